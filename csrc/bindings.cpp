@@ -29,6 +29,10 @@
 #include "ssd.cuh"
 #include "conv1d.cuh"
 
+namespace bw {
+void register_post_training(pybind11::module_& m);  // post_training.cpp
+}
+
 namespace {
 
 using torch::Tensor;
@@ -1383,4 +1387,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ce_fwd", &ce_fwd);
   m.def("ce_bwd_inplace", &ce_bwd_inplace);
   bw::register_projector(m);
+  bw::register_post_training(m);
 }

@@ -1,0 +1,406 @@
+// Bindings of the post-training operators: preference and policy losses from logits, the
+// router's balance loss, and head norms with rotation.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include <algorithm>
+#include <optional>
+#include <string>
+#include <vector>
+
+#include "logit_loss.cuh"
+#include "qk_norm.cuh"
+#include "router_balance.cuh"
+
+namespace {
+
+using torch::Tensor;
+using OptTensor = std::optional<Tensor>;
+
+bw::Elem elem_of(const Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case torch::kBFloat16:
+      return bw::Elem::kBF16;
+    case torch::kHalf:
+      return bw::Elem::kF16;
+    case torch::kFloat32:
+      return bw::Elem::kF32;
+    default:
+      TORCH_CHECK_TYPE(false, name, " must be bfloat16, float16 or float32, got ", t.scalar_type());
+  }
+}
+
+void check_like(const Tensor& t, const char* name, torch::ScalarType type, const Tensor& with) {
+  TORCH_CHECK(t.is_cuda() && t.device() == with.device(), name, " must be on ", with.device());
+  TORCH_CHECK_TYPE(t.scalar_type() == type, name, " must be ", type, ", got ", t.scalar_type());
+  TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+}
+
+const float* floats(const OptTensor& t) { return t.has_value() ? t->data_ptr<float>() : nullptr; }
+
+bw::LogitRows logit_rows(const Tensor& logits, const Tensor& labels, int64_t ignore, double temperature,
+                         const Tensor& err) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 3, "logits must be a (B, T, V) CUDA tensor");
+  const int64_t B = logits.size(0), T = logits.size(1), V = logits.size(2);
+  TORCH_CHECK(V >= 1 && V < (int64_t(1) << 30), "logits: the vocabulary must have 1 to 2^30 - 1 entries");
+  TORCH_CHECK(V == 1 || logits.stride(2) == 1 || logits.numel() == 0, "logits must be contiguous along the vocabulary");
+  TORCH_CHECK(B * T < (int64_t(1) << 31), "logits: at most 2^31 - 1 rows");
+  check_like(labels, "labels", torch::kInt64, logits);
+  TORCH_CHECK(labels.dim() == 2 && labels.size(0) == B && labels.size(1) == T, "labels must be (B, T)");
+  check_like(err, "err", torch::kInt32, logits);
+  return bw::LogitRows{logits.data_ptr(),          logits.stride(0), logits.stride(1), elem_of(logits, "logits"),
+                       (int)B,                     (int)T,           (int)V,           labels.data_ptr<int64_t>(),
+                       ignore,                     (float)(1.0 / temperature),         err.data_ptr<int>()};
+}
+
+// Memory for the gradient of `logits`. Its rows start at the same offset within 16 bytes as the rows of the logits
+// wherever those do not overlap, so that both sides move whole vectors.
+Tensor grad_like(const Tensor& logits) {
+  const int64_t n = 16 / logits.element_size(), V = logits.size(2);
+  const auto shift = (int64_t)(reinterpret_cast<uintptr_t>(logits.data_ptr()) % 16) / logits.element_size();
+  if (logits.is_contiguous() && shift == 0) return torch::empty(logits.sizes(), logits.options());
+  const bool even = V % n == 0;
+  if (even && shift == 0 && logits.stride(0) % n == 0 && logits.stride(1) % n == 0)
+    return torch::empty(logits.sizes(), logits.options());
+  const int64_t B = logits.size(0), T = logits.size(1), sb = logits.stride(0), st = logits.stride(1);
+  const bool apart = (T <= 1 || st >= V) && (B <= 1 || sb >= V) &&
+                     (T <= 1 || B <= 1 || sb >= (T - 1) * st + V || st >= (B - 1) * sb + V);
+  if (!apart || logits.numel() == 0) return torch::empty(logits.sizes(), logits.options());
+  const int64_t span = (B - 1) * sb + (T - 1) * st + V + shift;
+  if (span > 2 * logits.numel() + n) return torch::empty(logits.sizes(), logits.options());
+  return torch::empty({span}, logits.options()).as_strided(logits.sizes(), logits.strides(), shift);
+}
+
+// The float workspace of a preference loss: [stats 2 R | d (B) | scale (B) | token log-probabilities R | pair losses P | ticket].
+std::vector<Tensor> preference_fwd(Tensor logits, Tensor labels, Tensor ref, int64_t kind, double beta,
+                                   double smoothing, bool average, int64_t reduction, int64_t ignore, Tensor err) {
+  const c10::cuda::CUDAGuard guard(logits.device());
+  bw::PreferenceArgs a;
+  a.rows = logit_rows(logits, labels, ignore, 1.0, err);
+  const int64_t B = a.rows.B, P = B / 2, R = B * a.rows.T;
+  TORCH_CHECK(B >= 2 && B % 2 == 0, "a preference loss needs an even number of sequences: chosen, then rejected");
+  check_like(ref, "ref_logps", torch::kFloat32, logits);
+  TORCH_CHECK(ref.numel() == B, "ref_logps must be (B)");
+  const auto f32 = logits.options().dtype(torch::kFloat32);
+  auto ws = torch::empty({2 * R + 2 * B + R + P + 1}, f32);
+  auto logps = torch::empty({B}, f32);
+  auto loss = reduction == 0 ? torch::empty({P}, f32) : torch::empty({}, f32);
+  float* w = ws.data_ptr<float>();
+  a.ref = ref.data_ptr<float>();
+  a.stats = reinterpret_cast<bw::RowStat*>(w);
+  a.dseq = w + 2 * R;
+  a.scale = a.dseq + B;
+  a.logp_tok = a.scale + B;
+  a.pair_loss = a.logp_tok + R;
+  a.ticket = reinterpret_cast<unsigned*>(a.pair_loss + P);
+  a.logps = logps.data_ptr<float>();
+  a.loss = loss.data_ptr<float>();
+  a.kind = (bw::PairLoss)kind;
+  a.beta = (float)beta;
+  a.smoothing = (float)smoothing;
+  a.weight = reduction == 1 ? 1.f / (float)P : 1.f;
+  a.average = average;
+  a.reduced = reduction != 0;
+  bw::preference_fwd(a, at::cuda::getCurrentCUDAStream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {loss, logps, ws};
+}
+
+Tensor preference_bwd(Tensor logits, Tensor labels, Tensor ws, OptTensor g_loss, OptTensor g_logps, int64_t ignore,
+                      Tensor err) {
+  const c10::cuda::CUDAGuard guard(logits.device());
+  bw::LogitGradArgs a;
+  a.rows = logit_rows(logits, labels, ignore, 1.0, err);
+  const int64_t B = a.rows.B, R = B * a.rows.T;
+  check_like(ws, "workspace", torch::kFloat32, logits);
+  TORCH_CHECK(ws.numel() >= 3 * R + 2 * B, "workspace is too small");
+  if (g_loss.has_value()) {
+    check_like(*g_loss, "loss gradient", torch::kFloat32, logits);
+    TORCH_CHECK(g_loss->dim() == 0 || g_loss->numel() == B / 2, "loss gradient must be a scalar or (P)");
+  }
+  if (g_logps.has_value()) {
+    check_like(*g_logps, "logps gradient", torch::kFloat32, logits);
+    TORCH_CHECK(g_logps->numel() == B, "logps gradient must be (B)");
+  }
+  auto out = grad_like(logits);
+  const float* w = ws.data_ptr<float>();
+  a.stats = reinterpret_cast<const bw::RowStat*>(w);
+  a.d = w + 2 * R;
+  a.scale = a.d + B;
+  a.g_loss = floats(g_loss);
+  a.g_loss_mod = g_loss.has_value() && g_loss->dim() > 0 ? (int)(B / 2) : 0;
+  a.g_logps = floats(g_logps);
+  a.per_row = false;
+  a.out = out.data_ptr();
+  a.osb = out.stride(0);
+  a.ost = out.stride(1);
+  bw::logit_grad(a, at::cuda::getCurrentCUDAStream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return out;
+}
+
+// The float workspace of a policy loss: [stats 2 R | d R | sums of sequences 8 B | token counts B | ticket].
+std::vector<Tensor> policy_fwd(Tensor logits, Tensor labels, Tensor adv, OptTensor old_logps, OptTensor ref_logps,
+                               double clip_lo, double clip_hi, double kl_coef, double temperature, int64_t mean,
+                               int64_t ignore, Tensor err) {
+  const c10::cuda::CUDAGuard guard(logits.device());
+  bw::PolicyArgs a;
+  a.rows = logit_rows(logits, labels, ignore, temperature, err);
+  const int64_t B = a.rows.B, T = a.rows.T, R = B * T;
+  TORCH_CHECK(B >= 1, "a policy loss needs at least one sequence");
+  check_like(adv, "advantages", torch::kFloat32, logits);
+  TORCH_CHECK((adv.dim() == 1 && adv.size(0) == B) || (adv.dim() == 2 && adv.size(0) == B && adv.size(1) == T),
+              "advantages must be (B) or (B, T)");
+  for (const auto& [t, name] : {std::pair<const OptTensor&, const char*>{old_logps, "old_logps"}, {ref_logps, "ref_logps"}}) {
+    if (!t.has_value()) continue;
+    check_like(*t, name, torch::kFloat32, logits);
+    TORCH_CHECK(t->dim() == 2 && t->size(0) == B && t->size(1) == T, name, " must be (B, T)");
+  }
+  const auto f32 = logits.options().dtype(torch::kFloat32);
+  const int64_t even = R + (R & 1);
+  auto ws = torch::empty({2 * R + even + 8 * B + B + 1}, f32);
+  auto logps = torch::empty({B, T}, f32);
+  auto loss = torch::empty({}, f32), kl = torch::empty({}, f32), clipped = torch::empty({}, f32);
+  float* w = ws.data_ptr<float>();
+  a.adv = adv.data_ptr<float>();
+  a.old_logps = floats(old_logps);
+  a.ref_logps = floats(ref_logps);
+  a.adv_per_token = adv.dim() == 2;
+  a.clip_lo = (float)clip_lo;
+  a.clip_hi = (float)clip_hi;
+  a.kl_coef = (float)kl_coef;
+  a.mean = (bw::TokenMean)mean;
+  a.logps = logps.data_ptr<float>();
+  a.stats = reinterpret_cast<bw::RowStat*>(w);
+  a.dtok = w + 2 * R;
+  a.seq = reinterpret_cast<double*>(a.dtok + even);
+  a.count = reinterpret_cast<int*>(a.seq + 4 * B);
+  a.ticket = reinterpret_cast<unsigned*>(a.count + B);
+  a.loss = loss.data_ptr<float>();
+  a.kl = kl.data_ptr<float>();
+  a.clipped = clipped.data_ptr<float>();
+  bw::policy_fwd(a, at::cuda::getCurrentCUDAStream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {loss, logps, kl, clipped, ws};
+}
+
+Tensor policy_bwd(Tensor logits, Tensor labels, Tensor ws, OptTensor g_loss, OptTensor g_logps, double temperature,
+                  int64_t ignore, Tensor err) {
+  const c10::cuda::CUDAGuard guard(logits.device());
+  bw::LogitGradArgs a;
+  a.rows = logit_rows(logits, labels, ignore, temperature, err);
+  const int64_t R = (int64_t)a.rows.B * a.rows.T;
+  check_like(ws, "workspace", torch::kFloat32, logits);
+  TORCH_CHECK(ws.numel() >= 3 * R, "workspace is too small");
+  if (g_loss.has_value()) {
+    check_like(*g_loss, "loss gradient", torch::kFloat32, logits);
+    TORCH_CHECK(g_loss->numel() == 1, "loss gradient must be a scalar");
+  }
+  if (g_logps.has_value()) {
+    check_like(*g_logps, "logps gradient", torch::kFloat32, logits);
+    TORCH_CHECK(g_logps->numel() == R, "logps gradient must be (B, T)");
+  }
+  auto out = grad_like(logits);
+  const float* w = ws.data_ptr<float>();
+  a.stats = reinterpret_cast<const bw::RowStat*>(w);
+  a.d = w + 2 * R;
+  a.scale = nullptr;
+  a.g_loss = floats(g_loss);
+  a.g_loss_mod = 0;
+  a.g_logps = floats(g_logps);
+  a.per_row = true;
+  a.out = out.data_ptr();
+  a.osb = out.stride(0);
+  a.ost = out.stride(1);
+  bw::logit_grad(a, at::cuda::getCurrentCUDAStream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return out;
+}
+
+bw::BalanceArgs balance_args(const Tensor& logits, const OptTensor& ids, const OptTensor& mask, int64_t top_k,
+                             double z_coef, const Tensor& err) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 3, "router logits must be a (G, N, E) CUDA tensor");
+  bw::BalanceArgs a{};
+  const int64_t G = logits.size(0), N = logits.size(1), E = logits.size(2);
+  TORCH_CHECK(E >= 1 && E <= bw::kMaxExperts, "router logits: 1 to ", std::to_string(bw::kMaxExperts), " experts");
+  TORCH_CHECK(E == 1 || logits.stride(2) == 1 || logits.numel() == 0, "router logits must be contiguous along the experts");
+  TORCH_CHECK(top_k >= 1 && top_k <= E, "top_k must be between 1 and the number of experts");
+  TORCH_CHECK(G <= 65535, "router logits: at most 65535 groups");
+  TORCH_CHECK(N < (int64_t(1) << 31) / (top_k > 8 ? top_k : 8), "router logits: too many tokens in a group");
+  a.x = logits.data_ptr();
+  a.type = elem_of(logits, "router logits");
+  a.sg = logits.stride(0);
+  a.sn = logits.stride(1);
+  a.G = (int)G;
+  a.N = (int)N;
+  a.E = (int)E;
+  a.K = (int)top_k;
+  if (ids.has_value()) {
+    check_like(*ids, "expert_ids", torch::kInt64, logits);
+    TORCH_CHECK(ids->numel() == G * N * top_k, "expert_ids must be (..., N, top_k)");
+    a.ids = ids->data_ptr<int64_t>();
+  }
+  if (mask.has_value()) {
+    check_like(*mask, "mask", torch::kBool, logits);
+    TORCH_CHECK(mask->numel() == G * N, "mask must be (..., N)");
+    a.mask = reinterpret_cast<const uint8_t*>(mask->data_ptr<bool>());
+  }
+  a.z_coef = (float)z_coef;
+  const int64_t want = (148 * 4 + G - 1) / (G > 0 ? G : 1), have = (N + 63) / 64;
+  a.chunks = (int)std::max<int64_t>(1, std::min(want, have));
+  check_like(err, "err", torch::kInt32, logits);
+  a.err = err.data_ptr<int>();
+  return a;
+}
+
+std::vector<Tensor> balance_fwd(Tensor logits, OptTensor ids, OptTensor mask, int64_t top_k, double z_coef, Tensor err) {
+  const c10::cuda::CUDAGuard guard(logits.device());
+  bw::BalanceArgs a = balance_args(logits, ids, mask, top_k, z_coef, err);
+  const auto f32 = logits.options().dtype(torch::kFloat32);
+  const int64_t cells = (int64_t)a.G * a.chunks * (a.E + 1);
+  auto part = torch::empty({2 * cells}, f32);
+  auto loss = torch::empty({a.G}, f32), share = torch::empty({a.G, a.E + 1}, f32);
+  auto counts = torch::empty({a.G, a.E}, logits.options().dtype(torch::kInt64));
+  a.part = part.data_ptr<float>();
+  a.part_count = reinterpret_cast<int*>(a.part + cells);
+  a.loss = loss.data_ptr<float>();
+  a.counts = counts.data_ptr<int64_t>();
+  a.share = share.data_ptr<float>();
+  if (a.G > 0) bw::balance_fwd(a, at::cuda::getCurrentCUDAStream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {loss, counts, share};
+}
+
+Tensor balance_bwd(Tensor logits, OptTensor mask, Tensor share, Tensor g_loss, int64_t top_k, double z_coef, Tensor err) {
+  const c10::cuda::CUDAGuard guard(logits.device());
+  bw::BalanceGradArgs b;
+  b.f = balance_args(logits, std::nullopt, mask, top_k, z_coef, err);
+  check_like(share, "share", torch::kFloat32, logits);
+  TORCH_CHECK(share.numel() == (int64_t)b.f.G * (b.f.E + 1), "share must be (G, E + 1)");
+  TORCH_CHECK(g_loss.is_cuda() && g_loss.scalar_type() == torch::kFloat32 && g_loss.dim() == 1 && g_loss.size(0) == b.f.G,
+              "loss gradient must be (G) float32");
+  b.f.share = share.data_ptr<float>();
+  b.g_loss = g_loss.data_ptr<float>();
+  b.g_stride = g_loss.stride(0);
+  auto out = torch::empty(logits.sizes(), logits.options());
+  b.out = out.data_ptr();
+  if (out.numel() > 0) bw::balance_bwd(b, at::cuda::getCurrentCUDAStream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return out;
+}
+
+bw::HeadTensor head_tensor(const Tensor& x, const Tensor& w, const char* name) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 4, name, " must be a (B, T, H, D) CUDA tensor");
+  TORCH_CHECK(x.size(3) == 1 || x.stride(3) == 1 || x.numel() == 0, name, " must be contiguous along the head's elements");
+  TORCH_CHECK(w.is_cuda() && w.device() == x.device() && w.dim() == 1 && w.size(0) == x.size(3) && w.is_contiguous(),
+              name, " weight must be a contiguous (D) tensor on the same device");
+  return bw::HeadTensor{x.data_ptr(), x.stride(0), x.stride(1), x.stride(2), nullptr, w.data_ptr(), (int)x.size(2)};
+}
+
+bw::QkNormArgs qk_args(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw, const Tensor& cos,
+                       const Tensor& sin, const OptTensor& positions, double eps, const Tensor& err) {
+  bw::QkNormArgs a{};
+  a.q = head_tensor(q, qw, "q");
+  a.k = head_tensor(k, kw, "k");
+  TORCH_CHECK(q.size(0) == k.size(0) && q.size(1) == k.size(1) && q.size(3) == k.size(3) && q.device() == k.device(),
+              "q and k must be (B, T, H, D) with the same B, T and D");
+  a.type = elem_of(q, "q");
+  TORCH_CHECK_TYPE(k.scalar_type() == q.scalar_type(), "q and k must have one type");
+  a.wtype = elem_of(qw, "weights");
+  TORCH_CHECK_TYPE(kw.scalar_type() == qw.scalar_type(), "both weights must have one type");
+  a.B = (int)q.size(0);
+  a.T = (int)q.size(1);
+  a.D = (int)q.size(3);
+  TORCH_CHECK(a.D >= 2 && a.D % 2 == 0 && a.D <= bw::kMaxHeadDim, "the head dim must be even and at most ",
+              std::to_string(bw::kMaxHeadDim));
+  check_like(cos, "cos", torch::kFloat32, q);
+  check_like(sin, "sin", torch::kFloat32, q);
+  TORCH_CHECK(cos.dim() == 2 && sin.sizes() == cos.sizes() && 2 * cos.size(1) <= a.D,
+              "cos and sin must be (positions, R / 2) with R at most the head dim");
+  a.cos = cos.data_ptr<float>();
+  a.sin = sin.data_ptr<float>();
+  a.R = (int)(2 * cos.size(1));
+  TORCH_CHECK(cos.size(0) < (int64_t(1) << 31), "cos and sin: at most 2^31 - 1 positions");
+  a.table = (int)cos.size(0);
+  if (positions.has_value()) {
+    TORCH_CHECK(positions->is_cuda() && positions->device() == q.device() && positions->scalar_type() == torch::kInt64 &&
+                    positions->dim() == 2 && positions->size(0) == a.B && positions->size(1) == a.T,
+                "positions must be (B, T) int64 on the same device");
+    TORCH_CHECK(a.table > 0 || q.size(0) * q.size(1) == 0, "the tables of angles are empty");
+    a.positions = positions->data_ptr<int64_t>();
+    a.pb = positions->stride(0);
+    a.pt = positions->stride(1);
+  } else {
+    TORCH_CHECK(a.table >= a.T, "the tables of angles are shorter than the sequence");
+  }
+  a.eps = (float)eps;
+  check_like(err, "err", torch::kInt32, q);
+  a.err = err.data_ptr<int>();
+  return a;
+}
+
+std::vector<Tensor> qk_norm_fwd(Tensor q, Tensor k, Tensor qw, Tensor kw, Tensor cos, Tensor sin, OptTensor positions,
+                                double eps, Tensor err) {
+  const c10::cuda::CUDAGuard guard(q.device());
+  bw::QkNormArgs a = qk_args(q, k, qw, kw, cos, sin, positions, eps, err);
+  auto qo = torch::empty(q.sizes(), q.options()), ko = torch::empty(k.sizes(), k.options());
+  a.q.out = qo.data_ptr();
+  a.k.out = ko.data_ptr();
+  bw::qk_norm_fwd(a, at::cuda::getCurrentCUDAStream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {qo, ko};
+}
+
+void head_grad(const OptTensor& g, const Tensor& x, const char* name, const void*& p, long long& sb, long long& st,
+               long long& sh) {
+  p = nullptr;
+  sb = st = sh = 0;
+  if (!g.has_value()) return;
+  TORCH_CHECK(g->is_cuda() && g->device() == x.device() && g->sizes() == x.sizes() &&
+                  g->scalar_type() == x.scalar_type() && (x.size(3) == 1 || g->stride(3) == 1 || g->numel() == 0),
+              "the gradient of ", name, " must be like it, contiguous along the head's elements");
+  p = g->data_ptr();
+  sb = g->stride(0);
+  st = g->stride(1);
+  sh = g->stride(2);
+}
+
+std::vector<Tensor> qk_norm_bwd(OptTensor gq, OptTensor gk, Tensor q, Tensor k, Tensor qw, Tensor kw, Tensor cos,
+                                Tensor sin, OptTensor positions, double eps, Tensor err) {
+  const c10::cuda::CUDAGuard guard(q.device());
+  bw::QkNormGradArgs b{};
+  b.f = qk_args(q, k, qw, kw, cos, sin, positions, eps, err);
+  head_grad(gq, q, "q", b.gq, b.gqb, b.gqt, b.gqh);
+  head_grad(gk, k, "k", b.gk, b.gkb, b.gkt, b.gkh);
+  auto dq = torch::empty(q.sizes(), q.options()), dk = torch::empty(k.sizes(), k.options());
+  auto dqw = torch::empty(qw.sizes(), qw.options()), dkw = torch::empty(kw.sizes(), kw.options());
+  b.f.q.out = dq.data_ptr();
+  b.f.k.out = dk.data_ptr();
+  b.dqw = dqw.data_ptr();
+  b.dkw = dkw.data_ptr();
+  bw::qk_norm_blocks(b.f, &b.q_blocks, &b.k_blocks);
+  auto part = torch::empty({(int64_t)(b.q_blocks + b.k_blocks) * b.f.D}, q.options().dtype(torch::kFloat32));
+  b.part = part.data_ptr<float>();
+  bw::qk_norm_bwd(b, at::cuda::getCurrentCUDAStream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {dq, dk, dqw, dkw};
+}
+
+}  // namespace
+
+namespace bw {
+
+void register_post_training(pybind11::module_& m) {
+  m.def("preference_fwd", &::preference_fwd, "preference loss of pairs of sequences from logits");
+  m.def("preference_bwd", &::preference_bwd);
+  m.def("policy_fwd", &::policy_fwd, "clipped policy loss with a KL term from logits");
+  m.def("policy_bwd", &::policy_bwd);
+  m.def("balance_fwd", &::balance_fwd, "router balance loss and per-expert counts");
+  m.def("balance_bwd", &::balance_bwd);
+  m.def("qk_norm_fwd", &::qk_norm_fwd, "RMS norm of q and k heads with rotation by position");
+  m.def("qk_norm_bwd", &::qk_norm_bwd);
+}
+
+}  // namespace bw

@@ -116,7 +116,7 @@ _ERR_NAMES = {
     2: "a pipeline stage never drained (MMA wait timed out)",
     3: "the accumulator never completed",
     4: "a peer GPU flag never arrived",
-    5: "a kernel rejected its arguments",
+    5: "a kernel rejected its arguments (a label, expert id or position out of range)",
     6: "a peer-staged tile never became ready",
 }
 
@@ -138,6 +138,7 @@ def check_device_errors(device: torch.device | int | None = None) -> None:
             )
 
 
+from dattri_llm_b200.ops.fused import qk_norm_rope  # noqa: E402
 from dattri_llm_b200.ops.gemm import (  # noqa: E402
     STORE_ATOMIC_F32,
     STORE_BF16,
@@ -158,11 +159,22 @@ from dattri_llm_b200.ops.gram import (  # noqa: E402
     mask_gather,
     per_sample_outer,
 )
+from dattri_llm_b200.ops.losses import (  # noqa: E402
+    BalanceLoss,
+    PolicyLoss,
+    PreferenceLoss,
+    policy_loss,
+    preference_loss,
+    router_balance_loss,
+)
 from dattri_llm_b200.ops.norm import embedding_dense_grad, norm_per_sample_grad  # noqa: E402
 from dattri_llm_b200.ops.optim import adam_direction  # noqa: E402
 from dattri_llm_b200.ops.projection import projection_matrix_t  # noqa: E402
 
 __all__ = [
+    "BalanceLoss",
+    "PolicyLoss",
+    "PreferenceLoss",
     "STORE_ATOMIC_F32",
     "STORE_BF16",
     "STORE_BF16_T",
@@ -188,6 +200,10 @@ __all__ = [
     "embedding_dense_grad",
     "norm_per_sample_grad",
     "per_sample_outer",
+    "policy_loss",
+    "preference_loss",
     "projection_matrix_t",
+    "qk_norm_rope",
+    "router_balance_loss",
     "use_native",
 ]

@@ -337,3 +337,89 @@ def causal_conv_silu(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor |
     """``silu(conv1d(x^T, weight, bias, padding=3, groups=C)[..., :L])^T`` token-major, one kernel
     each way (the Mamba2 mixer's convolution and activation)."""
     return _CausalConvSiLU.apply(x, weight, bias)
+
+
+class _QkNormRope(torch.autograd.Function):
+    """RMS norm of each q / k head and rotation by position (``csrc/qk_norm.cu``)."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps):
+        from dattri_llm_b200.ops import count_launch, error_word, native
+
+        count_launch()
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
+        ctx.eps = eps
+        return tuple(native().qk_norm_fwd(q, k, q_weight, k_weight, cos, sin, positions, eps, error_word(q.device)))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk):
+        from dattri_llm_b200.ops import count_launch, error_word, native
+
+        if gq is None and gk is None:
+            return (None,) * 8
+        q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
+        gq, gk = (g if g is None or g.stride(-1) == 1 else g.contiguous() for g in (gq, gk))
+        count_launch(2)
+        grads = native().qk_norm_bwd(gq, gk, q, k, q_weight, k_weight, cos, sin, positions, ctx.eps, error_word(q.device))
+        return (*grads, None, None, None, None)
+
+
+def _qk_norm_rope_torch(x, weight, cos, sin, eps):
+    wide = torch.promote_types(x.dtype, torch.float32)
+    half = cos.shape[-1]
+    x32 = x.to(wide)
+    y = x32 * torch.rsqrt(x32.square().mean(-1, keepdim=True) + eps) * weight.to(wide)
+    a, b, rest = y[..., :half], y[..., half:2 * half], y[..., 2 * half:]
+    return torch.cat([a * cos - b * sin, b * cos + a * sin, rest], -1).to(x.dtype)
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, cos: torch.Tensor,
+                 sin: torch.Tensor, positions: torch.Tensor | None = None, *,
+                 eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMS norm of every query and key head, then the rotation of its first ``R`` elements by
+    position, in one pass: ``rotate(x * rsqrt(mean(x^2) + eps) * weight)``, rounded once.
+
+    Args:
+        q, k: ``(B, T, Hq, D)`` and ``(B, T, Hk, D)`` of one type (bf16, fp16 or fp32 on the
+            GPU), ``D`` even and at most 512; any strides, e.g. slices of one projection's output.
+        q_weight, k_weight: ``(D,)`` norm weights.
+        cos, sin: ``(positions, R / 2)`` tables of the angles, ``R <= D``; element *i* is
+            rotated with element ``i + R / 2``, elements from ``R`` on are not.
+        positions: rows of the tables, ``(T,)`` or ``(B, T)``; ``None``: ``0 .. T - 1``.  One
+            outside the tables is held to them and reported by
+            :func:`~dattri_llm_b200.ops.check_device_errors` (raised at once on CPU).
+
+    Returns:
+        The new q and k, contiguous.  Gradients reach q, k and both weights.
+    """
+    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3] or q.dtype != k.dtype:
+        raise ValueError(f"q and k must be (B, T, H, D) of one type with the same B, T and D, got {q.dtype} "
+                         f"{tuple(q.shape)} and {k.dtype} {tuple(k.shape)}")
+    b, t, _, d = q.shape
+    if q_weight.shape != (d,) or k_weight.shape != (d,) or q_weight.dtype != k_weight.dtype:
+        raise ValueError(f"both weights must be ({d},) of one type")
+    if cos.dim() != 2 or cos.shape != sin.shape or 2 * cos.shape[1] > d or d % 2:
+        raise ValueError(f"cos and sin must be (positions, R / 2) with R <= {d}, and D even, got {tuple(cos.shape)} and "
+                         f"{tuple(sin.shape)}")
+    if cos.requires_grad or sin.requires_grad:
+        raise ValueError("the tables of angles are constants: detach them")
+    if positions is not None:
+        if positions.shape not in ((t,), (b, t)) or positions.is_floating_point() or positions.dtype == torch.bool:
+            raise ValueError(f"positions must be whole numbers ({t},) or ({b}, {t}), got {positions.dtype} "
+                             f"{tuple(positions.shape)}")
+        positions = positions.long().expand(b, t)
+    elif cos.shape[0] < t:
+        raise ValueError(f"the tables hold {cos.shape[0]} positions, the sequence has {t}")
+    from dattri_llm_b200.ops import use_native
+
+    if not use_native(q):
+        if positions is not None and bool(((positions < 0) | (positions >= cos.shape[0])).any()):
+            raise ValueError(f"positions must be in [0, {cos.shape[0]})")
+        cos, sin = (x[:t] if positions is None else x[positions] for x in (cos, sin))
+        cos, sin = cos.unsqueeze(-2), sin.unsqueeze(-2)
+        return (_qk_norm_rope_torch(q, q_weight, cos, sin, eps), _qk_norm_rope_torch(k, k_weight, cos, sin, eps))
+    q, k = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k))
+    cos, sin = (x.to(torch.float32).contiguous() for x in (cos, sin))
+    return _QkNormRope.apply(q, k, q_weight.contiguous(), k_weight.contiguous(), cos, sin, positions, float(eps))

@@ -1,0 +1,400 @@
+"""Losses of post-training: preference pairs, clipped policy updates, router balance.
+
+Each takes logits and returns a loss that backpropagates into them:
+
+* :func:`preference_loss` -- paired log ratios of chosen and rejected sequences against a
+  reference model (sigmoid, hinge or squared form);
+* :func:`policy_loss` -- the clipped surrogate of sampled tokens with a KL term;
+* :func:`router_balance_loss` -- the auxiliary loss of an expert router, with the number of
+  tokens each expert received.
+
+On sm_100 they run the kernels of ``csrc/logit_loss.cu`` and ``csrc/router_balance.cu``
+(bf16, fp16 or fp32 logits; fp32 softmax statistics, sums over tokens in fp64); the same
+formulas in PyTorch serve CPU tensors.  The reference has neither: its losses are the
+user's own.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import NamedTuple
+
+import torch
+import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
+
+PAIR_LOSSES = {"sigmoid": 0, "hinge": 1, "ipo": 2}
+_PAIR_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+_TOKEN_REDUCTIONS = {"token_mean": 0, "sequence_mean": 1, "sum": 2}
+
+
+class PreferenceLoss(NamedTuple):
+    """``loss`` (a scalar, or ``(P,)`` with ``reduction="none"``) and the policy's log-probability
+    of each sequence ``logps (2P,)``; both backpropagate into the logits."""
+
+    loss: torch.Tensor
+    logps: torch.Tensor
+
+
+class PolicyLoss(NamedTuple):
+    """``loss`` (scalar) and the policy's token log-probabilities ``logps (B, T)`` (0 where
+    ignored), which backpropagate; the mean ``kl`` and the ``clip_fraction`` over the tokens
+    that count, which do not."""
+
+    loss: torch.Tensor
+    logps: torch.Tensor
+    kl: torch.Tensor
+    clip_fraction: torch.Tensor
+
+
+class BalanceLoss(NamedTuple):
+    """``loss`` of every group (the leading shape of the logits), which backpropagates, and the
+    tokens each expert received, ``counts (..., E)`` int64."""
+
+    loss: torch.Tensor
+    counts: torch.Tensor
+
+
+def _native(x: torch.Tensor) -> bool:
+    from dattri_llm_b200.ops import use_native
+
+    return use_native(x)
+
+
+def _constant(name: str, x: torch.Tensor | None) -> torch.Tensor | None:
+    """*x* as contiguous fp32, or an error if it would need a gradient."""
+    if x is None:
+        return None
+    if x.requires_grad:
+        raise ValueError(f"{name} is a constant of the loss: detach it")
+    return x.to(torch.float32).contiguous()
+
+
+def _check_logits(logits: torch.Tensor, labels: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    if logits.dim() != 3 or not logits.is_floating_point():
+        raise ValueError(f"logits must be floating (B, T, V), got {logits.dtype} {tuple(logits.shape)}")
+    if labels.shape != logits.shape[:2] or labels.is_floating_point() or labels.dtype == torch.bool:
+        raise ValueError(f"labels must be whole numbers (B, T) = {tuple(logits.shape[:2])}, got {labels.dtype} "
+                         f"{tuple(labels.shape)}")
+    if logits.shape[2] == 0:
+        raise ValueError("logits need a vocabulary of at least one entry")
+    if labels.device != logits.device:
+        raise ValueError(f"labels are on {labels.device}, logits on {logits.device}")
+    if logits.stride(2) != 1:
+        logits = logits.contiguous()
+    return logits, labels.long().contiguous()
+
+
+def _token_logps(logits: torch.Tensor, labels: torch.Tensor, ignore: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(log-probabilities of the labels, 0 where ignored, which tokens count)`` in PyTorch."""
+    valid = labels != ignore
+    if bool(((labels < 0) | (labels >= logits.shape[2]))[valid].any()):
+        raise ValueError(f"labels must be {ignore} or in [0, {logits.shape[2]})")
+    x = logits if logits.dtype == torch.float64 else logits.float()
+    x = x.masked_fill(~valid.unsqueeze(-1), 0.0)  # an ignored row may hold anything
+    logps = torch.log_softmax(x, -1).gather(2, labels.masked_fill(~valid, 0).unsqueeze(-1)).squeeze(-1)
+    return logps.masked_fill(~valid, 0.0), valid
+
+
+# ---------------------------------------------------------------- preference
+
+
+class _PreferenceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, ref, kind, beta, smoothing, average, reduction, ignore):
+        from dattri_llm_b200.ops import count_launch, error_word, native
+
+        err = error_word(logits.device)
+        count_launch(2)
+        loss, logps, ws = native().preference_fwd(logits, labels, ref, kind, beta, smoothing, average, reduction, ignore,
+                                                  err)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(logits, labels, ws)
+        ctx.ignore = ignore
+        return loss, logps
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_loss, g_logps):
+        from dattri_llm_b200.ops import count_launch, error_word, native
+
+        if g_loss is None and g_logps is None:
+            return (None,) * 9
+        logits, labels, ws = ctx.saved_tensors
+        g_loss, g_logps = (None if g is None else g.contiguous() for g in (g_loss, g_logps))
+        count_launch()
+        return (native().preference_bwd(logits, labels, ws, g_loss, g_logps, ctx.ignore, error_word(logits.device)),
+                *(None,) * 8)
+
+
+def _preference_torch(logits, labels, ref, kind, beta, smoothing, average, reduction, ignore) -> PreferenceLoss:
+    tokens, valid = _token_logps(logits, labels, ignore)
+    logps = tokens.sum(1)
+    if average:
+        logps = logps / valid.sum(1).clamp(min=1)
+    chosen, rejected = (logps - ref).chunk(2)
+    m = chosen - rejected
+    if kind == "sigmoid":
+        loss = -(1 - smoothing) * F.logsigmoid(beta * m)
+        if smoothing:
+            loss = loss - smoothing * F.logsigmoid(-beta * m)
+    elif kind == "hinge":
+        loss = torch.relu(1 - beta * m)
+    else:
+        loss = (m - 1 / (2 * beta)).square()
+    return PreferenceLoss(loss if reduction == "none" else loss.mean() if reduction == "mean" else loss.sum(), logps)
+
+
+def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch.Tensor, *, beta: float = 0.1,
+                    kind: str = "sigmoid", label_smoothing: float = 0.0, average_logps: bool = False,
+                    reduction: str = "mean", ignore_index: int = -100) -> PreferenceLoss:
+    """Preference loss of ``P`` pairs: sequences ``0 .. P-1`` of the batch are the chosen ones,
+    sequence ``P + i`` is the one rejected against sequence ``i``.
+
+    With ``L_b`` the summed (*average_logps*: mean) log-probability of sequence *b*'s labels
+    and ``m = (L_i - ref_i) - (L_{P+i} - ref_{P+i})``:
+
+    * ``"sigmoid"``: ``-(1 - s) log sigmoid(beta m) - s log sigmoid(-beta m)``, ``s`` = *label_smoothing*;
+    * ``"hinge"``: ``max(0, 1 - beta m)``;
+    * ``"ipo"``: ``(m - 1 / (2 beta))^2``.
+
+    Args:
+        logits: ``(2P, T, V)``, any batch and token strides.
+        labels: ``(2P, T)``, the token that ``logits[b, t]`` predicts (shift the labels, not
+            the logits: a shifted slice of the logits costs a copy of their gradient) or
+            *ignore_index*.  The logits of ignored positions are not read.
+        ref_logps: ``(2P,)`` the reference model's ``L_b``; a constant.
+        reduction: ``"mean"`` or ``"sum"`` over pairs, or ``"none"``.
+
+    Returns:
+        :class:`PreferenceLoss`.  A label outside the vocabulary is left out and reported by
+        :func:`~dattri_llm_b200.ops.check_device_errors` (raised at once on CPU).
+    """
+    logits, labels = _check_logits(logits, labels)
+    b = logits.shape[0]
+    if b < 2 or b % 2:
+        raise ValueError(f"a preference loss needs an even number of sequences (chosen, then rejected), got {b}")
+    if kind not in PAIR_LOSSES:
+        raise ValueError(f"kind must be one of {sorted(PAIR_LOSSES)}, got {kind!r}")
+    if reduction not in _PAIR_REDUCTIONS:
+        raise ValueError(f"reduction must be one of {sorted(_PAIR_REDUCTIONS)}, got {reduction!r}")
+    if not (beta > 0 and math.isfinite(beta)):
+        raise ValueError(f"beta must be positive, got {beta}")
+    if not 0 <= label_smoothing < 0.5 or (label_smoothing and kind != "sigmoid"):
+        raise ValueError(f"label_smoothing must be in [0, 0.5), and 0 unless kind is 'sigmoid', got {label_smoothing}")
+    if ref_logps.shape != (b,):
+        raise ValueError(f"ref_logps must be ({b},), got {tuple(ref_logps.shape)}")
+    if not _native(logits):
+        ref = _constant("ref_logps", ref_logps).to(torch.promote_types(logits.dtype, torch.float32))
+        return _preference_torch(logits, labels, ref, kind, beta, label_smoothing, average_logps, reduction, ignore_index)
+    return PreferenceLoss(*_PreferenceLoss.apply(
+        logits, labels, _constant("ref_logps", ref_logps), PAIR_LOSSES[kind], beta, label_smoothing, average_logps,
+        _PAIR_REDUCTIONS[reduction], ignore_index))
+
+
+# ---------------------------------------------------------------- policy
+
+
+class _PolicyLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, adv, old, ref, lo, hi, kl_coef, temperature, reduction, ignore):
+        from dattri_llm_b200.ops import count_launch, error_word, native
+
+        err = error_word(logits.device)
+        count_launch(3)
+        loss, logps, kl, clipped, ws = native().policy_fwd(logits, labels, adv, old, ref, lo, hi, kl_coef, temperature,
+                                                           reduction, ignore, err)
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(kl, clipped)
+        ctx.save_for_backward(logits, labels, ws)
+        ctx.temperature, ctx.ignore = temperature, ignore
+        return loss, logps, kl, clipped
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_loss, g_logps, _kl, _clipped):
+        from dattri_llm_b200.ops import count_launch, error_word, native
+
+        if g_loss is None and g_logps is None:
+            return (None,) * 11
+        logits, labels, ws = ctx.saved_tensors
+        g_loss, g_logps = (None if g is None else g.contiguous() for g in (g_loss, g_logps))
+        count_launch()
+        return (native().policy_bwd(logits, labels, ws, g_loss, g_logps, ctx.temperature, ctx.ignore,
+                                    error_word(logits.device)), *(None,) * 10)
+
+
+def _policy_torch(logits, labels, adv, old, ref, lo, hi, kl_coef, temperature, reduction, ignore) -> PolicyLoss:
+    logps, valid = _token_logps(logits if temperature == 1.0 else logits / temperature, labels, ignore)
+    adv = adv if adv.dim() == 2 else adv.unsqueeze(1)
+    base = logps.detach() if old is None else old
+    ratio = torch.exp((logps - base).masked_fill(~valid, 0.0))
+    free, held = ratio * adv, ratio.clamp(lo, hi) * adv
+    loss = -torch.where(free <= held, free, held)
+    kl = torch.zeros_like(logps)
+    if ref is not None:
+        d = (ref - logps).masked_fill(~valid, 0.0)
+        kl = torch.expm1(d) - d
+        loss = loss + kl_coef * kl
+    loss = loss.masked_fill(~valid, 0.0)
+    n = valid.sum().clamp(min=1)
+    if reduction == "token_mean":
+        total = loss.sum() / n
+    elif reduction == "sequence_mean":
+        total = (loss.sum(1) / valid.sum(1).clamp(min=1)).mean()
+    else:
+        total = loss.sum()
+    clipped = ((held < free) & valid).sum().to(logps.dtype) / n
+    return PolicyLoss(total, logps, kl.detach().masked_fill(~valid, 0.0).sum() / n, clipped)
+
+
+def policy_loss(logits: torch.Tensor, labels: torch.Tensor, advantages: torch.Tensor,
+                old_logps: torch.Tensor | None = None, ref_logps: torch.Tensor | None = None, *,
+                clip: tuple[float, float] = (0.2, 0.2), kl_coef: float = 0.0, temperature: float = 1.0,
+                reduction: str = "token_mean", ignore_index: int = -100) -> PolicyLoss:
+    """Clipped policy loss of sampled tokens with a KL term.
+
+    With ``logp`` the log-probability of a label under ``softmax(logits / temperature)``,
+    ``r = exp(logp - old)`` and ``d = ref - logp``, each token that counts adds
+    ``-min(r A, clamp(r, 1 - clip[0], 1 + clip[1]) A) + kl_coef (exp(d) - d - 1)``.
+
+    Args:
+        logits: ``(B, T, V)``, any batch and token strides.
+        labels: ``(B, T)``, the sampled token that ``logits[b, t]`` predicts or *ignore_index*.
+            The logits of ignored positions are not read.
+        advantages: ``(B,)`` or ``(B, T)``; a constant.
+        old_logps: ``(B, T)`` log-probabilities at sampling time, or ``None`` for an on-policy
+            step (``r = 1``, whose gradient is ``-A``); a constant.
+        ref_logps: ``(B, T)`` log-probabilities under the reference model, or ``None``: no KL
+            term (then *kl_coef* must be 0); a constant.
+        reduction: ``"token_mean"`` over all tokens that count, ``"sequence_mean"`` (the mean
+            of the sequences' means; one without tokens adds 0), or ``"sum"``.
+
+    Returns:
+        :class:`PolicyLoss`.  A label outside the vocabulary is left out and reported by
+        :func:`~dattri_llm_b200.ops.check_device_errors` (raised at once on CPU).
+    """
+    logits, labels = _check_logits(logits, labels)
+    b, t = labels.shape
+    if b == 0:
+        raise ValueError("a policy loss needs at least one sequence")
+    if advantages.shape not in ((b,), (b, t)):
+        raise ValueError(f"advantages must be ({b},) or ({b}, {t}), got {tuple(advantages.shape)}")
+    for name, x in (("old_logps", old_logps), ("ref_logps", ref_logps)):
+        if x is not None and x.shape != (b, t):
+            raise ValueError(f"{name} must be ({b}, {t}), got {tuple(x.shape)}")
+    if reduction not in _TOKEN_REDUCTIONS:
+        raise ValueError(f"reduction must be one of {sorted(_TOKEN_REDUCTIONS)}, got {reduction!r}")
+    if not (temperature > 0 and math.isfinite(temperature)):
+        raise ValueError(f"temperature must be positive, got {temperature}")
+    if not (0 <= clip[0] <= 1 and clip[1] >= 0):
+        raise ValueError(f"clip must be (low in [0, 1], high >= 0), got {clip}")
+    if kl_coef and ref_logps is None:
+        raise ValueError("a KL term needs ref_logps")
+    lo, hi = 1.0 - clip[0], 1.0 + clip[1]
+    consts = tuple(_constant(n, x) for n, x in (("advantages", advantages), ("old_logps", old_logps),
+                                                 ("ref_logps", ref_logps)))
+    if not _native(logits):
+        wide = torch.promote_types(logits.dtype, torch.float32)
+        consts = tuple(None if x is None else x.to(wide) for x in consts)
+        return _policy_torch(logits, labels, *consts, lo, hi, kl_coef, temperature, reduction, ignore_index)
+    return PolicyLoss(*_PolicyLoss.apply(logits, labels, *consts, lo, hi, kl_coef, temperature,
+                                         _TOKEN_REDUCTIONS[reduction], ignore_index))
+
+
+# ---------------------------------------------------------------- router balance
+
+
+class _BalanceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, mask, top_k, z_coef):
+        from dattri_llm_b200.ops import count_launch, error_word, native
+
+        count_launch(2)
+        loss, counts, share = native().balance_fwd(logits, ids, mask, top_k, z_coef, error_word(logits.device))
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(counts)
+        ctx.save_for_backward(logits, mask, share)
+        ctx.top_k, ctx.z_coef = top_k, z_coef
+        return loss, counts
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_loss, _counts):
+        from dattri_llm_b200.ops import count_launch, error_word, native
+
+        if g_loss is None:
+            return (None,) * 5
+        logits, mask, share = ctx.saved_tensors
+        count_launch()
+        return (native().balance_bwd(logits, mask, share, g_loss, ctx.top_k, ctx.z_coef, error_word(logits.device)),
+                None, None, None, None)
+
+
+def _balance_torch(logits, ids, mask, top_k, z_coef) -> BalanceLoss:
+    g, n, e = logits.shape
+    x = logits if logits.dtype == torch.float64 else logits.float()
+    keep = torch.ones(g, n, dtype=torch.bool, device=x.device) if mask is None else mask
+    x = x.masked_fill(~keep.unsqueeze(-1), 0.0)  # a masked token may hold anything
+    if ids is None:
+        ids = torch.sort(x.detach(), dim=-1, descending=True, stable=True).indices[..., :top_k]
+    elif bool(((ids < 0) | (ids >= e))[keep].any()):
+        raise ValueError(f"expert_ids must be in [0, {e})")
+    chosen = keep.unsqueeze(-1).expand_as(ids)
+    counts = torch.zeros(g, e, dtype=torch.int64, device=x.device)
+    counts.scatter_add_(1, torch.where(chosen, ids, 0).reshape(g, -1), chosen.reshape(g, -1).long())
+    tokens = keep.sum(1).clamp(min=1).unsqueeze(-1)
+    mean_p = torch.softmax(x, -1).masked_fill(~keep.unsqueeze(-1), 0.0).sum(1) / tokens
+    loss = e * (counts / tokens * mean_p).sum(1)
+    if z_coef:
+        lse = torch.logsumexp(x, -1).masked_fill(~keep, 0.0)
+        loss = loss + z_coef * lse.square().sum(1) / tokens.squeeze(-1)
+    return BalanceLoss(loss, counts)
+
+
+def router_balance_loss(logits: torch.Tensor, top_k: int, expert_ids: torch.Tensor | None = None,
+                        mask: torch.Tensor | None = None, *, z_coef: float = 0.0) -> BalanceLoss:
+    """Auxiliary balance loss of an expert router, for every group of tokens by itself.
+
+    With ``p = softmax(logits)``, ``f_e`` the choices of expert *e* per token and ``P_e`` the
+    mean of ``p_e``, both over the tokens that count, a group's loss is
+    ``E sum_e f_e P_e + z_coef mean(logsumexp(logits)^2)``; it is ``top_k`` when all experts
+    are used alike.  ``f`` carries no gradient.  A group without tokens has loss 0.
+
+    Args:
+        logits: ``(..., N, E)``; each index of the leading axes (layers, sequences) is a group.
+        top_k: choices of each token.
+        expert_ids: ``(..., N, top_k)`` the experts chosen, or ``None``: the largest logits, the
+            lowest index where they tie.
+        mask: ``(..., N)`` bool, the tokens that count, or ``None``: all.  The others get no
+            gradient, whatever their logits hold.
+
+    Returns:
+        :class:`BalanceLoss`.  An expert id outside ``[0, E)`` is left out and reported by
+        :func:`~dattri_llm_b200.ops.check_device_errors` (raised at once on CPU).
+    """
+    if logits.dim() < 2 or not logits.is_floating_point():
+        raise ValueError(f"router logits must be floating (..., N, E), got {logits.dtype} {tuple(logits.shape)}")
+    lead, (n, e) = logits.shape[:-2], logits.shape[-2:]
+    if not 1 <= top_k <= e:
+        raise ValueError(f"top_k must be between 1 and the number of experts {e}, got {top_k}")
+    if expert_ids is not None:
+        if expert_ids.shape != (*lead, n, top_k) or expert_ids.is_floating_point() or expert_ids.dtype == torch.bool:
+            raise ValueError(f"expert_ids must be whole numbers {(*lead, n, top_k)}, got {expert_ids.dtype} "
+                             f"{tuple(expert_ids.shape)}")
+        expert_ids = expert_ids.long().contiguous()
+    if mask is not None:
+        if mask.shape != (*lead, n):
+            raise ValueError(f"mask must be {(*lead, n)}, got {tuple(mask.shape)}")
+        mask = (mask if mask.dtype == torch.bool else mask != 0).contiguous()
+    x = logits if len(lead) == 1 else logits.reshape(-1, n, e) if lead else logits.unsqueeze(0)
+    if x.stride(2) != 1:
+        x = x.contiguous()
+    if _native(x):
+        loss, counts = _BalanceLoss.apply(x, expert_ids, mask, int(top_k), float(z_coef))
+    else:
+        loss, counts = _balance_torch(x, None if expert_ids is None else expert_ids.view(-1, n, top_k),
+                                      None if mask is None else mask.view(-1, n), top_k, z_coef)
+    if len(lead) == 1:
+        return BalanceLoss(loss, counts)
+    return BalanceLoss(loss.reshape(lead), counts.reshape(*lead, e))
