@@ -1,11 +1,16 @@
 // Bindings of the post-training operators: preference and policy losses from logits, the
 // router's balance loss, and head norms with rotation.
+//
+// Their autograd functions are C++: a backward node written in Python takes the interpreter
+// lock from the engine's thread, which cost more than the kernels of a small call (forward and
+// backward of 96 logit rows on one B200: 111 us with Python nodes, 87 us with these, of which 48 us are the engine's).
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <atomic>
 #include <optional>
 #include <string>
 #include <vector>
@@ -18,6 +23,18 @@ namespace {
 
 using torch::Tensor;
 using OptTensor = std::optional<Tensor>;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+std::atomic<int64_t> launches{0};
+
+// Gradients are the kernels' own results: they carry no graph.
+void once(const char* name) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), name, " cannot be differentiated twice");
+}
+
+// A gradient that a kernel reads as a dense array, or nothing.
+OptTensor dense(const Tensor& g) { return g.defined() ? OptTensor(g.contiguous()) : std::nullopt; }
 
 bw::Elem elem_of(const Tensor& t, const char* name) {
   switch (t.scalar_type()) {
@@ -74,8 +91,8 @@ Tensor grad_like(const Tensor& logits) {
 }
 
 // The float workspace of a preference loss: [stats 2 R | d (B) | scale (B) | token log-probabilities R | pair losses P | ticket].
-std::vector<Tensor> preference_fwd(Tensor logits, Tensor labels, Tensor ref, int64_t kind, double beta,
-                                   double smoothing, bool average, int64_t reduction, int64_t ignore, Tensor err) {
+variable_list preference_fwd(const Tensor& logits, const Tensor& labels, const Tensor& ref, int64_t kind, double beta,
+                             double smoothing, bool average, int64_t reduction, int64_t ignore, const Tensor& err) {
   const c10::cuda::CUDAGuard guard(logits.device());
   bw::PreferenceArgs a;
   a.rows = logit_rows(logits, labels, ignore, 1.0, err);
@@ -108,8 +125,8 @@ std::vector<Tensor> preference_fwd(Tensor logits, Tensor labels, Tensor ref, int
   return {loss, logps, ws};
 }
 
-Tensor preference_bwd(Tensor logits, Tensor labels, Tensor ws, OptTensor g_loss, OptTensor g_logps, int64_t ignore,
-                      Tensor err) {
+Tensor preference_bwd(const Tensor& logits, const Tensor& labels, const Tensor& ws, const OptTensor& g_loss,
+                      const OptTensor& g_logps, int64_t ignore, const Tensor& err) {
   const c10::cuda::CUDAGuard guard(logits.device());
   bw::LogitGradArgs a;
   a.rows = logit_rows(logits, labels, ignore, 1.0, err);
@@ -142,9 +159,9 @@ Tensor preference_bwd(Tensor logits, Tensor labels, Tensor ws, OptTensor g_loss,
 }
 
 // The float workspace of a policy loss: [stats 2 R | d R | sums of sequences 8 B | token counts B | ticket].
-std::vector<Tensor> policy_fwd(Tensor logits, Tensor labels, Tensor adv, OptTensor old_logps, OptTensor ref_logps,
-                               double clip_lo, double clip_hi, double kl_coef, double temperature, int64_t mean,
-                               int64_t ignore, Tensor err) {
+variable_list policy_fwd(const Tensor& logits, const Tensor& labels, const Tensor& adv, const OptTensor& old_logps,
+                         const OptTensor& ref_logps, double clip_lo, double clip_hi, double kl_coef, double temperature,
+                         int64_t mean, int64_t ignore, const Tensor& err) {
   const c10::cuda::CUDAGuard guard(logits.device());
   bw::PolicyArgs a;
   a.rows = logit_rows(logits, labels, ignore, temperature, err);
@@ -186,8 +203,8 @@ std::vector<Tensor> policy_fwd(Tensor logits, Tensor labels, Tensor adv, OptTens
   return {loss, logps, kl, clipped, ws};
 }
 
-Tensor policy_bwd(Tensor logits, Tensor labels, Tensor ws, OptTensor g_loss, OptTensor g_logps, double temperature,
-                  int64_t ignore, Tensor err) {
+Tensor policy_bwd(const Tensor& logits, const Tensor& labels, const Tensor& ws, const OptTensor& g_loss,
+                  const OptTensor& g_logps, double temperature, int64_t ignore, const Tensor& err) {
   const c10::cuda::CUDAGuard guard(logits.device());
   bw::LogitGradArgs a;
   a.rows = logit_rows(logits, labels, ignore, temperature, err);
@@ -255,7 +272,8 @@ bw::BalanceArgs balance_args(const Tensor& logits, const OptTensor& ids, const O
   return a;
 }
 
-std::vector<Tensor> balance_fwd(Tensor logits, OptTensor ids, OptTensor mask, int64_t top_k, double z_coef, Tensor err) {
+variable_list balance_fwd(const Tensor& logits, const OptTensor& ids, const OptTensor& mask, int64_t top_k, double z_coef,
+                          const Tensor& err) {
   const c10::cuda::CUDAGuard guard(logits.device());
   bw::BalanceArgs a = balance_args(logits, ids, mask, top_k, z_coef, err);
   const auto f32 = logits.options().dtype(torch::kFloat32);
@@ -273,7 +291,8 @@ std::vector<Tensor> balance_fwd(Tensor logits, OptTensor ids, OptTensor mask, in
   return {loss, counts, share};
 }
 
-Tensor balance_bwd(Tensor logits, OptTensor mask, Tensor share, Tensor g_loss, int64_t top_k, double z_coef, Tensor err) {
+Tensor balance_bwd(const Tensor& logits, const OptTensor& mask, const Tensor& share, const Tensor& g_loss, int64_t top_k,
+                   double z_coef, const Tensor& err) {
   const c10::cuda::CUDAGuard guard(logits.device());
   bw::BalanceGradArgs b;
   b.f = balance_args(logits, std::nullopt, mask, top_k, z_coef, err);
@@ -341,8 +360,8 @@ bw::QkNormArgs qk_args(const Tensor& q, const Tensor& k, const Tensor& qw, const
   return a;
 }
 
-std::vector<Tensor> qk_norm_fwd(Tensor q, Tensor k, Tensor qw, Tensor kw, Tensor cos, Tensor sin, OptTensor positions,
-                                double eps, Tensor err) {
+variable_list qk_norm_fwd(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw, const Tensor& cos,
+                          const Tensor& sin, const OptTensor& positions, double eps, const Tensor& err) {
   const c10::cuda::CUDAGuard guard(q.device());
   bw::QkNormArgs a = qk_args(q, k, qw, kw, cos, sin, positions, eps, err);
   auto qo = torch::empty(q.sizes(), q.options()), ko = torch::empty(k.sizes(), k.options());
@@ -367,8 +386,9 @@ void head_grad(const OptTensor& g, const Tensor& x, const char* name, const void
   sh = g->stride(2);
 }
 
-std::vector<Tensor> qk_norm_bwd(OptTensor gq, OptTensor gk, Tensor q, Tensor k, Tensor qw, Tensor kw, Tensor cos,
-                                Tensor sin, OptTensor positions, double eps, Tensor err) {
+variable_list qk_norm_bwd(const OptTensor& gq, const OptTensor& gk, const Tensor& q, const Tensor& k, const Tensor& qw,
+                          const Tensor& kw, const Tensor& cos, const Tensor& sin, const OptTensor& positions, double eps,
+                          const Tensor& err) {
   const c10::cuda::CUDAGuard guard(q.device());
   bw::QkNormGradArgs b{};
   b.f = qk_args(q, k, qw, kw, cos, sin, positions, eps, err);
@@ -388,19 +408,138 @@ std::vector<Tensor> qk_norm_bwd(OptTensor gq, OptTensor gk, Tensor q, Tensor k, 
   return {dq, dk, dqw, dkw};
 }
 
+// ---------------------------------------------------------------- autograd
+
+struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& labels, const Tensor& ref,
+                               int64_t kind, double beta, double smoothing, bool average, int64_t reduction,
+                               int64_t ignore, const Tensor& err) {
+    auto out = preference_fwd(logits, labels, ref, kind, beta, smoothing, average, reduction, ignore, err);
+    launches += 2;
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({logits, labels, out[2], err});
+    ctx->saved_data["ignore"] = ignore;
+    return {out[0], out[1]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    once("preference_loss");
+    variable_list out(10);
+    if (!g[0].defined() && !g[1].defined()) return out;
+    const auto s = ctx->get_saved_variables();
+    out[0] = preference_bwd(s[0], s[1], s[2], dense(g[0]), dense(g[1]), ctx->saved_data["ignore"].toInt(), s[3]);
+    ++launches;
+    return out;
+  }
+};
+
+struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& labels, const Tensor& adv,
+                               const OptTensor& old_logps, const OptTensor& ref_logps, double clip_lo, double clip_hi,
+                               double kl_coef, double temperature, int64_t mean, int64_t ignore, const Tensor& err) {
+    auto out = policy_fwd(logits, labels, adv, old_logps, ref_logps, clip_lo, clip_hi, kl_coef, temperature, mean,
+                          ignore, err);
+    launches += 3;
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({out[2], out[3]});
+    ctx->save_for_backward({logits, labels, out[4], err});
+    ctx->saved_data["ignore"] = ignore;
+    ctx->saved_data["temperature"] = temperature;
+    return {out[0], out[1], out[2], out[3]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    once("policy_loss");
+    variable_list out(12);
+    if (!g[0].defined() && !g[1].defined()) return out;
+    const auto s = ctx->get_saved_variables();
+    out[0] = policy_bwd(s[0], s[1], s[2], dense(g[0]), dense(g[1]), ctx->saved_data["temperature"].toDouble(),
+                        ctx->saved_data["ignore"].toInt(), s[3]);
+    ++launches;
+    return out;
+  }
+};
+
+struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const OptTensor& ids, const OptTensor& mask,
+                               int64_t top_k, double z_coef, const Tensor& err) {
+    auto out = balance_fwd(logits, ids, mask, top_k, z_coef, err);
+    launches += 2;
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({out[1]});
+    ctx->save_for_backward({logits, mask.value_or(Tensor()), out[2], err});
+    ctx->saved_data["top_k"] = top_k;
+    ctx->saved_data["z"] = z_coef;
+    return {out[0], out[1]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    once("router_balance_loss");
+    variable_list out(6);
+    if (!g[0].defined()) return out;
+    const auto s = ctx->get_saved_variables();
+    out[0] = balance_bwd(s[0], s[1].defined() ? OptTensor(s[1]) : std::nullopt, s[2], g[0],
+                         ctx->saved_data["top_k"].toInt(), ctx->saved_data["z"].toDouble(), s[3]);
+    ++launches;
+    return out;
+  }
+};
+
+struct QkNormRope : torch::autograd::Function<QkNormRope> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& qw,
+                               const Tensor& kw, const Tensor& cos, const Tensor& sin, const OptTensor& positions,
+                               double eps, const Tensor& err) {
+    auto out = qk_norm_fwd(q, k, qw, kw, cos, sin, positions, eps, err);
+    ++launches;
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({q, k, qw, kw, cos, sin, positions.value_or(Tensor()), err});
+    ctx->saved_data["eps"] = eps;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    once("qk_norm_rope");
+    variable_list out(9);
+    if (!g[0].defined() && !g[1].defined()) return out;
+    const auto s = ctx->get_saved_variables();
+    const auto row = [](const Tensor& t) {
+      return !t.defined() ? OptTensor() : OptTensor(t.stride(-1) == 1 ? t : t.contiguous());
+    };
+    auto d = qk_norm_bwd(row(g[0]), row(g[1]), s[0], s[1], s[2], s[3], s[4], s[5],
+                         s[6].defined() ? OptTensor(s[6]) : std::nullopt, ctx->saved_data["eps"].toDouble(), s[7]);
+    launches += 2;
+    std::copy(d.begin(), d.end(), out.begin());
+    return out;
+  }
+};
+
+variable_list preference_loss(Tensor logits, Tensor labels, Tensor ref, int64_t kind, double beta, double smoothing,
+                              bool average, int64_t reduction, int64_t ignore, Tensor err) {
+  return PreferenceLoss::apply(logits, labels, ref, kind, beta, smoothing, average, reduction, ignore, err);
+}
+
+variable_list policy_loss(Tensor logits, Tensor labels, Tensor adv, OptTensor old_logps, OptTensor ref_logps,
+                          double clip_lo, double clip_hi, double kl_coef, double temperature, int64_t mean,
+                          int64_t ignore, Tensor err) {
+  return PolicyLoss::apply(logits, labels, adv, old_logps, ref_logps, clip_lo, clip_hi, kl_coef, temperature, mean,
+                           ignore, err);
+}
+
+variable_list balance_loss(Tensor logits, OptTensor ids, OptTensor mask, int64_t top_k, double z_coef, Tensor err) {
+  return BalanceLoss::apply(logits, ids, mask, top_k, z_coef, err);
+}
+
+variable_list qk_norm_rope(Tensor q, Tensor k, Tensor qw, Tensor kw, Tensor cos, Tensor sin, OptTensor positions,
+                           double eps, Tensor err) {
+  return QkNormRope::apply(q, k, qw, kw, cos, sin, positions, eps, err);
+}
+
 }  // namespace
 
 namespace bw {
 
 void register_post_training(pybind11::module_& m) {
-  m.def("preference_fwd", &::preference_fwd, "preference loss of pairs of sequences from logits");
-  m.def("preference_bwd", &::preference_bwd);
-  m.def("policy_fwd", &::policy_fwd, "clipped policy loss with a KL term from logits");
-  m.def("policy_bwd", &::policy_bwd);
-  m.def("balance_fwd", &::balance_fwd, "router balance loss and per-expert counts");
-  m.def("balance_bwd", &::balance_bwd);
-  m.def("qk_norm_fwd", &::qk_norm_fwd, "RMS norm of q and k heads with rotation by position");
-  m.def("qk_norm_bwd", &::qk_norm_bwd);
+  m.def("preference_loss", &::preference_loss, "preference loss of pairs of sequences from logits");
+  m.def("policy_loss", &::policy_loss, "clipped policy loss with a KL term from logits");
+  m.def("balance_loss", &::balance_loss, "router balance loss and per-expert counts");
+  m.def("qk_norm_rope", &::qk_norm_rope, "RMS norm of q and k heads with rotation by position");
+  m.def("post_training_launches", [] { return launches.load(); }, "kernels that these functions launched");
 }
 
 }  // namespace bw

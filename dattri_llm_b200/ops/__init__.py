@@ -32,11 +32,12 @@ def count_launch(n: int = 1) -> None:
 
 def launch_count() -> int:
     """Native kernels launched by this process so far."""
-    return _LAUNCHES[0]
+    return _LAUNCHES[0] + (_C.post_training_launches() if _C is not None else 0)
 
 
 _lock = threading.Lock()
 _err_words: dict[int, torch.Tensor] = {}
+_sm100: dict[int, bool] = {}  # by device index: asking the driver costs 2 us a call
 _checked = None
 
 
@@ -91,9 +92,11 @@ def use_native(*tensors: torch.Tensor) -> bool:
     """
     if not tensors or not all(t.is_cuda for t in tensors):
         return False
-    dev = tensors[0].device
-    major, _ = torch.cuda.get_device_capability(dev)
-    if major != 10:
+    idx = tensors[0].device.index
+    sm100 = _sm100.get(idx)
+    if sm100 is None:
+        sm100 = _sm100[idx] = torch.cuda.get_device_capability(idx)[0] == 10
+    if not sm100:
         return False
     native()
     return True

@@ -339,33 +339,6 @@ def causal_conv_silu(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor |
     return _CausalConvSiLU.apply(x, weight, bias)
 
 
-class _QkNormRope(torch.autograd.Function):
-    """RMS norm of each q / k head and rotation by position (``csrc/qk_norm.cu``)."""
-
-    @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps):
-        from dattri_llm_b200.ops import count_launch, error_word, native
-
-        count_launch()
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
-        ctx.eps = eps
-        return tuple(native().qk_norm_fwd(q, k, q_weight, k_weight, cos, sin, positions, eps, error_word(q.device)))
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gq, gk):
-        from dattri_llm_b200.ops import count_launch, error_word, native
-
-        if gq is None and gk is None:
-            return (None,) * 8
-        q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
-        gq, gk = (g if g is None or g.stride(-1) == 1 else g.contiguous() for g in (gq, gk))
-        count_launch(2)
-        grads = native().qk_norm_bwd(gq, gk, q, k, q_weight, k_weight, cos, sin, positions, ctx.eps, error_word(q.device))
-        return (*grads, None, None, None, None)
-
-
 def _qk_norm_rope_torch(x, weight, cos, sin, eps):
     wide = torch.promote_types(x.dtype, torch.float32)
     half = cos.shape[-1]
@@ -379,7 +352,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
                  sin: torch.Tensor, positions: torch.Tensor | None = None, *,
                  eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
     """RMS norm of every query and key head, then the rotation of its first ``R`` elements by
-    position, in one pass: ``rotate(x * rsqrt(mean(x^2) + eps) * weight)``, rounded once.
+    position, in one pass (``csrc/qk_norm.cu``): ``rotate(x * rsqrt(mean(x^2) + eps) * weight)``, rounded once.
 
     Args:
         q, k: ``(B, T, Hq, D)`` and ``(B, T, Hk, D)`` of one type (bf16, fp16 or fp32 on the
@@ -412,7 +385,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
         positions = positions.long().expand(b, t)
     elif cos.shape[0] < t:
         raise ValueError(f"the tables hold {cos.shape[0]} positions, the sequence has {t}")
-    from dattri_llm_b200.ops import use_native
+    from dattri_llm_b200.ops import error_word, native, use_native
 
     if not use_native(q):
         if positions is not None and bool(((positions < 0) | (positions >= cos.shape[0])).any()):
@@ -422,4 +395,5 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
         return (_qk_norm_rope_torch(q, q_weight, cos, sin, eps), _qk_norm_rope_torch(k, k_weight, cos, sin, eps))
     q, k = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k))
     cos, sin = (x.to(torch.float32).contiguous() for x in (cos, sin))
-    return _QkNormRope.apply(q, k, q_weight.contiguous(), k_weight.contiguous(), cos, sin, positions, float(eps))
+    return tuple(native().qk_norm_rope(q, k, q_weight.contiguous(), k_weight.contiguous(), cos, sin, positions, eps,
+                                       error_word(q.device)))

@@ -21,7 +21,6 @@ from typing import NamedTuple
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 PAIR_LOSSES = {"sigmoid": 0, "hinge": 1, "ipo": 2}
 _PAIR_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
@@ -53,12 +52,6 @@ class BalanceLoss(NamedTuple):
 
     loss: torch.Tensor
     counts: torch.Tensor
-
-
-def _native(x: torch.Tensor) -> bool:
-    from dattri_llm_b200.ops import use_native
-
-    return use_native(x)
 
 
 def _constant(name: str, x: torch.Tensor | None) -> torch.Tensor | None:
@@ -97,34 +90,6 @@ def _token_logps(logits: torch.Tensor, labels: torch.Tensor, ignore: int) -> tup
 
 
 # ---------------------------------------------------------------- preference
-
-
-class _PreferenceLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, labels, ref, kind, beta, smoothing, average, reduction, ignore):
-        from dattri_llm_b200.ops import count_launch, error_word, native
-
-        err = error_word(logits.device)
-        count_launch(2)
-        loss, logps, ws = native().preference_fwd(logits, labels, ref, kind, beta, smoothing, average, reduction, ignore,
-                                                  err)
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(logits, labels, ws)
-        ctx.ignore = ignore
-        return loss, logps
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_loss, g_logps):
-        from dattri_llm_b200.ops import count_launch, error_word, native
-
-        if g_loss is None and g_logps is None:
-            return (None,) * 9
-        logits, labels, ws = ctx.saved_tensors
-        g_loss, g_logps = (None if g is None else g.contiguous() for g in (g_loss, g_logps))
-        count_launch()
-        return (native().preference_bwd(logits, labels, ws, g_loss, g_logps, ctx.ignore, error_word(logits.device)),
-                *(None,) * 8)
 
 
 def _preference_torch(logits, labels, ref, kind, beta, smoothing, average, reduction, ignore) -> PreferenceLoss:
@@ -170,6 +135,8 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
         :class:`PreferenceLoss`.  A label outside the vocabulary is left out and reported by
         :func:`~dattri_llm_b200.ops.check_device_errors` (raised at once on CPU).
     """
+    from dattri_llm_b200.ops import error_word, native, use_native
+
     logits, labels = _check_logits(logits, labels)
     b = logits.shape[0]
     if b < 2 or b % 2:
@@ -184,44 +151,15 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
         raise ValueError(f"label_smoothing must be in [0, 0.5), and 0 unless kind is 'sigmoid', got {label_smoothing}")
     if ref_logps.shape != (b,):
         raise ValueError(f"ref_logps must be ({b},), got {tuple(ref_logps.shape)}")
-    if not _native(logits):
+    if not use_native(logits):
         ref = _constant("ref_logps", ref_logps).to(torch.promote_types(logits.dtype, torch.float32))
         return _preference_torch(logits, labels, ref, kind, beta, label_smoothing, average_logps, reduction, ignore_index)
-    return PreferenceLoss(*_PreferenceLoss.apply(
+    return PreferenceLoss(*native().preference_loss(
         logits, labels, _constant("ref_logps", ref_logps), PAIR_LOSSES[kind], beta, label_smoothing, average_logps,
-        _PAIR_REDUCTIONS[reduction], ignore_index))
+        _PAIR_REDUCTIONS[reduction], ignore_index, error_word(logits.device)))
 
 
 # ---------------------------------------------------------------- policy
-
-
-class _PolicyLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, labels, adv, old, ref, lo, hi, kl_coef, temperature, reduction, ignore):
-        from dattri_llm_b200.ops import count_launch, error_word, native
-
-        err = error_word(logits.device)
-        count_launch(3)
-        loss, logps, kl, clipped, ws = native().policy_fwd(logits, labels, adv, old, ref, lo, hi, kl_coef, temperature,
-                                                           reduction, ignore, err)
-        ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(kl, clipped)
-        ctx.save_for_backward(logits, labels, ws)
-        ctx.temperature, ctx.ignore = temperature, ignore
-        return loss, logps, kl, clipped
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_loss, g_logps, _kl, _clipped):
-        from dattri_llm_b200.ops import count_launch, error_word, native
-
-        if g_loss is None and g_logps is None:
-            return (None,) * 11
-        logits, labels, ws = ctx.saved_tensors
-        g_loss, g_logps = (None if g is None else g.contiguous() for g in (g_loss, g_logps))
-        count_launch()
-        return (native().policy_bwd(logits, labels, ws, g_loss, g_logps, ctx.temperature, ctx.ignore,
-                                    error_word(logits.device)), *(None,) * 10)
 
 
 def _policy_torch(logits, labels, adv, old, ref, lo, hi, kl_coef, temperature, reduction, ignore) -> PolicyLoss:
@@ -274,6 +212,8 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, advantages: torch.Te
         :class:`PolicyLoss`.  A label outside the vocabulary is left out and reported by
         :func:`~dattri_llm_b200.ops.check_device_errors` (raised at once on CPU).
     """
+    from dattri_llm_b200.ops import error_word, native, use_native
+
     logits, labels = _check_logits(logits, labels)
     b, t = labels.shape
     if b == 0:
@@ -294,41 +234,15 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, advantages: torch.Te
     lo, hi = 1.0 - clip[0], 1.0 + clip[1]
     consts = tuple(_constant(n, x) for n, x in (("advantages", advantages), ("old_logps", old_logps),
                                                  ("ref_logps", ref_logps)))
-    if not _native(logits):
+    if not use_native(logits):
         wide = torch.promote_types(logits.dtype, torch.float32)
         consts = tuple(None if x is None else x.to(wide) for x in consts)
         return _policy_torch(logits, labels, *consts, lo, hi, kl_coef, temperature, reduction, ignore_index)
-    return PolicyLoss(*_PolicyLoss.apply(logits, labels, *consts, lo, hi, kl_coef, temperature,
-                                         _TOKEN_REDUCTIONS[reduction], ignore_index))
+    return PolicyLoss(*native().policy_loss(logits, labels, *consts, lo, hi, kl_coef, temperature,
+                                            _TOKEN_REDUCTIONS[reduction], ignore_index, error_word(logits.device)))
 
 
 # ---------------------------------------------------------------- router balance
-
-
-class _BalanceLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, ids, mask, top_k, z_coef):
-        from dattri_llm_b200.ops import count_launch, error_word, native
-
-        count_launch(2)
-        loss, counts, share = native().balance_fwd(logits, ids, mask, top_k, z_coef, error_word(logits.device))
-        ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(counts)
-        ctx.save_for_backward(logits, mask, share)
-        ctx.top_k, ctx.z_coef = top_k, z_coef
-        return loss, counts
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_loss, _counts):
-        from dattri_llm_b200.ops import count_launch, error_word, native
-
-        if g_loss is None:
-            return (None,) * 5
-        logits, mask, share = ctx.saved_tensors
-        count_launch()
-        return (native().balance_bwd(logits, mask, share, g_loss, ctx.top_k, ctx.z_coef, error_word(logits.device)),
-                None, None, None, None)
 
 
 def _balance_torch(logits, ids, mask, top_k, z_coef) -> BalanceLoss:
@@ -373,6 +287,8 @@ def router_balance_loss(logits: torch.Tensor, top_k: int, expert_ids: torch.Tens
         :class:`BalanceLoss`.  An expert id outside ``[0, E)`` is left out and reported by
         :func:`~dattri_llm_b200.ops.check_device_errors` (raised at once on CPU).
     """
+    from dattri_llm_b200.ops import error_word, native, use_native
+
     if logits.dim() < 2 or not logits.is_floating_point():
         raise ValueError(f"router logits must be floating (..., N, E), got {logits.dtype} {tuple(logits.shape)}")
     lead, (n, e) = logits.shape[:-2], logits.shape[-2:]
@@ -390,8 +306,8 @@ def router_balance_loss(logits: torch.Tensor, top_k: int, expert_ids: torch.Tens
     x = logits if len(lead) == 1 else logits.reshape(-1, n, e) if lead else logits.unsqueeze(0)
     if x.stride(2) != 1:
         x = x.contiguous()
-    if _native(x):
-        loss, counts = _BalanceLoss.apply(x, expert_ids, mask, int(top_k), float(z_coef))
+    if use_native(x):
+        loss, counts = native().balance_loss(x, expert_ids, mask, top_k, z_coef, error_word(x.device))
     else:
         loss, counts = _balance_torch(x, None if expert_ids is None else expert_ids.view(-1, n, top_k),
                                       None if mask is None else mask.view(-1, n), top_k, z_coef)
