@@ -42,54 +42,62 @@ struct ElemOf<float> {
 template <typename T>
 constexpr int kVecOf = 16 / (int)sizeof(T);
 
-__device__ __forceinline__ void unpack(const uint4& r, float (&f)[8], __nv_bfloat16) {
-  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+// Two elements of a 32-bit word (one for fp32), converted together: single conversions run at a fraction of the rate.
+__device__ __forceinline__ void word_up(uint32_t w, float* f, __nv_bfloat16) {
+  f[0] = __uint_as_float(w << 16);
+  f[1] = __uint_as_float(w & 0xffff0000u);
+}
+__device__ __forceinline__ void word_up(uint32_t w, float* f, __half) {
+  const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  f[0] = p.x;
+  f[1] = p.y;
+}
+__device__ __forceinline__ void word_up(uint32_t w, float* f, float) { f[0] = __uint_as_float(w); }
+
+__device__ __forceinline__ uint32_t word_down(const float* f, __nv_bfloat16) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(f[0], f[1]);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+__device__ __forceinline__ uint32_t word_down(const float* f, __half) {
+  const __half2 p = __floats2half2_rn(f[0], f[1]);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+__device__ __forceinline__ uint32_t word_down(const float* f, float) { return __float_as_uint(f[0]); }
+
+// An access of 4, 8 or 16 bytes as words, and its elements in fp32.
+__device__ __forceinline__ void words_of(const uint4& r, uint32_t* w) {
+  w[0] = r.x;
+  w[1] = r.y;
+  w[2] = r.z;
+  w[3] = r.w;
+}
+__device__ __forceinline__ void words_of(const uint2& r, uint32_t* w) {
+  w[0] = r.x;
+  w[1] = r.y;
+}
+__device__ __forceinline__ void words_of(const uint32_t& r, uint32_t* w) { w[0] = r; }
+__device__ __forceinline__ void of_words(uint4& r, const uint32_t* w) { r = make_uint4(w[0], w[1], w[2], w[3]); }
+__device__ __forceinline__ void of_words(uint2& r, const uint32_t* w) { r = make_uint2(w[0], w[1]); }
+__device__ __forceinline__ void of_words(uint32_t& r, const uint32_t* w) { r = w[0]; }
+
+template <typename T, typename Raw>
+__device__ __forceinline__ void raw_up(const Raw& r, float* f) {
+  constexpr int kWords = sizeof(Raw) / 4, kPer = 4 / sizeof(T);
+  uint32_t w[kWords];
+  words_of(r, w);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = __uint_as_float(w[i] << 16);
-    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
+  for (int i = 0; i < kWords; ++i) word_up(w[i], f + i * kPer, T());
 }
 
-__device__ __forceinline__ void unpack(const uint4& r, float (&f)[8], __half) {
-  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+template <typename T, typename Raw>
+__device__ __forceinline__ Raw raw_down(const float* f) {
+  constexpr int kWords = sizeof(Raw) / 4, kPer = 4 / sizeof(T);
+  uint32_t w[kWords];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    f[2 * i] = p.x;
-    f[2 * i + 1] = p.y;
-  }
-}
-
-__device__ __forceinline__ void unpack(const uint4& r, float (&f)[4], float) {
-  f[0] = __uint_as_float(r.x);
-  f[1] = __uint_as_float(r.y);
-  f[2] = __uint_as_float(r.z);
-  f[3] = __uint_as_float(r.w);
-}
-
-__device__ __forceinline__ uint4 pack(const float (&f)[8], __nv_bfloat16) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __nv_bfloat162 p = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-    w[i] = *reinterpret_cast<const uint32_t*>(&p);
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-__device__ __forceinline__ uint4 pack(const float (&f)[8], __half) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __half2 p = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-    w[i] = *reinterpret_cast<const uint32_t*>(&p);
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-__device__ __forceinline__ uint4 pack(const float (&f)[4], float) {
-  return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  for (int i = 0; i < kWords; ++i) w[i] = word_down(f + i * kPer, T());
+  Raw r;
+  of_words(r, w);
+  return r;
 }
 
 template <typename V>

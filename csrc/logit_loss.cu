@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kThreads) row_stats_kernel(LogitRows r, float*
   float m = -INFINITY, base = 0.f, s = 0.f;
   for (int j = threadIdx.x; j < span.nv; j += kThreads) {
     float f[N];
-    unpack(span.load(j), f, T());
+    raw_up<T>(span.load(j), f);
     float top = f[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) top = fmaxf(top, f[i]);
@@ -183,14 +183,14 @@ __global__ void __launch_bounds__(kThreads) logit_grad_kernel(LogitGradArgs a) {
   const float c = kLog2e * r.inv_temp, k = -coef * st.inv_s;
   for (int j = threadIdx.x; j < span.nv; j += kThreads) {
     float f[N];
-    unpack(span.load(j), f, T());
+    raw_up<T>(span.load(j), f);
     const int lo = j * N - span.shift;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       f[i] = ex2((f[i] - st.m) * c) * k;
       if (lo + i == y) f[i] += coef;
     }
-    store_vec<T>(out, r.V, lo, pack(f, T()), aligned);
+    store_vec<T>(out, r.V, lo, raw_down<T, uint4>(f), aligned);
   }
 }
 

@@ -400,7 +400,7 @@ variable_list qk_norm_bwd(const OptTensor& gq, const OptTensor& gk, const Tensor
   b.f.k.out = dk.data_ptr();
   b.dqw = dqw.data_ptr();
   b.dkw = dkw.data_ptr();
-  bw::qk_norm_blocks(b.f, &b.q_blocks, &b.k_blocks);
+  bw::qk_norm_blocks(b, &b.q_blocks, &b.k_blocks);
   auto part = torch::empty({(int64_t)(b.q_blocks + b.k_blocks) * b.f.D}, q.options().dtype(torch::kFloat32));
   b.part = part.data_ptr<float>();
   bw::qk_norm_bwd(b, at::cuda::getCurrentCUDAStream());

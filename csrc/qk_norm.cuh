@@ -43,6 +43,6 @@ struct QkNormGradArgs {
 void qk_norm_fwd(const QkNormArgs& a, cudaStream_t s);
 void qk_norm_bwd(const QkNormGradArgs& a, cudaStream_t s);
 // CTAs that the backward wants for q and for k.
-void qk_norm_blocks(const QkNormArgs& a, int* q_blocks, int* k_blocks);
+void qk_norm_blocks(const QkNormGradArgs& g, int* q_blocks, int* k_blocks);
 
 }  // namespace bw
