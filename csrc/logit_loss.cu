@@ -13,6 +13,10 @@
 #include "logit_loss.cuh"
 
 #include <cmath>
+#include <cstring>
+#include <cstring>
+
+#include "tc_common.cuh"
 
 namespace bw {
 namespace {
@@ -38,17 +42,32 @@ struct RowSpan {
     shift = (int)((reinterpret_cast<uintptr_t>(p) % 16) / sizeof(T));
     nv = (V + shift + N - 1) / N;
   }
-  // Vector j; elements outside the row are -inf.
+  __device__ __forceinline__ int first(int j) const { return j * N - shift; }
+  // Vector j; elements outside the row are -inf. kLast: nothing reads it again soon.
+  template <bool kLast>
   __device__ __forceinline__ uint4 load(int j) const {
-    const int lo = j * N - shift;
-    if (lo >= 0 && lo + N <= V) return __ldg(reinterpret_cast<const uint4*>(row + lo));
+    const int lo = first(j);
+    if (lo >= 0 && lo + N <= V) {
+      const uint4* p = reinterpret_cast<const uint4*>(row + lo);
+      return kLast ? __ldcs(p) : __ldcg(p);
+    }
     constexpr uint32_t kFill = sizeof(T) == 2 ? ElemOf<T>::kNegInf * 0x10001u : ElemOf<T>::kNegInf;
-    uint4 r = make_uint4(kFill, kFill, kFill, kFill);
-    T* e = reinterpret_cast<T*>(&r);
+    uint32_t w[4] = {kFill, kFill, kFill, kFill};
+    if (j < nv) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (lo + i >= 0 && lo + i < V) e[i] = row[lo + i];
-    return r;
+      for (int i = 0; i < N; ++i)
+        if (lo + i >= 0 && lo + i < V) put(w, i, row[lo + i]);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  static __device__ __forceinline__ void put(uint32_t* w, int i, T v) {
+    if constexpr (sizeof(T) == 2) {
+      uint16_t b;
+      memcpy(&b, &v, 2);
+      w[i / 2] = (w[i / 2] & (i & 1 ? 0xffffu : 0xffff0000u)) | (uint32_t)b << (i & 1 ? 16 : 0);
+    } else {
+      memcpy(&w[i], &v, 4);
+    }
   }
 };
 
@@ -59,44 +78,123 @@ __device__ __forceinline__ void store_vec(T* row, int V, int lo, const uint4& v,
     __stcs(reinterpret_cast<uint4*>(row + lo), v);
     return;
   }
-  const T* e = reinterpret_cast<const T*>(&v);
+  float f[N];
+  raw_up<T>(v, f);  // exact: the values came from T
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    if (lo + i >= 0 && lo + i < V) row[lo + i] = e[i];
+    if (lo + i >= 0 && lo + i < V) row[lo + i] = ElemOf<T>::down(f[i]);
 }
 
 // What the terms of a part with maximum m are taken off: 0 where all of it is -inf, so that its terms are 0.
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
 
-template <int kThreads>
-__device__ __forceinline__ void block_max_sum(float& m, float& s, float c, float* red) {
+// The larger of each element of two words; a NaN is passed over here and found again in the sum.
+__device__ __forceinline__ uint32_t word_max(uint32_t a, uint32_t b, __nv_bfloat16) {
+  const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t word_max(uint32_t a, uint32_t b, __half) {
+  const __half2 m = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t word_max(uint32_t a, uint32_t b, float) {
+  return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+}
+
+template <typename T, int K>
+__device__ __forceinline__ float max_of(const uint4 (&r)[K]) {
+  uint32_t m = word_max(word_max(r[0].x, r[0].y, T()), word_max(r[0].z, r[0].w, T()), T());
+#pragma unroll
+  for (int k = 1; k < K; ++k)
+    m = word_max(m, word_max(word_max(r[k].x, r[k].y, T()), word_max(r[k].z, r[k].w, T()), T()), T());
+  float f[4 / sizeof(T)];
+  word_up(m, f, T());
+  return sizeof(T) == 2 ? fmaxf(f[0], f[4 / sizeof(T) - 1]) : f[0];
+}
+
+// 2^((x - base) c) of a vector's elements, by twos.
+template <typename T>
+__device__ __forceinline__ void powers(const uint4& r, float base, float c, float2 (&e)[kVecOf<T> / 2]) {
+  constexpr int N = kVecOf<T>;
+  float f[N];
+  raw_up<T>(r, f);
+  const float2 off = make_float2(-base, -base), cc = make_float2(c, c);
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    const float2 t = __fmul2_rn(__fadd2_rn(make_float2(f[2 * i], f[2 * i + 1]), off), cc);
+    e[i] = make_float2(ex2(t.x), ex2(t.y));
+  }
+}
+
+template <typename T, int K>
+__device__ __forceinline__ float sum_of(const uint4 (&r)[K], float base, float c) {
+  float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    float2 e[kVecOf<T> / 2];
+    powers<T>(r[k], base, c, e);
+#pragma unroll
+    for (int i = 0; i < kVecOf<T> / 2; ++i) s = __fadd2_rn(s, e[i]);
+  }
+  return s.x + s.y;
+}
+
+// coef (onehot(y) - softmax) of a vector whose first element is `lo`: k = -coef / s.
+template <typename T>
+__device__ __forceinline__ uint4 grad_of(const uint4& r, int lo, int y, float base, float c, float k, float coef) {
+  constexpr int N = kVecOf<T>;
+  float2 e[N / 2];
+  powers<T>(r, base, c, e);
+  float f[N];
+  const float2 kk = make_float2(k, k);
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    const float2 g = __fmul2_rn(e[i], kk);
+    f[2 * i] = g.x;
+    f[2 * i + 1] = g.y;
+  }
+  if ((unsigned)(y - lo) < (unsigned)N) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (lo + i == y) f[i] += coef;
+  }
+  return raw_down<T, uint4>(f);
+}
+
+// The maximum and the sum of a warp's parts (m, s), s counting 2^((x - m) c); in every lane.
+__device__ __forceinline__ void merge_warp(float& m, float& s, float c) {
   float M = m;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kW = kThreads / 32;
-  if (lane == 0) red[warp] = M;
-  __syncthreads();
-  M = red[0];
-#pragma unroll
-  for (int k = 1; k < kW; ++k) M = fmaxf(M, red[k]);
-  // A thread that saw only -inf has s = 0 (or NaN from a NaN logit): its factor only has to be finite.
-  s *= m == -INFINITY ? 1.f : ex2((m - M) * c);
-  s = lanes_sum(s);
-  if (lane == 0) red[32 + warp] = s;
-  __syncthreads();
-  s = red[32];
-#pragma unroll
-  for (int k = 1; k < kW; ++k) s += red[32 + k];
+  // A part that saw only -inf has s = 0 (or NaN from a NaN logit): its factor only has to be finite.
+  s = lanes_sum(s * (m == -INFINITY ? 1.f : ex2((m - M) * c)));
   m = M;
 }
+
+// The same over the threads of a row.
+template <int kGroup>
+__device__ __forceinline__ void merge_group(float& m, float& s, float c, float2* parts) {
+  constexpr int kW = kGroup / 32;
+  merge_warp(m, s, c);
+  if constexpr (kW > 1) {
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) parts[threadIdx.x >> 5] = make_float2(m, s);
+    __syncthreads();
+    const float2 p = lane < kW ? parts[lane] : make_float2(-INFINITY, 0.f);
+    m = p.x;
+    s = p.y;
+    merge_warp(m, s, c);
+  }
+}
+
+constexpr int kUnroll = 4;  // vectors of a thread in one step
 
 // The row's label, or -1 where the row does not count.
 __device__ __forceinline__ int row_label(const LogitRows& r, long long row) {
   const int64_t y = r.labels[row];
   if (y == r.ignore) return -1;
   if (y < 0 || y >= r.V) {
-    if (threadIdx.x == 0) *r.err = kErrArgument;
+    if ((threadIdx.x & 31) == 0) report_error(r.err, kErrBadArg);
     return -1;
   }
   return (int)y;
@@ -109,56 +207,134 @@ __device__ __forceinline__ const T* row_ptr(const LogitRows& r, long long row) {
 }
 
 // ---------------------------------------------------------------- row statistics
-// One CTA for each row, one pass with a running maximum and sum in every thread.
-template <typename T, int kThreads>
-__global__ void __launch_bounds__(kThreads) row_stats_kernel(LogitRows r, float* __restrict__ logps,
-                                                             RowStat* __restrict__ stats,
-                                                             unsigned* __restrict__ ticket) {
-  constexpr int N = kVecOf<T>;
-  __shared__ float red[64];
-  const long long row = blockIdx.x;
-  if (row == 0 && threadIdx.x == 0) *ticket = 0;
+// Rows go to groups of kGroup threads: whole CTAs, or the warps of a CTA of four (a short row leaves a wider group
+// waiting on its own barriers, and an SM takes 32 CTAs at most).
+template <int kGroup>
+struct Place {
+  static constexpr int kRows = kGroup == 32 ? 4 : 1, kThreads = kGroup * kRows;
+  static __device__ __forceinline__ int tid() { return kRows > 1 ? threadIdx.x & 31 : threadIdx.x; }
+  static __device__ __forceinline__ long long row() {
+    return kRows > 1 ? (long long)blockIdx.x * kRows + (threadIdx.x >> 5) : blockIdx.x;
+  }
+};
+
+// The maximum and the sum of a row, in every thread of its group: one pass with a running maximum and sum in each. Vectors
+// before `kept` (whole steps of the loop, or all) also stay in `keep`, where the thread that read them finds them again.
+// kAhead: a step's loads are issued before the step in front is used, for groups too few on an SM to hide them.
+template <typename T, int kGroup, bool kKeep, bool kAhead>
+__device__ __forceinline__ void row_stats(const RowSpan<T>& span, float c, float& m, float& s, float2* parts, uint4* keep,
+                                          int kept) {
+  constexpr int kHold = kGroup * kUnroll;
+  m = -INFINITY;
+  s = 0.f;
+  const int tid = Place<kGroup>::tid();
+  uint4 v[kUnroll], next[kUnroll];
+  auto fetch = [&](uint4 (&to)[kUnroll], int j) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) to[u] = span.template load<false>(j + u * kGroup);
+  };
+  if (kAhead) fetch(next, tid);
+  for (int j = tid; j < span.nv; j += kHold) {
+    if constexpr (kAhead) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) v[u] = next[u];
+      if (j + kHold < span.nv) fetch(next, j + kHold);
+    } else {
+      fetch(v, j);
+    }
+    if (kKeep && j < kept) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (j + u * kGroup < kept) keep[j + u * kGroup] = v[u];
+    }
+    const float top = max_of<T>(v);
+    if (top > m) {
+      s *= m == -INFINITY ? 1.f : ex2((m - top) * c);
+      m = top;
+    }
+    s += sum_of<T>(v, base_of(m), c);
+  }
+  merge_group<kGroup>(m, s, c, parts);
+}
+
+template <typename T, int kGroup>
+__global__ void __launch_bounds__(Place<kGroup>::kThreads) row_stats_kernel(LogitRows r, float* __restrict__ logps,
+                                                                            RowStat* __restrict__ stats,
+                                                                            unsigned* __restrict__ ticket) {
+  __shared__ float2 parts[32];
+  const long long row = Place<kGroup>::row();
+  const int tid = Place<kGroup>::tid();
+  if (row == 0 && tid == 0) *ticket = 0;
+  if (row >= (long long)r.B * r.T) return;
   const int y = row_label(r, row);
   if (y < 0) {
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
       logps[row] = 0.f;
       stats[row] = RowStat{0.f, 0.f};
     }
     return;
   }
   const T* x = row_ptr<T>(r, row);
-  const RowSpan<T> span(x, r.V);
   const float c = kLog2e * r.inv_temp;
-  float m = -INFINITY, base = 0.f, s = 0.f;
-  for (int j = threadIdx.x; j < span.nv; j += kThreads) {
-    float f[N];
-    raw_up<T>(span.load(j), f);
-    float top = f[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) top = fmaxf(top, f[i]);
-    if (top > m) {
-      s *= m == -INFINITY ? 1.f : ex2((m - top) * c);
-      m = base = top;
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) s += ex2((f[i] - base) * c);
-  }
-  block_max_sum<kThreads>(m, s, c, red);
-  if (threadIdx.x == 0) {
-    base = base_of(m);
+  float m, s;
+  row_stats<T, kGroup, false, false>(RowSpan<T>(x, r.V), c, m, s, parts, nullptr, 0);
+  if (tid == 0) {
+    const float base = base_of(m);
     logps[row] = kLn2 * ((ElemOf<T>::up(x[y]) - base) * c - log2f(s));
     stats[row] = RowStat{base, 1.f / s};
   }
 }
 
 // ---------------------------------------------------------------- gradient
-// One CTA for each row: coef (onehot - softmax) / temperature. A zero coefficient (an ignored row, a clipped token)
-// writes zeros without reading the row.
-template <typename T, int kThreads>
-__global__ void __launch_bounds__(kThreads) logit_grad_kernel(LogitGradArgs a) {
-  constexpr int N = kVecOf<T>;
+template <typename T, int kGroup>
+__device__ __forceinline__ void zero_row(T* out, int V) {
+  const RowSpan<T> span(out, V);
+  for (int j = Place<kGroup>::tid(); j < span.nv; j += kGroup) store_vec<T>(out, V, span.first(j), make_uint4(0, 0, 0, 0), true);
+}
+
+// coef (onehot - softmax) of a row, read for the last time: from `keep` what row_stats left there.
+template <typename T, int kGroup, bool kKeep, bool kAhead>
+__device__ __forceinline__ void row_grad(const RowSpan<T>& span, T* out, int y, float base, float inv_s, float c, float coef,
+                                         const uint4* keep, int kept) {
+  constexpr int kHold = kGroup * kUnroll;
+  const bool aligned = (int)((reinterpret_cast<uintptr_t>(out) % 16) / sizeof(T)) == span.shift;
+  const float k = -coef * inv_s;
+  const int tid = Place<kGroup>::tid();
+  uint4 v[kUnroll], next[kUnroll];
+  auto fetch = [&](uint4 (&to)[kUnroll], int j) {
+    if (kKeep && j < kept) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (j + u * kGroup < kept) to[u] = keep[j + u * kGroup];
+    } else {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) to[u] = span.template load<true>(j + u * kGroup);
+    }
+  };
+  if (kAhead) fetch(next, tid);
+  for (int j = tid; j < span.nv; j += kHold) {
+    if constexpr (kAhead) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) v[u] = next[u];
+      if (j + kHold < span.nv) fetch(next, j + kHold);
+    } else {
+      fetch(v, j);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int lo = span.first(j + u * kGroup);
+      if (lo < span.V) store_vec<T>(out, span.V, lo, grad_of<T>(v[u], lo, y, base, c, k, coef), aligned);
+    }
+  }
+}
+
+// coef (onehot - softmax) / temperature of every row. A zero coefficient (an ignored row, a clipped token)
+// writes zeros without reading the row. Rows run backwards: the last ones read before are the likeliest still in L2.
+template <typename T, int kGroup>
+__global__ void __launch_bounds__(Place<kGroup>::kThreads) logit_grad_kernel(LogitGradArgs a) {
   const LogitRows& r = a.rows;
-  const long long row = blockIdx.x;
+  const long long row = (long long)r.B * r.T - 1 - Place<kGroup>::row();
+  if (row < 0) return;
   const long long b = row / r.T, t = row - b * r.T;
   const int y = row_label(r, row);
   T* out = reinterpret_cast<T*>(a.out) + b * a.osb + t * a.ost;
@@ -171,27 +347,12 @@ __global__ void __launch_bounds__(kThreads) logit_grad_kernel(LogitGradArgs a) {
     coef *= r.inv_temp;
   }
   if (coef == 0.f) {
-    const RowSpan<T> span(out, r.V);
-    for (int j = threadIdx.x; j < span.nv; j += kThreads)
-      store_vec<T>(out, r.V, j * N - span.shift, make_uint4(0, 0, 0, 0), true);
+    zero_row<T, kGroup>(out, r.V);
     return;
   }
-  const T* x = row_ptr<T>(r, row);
-  const RowSpan<T> span(x, r.V);
-  const bool aligned = (int)((reinterpret_cast<uintptr_t>(out) % 16) / sizeof(T)) == span.shift;
   const RowStat st = a.stats[row];
-  const float c = kLog2e * r.inv_temp, k = -coef * st.inv_s;
-  for (int j = threadIdx.x; j < span.nv; j += kThreads) {
-    float f[N];
-    raw_up<T>(span.load(j), f);
-    const int lo = j * N - span.shift;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      f[i] = ex2((f[i] - st.m) * c) * k;
-      if (lo + i == y) f[i] += coef;
-    }
-    store_vec<T>(out, r.V, lo, raw_down<T, uint4>(f), aligned);
-  }
+  row_grad<T, kGroup, false, false>(RowSpan<T>(row_ptr<T>(r, row), r.V), out, y, st.m, st.inv_s, kLog2e * r.inv_temp, coef,
+                                    nullptr, 0);
 }
 
 // ---------------------------------------------------------------- sums over tokens
@@ -282,9 +443,19 @@ struct TokenTerms {
   float loss, kl, clipped, slope;  // slope: d loss / d logp
 };
 
-__device__ __forceinline__ TokenTerms policy_token(const PolicyArgs& a, long long row, long long b, float logp) {
-  const float adv = a.adv[a.adv_per_token ? row : b];
-  const float r = a.old_logps != nullptr ? expf(logp - a.old_logps[row]) : (logp != logp ? logp : 1.f);
+// What a token brings along, read before it is needed.
+struct TokenIn {
+  float adv, old_logp, ref_logp;
+};
+
+__device__ __forceinline__ TokenIn token_in(const PolicyArgs& a, long long row, long long b) {
+  return TokenIn{a.adv[a.adv_per_token ? row : b], a.old_logps != nullptr ? a.old_logps[row] : 0.f,
+                 a.ref_logps != nullptr ? a.ref_logps[row] : 0.f};
+}
+
+__device__ __forceinline__ TokenTerms policy_token(const PolicyArgs& a, const TokenIn& in, float logp) {
+  const float adv = in.adv;
+  const float r = a.old_logps != nullptr ? expf(logp - in.old_logp) : (logp != logp ? logp : 1.f);
   const float held_r = r < a.clip_lo ? a.clip_lo : (r > a.clip_hi ? a.clip_hi : r);
   const float free = r * adv, held = held_r * adv;
   TokenTerms t;
@@ -293,7 +464,7 @@ __device__ __forceinline__ TokenTerms policy_token(const PolicyArgs& a, long lon
   t.clipped = held < free ? 1.f : 0.f;
   t.kl = 0.f;
   if (a.ref_logps != nullptr) {
-    const float d = a.ref_logps[row] - logp;
+    const float d = in.ref_logp - logp;
     t.kl = exp_excess(d);
     t.loss += a.kl_coef * t.kl;
     t.slope -= a.kl_coef * expm1f(d);
@@ -317,72 +488,177 @@ __global__ void __launch_bounds__(256) policy_count_kernel(PolicyArgs a) {
   }
 }
 
-// One CTA for each sequence: its tokens' terms, sums and derivatives; the last CTA adds the sequences in order.
+// A token's share in the loss, from the tokens that count; the same in every lane of a warp.
+__device__ __forceinline__ float token_weight(const PolicyArgs& a, long long b) {
+  if (a.mean == TokenMean::kSum) return 1.f;
+  if (a.mean == TokenMean::kSequences) return 1.f / ((float)max(a.count[b], 1) * a.rows.B);
+  int n = 0;
+  for (int k = threadIdx.x & 31; k < a.rows.B; k += 32) n += a.count[k];
+  n = lanes_sum(n);
+  return 1.f / max(n, 1);
+}
+
+// The terms of every token, for calls that take no gradient along.
+__global__ void __launch_bounds__(256) policy_token_kernel(PolicyArgs a) {
+  const long long b = blockIdx.x, base = b * a.rows.T;
+  const float w = token_weight(a, b);
+  for (int t = threadIdx.x; t < a.rows.T; t += blockDim.x) {
+    const long long row = base + t;
+    const int64_t y = a.rows.labels[row];
+    TokenTerms k{0.f, 0.f, 0.f, 0.f};
+    if (y != a.rows.ignore && y >= 0 && y < a.rows.V) k = policy_token(a, token_in(a, row, b), a.logps[row]);
+    a.dtok[row] = k.slope * w;
+    a.tok[row] = make_float4(k.loss * w, k.kl, k.clipped, 0.f);
+  }
+}
+
+// One CTA for each sequence: its tokens' sums; the last CTA adds the sequences in order.
 __global__ void __launch_bounds__(256) policy_finish_kernel(PolicyArgs a) {
   __shared__ double red[8];
   const int B = gridDim.x, b = blockIdx.x, T = a.rows.T;
-  double total = 0;
-  for (int k = threadIdx.x; k < B; k += blockDim.x) total += a.count[k];
-  total = block_sum(total, red);
-  const double mine = a.count[b];
-  const double w = a.mean == TokenMean::kTokens      ? 1 / fmax(total, 1.0)
-                   : a.mean == TokenMean::kSequences ? 1 / (fmax(mine, 1.0) * B)
-                                                     : 1.0;
   const long long base = (long long)b * T;
   double v[3] = {0, 0, 0};
   for (int t = threadIdx.x; t < T; t += blockDim.x) {
-    const long long row = base + t;
-    const int64_t y = a.rows.labels[row];
-    if (y == a.rows.ignore || y < 0 || y >= a.rows.V) {
-      a.dtok[row] = 0.f;
-      continue;
-    }
-    const TokenTerms k = policy_token(a, row, b, a.logps[row]);
-    a.dtok[row] = (float)(k.slope * w);
-    v[0] += k.loss;
-    v[1] += k.kl;
-    v[2] += k.clipped;
+    const float4 k = a.tok[base + t];
+    v[0] += k.x;
+    v[1] += k.y;
+    v[2] += k.z;
   }
 #pragma unroll
   for (int i = 0; i < 3; ++i) {
     v[i] = block_sum(v[i], red);
-    if (threadIdx.x == 0) a.seq[4 * b + i] = i == 0 ? v[i] * w : v[i];
+    if (threadIdx.x == 0) a.seq[4 * b + i] = v[i];
   }
   if (!last_block(a.ticket)) return;
+  double n = 0;
+  for (int k = threadIdx.x; k < B; k += blockDim.x) n += a.count[k];
+  n = fmax(block_sum(n, red), 1.0);
 #pragma unroll
   for (int i = 0; i < 3; ++i) {
     double u = 0;
     for (int k = threadIdx.x; k < B; k += blockDim.x) u += __ldcg(a.seq + 4 * k + i);
     u = block_sum(u, red);
-    if (threadIdx.x == 0) (i == 0 ? a.loss : i == 1 ? a.kl : a.clipped)[0] = (float)(i == 0 ? u : u / fmax(total, 1.0));
+    if (threadIdx.x == 0) (i == 0 ? a.loss : i == 1 ? a.kl : a.clipped)[0] = (float)(i == 0 ? u : u / n);
   }
+}
+
+// ---------------------------------------------------------------- loss and gradient in one kernel
+// A token's coefficient needs its own row only, so the group that took a row's statistics writes its gradient at once: the
+// row's first `kept` vectors wait in shared memory, the rest is read a second time from L2, where few enough rows are
+// between their two passes at any time.
+template <typename T, int kGroup, int kMin, bool kLong>
+__global__ void __launch_bounds__(Place<kGroup>::kThreads, kMin) policy_row_kernel(PolicyArgs a, int kept) {
+  extern __shared__ uint4 keep[];
+  __shared__ float2 parts[32];
+  const LogitRows& r = a.rows;
+  const long long row = Place<kGroup>::row();
+  if (row >= (long long)r.B * r.T) return;
+  const int tid = Place<kGroup>::tid();
+  const long long b = row / r.T, t = row - b * r.T;
+  const int y = row_label(r, row);
+  T* out = reinterpret_cast<T*>(a.grad) + b * a.gsb + t * a.gst;
+  if (y < 0) {
+    if (tid == 0) {
+      a.logps[row] = a.dtok[row] = 0.f;
+      a.stats[row] = RowStat{0.f, 0.f};
+      a.tok[row] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    zero_row<T, kGroup>(out, r.V);
+    return;
+  }
+  const T* x = row_ptr<T>(r, row);
+  const RowSpan<T> span(x, r.V);
+  const float c = kLog2e * r.inv_temp, xy = ElemOf<T>::up(x[y]), w = token_weight(a, b);
+  const TokenIn in = token_in(a, row, b);
+  float m, s;
+  row_stats<T, kGroup, kLong, kLong>(span, c, m, s, parts, keep, kept);
+  const float base = base_of(m), inv_s = 1.f / s, logp = kLn2 * ((xy - base) * c - log2f(s));
+  const TokenTerms k = policy_token(a, in, logp);  // the same in every thread
+  if (tid == 0) {
+    a.logps[row] = logp;
+    a.stats[row] = RowStat{base, inv_s};
+    a.dtok[row] = k.slope * w;
+    a.tok[row] = make_float4(k.loss * w, k.kl, k.clipped, 0.f);
+  }
+  const float coef = k.slope * w * r.inv_temp;
+  if (coef == 0.f)
+    zero_row<T, kGroup>(out, r.V);
+  else
+    row_grad<T, kGroup, kLong, kLong>(span, out, y, base, inv_s, c, coef, keep, kept);
+}
+
+// grad *= g unless g is 1, which is what a loss that ends the graph sends.
+template <typename T>
+__global__ void __launch_bounds__(512) logit_scale_kernel(LogitRows r, T* grad, long long sb, long long st,
+                                                          const float* __restrict__ g) {
+  constexpr int N = kVecOf<T>;
+  const float by = *g;
+  if (by == 1.f) return;
+  const long long rows = (long long)r.B * r.T;
+  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+    const long long b = row / r.T;
+    T* out = grad + b * sb + (row - b * r.T) * st;
+    const RowSpan<T> span(out, r.V);
+    for (int j = threadIdx.x; j < span.nv; j += blockDim.x) {
+      float f[N];
+      raw_up<T>(span.template load<true>(j), f);
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] *= by;
+      store_vec<T>(out, r.V, span.first(j), raw_down<T, uint4>(f), true);
+    }
+  }
+}
+
+template <int kGroup>
+unsigned grid_of(const LogitRows& r) {
+  return (unsigned)(((long long)r.B * r.T + Place<kGroup>::kRows - 1) / Place<kGroup>::kRows);
+}
+
+// The threads of a row by its vectors of 16 bytes; times of bf16 rows on one B200 (a quarter of them ignored):
+// 65536 rows of 1024 and 32768 of 4000 logits, 16384 of 16000, 8192 of 128256.
+constexpr int kShort = 768;
+
+template <typename T, int kGroup, int kMin, bool kLong>
+void policy_rows(const PolicyArgs& a, int bytes, cudaStream_t s) {
+  const int all = (a.rows.V + 2 * (kVecOf<T> - 1)) / kVecOf<T>, step = kGroup * kUnroll;
+  const int kept = bytes / 16 >= all ? all : bytes / 16 / step * step;
+  const auto kernel = policy_row_kernel<T, kGroup, kMin, kLong>;
+  if (kLong) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kept * 16);
+  kernel<<<grid_of<kGroup>(a.rows), Place<kGroup>::kThreads, kept * 16, s>>>(a, kept);
+}
+
+template <typename T>
+void rows_of(const PolicyArgs& a, cudaStream_t s) {
+  const int n = a.rows.V / kVecOf<T>;
+  if (n <= kShort) return policy_rows<T, 32, 8, false>(a, 0, s);
+  if (n <= 3072) return policy_rows<T, 128, 8, false>(a, 0, s);
+  if (n <= 6144) return policy_rows<T, 256, 4, false>(a, 0, s);
+  policy_rows<T, 512, 2, true>(a, 100 * 1024, s);
 }
 
 template <typename T>
 void launch_stats(const LogitRows& r, float* logps, RowStat* stats, unsigned* ticket, cudaStream_t s) {
-  const long long rows = (long long)r.B * r.T;
-  if (rows == 0) {
-    cudaMemsetAsync(ticket, 0, sizeof(unsigned), s);
-    return;
-  }
-  if (r.V > 8192)
-    row_stats_kernel<T, 512><<<(unsigned)rows, 512, 0, s>>>(r, logps, stats, ticket);
+  if (r.V / kVecOf<T> <= kShort)
+    row_stats_kernel<T, 32><<<grid_of<32>(r), Place<32>::kThreads, 0, s>>>(r, logps, stats, ticket);
   else
-    row_stats_kernel<T, 128><<<(unsigned)rows, 128, 0, s>>>(r, logps, stats, ticket);
+    row_stats_kernel<T, 128><<<grid_of<128>(r), 128, 0, s>>>(r, logps, stats, ticket);
 }
 
 template <typename T>
 void launch_grad(const LogitGradArgs& a, cudaStream_t s) {
-  const long long rows = (long long)a.rows.B * a.rows.T;
-  if (rows == 0) return;
-  if (a.rows.V > 8192)
-    logit_grad_kernel<T, 512><<<(unsigned)rows, 512, 0, s>>>(a);
+  const int n = a.rows.V / kVecOf<T>;
+  if (n <= kShort)
+    logit_grad_kernel<T, 32><<<grid_of<32>(a.rows), Place<32>::kThreads, 0, s>>>(a);
+  else if (n <= 8192)
+    logit_grad_kernel<T, 256><<<grid_of<256>(a.rows), 256, 0, s>>>(a);
   else
-    logit_grad_kernel<T, 128><<<(unsigned)rows, 128, 0, s>>>(a);
+    logit_grad_kernel<T, 512><<<grid_of<512>(a.rows), 512, 0, s>>>(a);
 }
 
 void stats_of(const LogitRows& r, float* logps, RowStat* stats, unsigned* ticket, cudaStream_t s) {
-  if (r.type == Elem::kBF16)
+  if ((long long)r.B * r.T == 0)
+    cudaMemsetAsync(ticket, 0, sizeof(unsigned), s);
+  else if (r.type == Elem::kBF16)
     launch_stats<__nv_bfloat16>(r, logps, stats, ticket, s);
   else if (r.type == Elem::kF16)
     launch_stats<__half>(r, logps, stats, ticket, s);
@@ -397,13 +673,36 @@ void preference_fwd(const PreferenceArgs& a, cudaStream_t s) {
   preference_finish_kernel<<<a.rows.B / 2, 256, 0, s>>>(a);
 }
 
-void policy_fwd(const PolicyArgs& a, cudaStream_t s) {
-  stats_of(a.rows, a.logps, a.stats, a.ticket, s);
+int policy_fwd(const PolicyArgs& a, cudaStream_t s) {
+  const bool rows = (long long)a.rows.B * a.rows.T > 0;
+  if (a.grad == nullptr || !rows) stats_of(a.rows, a.logps, a.stats, a.ticket, s);
   policy_count_kernel<<<a.rows.B, 256, 0, s>>>(a);
+  if (a.grad == nullptr || !rows)
+    policy_token_kernel<<<a.rows.B, 256, 0, s>>>(a);
+  else if (a.rows.type == Elem::kBF16)
+    rows_of<__nv_bfloat16>(a, s);
+  else if (a.rows.type == Elem::kF16)
+    rows_of<__half>(a, s);
+  else
+    rows_of<float>(a, s);
   policy_finish_kernel<<<a.rows.B, 256, 0, s>>>(a);
+  return a.grad == nullptr ? 4 : 3;
+}
+
+void logit_scale(const LogitRows& r, void* grad, long long sb, long long st, const float* g, cudaStream_t s) {
+  const long long rows = (long long)r.B * r.T;
+  if (rows == 0) return;
+  const unsigned grid = (unsigned)(rows < 148 * 4 ? rows : 148 * 4);
+  if (r.type == Elem::kBF16)
+    logit_scale_kernel<<<grid, 512, 0, s>>>(r, reinterpret_cast<__nv_bfloat16*>(grad), sb, st, g);
+  else if (r.type == Elem::kF16)
+    logit_scale_kernel<<<grid, 512, 0, s>>>(r, reinterpret_cast<__half*>(grad), sb, st, g);
+  else
+    logit_scale_kernel<<<grid, 512, 0, s>>>(r, reinterpret_cast<float*>(grad), sb, st, g);
 }
 
 void logit_grad(const LogitGradArgs& a, cudaStream_t s) {
+  if ((long long)a.rows.B * a.rows.T == 0) return;
   if (a.rows.type == Elem::kBF16)
     launch_grad<__nv_bfloat16>(a, s);
   else if (a.rows.type == Elem::kF16)

@@ -22,15 +22,13 @@ struct LogitRows {
   const int64_t* labels;
   int64_t ignore;
   float inv_temp;
-  int* err;  // set to kErrArgument where a label is outside [0, V) and not `ignore`
+  int* err;  // the device's error word, set where a label is outside [0, V) and not `ignore`
 };
 
 // What a row's softmax needs again: exp2((x - m) * c) * inv_s is a probability, c = log2(e) / temperature.
 struct RowStat {
   float m, inv_s;
 };
-
-constexpr int kErrArgument = 5;
 
 struct PreferenceArgs {
   LogitRows rows;
@@ -62,6 +60,8 @@ struct PolicyArgs {
   int* count;          // (B) tokens of each sequence that count
   unsigned* ticket;
   float *loss, *kl, *clipped;  // (1) each
+  void* grad;          // like the logits, or null: no gradient now
+  long long gsb, gst;
 };
 
 // d loss / d logits = coef (onehot - softmax) / temperature,
@@ -80,7 +80,10 @@ struct LogitGradArgs {
 };
 
 void preference_fwd(const PreferenceArgs& a, cudaStream_t s);
-void policy_fwd(const PolicyArgs& a, cudaStream_t s);
+// Returns the kernels launched.
+int policy_fwd(const PolicyArgs& a, cudaStream_t s);
+// grad *= *g, unless *g is 1; rows as in `rows`.
+void logit_scale(const LogitRows& rows, void* grad, long long sb, long long st, const float* g, cudaStream_t s);
 void logit_grad(const LogitGradArgs& a, cudaStream_t s);
 
 }  // namespace bw

@@ -158,10 +158,11 @@ Tensor preference_bwd(const Tensor& logits, const Tensor& labels, const Tensor& 
   return out;
 }
 
-// The float workspace of a policy loss: [stats 2 R | d R | sums of sequences 8 B | token counts B | ticket].
+// The float workspace of a policy loss: [stats 2 R | d R | (4 R of tokens) | sums of sequences 8 B | token counts B | ticket].
+// With want_grad the result's last tensor is the gradient for a loss gradient of 1.
 variable_list policy_fwd(const Tensor& logits, const Tensor& labels, const Tensor& adv, const OptTensor& old_logps,
                          const OptTensor& ref_logps, double clip_lo, double clip_hi, double kl_coef, double temperature,
-                         int64_t mean, int64_t ignore, const Tensor& err) {
+                         int64_t mean, int64_t ignore, const Tensor& err, bool want_grad) {
   const c10::cuda::CUDAGuard guard(logits.device());
   bw::PolicyArgs a;
   a.rows = logit_rows(logits, labels, ignore, temperature, err);
@@ -176,8 +177,8 @@ variable_list policy_fwd(const Tensor& logits, const Tensor& labels, const Tenso
     TORCH_CHECK(t->dim() == 2 && t->size(0) == B && t->size(1) == T, name, " must be (B, T)");
   }
   const auto f32 = logits.options().dtype(torch::kFloat32);
-  const int64_t even = R + (R & 1);
-  auto ws = torch::empty({2 * R + even + 8 * B + B + 1}, f32);
+  const int64_t even = (2 * R + R + 3) / 4 * 4;  // the tokens' float4 start on their boundary
+  auto ws = torch::empty({even + 4 * R + 8 * B + B + 1}, f32);
   auto logps = torch::empty({B, T}, f32);
   auto loss = torch::empty({}, f32), kl = torch::empty({}, f32), clipped = torch::empty({}, f32);
   float* w = ws.data_ptr<float>();
@@ -192,15 +193,24 @@ variable_list policy_fwd(const Tensor& logits, const Tensor& labels, const Tenso
   a.logps = logps.data_ptr<float>();
   a.stats = reinterpret_cast<bw::RowStat*>(w);
   a.dtok = w + 2 * R;
-  a.seq = reinterpret_cast<double*>(a.dtok + even);
+  a.tok = reinterpret_cast<float4*>(w + even);
+  a.seq = reinterpret_cast<double*>(a.tok + R);
   a.count = reinterpret_cast<int*>(a.seq + 4 * B);
   a.ticket = reinterpret_cast<unsigned*>(a.count + B);
   a.loss = loss.data_ptr<float>();
   a.kl = kl.data_ptr<float>();
   a.clipped = clipped.data_ptr<float>();
-  bw::policy_fwd(a, at::cuda::getCurrentCUDAStream());
+  Tensor grad;
+  a.grad = nullptr;
+  if (want_grad) {
+    grad = grad_like(logits);
+    a.grad = grad.data_ptr();
+    a.gsb = grad.stride(0);
+    a.gst = grad.stride(1);
+  }
+  launches += bw::policy_fwd(a, at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  return {loss, logps, kl, clipped, ws};
+  return {loss, logps, kl, clipped, ws, grad};
 }
 
 Tensor policy_bwd(const Tensor& logits, const Tensor& labels, const Tensor& ws, const OptTensor& g_loss,
@@ -435,22 +445,40 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
 struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& labels, const Tensor& adv,
                                const OptTensor& old_logps, const OptTensor& ref_logps, double clip_lo, double clip_hi,
-                               double kl_coef, double temperature, int64_t mean, int64_t ignore, const Tensor& err) {
+                               double kl_coef, double temperature, int64_t mean, int64_t ignore, const Tensor& err,
+                               bool want_grad) {
     auto out = policy_fwd(logits, labels, adv, old_logps, ref_logps, clip_lo, clip_hi, kl_coef, temperature, mean,
-                          ignore, err);
-    launches += 3;
+                          ignore, err, want_grad);
     ctx->set_materialize_grads(false);
     ctx->mark_non_differentiable({out[2], out[3]});
     ctx->save_for_backward({logits, labels, out[4], err});
     ctx->saved_data["ignore"] = ignore;
     ctx->saved_data["temperature"] = temperature;
+    if (out[5].defined()) ctx->saved_data["grad"] = out[5];
     return {out[0], out[1], out[2], out[3]};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     once("policy_loss");
-    variable_list out(12);
+    variable_list out(13);
     if (!g[0].defined() && !g[1].defined()) return out;
     const auto s = ctx->get_saved_variables();
+    // The gradient written by the forward is given away once; another backward through the graph computes it again.
+    const auto kept = ctx->saved_data.find("grad");
+    if (kept != ctx->saved_data.end()) {
+      Tensor grad = kept->second.toTensor();
+      ctx->saved_data.erase(kept);
+      if (!g[1].defined()) {
+        const c10::cuda::CUDAGuard guard(grad.device());
+        const auto by = *dense(g[0]);
+        check_like(by, "loss gradient", torch::kFloat32, grad);
+        bw::logit_scale(logit_rows(s[0], s[1], 0, 1.0, s[3]), grad.data_ptr(), grad.stride(0), grad.stride(1),
+                        by.data_ptr<float>(), at::cuda::getCurrentCUDAStream());
+        C10_CUDA_KERNEL_LAUNCH_CHECK();
+        ++launches;
+        out[0] = std::move(grad);
+        return out;
+      }
+    }
     out[0] = policy_bwd(s[0], s[1], s[2], dense(g[0]), dense(g[1]), ctx->saved_data["temperature"].toDouble(),
                         ctx->saved_data["ignore"].toInt(), s[3]);
     ++launches;
@@ -517,8 +545,9 @@ variable_list preference_loss(Tensor logits, Tensor labels, Tensor ref, int64_t 
 variable_list policy_loss(Tensor logits, Tensor labels, Tensor adv, OptTensor old_logps, OptTensor ref_logps,
                           double clip_lo, double clip_hi, double kl_coef, double temperature, int64_t mean,
                           int64_t ignore, Tensor err) {
+  const bool want_grad = logits.requires_grad() && at::GradMode::is_enabled();
   return PolicyLoss::apply(logits, labels, adv, old_logps, ref_logps, clip_lo, clip_hi, kl_coef, temperature, mean,
-                           ignore, err);
+                           ignore, err, want_grad);
 }
 
 variable_list balance_loss(Tensor logits, OptTensor ids, OptTensor mask, int64_t top_k, double z_coef, Tensor err) {

@@ -7,7 +7,7 @@
 // Arithmetic is fp32; the result is rounded once.
 #include "qk_norm.cuh"
 
-#include "logit_loss.cuh"
+#include "tc_common.cuh"
 
 namespace bw {
 namespace {
@@ -45,7 +45,7 @@ __device__ __forceinline__ void pair_at(int j, int half, int& lo, int& hi) {
 __device__ __forceinline__ int table_row(const QkNormArgs& a, int b, int t) {
   const int64_t p = a.positions != nullptr ? a.positions[b * a.pb + t * a.pt] : t;
   if (p >= 0 && p < a.table) return (int)p;
-  *a.err = kErrArgument;
+  report_error(a.err, kErrBadArg);
   return p < 0 ? 0 : a.table - 1;
 }
 

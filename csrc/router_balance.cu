@@ -8,7 +8,7 @@
 
 #include <cmath>
 
-#include "logit_loss.cuh"
+#include "tc_common.cuh"
 
 namespace bw {
 namespace {
@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(kWarps * 32) balance_fwd_kernel(BalanceArgs a)
         if (e >= 0 && e < a.E)
           atomicAdd(hist + e, 1);
         else
-          *a.err = kErrArgument;
+          report_error(a.err, kErrBadArg);
       }
     }
 #pragma unroll
