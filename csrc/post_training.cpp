@@ -275,8 +275,7 @@ bw::BalanceArgs balance_args(const Tensor& logits, const OptTensor& ids, const O
     a.mask = reinterpret_cast<const uint8_t*>(mask->data_ptr<bool>());
   }
   a.z_coef = (float)z_coef;
-  const int64_t want = (148 * 4 + G - 1) / (G > 0 ? G : 1), have = (N + 63) / 64;
-  a.chunks = (int)std::max<int64_t>(1, std::min(want, have));
+  a.chunks = bw::balance_chunks(a);
   check_like(err, "err", torch::kInt32, logits);
   a.err = err.data_ptr<int>();
   return a;

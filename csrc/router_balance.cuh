@@ -36,6 +36,8 @@ struct BalanceGradArgs {
   void* out;            // (G, N, E) contiguous
 };
 
+// CTAs of one group in the forward.
+int balance_chunks(const BalanceArgs& a);
 void balance_fwd(const BalanceArgs& a, cudaStream_t s);
 void balance_bwd(const BalanceGradArgs& a, cudaStream_t s);
 
