@@ -13,7 +13,8 @@ B200 execution choices:
   computes its projections inside those GEMMs;
 * attention is ``scaled_dot_product_attention`` with grouped KV heads (no K/V
   repetition in memory);
-* RMSNorm and SwiGLU use the library's fused elementwise kernels on sm_100;
+* RMSNorm and SwiGLU use the library's fused elementwise kernels on sm_100; with
+  ``qk_norm=True`` the norms of the query and key heads run in the rotation's pass;
 * the LM loss never materializes fp32 logits: bf16 logits from one GEMM, then a
   fused kernel computes per-row log-sum-exp and the loss, and in the backward the
   same bf16 buffer is turned into ``dlogits`` in place;
@@ -54,6 +55,7 @@ class LlamaConfig:
     max_position_embeddings: int = 131072
     tie_word_embeddings: bool = True
     initializer_range: float = 0.02
+    qk_norm: bool = False  # RMS norms of every query and key head before the rotation
 
     @property
     def dim_per_head(self) -> int:
@@ -166,6 +168,22 @@ class LlamaAttention(nn.Module):
         self.k_proj = TcLinear(d, self.n_kv * hd, bias=False)
         self.v_proj = TcLinear(d, self.n_kv * hd, bias=False)
         self.o_proj = TcLinear(self.n_heads * hd, d, bias=False)
+        if cfg.qk_norm:
+            self.q_norm = RMSNorm(hd, eps=cfg.rms_norm_eps)
+            self.k_norm = RMSNorm(hd, eps=cfg.rms_norm_eps)
+        self.qk_norm = cfg.qk_norm
+
+    def _norm_and_rotate(self, q, k, cos, sin, half_tables):
+        """Head norms and rotation of ``q, k (B, T, H, d)``, returned as ``(B, H, T, d)``: one
+        kernel, or the modules one by one where a hook watches a norm."""
+        from dattri_llm_b200.ops import fused
+
+        watched = any(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks
+                      for m in (self.q_norm, self.k_norm))
+        if half_tables is not None and fused.enabled(q) and not watched:
+            q, k = fused.qk_norm_rope(q, k, self.q_norm.weight, self.k_norm.weight, *half_tables, eps=self.q_norm.eps)
+            return q.transpose(1, 2), k.transpose(1, 2)
+        return apply_rope(self.q_norm(q).transpose(1, 2), self.k_norm(k).transpose(1, 2), cos, sin)
 
     def forward(self, x: torch.Tensor, cos, sin, attention_mask: torch.Tensor | None = None,
                 half_tables: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
@@ -175,7 +193,9 @@ class LlamaAttention(nn.Module):
         q = self.q_proj(x).view(b, t, self.n_heads, self.head_dim)
         k = self.k_proj(x).view(b, t, self.n_kv, self.head_dim)
         v = self.v_proj(x).view(b, t, self.n_kv, self.head_dim).transpose(1, 2)
-        if (half_tables is not None and fused.rope_enabled(q) and fused.rope_enabled(k)
+        if self.qk_norm:
+            q, k = self._norm_and_rotate(q, k, cos, sin, half_tables)
+        elif (half_tables is not None and fused.rope_enabled(q) and fused.rope_enabled(k)
                 and (self.n_heads + self.n_kv) * self.head_dim // 16 <= 1024):
             q, k = fused.rope(q, k, *half_tables)
             q, k = q.transpose(1, 2), k.transpose(1, 2)

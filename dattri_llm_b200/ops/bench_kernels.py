@@ -25,6 +25,10 @@ Rows (ids of the hot-op inventory):
   gated_norm      Mamba2 gated RMSNorm, forward + backward   vs the module's elementwise chain
   causal_conv     Mamba2 conv1d (4 taps) + SiLU, fwd + bwd    vs cuDNN depthwise conv + SiLU
   ssd_intra       Mamba2 intra-chunk SSD, fwd + bwd          vs materialized decay + einsum
+  preference      preference loss from logits, fwd + bwd     vs log_softmax + gather + logsigmoid under autograd
+  policy          clipped policy loss with KL, fwd + bwd     vs log_softmax + gather + the surrogate under autograd
+  balance         router balance loss and counts, fwd + bwd  vs softmax + topk + one-hot mean under autograd
+  qk_norm         head norms + rotation, fwd + bwd           vs rms_norm + rotate-half under autograd
 """
 
 from __future__ import annotations
@@ -343,6 +347,94 @@ def bench_ssd_intra(peaks):
          {"shape": f"B={b} C={c} S={s} H={h} G={g} P={p}", "note": "fp32 CUDA cores; tensor_frac vs the bf16 peak"})
 
 
+def _logits_and_labels(b, t, v):
+    x = torch.randn(b, t, v, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    y = torch.randint(0, v, (b, t), device="cuda")
+    y[:, : t // 4] = -100
+    return x, y
+
+
+def _torch_logps(x, y):
+    keep = y != -100
+    return torch.log_softmax(x.float(), -1).gather(2, y.clamp(min=0)[..., None])[..., 0] * keep, keep
+
+
+def bench_preference(peaks):
+    from dattri_llm_b200 import ops
+
+    b, t, v = 8, 512, 128256
+    x, y = _logits_and_labels(b, t, v)
+    ref = torch.zeros(b, device="cuda")
+
+    def torch_fn():
+        lp = _torch_logps(x, y)[0].sum(1)
+        loss = -torch.nn.functional.logsigmoid(0.1 * (lp[: b // 2] - lp[b // 2:])).mean()
+        return torch.autograd.grad(loss, x)
+
+    ours = _time(lambda: torch.autograd.grad(ops.preference_loss(x, y, ref).loss, x))
+    _row("preference", ours, _time(torch_fn, 3), int(x.numel() * 2 * 1.75), x.numel() * 7, peaks,
+         {"shape": f"B={b} T={t} V={v}"})
+
+
+def bench_policy(peaks):
+    from dattri_llm_b200 import ops
+
+    b, t, v = 8, 512, 128256
+    x, y = _logits_and_labels(b, t, v)
+    adv, old = torch.randn(b, device="cuda"), torch.full((b, t), -12.0, device="cuda")
+
+    def torch_fn():
+        lp, keep = _torch_logps(x, y)
+        r, d = torch.exp((lp - old) * keep), (old - lp) * keep
+        a = adv[:, None]
+        tok = -torch.minimum(r * a, r.clamp(0.8, 1.2) * a) + 0.04 * (torch.exp(d) - d - 1)
+        return torch.autograd.grad((tok * keep).sum() / keep.sum(), x)
+
+    ours = _time(lambda: torch.autograd.grad(ops.policy_loss(x, y, adv, old, old, kl_coef=0.04).loss, x))
+    _row("policy", ours, _time(torch_fn, 3), int(x.numel() * 2 * 1.75), x.numel() * 7, peaks,
+         {"shape": f"B={b} T={t} V={v}"})
+
+
+def bench_balance(peaks):
+    from dattri_llm_b200 import ops
+
+    g, n, e, k = 16, 65536, 64, 8
+    x = torch.randn(g, n, e, device="cuda").bfloat16().requires_grad_()
+
+    def torch_fn():
+        p = torch.softmax(x.float(), -1)
+        ids = p.topk(k, -1).indices
+        f = torch.zeros(g, e, device="cuda").scatter_add_(1, ids.reshape(g, -1), torch.ones(1, device="cuda").expand(g, n * k)) / n
+        return torch.autograd.grad((e * (f * p.mean(1)).sum(1)).sum(), x)
+
+    ours = _time(lambda: torch.autograd.grad(ops.router_balance_loss(x, k).loss.sum(), x))
+    _row("balance", ours, _time(torch_fn, 3), x.numel() * 4, x.numel() * 10, peaks, {"shape": f"G={g} N={n} E={e} K={k}"})
+
+
+def bench_qk_norm(peaks):
+    from dattri_llm_b200 import ops
+
+    b, t, h, hk, d = 8, 2048, 32, 8, 128
+    q, k = (torch.randn(b, t, n, d, device="cuda").bfloat16().requires_grad_() for n in (h, hk))
+    qw, kw = (torch.ones(d, device="cuda", dtype=torch.bfloat16).requires_grad_() for _ in range(2))
+    ang = torch.outer(torch.arange(t, device="cuda").float(), 10000.0 ** (-torch.arange(d // 2, device="cuda") / (d // 2)))
+    cos, sin = ang.cos(), ang.sin()
+    gq, gk = (torch.randn(b, n, t, d, device="cuda").bfloat16().transpose(1, 2) for n in (h, hk))
+
+    def one(x, w):
+        y = torch.nn.functional.rms_norm(x, (d,), w, 1e-6)
+        a, c = y[..., : d // 2], y[..., d // 2:]
+        co, si = cos[None, :, None].to(x.dtype), sin[None, :, None].to(x.dtype)
+        return torch.cat([a * co - c * si, c * co + a * si], -1)
+
+    def torch_fn():
+        return torch.autograd.grad((one(q, qw), one(k, kw)), (q, k, qw, kw), (gq, gk))
+
+    ours = _time(lambda: torch.autograd.grad(ops.qk_norm_rope(q, k, qw, kw, cos, sin), (q, k, qw, kw), (gq, gk)))
+    n = q.numel() + k.numel()
+    _row("qk_norm", ours, _time(torch_fn, 3), n * 8, n * 18, peaks, {"shape": f"B={b} T={t} H={h}/{hk} D={d}"})
+
+
 BENCHES = {
     "ghost_gram": bench_ghost_gram,
     "ghost_dot": bench_ghost_dot,
@@ -358,6 +450,10 @@ BENCHES = {
     "gated_norm": bench_gated_norm,
     "causal_conv": bench_causal_conv,
     "ssd_intra": bench_ssd_intra,
+    "preference": bench_preference,
+    "policy": bench_policy,
+    "balance": bench_balance,
+    "qk_norm": bench_qk_norm,
 }
 
 

@@ -107,6 +107,16 @@ def check_mask_coords(name: str, rows: torch.Tensor, cols: torch.Tensor, k_rows:
     _in_range(name, cols, 0, k_cols, "column coordinate")
 
 
+def check_labels(name: str, labels: torch.Tensor, vocab: int, ignore: int) -> None:
+    """Labels that count address the vocabulary axis of the logits."""
+    _in_range(name, torch.where(labels == ignore, 0, labels), 0, vocab, "label")
+
+
+def check_positions(name: str, positions: torch.Tensor, table: int) -> None:
+    """Positions address the rows of the tables of angles."""
+    _in_range(name, positions, 0, table, "position")
+
+
 def _opt(args: tuple, kwargs: dict, i: int, key: str, default=None):
     if len(args) > i:
         return args[i]
@@ -147,6 +157,29 @@ def _v_mask_gather(args, kwargs):
     check_mask_coords("mask_gather", args[2], args[3], int(args[0].shape[-1]), int(args[1].shape[-1]))
 
 
+def _v_preference_loss(args, kwargs):
+    # (logits, labels, ref, kind, beta, smoothing, average, reduction, ignore, err)
+    check_labels("preference_loss", args[1], int(args[0].shape[2]), int(args[8]))
+
+
+def _v_policy_loss(args, kwargs):
+    # (logits, labels, adv, old, ref, lo, hi, kl_coef, temperature, reduction, ignore, err)
+    check_labels("policy_loss", args[1], int(args[0].shape[2]), int(args[10]))
+
+
+def _v_balance_loss(args, kwargs):
+    # (logits, ids, mask, top_k, z_coef, err)
+    if args[1] is not None:
+        ids, mask = args[1].reshape(-1, int(args[3])), args[2]
+        check_expert_ids("balance_loss", ids if mask is None else ids[mask.reshape(-1)], int(args[0].shape[2]))
+
+
+def _v_qk_norm_rope(args, kwargs):
+    # (q, k, q_weight, k_weight, cos, sin, positions, eps, err)
+    if args[6] is not None:
+        check_positions("qk_norm_rope", args[6], int(args[4].shape[0]))
+
+
 VALIDATORS: dict[str, Callable[[tuple, dict], None]] = {
     "moe_dispatch": _v_moe_dispatch,
     "moe_combine_bwd_dispatch": _v_moe_combine_bwd_dispatch,
@@ -154,6 +187,10 @@ VALIDATORS: dict[str, Callable[[tuple, dict], None]] = {
     "moe_count": _v_moe_count,
     "moe_place": _v_moe_place,
     "mask_gather": _v_mask_gather,
+    "preference_loss": _v_preference_loss,
+    "policy_loss": _v_policy_loss,
+    "balance_loss": _v_balance_loss,
+    "qk_norm_rope": _v_qk_norm_rope,
 }
 
 

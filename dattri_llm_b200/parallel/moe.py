@@ -44,6 +44,7 @@ import torch.distributed as dist
 import torch.nn.functional as F
 from torch import nn
 
+from dattri_llm_b200.ops.losses import router_balance_loss
 from dattri_llm_b200.parallel.symm import PeerBarrier, SymmetricBuffer
 
 
@@ -591,11 +592,15 @@ class ExpertParallelMoE(nn.Module):
     capture (one LoGra projection per side, materialized), it is the same fused path with the
     captures taken inside it (:class:`_EPGroupedMoE`); under other captures, and on other
     devices or dtypes, it is the two-stage all-to-all form (``torch.distributed`` all-to-all,
-    any backend)."""
+    any backend).
+
+    With ``track_balance`` each forward leaves the router's balance loss and expert counts of
+    this rank's tokens in ``balance`` (:func:`dattri_llm_b200.ops.router_balance_loss`); add
+    :func:`balance_loss` of the model to a training loss."""
 
     def __init__(self, hidden: int, intermediate: int, n_experts: int, top_k: int, *, max_tokens: int,
                  norm_topk_prob: bool = False, group=None, device: torch.device | None = None,
-                 dtype: torch.dtype = torch.bfloat16) -> None:
+                 dtype: torch.dtype = torch.bfloat16, track_balance: bool = False) -> None:
         super().__init__()
         self.group = group
         self.world = dist.get_world_size(group) if dist.is_initialized() else 1
@@ -609,6 +614,8 @@ class ExpertParallelMoE(nn.Module):
         self.hidden, self.intermediate, self.n_experts, self.top_k = hidden, intermediate, n_experts, top_k
         self.experts_per_rank = n_experts // self.world
         self.norm_topk_prob = norm_topk_prob
+        self.track_balance = track_balance
+        self.balance = None
         self.max_tokens = max_tokens
         self.capacity = self.world * max_tokens * top_k
         self.dtype = dtype
@@ -651,8 +658,11 @@ class ExpertParallelMoE(nn.Module):
 
         The router runs on *x* in its own shape, so a capture hook on ``gate`` sees the
         ``(B, T, H)`` layout of the samples."""
-        probs = torch.softmax(self.gate(x).float().reshape(-1, self.n_experts), dim=-1)
+        logits = self.gate(x)
+        probs = torch.softmax(logits.float().reshape(-1, self.n_experts), dim=-1)
         topv, topi = probs.topk(self.top_k, dim=-1)
+        if self.track_balance:
+            self.balance = router_balance_loss(logits.reshape(-1, self.n_experts), self.top_k, topi)
         if self.norm_topk_prob:
             topv = topv / topv.sum(-1, keepdim=True)
         return topv, topi
@@ -745,6 +755,15 @@ def expert_parallelize(model: nn.Module, *, max_tokens: int, group=None, device:
         setattr(parent, child, ep)
         replaced.append(name)
     return replaced
+
+
+def balance_loss(model: nn.Module) -> torch.Tensor:
+    """Mean of the balance losses that the last forward left in *model*'s tracking
+    :class:`ExpertParallelMoE` blocks."""
+    found = [m.balance.loss for m in model.modules() if isinstance(m, ExpertParallelMoE) and m.balance is not None]
+    if not found:
+        raise ValueError("no expert block of the model tracked its balance in a forward (track_balance=True)")
+    return torch.stack(found).mean()
 
 
 def expert_parallel_buffers(model: nn.Module) -> list[str]:
