@@ -43,6 +43,12 @@ struct RowSpan {
     nv = (V + shift + N - 1) / N;
   }
   __device__ __forceinline__ int first(int j) const { return j * N - shift; }
+  // Whether vectors [j0, j0 + n) all belong to the row whole.
+  __device__ __forceinline__ bool inner(int j0, int n) const {
+    return (j0 > 0 || shift == 0) && j0 + n <= (V + shift) / N;
+  }
+  __device__ __forceinline__ bool whole(int lo) const { return lo >= 0 && lo + N <= V; }
+  __device__ __forceinline__ const uint4* vec(int j) const { return reinterpret_cast<const uint4*>(row - shift) + j; }
   // Vector j; elements outside the row are -inf. kLast: nothing reads it again soon.
   template <bool kLast>
   __device__ __forceinline__ uint4 load(int j) const {
@@ -218,47 +224,47 @@ struct Place {
   }
 };
 
-// The maximum and the sum of a row, in every thread of its group: one pass with a running maximum and sum in each. Vectors
-// before `kept` (whole steps of the loop, or all) also stay in `keep`, where the thread that read them finds them again.
-// kAhead: a step's loads are issued before the step in front is used, for groups too few on an SM to hide them.
-template <typename T, int kGroup, bool kKeep, bool kAhead>
-__device__ __forceinline__ void row_stats(const RowSpan<T>& span, float c, float& m, float& s, float2* parts, uint4* keep,
-                                          int kept) {
+// kUnroll vectors of a thread from vector j on, kStride apart; `whole`: all of the row. kLast: nothing reads them again soon.
+template <typename T, int kStride, bool kLast>
+__device__ __forceinline__ void fetch(const RowSpan<T>& span, int j, bool whole, uint4 (&to)[kUnroll]) {
+  if (whole) {
+    const uint4* p = span.vec(j);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) to[u] = kLast ? __ldcs(p + u * kStride) : __ldcg(p + u * kStride);
+  } else {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) to[u] = span.template load<kLast>(j + u * kStride);
+  }
+}
+
+// Takes vectors into a thread's running maximum and sum.
+template <typename T>
+__device__ __forceinline__ void take(const uint4 (&v)[kUnroll], float c, float& m, float& s) {
+  const float top = max_of<T>(v);
+  if (top > m) {
+    s *= m == -INFINITY ? 1.f : ex2((m - top) * c);
+    m = top;
+  }
+  s += sum_of<T>(v, base_of(m), c);
+}
+
+// The maximum and the sum of a row, in every thread of its group: one pass with a running maximum and sum in each.
+template <typename T, int kGroup>
+__device__ __forceinline__ void row_stats(const RowSpan<T>& span, float c, float& m, float& s, float2* parts) {
   constexpr int kHold = kGroup * kUnroll;
   m = -INFINITY;
   s = 0.f;
   const int tid = Place<kGroup>::tid();
-  uint4 v[kUnroll], next[kUnroll];
-  auto fetch = [&](uint4 (&to)[kUnroll], int j) {
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) to[u] = span.template load<false>(j + u * kGroup);
-  };
-  if (kAhead) fetch(next, tid);
   for (int j = tid; j < span.nv; j += kHold) {
-    if constexpr (kAhead) {
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) v[u] = next[u];
-      if (j + kHold < span.nv) fetch(next, j + kHold);
-    } else {
-      fetch(v, j);
-    }
-    if (kKeep && j < kept) {
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (j + u * kGroup < kept) keep[j + u * kGroup] = v[u];
-    }
-    const float top = max_of<T>(v);
-    if (top > m) {
-      s *= m == -INFINITY ? 1.f : ex2((m - top) * c);
-      m = top;
-    }
-    s += sum_of<T>(v, base_of(m), c);
+    uint4 v[kUnroll];
+    fetch<T, kGroup, false>(span, j, span.inner(j - tid, kHold), v);
+    take<T>(v, c, m, s);
   }
   merge_group<kGroup>(m, s, c, parts);
 }
 
 template <typename T, int kGroup>
-__global__ void __launch_bounds__(Place<kGroup>::kThreads) row_stats_kernel(LogitRows r, float* __restrict__ logps,
+__global__ void __launch_bounds__(Place<kGroup>::kThreads, kGroup == 32 ? 10 : 12) row_stats_kernel(LogitRows r, float* __restrict__ logps,
                                                                             RowStat* __restrict__ stats,
                                                                             unsigned* __restrict__ ticket) {
   __shared__ float2 parts[32];
@@ -277,7 +283,7 @@ __global__ void __launch_bounds__(Place<kGroup>::kThreads) row_stats_kernel(Logi
   const T* x = row_ptr<T>(r, row);
   const float c = kLog2e * r.inv_temp;
   float m, s;
-  row_stats<T, kGroup, false, false>(RowSpan<T>(x, r.V), c, m, s, parts, nullptr, 0);
+  row_stats<T, kGroup>(RowSpan<T>(x, r.V), c, m, s, parts);
   if (tid == 0) {
     const float base = base_of(m);
     logps[row] = kLn2 * ((ElemOf<T>::up(x[y]) - base) * c - log2f(s));
@@ -292,39 +298,49 @@ __device__ __forceinline__ void zero_row(T* out, int V) {
   for (int j = Place<kGroup>::tid(); j < span.nv; j += kGroup) store_vec<T>(out, V, span.first(j), make_uint4(0, 0, 0, 0), true);
 }
 
-// coef (onehot - softmax) of a row, read for the last time: from `keep` what row_stats left there.
-template <typename T, int kGroup, bool kKeep, bool kAhead>
-__device__ __forceinline__ void row_grad(const RowSpan<T>& span, T* out, int y, float base, float inv_s, float c, float coef,
-                                         const uint4* keep, int kept) {
-  constexpr int kHold = kGroup * kUnroll;
+// Writes coef (onehot - softmax) of kUnroll vectors. What a gradient needs of its row:
+struct RowGrad {
+  int y;
+  float base, c, k, coef;  // k = -coef / s
+  bool aligned;            // the gradient's row starts at the same place within 16 bytes
+};
+
+template <typename T, int kStride>
+__device__ __forceinline__ void put(const RowSpan<T>& span, T* out, int j, bool whole, const uint4 (&v)[kUnroll],
+                                    const RowGrad& g) {
+  constexpr int N = kVecOf<T>;
+  if (whole && g.aligned) {
+    const int lo = span.first(j);
+    uint4* p = reinterpret_cast<uint4*>(out + lo);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      __stcs(p + u * kStride, grad_of<T>(v[u], lo + u * kStride * N, g.y, g.base, g.c, g.k, g.coef));
+    return;
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int lo = span.first(j + u * kStride);
+    if (lo < span.V) store_vec<T>(out, span.V, lo, grad_of<T>(v[u], lo, g.y, g.base, g.c, g.k, g.coef), g.aligned);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ RowGrad row_grad_of(const RowSpan<T>& span, const T* out, int y, float base, float inv_s, float c,
+                                               float coef) {
   const bool aligned = (int)((reinterpret_cast<uintptr_t>(out) % 16) / sizeof(T)) == span.shift;
-  const float k = -coef * inv_s;
+  return RowGrad{y, base, c, -coef * inv_s, coef, aligned};
+}
+
+// The gradient of a row, read for the last time.
+template <typename T, int kGroup>
+__device__ __forceinline__ void row_grad(const RowSpan<T>& span, T* out, const RowGrad& g) {
+  constexpr int kHold = kGroup * kUnroll;
   const int tid = Place<kGroup>::tid();
-  uint4 v[kUnroll], next[kUnroll];
-  auto fetch = [&](uint4 (&to)[kUnroll], int j) {
-    if (kKeep && j < kept) {
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (j + u * kGroup < kept) to[u] = keep[j + u * kGroup];
-    } else {
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) to[u] = span.template load<true>(j + u * kGroup);
-    }
-  };
-  if (kAhead) fetch(next, tid);
   for (int j = tid; j < span.nv; j += kHold) {
-    if constexpr (kAhead) {
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) v[u] = next[u];
-      if (j + kHold < span.nv) fetch(next, j + kHold);
-    } else {
-      fetch(v, j);
-    }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int lo = span.first(j + u * kGroup);
-      if (lo < span.V) store_vec<T>(out, span.V, lo, grad_of<T>(v[u], lo, y, base, c, k, coef), aligned);
-    }
+    const bool whole = span.inner(j - tid, kHold);
+    uint4 v[kUnroll];
+    fetch<T, kGroup, true>(span, j, whole, v);
+    put<T, kGroup>(span, out, j, whole, v, g);
   }
 }
 
@@ -351,8 +367,8 @@ __global__ void __launch_bounds__(Place<kGroup>::kThreads) logit_grad_kernel(Log
     return;
   }
   const RowStat st = a.stats[row];
-  row_grad<T, kGroup, false, false>(RowSpan<T>(row_ptr<T>(r, row), r.V), out, y, st.m, st.inv_s, kLog2e * r.inv_temp, coef,
-                                    nullptr, 0);
+  const RowSpan<T> span(row_ptr<T>(r, row), r.V);
+  row_grad<T, kGroup>(span, out, row_grad_of(span, out, y, st.m, st.inv_s, kLog2e * r.inv_temp, coef));
 }
 
 // ---------------------------------------------------------------- sums over tokens
@@ -543,48 +559,124 @@ __global__ void __launch_bounds__(256) policy_finish_kernel(PolicyArgs a) {
 }
 
 // ---------------------------------------------------------------- loss and gradient in one kernel
-// A token's coefficient needs its own row only, so the group that took a row's statistics writes its gradient at once: the
-// row's first `kept` vectors wait in shared memory, the rest is read a second time from L2, where few enough rows are
-// between their two passes at any time.
-template <typename T, int kGroup, int kMin, bool kLong>
-__global__ void __launch_bounds__(Place<kGroup>::kThreads, kMin) policy_row_kernel(PolicyArgs a, int kept) {
-  extern __shared__ uint4 keep[];
+// A token's coefficient needs its own row only, so the group that took a row's statistics writes its gradient at once and
+// reads the row a second time: from L2, which holds the few rows that are between their two passes at any time.
+
+// What of a row that counts goes out, from its maximum and sum; the gradient's coefficient, the same in every thread.
+__device__ __forceinline__ float policy_out(const PolicyArgs& a, long long row, const TokenIn& in, float w, float xy, float m,
+                                            float s, float c, bool first) {
+  const float base = base_of(m), logp = kLn2 * ((xy - base) * c - log2f(s));
+  const TokenTerms k = policy_token(a, in, logp);
+  if (first) {
+    a.logps[row] = logp;
+    a.stats[row] = RowStat{base, 1.f / s};
+    a.dtok[row] = k.slope * w;
+    a.tok[row] = make_float4(k.loss * w, k.kl, k.clipped, 0.f);
+  }
+  return k.slope * w * a.rows.inv_temp;
+}
+
+// The same of a row that does not.
+template <typename T, int kGroup>
+__device__ __forceinline__ void policy_skip(const PolicyArgs& a, long long row, T* out) {
+  if (Place<kGroup>::tid() == 0) {
+    a.logps[row] = a.dtok[row] = 0.f;
+    a.stats[row] = RowStat{0.f, 0.f};
+    a.tok[row] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  zero_row<T, kGroup>(out, a.rows.V);
+}
+
+template <typename T>
+__device__ __forceinline__ T* grad_row(const PolicyArgs& a, long long row) {
+  const long long b = row / a.rows.T;
+  return reinterpret_cast<T*>(a.grad) + b * a.gsb + (row - b * a.rows.T) * a.gst;
+}
+
+template <typename T, int kGroup, int kMin>
+__global__ void __launch_bounds__(Place<kGroup>::kThreads, kMin) policy_row_kernel(PolicyArgs a) {
   __shared__ float2 parts[32];
   const LogitRows& r = a.rows;
   const long long row = Place<kGroup>::row();
   if (row >= (long long)r.B * r.T) return;
-  const int tid = Place<kGroup>::tid();
-  const long long b = row / r.T, t = row - b * r.T;
   const int y = row_label(r, row);
-  T* out = reinterpret_cast<T*>(a.grad) + b * a.gsb + t * a.gst;
+  T* out = grad_row<T>(a, row);
   if (y < 0) {
-    if (tid == 0) {
-      a.logps[row] = a.dtok[row] = 0.f;
-      a.stats[row] = RowStat{0.f, 0.f};
-      a.tok[row] = make_float4(0.f, 0.f, 0.f, 0.f);
-    }
+    policy_skip<T, kGroup>(a, row, out);
+    return;
+  }
+  const T* x = row_ptr<T>(r, row);
+  const RowSpan<T> span(x, r.V);
+  const long long b = row / r.T;
+  const float c = kLog2e * r.inv_temp, xy = ElemOf<T>::up(x[y]), w = token_weight(a, b);
+  const TokenIn in = token_in(a, row, b);
+  float m, s;
+  row_stats<T, kGroup>(span, c, m, s, parts);
+  const float coef = policy_out(a, row, in, w, xy, m, s, c, Place<kGroup>::tid() == 0);
+  if (coef == 0.f)
     zero_row<T, kGroup>(out, r.V);
+  else
+    row_grad<T, kGroup>(span, out, row_grad_of(span, out, y, base_of(m), 1.f / s, c, coef));
+}
+
+// Long rows, two CTAs of an SM: the first kKept vectors wait in shared memory for the second pass, where the thread that read
+// them finds them again, and only the rest is read again from L2. A step's loads are issued before the step in front is used.
+constexpr int kLongThreads = 512, kLongHold = kLongThreads * kUnroll, kKept = 3 * kLongHold;
+
+template <typename T>
+__global__ void __launch_bounds__(kLongThreads, 2) policy_long_kernel(PolicyArgs a) {
+  extern __shared__ uint4 keep[];  // [kKept]
+  __shared__ float2 parts[32];
+  const LogitRows& r = a.rows;
+  const long long row = blockIdx.x, b = row / r.T;
+  const int tid = threadIdx.x, y = row_label(r, row);
+  T* out = grad_row<T>(a, row);
+  if (y < 0) {
+    policy_skip<T, kLongThreads>(a, row, out);
     return;
   }
   const T* x = row_ptr<T>(r, row);
   const RowSpan<T> span(x, r.V);
   const float c = kLog2e * r.inv_temp, xy = ElemOf<T>::up(x[y]), w = token_weight(a, b);
   const TokenIn in = token_in(a, row, b);
-  float m, s;
-  row_stats<T, kGroup, kLong, kLong>(span, c, m, s, parts, keep, kept);
-  const float base = base_of(m), inv_s = 1.f / s, logp = kLn2 * ((xy - base) * c - log2f(s));
-  const TokenTerms k = policy_token(a, in, logp);  // the same in every thread
-  if (tid == 0) {
-    a.logps[row] = logp;
-    a.stats[row] = RowStat{base, inv_s};
-    a.dtok[row] = k.slope * w;
-    a.tok[row] = make_float4(k.loss * w, k.kl, k.clipped, 0.f);
+  uint4 v[kUnroll], ahead[kUnroll];
+  const auto load = [&](int j0) {
+    fetch<T, kLongThreads, false>(span, j0 + tid, span.inner(j0, kLongHold), ahead);
+  };
+  load(0);
+  float m = -INFINITY, s = 0.f;
+  for (int j0 = 0; j0 < span.nv; j0 += kLongHold) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) v[u] = ahead[u];
+    if (j0 + kLongHold < span.nv) load(j0 + kLongHold);
+    if (j0 < kKept) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) keep[j0 + u * kLongThreads + tid] = v[u];
+    }
+    take<T>(v, c, m, s);
   }
-  const float coef = k.slope * w * r.inv_temp;
-  if (coef == 0.f)
-    zero_row<T, kGroup>(out, r.V);
-  else
-    row_grad<T, kGroup, kLong, kLong>(span, out, y, base, inv_s, c, coef, keep, kept);
+  merge_group<kLongThreads>(m, s, c, parts);
+  const float coef = policy_out(a, row, in, w, xy, m, s, c, tid == 0);
+  if (coef == 0.f) {
+    zero_row<T, kLongThreads>(out, r.V);
+    return;
+  }
+  const RowGrad g = row_grad_of(span, out, y, base_of(m), 1.f / s, c, coef);
+  const auto again = [&](int j0) {
+    if (j0 < kKept) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) ahead[u] = keep[j0 + u * kLongThreads + tid];
+    } else {
+      fetch<T, kLongThreads, true>(span, j0 + tid, span.inner(j0, kLongHold), ahead);
+    }
+  };
+  again(0);
+  for (int j0 = 0; j0 < span.nv; j0 += kLongHold) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) v[u] = ahead[u];
+    if (j0 + kLongHold < span.nv) again(j0 + kLongHold);
+    put<T, kLongThreads>(span, out, j0 + tid, span.inner(j0, kLongHold), v, g);
+  }
 }
 
 // grad *= g unless g is 1, which is what a loss that ends the graph sends.
@@ -618,22 +710,20 @@ unsigned grid_of(const LogitRows& r) {
 // 65536 rows of 1024 and 32768 of 4000 logits, 16384 of 16000, 8192 of 128256.
 constexpr int kShort = 768;
 
-template <typename T, int kGroup, int kMin, bool kLong>
-void policy_rows(const PolicyArgs& a, int bytes, cudaStream_t s) {
-  const int all = (a.rows.V + 2 * (kVecOf<T> - 1)) / kVecOf<T>, step = kGroup * kUnroll;
-  const int kept = bytes / 16 >= all ? all : bytes / 16 / step * step;
-  const auto kernel = policy_row_kernel<T, kGroup, kMin, kLong>;
-  if (kLong) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kept * 16);
-  kernel<<<grid_of<kGroup>(a.rows), Place<kGroup>::kThreads, kept * 16, s>>>(a, kept);
+template <typename T, int kGroup, int kMin>
+void policy_rows(const PolicyArgs& a, cudaStream_t s) {
+  policy_row_kernel<T, kGroup, kMin><<<grid_of<kGroup>(a.rows), Place<kGroup>::kThreads, 0, s>>>(a);
 }
 
 template <typename T>
 void rows_of(const PolicyArgs& a, cudaStream_t s) {
   const int n = a.rows.V / kVecOf<T>;
-  if (n <= kShort) return policy_rows<T, 32, 8, false>(a, 0, s);
-  if (n <= 3072) return policy_rows<T, 128, 8, false>(a, 0, s);
-  if (n <= 6144) return policy_rows<T, 256, 4, false>(a, 0, s);
-  policy_rows<T, 512, 2, true>(a, 100 * 1024, s);
+  if (n <= kShort) return policy_rows<T, 32, 8>(a, s);
+  if (n <= 3072) return policy_rows<T, 128, 8>(a, s);
+  if (n <= kKept) return policy_rows<T, 256, 4>(a, s);
+  constexpr int kBytes = kKept * 16;
+  cudaFuncSetAttribute(policy_long_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+  policy_long_kernel<T><<<grid_of<kLongThreads>(a.rows), kLongThreads, kBytes, s>>>(a);
 }
 
 template <typename T>
