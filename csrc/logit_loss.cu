@@ -504,13 +504,28 @@ __global__ void __launch_bounds__(256) policy_count_kernel(PolicyArgs a) {
   }
 }
 
+// The sequences' counts in one: with up to kFewSequences every row adds them itself.
+constexpr int kFewSequences = 32;
+
+__global__ void __launch_bounds__(1024) policy_total_kernel(PolicyArgs a) {
+  __shared__ double red[32];
+  double n = 0;
+  for (int k = threadIdx.x; k < a.rows.B; k += blockDim.x) n += a.count[k];
+  n = block_sum(n, red);
+  if (threadIdx.x == 0) a.count[a.rows.B] = (int)n;
+}
+
 // A token's share in the loss, from the tokens that count; the same in every lane of a warp.
 __device__ __forceinline__ float token_weight(const PolicyArgs& a, long long b) {
   if (a.mean == TokenMean::kSum) return 1.f;
   if (a.mean == TokenMean::kSequences) return 1.f / ((float)max(a.count[b], 1) * a.rows.B);
-  int n = 0;
-  for (int k = threadIdx.x & 31; k < a.rows.B; k += 32) n += a.count[k];
-  n = lanes_sum(n);
+  int n;
+  if (a.rows.B > kFewSequences) {
+    n = a.count[a.rows.B];
+  } else {
+    const int lane = threadIdx.x & 31;
+    n = lanes_sum(lane < a.rows.B ? a.count[lane] : 0);
+  }
   return 1.f / max(n, 1);
 }
 
@@ -767,6 +782,8 @@ int policy_fwd(const PolicyArgs& a, cudaStream_t s) {
   const bool rows = (long long)a.rows.B * a.rows.T > 0;
   if (a.grad == nullptr || !rows) stats_of(a.rows, a.logps, a.stats, a.ticket, s);
   policy_count_kernel<<<a.rows.B, 256, 0, s>>>(a);
+  const bool many = a.rows.B > kFewSequences;
+  if (many) policy_total_kernel<<<1, 1024, 0, s>>>(a);
   if (a.grad == nullptr || !rows)
     policy_token_kernel<<<a.rows.B, 256, 0, s>>>(a);
   else if (a.rows.type == Elem::kBF16)
@@ -776,7 +793,7 @@ int policy_fwd(const PolicyArgs& a, cudaStream_t s) {
   else
     rows_of<float>(a, s);
   policy_finish_kernel<<<a.rows.B, 256, 0, s>>>(a);
-  return a.grad == nullptr ? 4 : 3;
+  return (a.grad == nullptr ? 4 : 3) + many;
 }
 
 void logit_scale(const LogitRows& r, void* grad, long long sb, long long st, const float* g, cudaStream_t s) {

@@ -57,7 +57,7 @@ struct PolicyArgs {
   float* dtok;         // (B, T): d loss / d logps
   float4* tok;         // (B, T) workspace: loss, kl, clipped, unused
   double* seq;         // (B, 4) workspace
-  int* count;          // (B) tokens of each sequence that count
+  int* count;          // (B + 1): tokens of each sequence that count, and of all where there are more than a warp's
   unsigned* ticket;
   float *loss, *kl, *clipped;  // (1) each
   void* grad;          // like the logits, or null: no gradient now

@@ -7,6 +7,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -28,9 +29,18 @@ using torch::autograd::variable_list;
 
 std::atomic<int64_t> launches{0};
 
-// Gradients are the kernels' own results: they carry no graph.
-void once(const char* name) {
-  TORCH_CHECK(!at::GradMode::is_enabled(), name, " cannot be differentiated twice");
+// Gradients are the kernels' own results: they carry no graph. Under create_graph they come with a node that raises
+// when something is differentiated through them.
+variable_list once(variable_list grads, const char* name) {
+  if (!at::GradMode::is_enabled()) return grads;
+  for (auto& g : grads) {
+    if (!g.defined()) continue;
+    g = g.detach().requires_grad_();
+    auto node = std::make_shared<torch::autograd::DelayedError>(
+        std::string("the gradient of ") + name + " cannot be differentiated", 1);
+    g = (*node)({g})[0];
+  }
+  return grads;
 }
 
 // A gradient that a kernel reads as a dense array, or nothing.
@@ -158,7 +168,7 @@ Tensor preference_bwd(const Tensor& logits, const Tensor& labels, const Tensor& 
   return out;
 }
 
-// The float workspace of a policy loss: [stats 2 R | d R | (4 R of tokens) | sums of sequences 8 B | token counts B | ticket].
+// The float workspace of a policy loss: [stats 2 R | d R | (4 R of tokens) | sums of sequences 8 B | token counts B, all | ticket].
 // With want_grad the result's last tensor is the gradient for a loss gradient of 1.
 variable_list policy_fwd(const Tensor& logits, const Tensor& labels, const Tensor& adv, const OptTensor& old_logps,
                          const OptTensor& ref_logps, double clip_lo, double clip_hi, double kl_coef, double temperature,
@@ -178,7 +188,7 @@ variable_list policy_fwd(const Tensor& logits, const Tensor& labels, const Tenso
   }
   const auto f32 = logits.options().dtype(torch::kFloat32);
   const int64_t even = (2 * R + R + 3) / 4 * 4;  // the tokens' float4 start on their boundary
-  auto ws = torch::empty({even + 4 * R + 8 * B + B + 1}, f32);
+  auto ws = torch::empty({even + 4 * R + 8 * B + B + 2}, f32);
   auto logps = torch::empty({B, T}, f32);
   auto loss = torch::empty({}, f32), kl = torch::empty({}, f32), clipped = torch::empty({}, f32);
   float* w = ws.data_ptr<float>();
@@ -196,7 +206,7 @@ variable_list policy_fwd(const Tensor& logits, const Tensor& labels, const Tenso
   a.tok = reinterpret_cast<float4*>(w + even);
   a.seq = reinterpret_cast<double*>(a.tok + R);
   a.count = reinterpret_cast<int*>(a.seq + 4 * B);
-  a.ticket = reinterpret_cast<unsigned*>(a.count + B);
+  a.ticket = reinterpret_cast<unsigned*>(a.count + B + 1);
   a.loss = loss.data_ptr<float>();
   a.kl = kl.data_ptr<float>();
   a.clipped = clipped.data_ptr<float>();
@@ -364,6 +374,8 @@ bw::QkNormArgs qk_args(const Tensor& q, const Tensor& k, const Tensor& qw, const
     TORCH_CHECK(a.table >= a.T, "the tables of angles are shorter than the sequence");
   }
   a.eps = (float)eps;
+  TORCH_CHECK(q.size(0) * q.size(1) < (int64_t(1) << 31) && q.size(0) * q.size(1) * (q.size(2) + k.size(2)) < (int64_t(1) << 33),
+              "q and k: too many heads");
   check_like(err, "err", torch::kInt32, q);
   a.err = err.data_ptr<int>();
   return a;
@@ -431,13 +443,12 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
     return {out[0], out[1]};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    once("preference_loss");
     variable_list out(10);
     if (!g[0].defined() && !g[1].defined()) return out;
     const auto s = ctx->get_saved_variables();
     out[0] = preference_bwd(s[0], s[1], s[2], dense(g[0]), dense(g[1]), ctx->saved_data["ignore"].toInt(), s[3]);
     ++launches;
-    return out;
+    return once(std::move(out), "preference_loss");
   }
 };
 
@@ -457,7 +468,6 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     return {out[0], out[1], out[2], out[3]};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    once("policy_loss");
     variable_list out(13);
     if (!g[0].defined() && !g[1].defined()) return out;
     const auto s = ctx->get_saved_variables();
@@ -475,13 +485,13 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
         C10_CUDA_KERNEL_LAUNCH_CHECK();
         ++launches;
         out[0] = std::move(grad);
-        return out;
+        return once(std::move(out), "policy_loss");
       }
     }
     out[0] = policy_bwd(s[0], s[1], s[2], dense(g[0]), dense(g[1]), ctx->saved_data["temperature"].toDouble(),
                         ctx->saved_data["ignore"].toInt(), s[3]);
     ++launches;
-    return out;
+    return once(std::move(out), "policy_loss");
   }
 };
 
@@ -498,14 +508,13 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
     return {out[0], out[1]};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    once("router_balance_loss");
     variable_list out(6);
     if (!g[0].defined()) return out;
     const auto s = ctx->get_saved_variables();
     out[0] = balance_bwd(s[0], s[1].defined() ? OptTensor(s[1]) : std::nullopt, s[2], g[0],
                          ctx->saved_data["top_k"].toInt(), ctx->saved_data["z"].toDouble(), s[3]);
     ++launches;
-    return out;
+    return once(std::move(out), "router_balance_loss");
   }
 };
 
@@ -521,7 +530,6 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    once("qk_norm_rope");
     variable_list out(9);
     if (!g[0].defined() && !g[1].defined()) return out;
     const auto s = ctx->get_saved_variables();
@@ -532,7 +540,7 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
                          s[6].defined() ? OptTensor(s[6]) : std::nullopt, ctx->saved_data["eps"].toDouble(), s[7]);
     launches += 2;
     std::copy(d.begin(), d.end(), out.begin());
-    return out;
+    return once(std::move(out), "qk_norm_rope");
   }
 };
 

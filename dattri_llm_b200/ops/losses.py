@@ -256,7 +256,7 @@ def _balance_torch(logits, ids, mask, top_k, z_coef) -> BalanceLoss:
         raise ValueError(f"expert_ids must be in [0, {e})")
     chosen = keep.unsqueeze(-1).expand_as(ids)
     counts = torch.zeros(g, e, dtype=torch.int64, device=x.device)
-    counts.scatter_add_(1, torch.where(chosen, ids, 0).reshape(g, -1), chosen.reshape(g, -1).long())
+    counts.scatter_add_(1, torch.where(chosen, ids, 0).reshape(g, n * top_k), chosen.reshape(g, n * top_k).long())
     tokens = keep.sum(1).clamp(min=1).unsqueeze(-1)
     mean_p = torch.softmax(x, -1).masked_fill(~keep.unsqueeze(-1), 0.0).sum(1) / tokens
     loss = e * (counts / tokens * mean_p).sum(1)
@@ -303,14 +303,14 @@ def router_balance_loss(logits: torch.Tensor, top_k: int, expert_ids: torch.Tens
         if mask.shape != (*lead, n):
             raise ValueError(f"mask must be {(*lead, n)}, got {tuple(mask.shape)}")
         mask = (mask if mask.dtype == torch.bool else mask != 0).contiguous()
-    x = logits if len(lead) == 1 else logits.reshape(-1, n, e) if lead else logits.unsqueeze(0)
+    x = logits if len(lead) == 1 else logits.reshape(math.prod(lead), n, e) if lead else logits.unsqueeze(0)
     if x.stride(2) != 1:
         x = x.contiguous()
     if use_native(x):
         loss, counts = native().balance_loss(x, expert_ids, mask, top_k, z_coef, error_word(x.device))
     else:
-        loss, counts = _balance_torch(x, None if expert_ids is None else expert_ids.view(-1, n, top_k),
-                                      None if mask is None else mask.view(-1, n), top_k, z_coef)
+        loss, counts = _balance_torch(x, None if expert_ids is None else expert_ids.view(*x.shape[:2], top_k),
+                                      None if mask is None else mask.view(x.shape[:2]), top_k, z_coef)
     if len(lead) == 1:
         return BalanceLoss(loss, counts)
     return BalanceLoss(loss.reshape(lead), counts.reshape(*lead, e))

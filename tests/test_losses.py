@@ -652,6 +652,46 @@ def test_results_repeat_bit_for_bit_and_follow_the_current_stream():
         assert all(torch.equal(a, b) for a, b in zip(first, out))
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("b", [33, 100, 1026])
+def test_many_short_sequences(dev, b):
+    got, x, want, x64, _ = _policy(dev, (b, 2, 19), torch.float32, has_ref=True, kl_coef=0.1)
+    _check_policy(got, want, 1)
+    got.loss.backward()
+    want[0].backward()
+    _close(x.grad, x64.grad, 4e-5, 4e-5 * 15)
+    got, x, want, x64 = _preference(dev, (b, 2, 19), torch.float32)
+    _check_preference(got, x, want, x64)
+    got.loss.backward()
+    want[0].backward()
+    _close(x.grad, x64.grad, 4e-5, 4e-6)
+
+
+@pytest.mark.gpu
+def test_gradients_are_not_differentiated_again():
+    """Under create_graph the gradients are there; what differentiates them raises and says why."""
+    x = torch.randn(2, 3, 50, device="cuda", requires_grad=True)
+    y, zero = torch.zeros(2, 3, dtype=torch.long, device="cuda"), torch.zeros(2, device="cuda")
+    for loss in (lambda: ops.preference_loss(x, y, zero).loss, lambda: ops.policy_loss(x, y, zero + 1).loss,
+                 lambda: ops.router_balance_loss(x, 2).loss.sum()):
+        (want,) = torch.autograd.grad(loss(), x)
+        (grad,) = torch.autograd.grad(loss(), x, create_graph=True)
+        assert torch.equal(grad, want)
+        with pytest.raises(RuntimeError, match="cannot be differentiated"):
+            grad.sum().backward()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_balance_of_no_groups(dev):
+    for shape in [(0, 5, 4), (2, 0, 3, 4), (2, 3, 0, 4)]:
+        x = torch.zeros(shape, device=dev, requires_grad=True)
+        got = ops.router_balance_loss(x, 2, torch.zeros(*shape[:-1], 2, dtype=torch.long, device=dev),
+                                      torch.ones(shape[:-1], dtype=torch.bool, device=dev))
+        assert got.loss.shape == shape[:-2] and got.counts.shape == (*shape[:-2], 4) and not got.loss.any()
+        got.loss.sum().backward()
+        assert x.grad.shape == x.shape
+
+
 @pytest.mark.gpu
 def test_rows_beyond_32_bit_offsets():
     """The last rows of logits with more than 2^31 elements, and of rows far apart."""
