@@ -10,10 +10,22 @@
 //
 // A row whose label is ignored is not read: whatever stands there, its log-probability is 0
 // and its gradient is 0.
+//
+// What bounds them: memory. Figures are of 8 x 1024 x 128256 bf16 logits, a quarter of the rows ignored, on one B200
+// whose copy rate is 6.55 TB/s:
+//     statistics  read 1.58 GB            266 us   5.9 TB/s   (the exponential's unit is 75 % busy beside it)
+//     gradient    read 1.58, write 2.10   607 us   6.1 TB/s
+//     policy      the same bytes, once    679 us   5.4 TB/s   with its two small kernels
+// The preference loss needs both passes over HBM, since a pair's coefficient needs every token of both sequences. The
+// policy's does not, and takes them in one kernel.
+// Tried and slower for the policy: the row in registers over a cluster of CTAs, joined through distributed shared memory
+// (1020 us: a row's chain of load, barrier and store is too long for the few CTAs that fit); persistent CTAs with an
+// asynchronous ring across rows (843 us: too few warps for the arithmetic); the kept part refilled with the next row's head
+// during the second pass (767 us). A polynomial on the FMA pipe for a quarter of the exponentials costs more issue slots
+// than it frees (statistics 266 -> 288 us).
 #include "logit_loss.cuh"
 
 #include <cmath>
-#include <cstring>
 #include <cstring>
 
 #include "tc_common.cuh"
@@ -721,8 +733,14 @@ unsigned grid_of(const LogitRows& r) {
   return (unsigned)(((long long)r.B * r.T + Place<kGroup>::kRows - 1) / Place<kGroup>::kRows);
 }
 
-// The threads of a row by its vectors of 16 bytes; times of bf16 rows on one B200 (a quarter of them ignored):
-// 65536 rows of 1024 and 32768 of 4000 logits, 16384 of 16000, 8192 of 128256.
+// The threads of a row by its vectors of 16 bytes. Short rows want warps (no barrier, four to a CTA), long ones threads
+// enough for their loads; measured in us on one B200, bf16, a quarter of the rows ignored, by threads of a row:
+//     rows x logits       vectors   statistics             gradient               policy
+//     65536 x 1024            128   32: 57,  128: 124      32: 76,  128: 123      32: 101, 128: 235
+//     32768 x 4000            500   32: 70,  128: 83       32: 112, 128: 115      32: 136, 128: 178
+//     16384 x 16000          2000   32: 103, 128: 94       32: 191, 256: 175      32: 242, 128: 212, 256: 243
+//     1998 x 32003 (fp16)    4000   128: 46, 512: 49       256: 78, 512: 79       128: 92, 256: 86, long: 92
+//     8192 x 128256         16032   128: 266, 512: 280     256: 620, 512: 605     256: 842, long: 679
 constexpr int kShort = 768;
 
 template <typename T, int kGroup, int kMin>

@@ -4,7 +4,11 @@
 //     (y_i, y_{i+R/2}) -> (y_i cos - y_{i+R/2} sin, y_{i+R/2} cos + y_i sin)     i < R / 2
 // Backward, with dy the gradient rotated by the opposite angle:
 //     dw = sum over tokens and heads of dy n,    dx = r (w dy - n mean(w dy n)).
-// Arithmetic is fp32; the result is rounded once.
+// Arithmetic is fp32; the result is rounded once. r is computed again in the backward, which reads x anyway.
+//
+// 8 x 2048 tokens, 32 + 8 heads of 128, bf16, on one B200 (copy rate 6.55 TB/s): forward 63 us for 336 MB, backward 92 us
+// for 503 MB, 5.3 and 5.5 TB/s; both in one pass of a program 159 us with the sum of the weight gradients. What is left is
+// the latency of each step's chain (load, sum over the lanes, root, store) with the few warps that the registers allow.
 #include "qk_norm.cuh"
 
 #include "tc_common.cuh"
@@ -166,6 +170,7 @@ __device__ __forceinline__ float rsqrt_of(float v) {
   return r;
 }
 
+// A head of 128 takes 8 lanes with two 16-byte chunks each: half as wide chunks on 16 lanes took 1.4 times as long.
 // A warp's walk over one tensor: its tasks are (token, run of per_task heads), the steps of a task
 // 32 / 2^log heads each. Loading and computing walk the same steps, the loads kStages - 1 ahead.
 // The next task is a fixed number of tasks away: (batch, token, part) are carried along, not divided out.
@@ -208,7 +213,9 @@ struct Stride {
 };
 
 constexpr int kVecWarps = 4;
-constexpr int kStages = 4;  // steps in flight of each warp; a lane reads back only what it copied itself, so none waits for another
+// Steps of the ring, kStages - 1 of them on their way; a lane reads back only what it copied itself, so none waits for
+// another. The pass above with 2, 3 and 4 stages: 176, 159 and 170 us.
+constexpr int kStages = 3;
 
 // CTAs [0, q_blocks) walk q's tasks, the others k's.
 template <typename T, int VEC, int kLog>

@@ -4,6 +4,11 @@
 // P_e the mean of p_e:
 //     loss = E sum_e f_e P_e + z mean(lse^2)
 //     dx_ne = g [ E p_ne (f_e - sum_j f_j p_nj) + 2 z lse_n p_ne ] / N        (f is a constant)
+// p is computed again in the backward: writing it would cost as much as reading the logits.
+//
+// 16 groups of 65536 tokens, 64 experts, top 8, bf16, on one B200: forward 97 us + 8 us for the joining of the CTAs' sums,
+// backward 58 us (4.6 TB/s of its 268 MB). The forward reads 134 MB, 20 us at the copy rate: it is bound by the min / max
+// instructions of the selection (ALU 73 % busy). Where the choices are given it has none of them.
 #include "router_balance.cuh"
 
 #include <cmath>
@@ -26,6 +31,9 @@ __device__ __forceinline__ uint32_t order_key(float v) {
 // 2^log lanes share a token, lane l holds its experts 8 l .. 8 l + 7, and two tokens at once (A, B), whose logits of
 // one expert go through the selection side by side: in the halves of a word for 16-bit types. The K-th largest is found by
 // sorting each lane's 8 and merging sorted lists over the lanes; then each lane counts its own experts at or above it.
+// K rounds of "the largest that is left" took 5 times as long in the kernels below: each round waits for the lanes' maximum.
+// Sums and counts stay in registers until a CTA is done, and CTAs leave theirs in a row of a table that one more kernel
+// adds in order: no floating atomics, the same result each time.
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float ex2(float x) {
