@@ -25,7 +25,7 @@ struct BalanceArgs {
   int* part_count;      // (G, chunks, E + 1): choices, then tokens that count
   float* loss;          // (G)
   int64_t* counts;      // (G, E)
-  float* share;         // (G, E + 1): choices of each expert per token, then 1 / tokens
+  float* share;         // (G, E + 1): E times the choices of each expert per token, less K; then 1 / tokens
   int* err;
 };
 

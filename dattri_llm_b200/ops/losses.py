@@ -22,6 +22,8 @@ from typing import NamedTuple
 import torch
 import torch.nn.functional as F
 
+from dattri_llm_b200.ops import error_word, native, use_native
+
 PAIR_LOSSES = {"sigmoid": 0, "hinge": 1, "ipo": 2}
 _PAIR_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 _TOKEN_REDUCTIONS = {"token_mean": 0, "sequence_mean": 1, "sum": 2}
@@ -135,8 +137,6 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
         :class:`PreferenceLoss`.  A label outside the vocabulary is left out and reported by
         :func:`~dattri_llm_b200.ops.check_device_errors` (raised at once on CPU).
     """
-    from dattri_llm_b200.ops import error_word, native, use_native
-
     logits, labels = _check_logits(logits, labels)
     b = logits.shape[0]
     if b < 2 or b % 2:
@@ -212,8 +212,6 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, advantages: torch.Te
         :class:`PolicyLoss`.  A label outside the vocabulary is left out and reported by
         :func:`~dattri_llm_b200.ops.check_device_errors` (raised at once on CPU).
     """
-    from dattri_llm_b200.ops import error_word, native, use_native
-
     logits, labels = _check_logits(logits, labels)
     b, t = labels.shape
     if b == 0:
@@ -287,8 +285,6 @@ def router_balance_loss(logits: torch.Tensor, top_k: int, expert_ids: torch.Tens
         :class:`BalanceLoss`.  An expert id outside ``[0, E)`` is left out and reported by
         :func:`~dattri_llm_b200.ops.check_device_errors` (raised at once on CPU).
     """
-    from dattri_llm_b200.ops import error_word, native, use_native
-
     if logits.dim() < 2 or not logits.is_floating_point():
         raise ValueError(f"router logits must be floating (..., N, E), got {logits.dtype} {tuple(logits.shape)}")
     lead, (n, e) = logits.shape[:-2], logits.shape[-2:]

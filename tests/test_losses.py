@@ -541,6 +541,23 @@ def test_balance_masked_experts_and_no_tokens(dev):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("e,k", [(8, 8), (60, 60), (64, 1), (300, 3)])
+def test_balance_of_experts_used_alike(dev, e, k):
+    """The loss is top_k and there is nothing to push: the gradient keeps no rounding of the shares."""
+    n = 3 * e
+    x = _router((1, n, e, k), torch.float32, 0, dev)
+    ids = (torch.arange(n)[:, None] * k + torch.arange(k)).remainder(e).unsqueeze(0)  # each expert n k / e times
+    got = ops.router_balance_loss(x, k, ids.to(dev))
+    assert got.counts.unique().tolist() == [n * k // e]
+    _close(got.loss, torch.full((1,), float(k)), 2e-6, 0)
+    got.loss.sum().backward()
+    if dev == "cuda":
+        assert not x.grad.any()
+    else:  # the sums of the shares, each within 2^-22 of k, over the tokens
+        assert float(x.grad.abs().max()) <= 2e-6 * k / n
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 def test_balance_gradient_against_differences(dev):
     x = _router((1, 9, 10, 2), torch.float32, 3, dev)
     ids = torch.randint(0, 10, (1, 9, 2), generator=_gen(1))
