@@ -15,7 +15,7 @@
 // whose copy rate is 6.55 TB/s:
 //     statistics  read 1.58 GB            266 us   5.9 TB/s   (the exponential's unit is 75 % busy beside it)
 //     gradient    read 1.58, write 2.10   607 us   6.1 TB/s
-//     policy      the same bytes, once    679 us   5.4 TB/s   with its two small kernels
+//     policy      the same bytes, once    679 us   5.4 TB/s   with its two small kernels (699 us a pass with the backward's scaling)
 // The preference loss needs both passes over HBM, since a pair's coefficient needs every token of both sequences. The
 // policy's does not, and takes them in one kernel.
 // Tried and slower for the policy: the row in registers over a cluster of CTAs, joined through distributed shared memory

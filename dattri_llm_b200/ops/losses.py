@@ -196,6 +196,10 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, advantages: torch.Te
     ``r = exp(logp - old)`` and ``d = ref - logp``, each token that counts adds
     ``-min(r A, clamp(r, 1 - clip[0], 1 + clip[1]) A) + kl_coef (exp(d) - d - 1)``.
 
+    On the GPU the gradient is written along with the loss (memory of the logits' size from the
+    forward on, unless the logits need none) and scaled by the loss's own gradient in the
+    backward; a second backward through the graph computes it again.
+
     Args:
         logits: ``(B, T, V)``, any batch and token strides.
         labels: ``(B, T)``, the sampled token that ``logits[b, t]`` predicts or *ignore_index*.
