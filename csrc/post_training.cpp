@@ -12,6 +12,8 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
+#include <initializer_list>
 #include <optional>
 #include <string>
 #include <vector>
@@ -455,20 +457,19 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
 struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& labels, const Tensor& adv,
                                const OptTensor& old_logps, const OptTensor& ref_logps, double clip_lo, double clip_hi,
-                               double kl_coef, double temperature, int64_t mean, int64_t ignore, const Tensor& err,
-                               bool want_grad) {
+                               double kl_coef, double temperature, int64_t mean, int64_t ignore, const Tensor& err) {
     auto out = policy_fwd(logits, labels, adv, old_logps, ref_logps, clip_lo, clip_hi, kl_coef, temperature, mean,
-                          ignore, err, want_grad);
+                          ignore, err, true);
     ctx->set_materialize_grads(false);
     ctx->mark_non_differentiable({out[2], out[3]});
     ctx->save_for_backward({logits, labels, out[4], err});
     ctx->saved_data["ignore"] = ignore;
     ctx->saved_data["temperature"] = temperature;
-    if (out[5].defined()) ctx->saved_data["grad"] = out[5];
+    ctx->saved_data["grad"] = out[5];
     return {out[0], out[1], out[2], out[3]};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    variable_list out(13);
+    variable_list out(12);
     if (!g[0].defined() && !g[1].defined()) return out;
     const auto s = ctx->get_saved_variables();
     // The gradient written by the forward is given away once; another backward through the graph computes it again.
@@ -544,25 +545,155 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
   }
 };
 
-variable_list preference_loss(Tensor logits, Tensor labels, Tensor ref, int64_t kind, double beta, double smoothing,
-                              bool average, int64_t reduction, int64_t ignore, Tensor err) {
-  return PreferenceLoss::apply(logits, labels, ref, kind, beta, smoothing, average, reduction, ignore, err);
+// ---------------------------------------------------------------- entry points
+// The arguments are checked here and not in Python, where the checks took as long as the rest of a small call.
+
+// Without a gradient to come there is no node.
+bool wants_grad(const Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
+
+bool whole_numbers(const Tensor& t) { return at::isIntegralType(t.scalar_type(), false); }
+
+void take_logits(Tensor& logits, Tensor& labels) {
+  TORCH_CHECK_VALUE(logits.dim() == 3 && at::isFloatingType(logits.scalar_type()), "logits must be floating (B, T, V), got ",
+                    logits.scalar_type());
+  TORCH_CHECK_VALUE(labels.dim() == 2 && labels.size(0) == logits.size(0) && labels.size(1) == logits.size(1) &&
+                        whole_numbers(labels),
+                    "labels must be whole numbers (B, T), got ", labels.scalar_type());
+  TORCH_CHECK_VALUE(logits.size(2) > 0, "logits need a vocabulary of at least one entry");
+  TORCH_CHECK_VALUE(labels.device() == logits.device(), "labels are on ", labels.device(), ", logits on ", logits.device());
+  if (logits.stride(2) != 1) logits = logits.contiguous();
+  labels = labels.to(torch::kInt64).contiguous();
 }
 
-variable_list policy_loss(Tensor logits, Tensor labels, Tensor adv, OptTensor old_logps, OptTensor ref_logps,
-                          double clip_lo, double clip_hi, double kl_coef, double temperature, int64_t mean,
-                          int64_t ignore, Tensor err) {
-  const bool want_grad = logits.requires_grad() && at::GradMode::is_enabled();
-  return PolicyLoss::apply(logits, labels, adv, old_logps, ref_logps, clip_lo, clip_hi, kl_coef, temperature, mean,
-                           ignore, err, want_grad);
+Tensor constant(const Tensor& t, const char* name) {
+  TORCH_CHECK_VALUE(!t.requires_grad(), name, " is a constant of the loss: detach it");
+  return t.to(torch::kFloat32).contiguous();
+}
+
+// The place of `name` among the choices.
+int64_t choice(const std::string& name, const char* what, std::initializer_list<const char*> of) {
+  int64_t k = 0;
+  std::string all;
+  for (const char* o : of) {
+    if (name == o) return k;
+    all += (k++ ? ", '" : "'") + std::string(o) + "'";
+  }
+  TORCH_CHECK_VALUE(false, what, " must be one of ", all, ", got '", name, "'");
+}
+
+variable_list preference_loss(Tensor logits, Tensor labels, Tensor ref, const std::string& kind, double beta,
+                              double smoothing, bool average, const std::string& reduction, int64_t ignore, Tensor err) {
+  take_logits(logits, labels);
+  const int64_t B = logits.size(0);
+  TORCH_CHECK_VALUE(B >= 2 && B % 2 == 0, "a preference loss needs an even number of sequences (chosen, then rejected)");
+  const int64_t kind_at = choice(kind, "kind", {"sigmoid", "hinge", "ipo"});
+  const int64_t reduction_at = choice(reduction, "reduction", {"none", "mean", "sum"});
+  TORCH_CHECK_VALUE(beta > 0 && std::isfinite(beta), "beta must be positive");
+  TORCH_CHECK_VALUE(smoothing >= 0 && smoothing < 0.5 && (smoothing == 0 || kind_at == 0),
+                    "label_smoothing must be in [0, 0.5), and 0 unless kind is 'sigmoid'");
+  TORCH_CHECK_VALUE(ref.dim() == 1 && ref.size(0) == B, "ref_logps must have one entry for each sequence");
+  ref = constant(ref, "ref_logps");
+  if (!wants_grad(logits)) {
+    auto out = preference_fwd(logits, labels, ref, kind_at, beta, smoothing, average, reduction_at, ignore, err);
+    launches += 2;
+    return {out[0], out[1]};
+  }
+  return PreferenceLoss::apply(logits, labels, ref, kind_at, beta, smoothing, average, reduction_at, ignore, err);
+}
+
+variable_list policy_loss(Tensor logits, Tensor labels, Tensor adv, OptTensor old_logps, OptTensor ref_logps, double low,
+                          double high, double kl_coef, double temperature, const std::string& reduction, int64_t ignore,
+                          Tensor err) {
+  take_logits(logits, labels);
+  const int64_t B = logits.size(0), T = logits.size(1);
+  TORCH_CHECK_VALUE(B > 0, "a policy loss needs at least one sequence");
+  const auto per_token = [&](const Tensor& t) { return t.dim() == 2 && t.size(0) == B && t.size(1) == T; };
+  TORCH_CHECK_VALUE((adv.dim() == 1 && adv.size(0) == B) || per_token(adv), "advantages must be (B,) or (B, T)");
+  TORCH_CHECK_VALUE(!old_logps.has_value() || per_token(*old_logps), "old_logps must be (B, T)");
+  TORCH_CHECK_VALUE(!ref_logps.has_value() || per_token(*ref_logps), "ref_logps must be (B, T)");
+  const int64_t mean = choice(reduction, "reduction", {"token_mean", "sequence_mean", "sum"});
+  TORCH_CHECK_VALUE(temperature > 0 && std::isfinite(temperature), "temperature must be positive");
+  TORCH_CHECK_VALUE(low >= 0 && low <= 1 && high >= 0, "clip must be (low in [0, 1], high >= 0)");
+  TORCH_CHECK_VALUE(kl_coef == 0 || ref_logps.has_value(), "a KL term needs ref_logps");
+  adv = constant(adv, "advantages");
+  if (old_logps.has_value()) old_logps = constant(*old_logps, "old_logps");
+  if (ref_logps.has_value()) ref_logps = constant(*ref_logps, "ref_logps");
+  if (!wants_grad(logits)) {
+    auto out = policy_fwd(logits, labels, adv, old_logps, ref_logps, 1 - low, 1 + high, kl_coef, temperature, mean, ignore,
+                          err, false);
+    return {out[0], out[1], out[2], out[3]};
+  }
+  return PolicyLoss::apply(logits, labels, adv, old_logps, ref_logps, 1 - low, 1 + high, kl_coef, temperature, mean,
+                           ignore, err);
 }
 
 variable_list balance_loss(Tensor logits, OptTensor ids, OptTensor mask, int64_t top_k, double z_coef, Tensor err) {
-  return BalanceLoss::apply(logits, ids, mask, top_k, z_coef, err);
+  TORCH_CHECK_VALUE(logits.dim() >= 2 && at::isFloatingType(logits.scalar_type()),
+                    "router logits must be floating (..., N, E), got ", logits.scalar_type());
+  const auto lead = logits.sizes().slice(0, logits.dim() - 2).vec();
+  const int64_t N = logits.size(-2), E = logits.size(-1), G = c10::multiply_integers(lead);
+  TORCH_CHECK_VALUE(top_k >= 1 && top_k <= E, "top_k must be between 1 and the number of experts");
+  if (ids.has_value()) {
+    auto want = logits.sizes().vec();
+    want.back() = top_k;
+    TORCH_CHECK_VALUE(ids->sizes() == at::IntArrayRef(want) && whole_numbers(*ids),
+                      "expert_ids must be whole numbers (..., N, top_k), got ", ids->scalar_type());
+    ids = ids->to(torch::kInt64).contiguous();
+  }
+  if (mask.has_value()) {
+    TORCH_CHECK_VALUE(mask->sizes() == logits.sizes().slice(0, logits.dim() - 1), "mask must be (..., N)");
+    mask = (mask->scalar_type() == torch::kBool ? *mask : mask->ne(0)).contiguous();
+  }
+  if (lead.size() != 1) logits = logits.reshape({G, N, E});
+  if (logits.stride(2) != 1) logits = logits.contiguous();
+  variable_list out;
+  if (!wants_grad(logits)) {
+    out = balance_fwd(logits, ids, mask, top_k, z_coef, err);
+    launches += 2;
+    out.pop_back();
+  } else {
+    out = BalanceLoss::apply(logits, ids, mask, top_k, z_coef, err);
+  }
+  if (lead.size() != 1) {
+    auto cells = lead;
+    cells.push_back(E);
+    out = {out[0].reshape(lead), out[1].reshape(cells)};
+  }
+  return out;
 }
 
+// A call by a decoder's every layer and token: its arguments are checked here, not in Python.
 variable_list qk_norm_rope(Tensor q, Tensor k, Tensor qw, Tensor kw, Tensor cos, Tensor sin, OptTensor positions,
                            double eps, Tensor err) {
+  TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && q.size(0) == k.size(0) && q.size(1) == k.size(1) &&
+                        q.size(3) == k.size(3) && q.scalar_type() == k.scalar_type(),
+                    "q and k must be (B, T, H, D) of one type with the same B, T and D");
+  const int64_t B = q.size(0), T = q.size(1), D = q.size(3);
+  TORCH_CHECK_VALUE(qw.dim() == 1 && kw.dim() == 1 && qw.size(0) == D && kw.size(0) == D && qw.scalar_type() == kw.scalar_type(),
+                    "both weights must be (D,) of one type");
+  TORCH_CHECK_VALUE(cos.dim() == 2 && cos.sizes() == sin.sizes() && 2 * cos.size(1) <= D && D % 2 == 0,
+                    "cos and sin must be (positions, R / 2) with R at most D, and D even");
+  TORCH_CHECK_VALUE(!cos.requires_grad() && !sin.requires_grad(), "the tables of angles are constants: detach them");
+  if (positions.has_value()) {
+    const Tensor& p = *positions;
+    TORCH_CHECK_VALUE(((p.dim() == 1 && p.size(0) == T) || (p.dim() == 2 && p.size(0) == B && p.size(1) == T)) &&
+                          whole_numbers(p),
+                      "positions must be whole numbers (T,) or (B, T)");
+    positions = p.to(torch::kInt64);
+    if (positions->dim() == 1) positions = positions->expand({B, T});
+  } else {
+    TORCH_CHECK_VALUE(cos.size(0) >= T, "the tables of angles are shorter than the sequence");
+  }
+  if (q.stride(3) != 1) q = q.contiguous();
+  if (k.stride(3) != 1) k = k.contiguous();
+  qw = qw.contiguous();
+  kw = kw.contiguous();
+  cos = cos.to(torch::kFloat32).contiguous();
+  sin = sin.to(torch::kFloat32).contiguous();
+  if (!wants_grad(q) && !wants_grad(k) && !wants_grad(qw) && !wants_grad(kw)) {
+    ++launches;
+    return qk_norm_fwd(q, k, qw, kw, cos, sin, positions, eps, err);
+  }
   return QkNormRope::apply(q, k, qw, kw, cos, sin, positions, eps, err);
 }
 

@@ -159,19 +159,19 @@ def _v_mask_gather(args, kwargs):
 
 def _v_preference_loss(args, kwargs):
     # (logits, labels, ref, kind, beta, smoothing, average, reduction, ignore, err)
-    check_labels("preference_loss", args[1], int(args[0].shape[2]), int(args[8]))
+    check_labels("preference_loss", args[1], int(args[0].shape[-1]), int(args[8]))
 
 
 def _v_policy_loss(args, kwargs):
     # (logits, labels, adv, old, ref, lo, hi, kl_coef, temperature, reduction, ignore, err)
-    check_labels("policy_loss", args[1], int(args[0].shape[2]), int(args[10]))
+    check_labels("policy_loss", args[1], int(args[0].shape[-1]), int(args[10]))
 
 
 def _v_balance_loss(args, kwargs):
     # (logits, ids, mask, top_k, z_coef, err)
     if args[1] is not None:
         ids, mask = args[1].reshape(-1, int(args[3])), args[2]
-        check_expert_ids("balance_loss", ids if mask is None else ids[mask.reshape(-1)], int(args[0].shape[2]))
+        check_expert_ids("balance_loss", ids if mask is None else ids[mask.reshape(-1) != 0], int(args[0].shape[-1]))
 
 
 def _v_qk_norm_rope(args, kwargs):

@@ -10,6 +10,8 @@ from __future__ import annotations
 
 import torch
 
+from dattri_llm_b200.ops import error_word, native, use_native
+
 
 def enabled(x: torch.Tensor) -> bool:
     """Whether the fused kernels apply to *x*."""
@@ -367,6 +369,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     Returns:
         The new q and k, contiguous.  Gradients reach q, k and both weights.
     """
+    if use_native(q):
+        return tuple(native().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, error_word(q.device)))
     if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3] or q.dtype != k.dtype:
         raise ValueError(f"q and k must be (B, T, H, D) of one type with the same B, T and D, got {q.dtype} "
                          f"{tuple(q.shape)} and {k.dtype} {tuple(k.shape)}")
@@ -385,15 +389,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
         positions = positions.long().expand(b, t)
     elif cos.shape[0] < t:
         raise ValueError(f"the tables hold {cos.shape[0]} positions, the sequence has {t}")
-    from dattri_llm_b200.ops import error_word, native, use_native
-
-    if not use_native(q):
-        if positions is not None and bool(((positions < 0) | (positions >= cos.shape[0])).any()):
-            raise ValueError(f"positions must be in [0, {cos.shape[0]})")
-        cos, sin = (x[:t] if positions is None else x[positions] for x in (cos, sin))
-        cos, sin = cos.unsqueeze(-2), sin.unsqueeze(-2)
-        return (_qk_norm_rope_torch(q, q_weight, cos, sin, eps), _qk_norm_rope_torch(k, k_weight, cos, sin, eps))
-    q, k = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k))
-    cos, sin = (x.to(torch.float32).contiguous() for x in (cos, sin))
-    return tuple(native().qk_norm_rope(q, k, q_weight.contiguous(), k_weight.contiguous(), cos, sin, positions, eps,
-                                       error_word(q.device)))
+    if positions is not None and bool(((positions < 0) | (positions >= cos.shape[0])).any()):
+        raise ValueError(f"positions must be in [0, {cos.shape[0]})")
+    cos, sin = (x[:t] if positions is None else x[positions] for x in (cos, sin))
+    cos, sin = cos.unsqueeze(-2), sin.unsqueeze(-2)
+    return (_qk_norm_rope_torch(q, q_weight, cos, sin, eps), _qk_norm_rope_torch(k, k_weight, cos, sin, eps))

@@ -24,9 +24,7 @@ import torch.nn.functional as F
 
 from dattri_llm_b200.ops import error_word, native, use_native
 
-PAIR_LOSSES = {"sigmoid": 0, "hinge": 1, "ipo": 2}
-_PAIR_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
-_TOKEN_REDUCTIONS = {"token_mean": 0, "sequence_mean": 1, "sum": 2}
+PAIR_LOSSES = ("sigmoid", "hinge", "ipo")
 
 
 class PreferenceLoss(NamedTuple):
@@ -137,26 +135,25 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
         :class:`PreferenceLoss`.  A label outside the vocabulary is left out and reported by
         :func:`~dattri_llm_b200.ops.check_device_errors` (raised at once on CPU).
     """
+    if use_native(logits):
+        return PreferenceLoss(*native().preference_loss(logits, labels, ref_logps, kind, beta, label_smoothing, average_logps,
+                                                        reduction, ignore_index, error_word(logits.device)))
     logits, labels = _check_logits(logits, labels)
     b = logits.shape[0]
     if b < 2 or b % 2:
         raise ValueError(f"a preference loss needs an even number of sequences (chosen, then rejected), got {b}")
     if kind not in PAIR_LOSSES:
-        raise ValueError(f"kind must be one of {sorted(PAIR_LOSSES)}, got {kind!r}")
-    if reduction not in _PAIR_REDUCTIONS:
-        raise ValueError(f"reduction must be one of {sorted(_PAIR_REDUCTIONS)}, got {reduction!r}")
+        raise ValueError(f"kind must be one of {PAIR_LOSSES}, got {kind!r}")
+    if reduction not in ("none", "mean", "sum"):
+        raise ValueError(f"reduction must be 'none', 'mean' or 'sum', got {reduction!r}")
     if not (beta > 0 and math.isfinite(beta)):
         raise ValueError(f"beta must be positive, got {beta}")
     if not 0 <= label_smoothing < 0.5 or (label_smoothing and kind != "sigmoid"):
         raise ValueError(f"label_smoothing must be in [0, 0.5), and 0 unless kind is 'sigmoid', got {label_smoothing}")
     if ref_logps.shape != (b,):
         raise ValueError(f"ref_logps must be ({b},), got {tuple(ref_logps.shape)}")
-    if not use_native(logits):
-        ref = _constant("ref_logps", ref_logps).to(torch.promote_types(logits.dtype, torch.float32))
-        return _preference_torch(logits, labels, ref, kind, beta, label_smoothing, average_logps, reduction, ignore_index)
-    return PreferenceLoss(*native().preference_loss(
-        logits, labels, _constant("ref_logps", ref_logps), PAIR_LOSSES[kind], beta, label_smoothing, average_logps,
-        _PAIR_REDUCTIONS[reduction], ignore_index, error_word(logits.device)))
+    ref = _constant("ref_logps", ref_logps).to(torch.promote_types(logits.dtype, torch.float32))
+    return _preference_torch(logits, labels, ref, kind, beta, label_smoothing, average_logps, reduction, ignore_index)
 
 
 # ---------------------------------------------------------------- policy
@@ -216,6 +213,9 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, advantages: torch.Te
         :class:`PolicyLoss`.  A label outside the vocabulary is left out and reported by
         :func:`~dattri_llm_b200.ops.check_device_errors` (raised at once on CPU).
     """
+    if use_native(logits):
+        return PolicyLoss(*native().policy_loss(logits, labels, advantages, old_logps, ref_logps, clip[0], clip[1], kl_coef,
+                                                temperature, reduction, ignore_index, error_word(logits.device)))
     logits, labels = _check_logits(logits, labels)
     b, t = labels.shape
     if b == 0:
@@ -225,8 +225,8 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, advantages: torch.Te
     for name, x in (("old_logps", old_logps), ("ref_logps", ref_logps)):
         if x is not None and x.shape != (b, t):
             raise ValueError(f"{name} must be ({b}, {t}), got {tuple(x.shape)}")
-    if reduction not in _TOKEN_REDUCTIONS:
-        raise ValueError(f"reduction must be one of {sorted(_TOKEN_REDUCTIONS)}, got {reduction!r}")
+    if reduction not in ("token_mean", "sequence_mean", "sum"):
+        raise ValueError(f"reduction must be 'token_mean', 'sequence_mean' or 'sum', got {reduction!r}")
     if not (temperature > 0 and math.isfinite(temperature)):
         raise ValueError(f"temperature must be positive, got {temperature}")
     if not (0 <= clip[0] <= 1 and clip[1] >= 0):
@@ -236,12 +236,9 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, advantages: torch.Te
     lo, hi = 1.0 - clip[0], 1.0 + clip[1]
     consts = tuple(_constant(n, x) for n, x in (("advantages", advantages), ("old_logps", old_logps),
                                                  ("ref_logps", ref_logps)))
-    if not use_native(logits):
-        wide = torch.promote_types(logits.dtype, torch.float32)
-        consts = tuple(None if x is None else x.to(wide) for x in consts)
-        return _policy_torch(logits, labels, *consts, lo, hi, kl_coef, temperature, reduction, ignore_index)
-    return PolicyLoss(*native().policy_loss(logits, labels, *consts, lo, hi, kl_coef, temperature,
-                                            _TOKEN_REDUCTIONS[reduction], ignore_index, error_word(logits.device)))
+    wide = torch.promote_types(logits.dtype, torch.float32)
+    consts = tuple(None if x is None else x.to(wide) for x in consts)
+    return _policy_torch(logits, labels, *consts, lo, hi, kl_coef, temperature, reduction, ignore_index)
 
 
 # ---------------------------------------------------------------- router balance
@@ -289,6 +286,8 @@ def router_balance_loss(logits: torch.Tensor, top_k: int, expert_ids: torch.Tens
         :class:`BalanceLoss`.  An expert id outside ``[0, E)`` is left out and reported by
         :func:`~dattri_llm_b200.ops.check_device_errors` (raised at once on CPU).
     """
+    if use_native(logits):
+        return BalanceLoss(*native().balance_loss(logits, expert_ids, mask, top_k, z_coef, error_word(logits.device)))
     if logits.dim() < 2 or not logits.is_floating_point():
         raise ValueError(f"router logits must be floating (..., N, E), got {logits.dtype} {tuple(logits.shape)}")
     lead, (n, e) = logits.shape[:-2], logits.shape[-2:]
@@ -303,14 +302,7 @@ def router_balance_loss(logits: torch.Tensor, top_k: int, expert_ids: torch.Tens
         if mask.shape != (*lead, n):
             raise ValueError(f"mask must be {(*lead, n)}, got {tuple(mask.shape)}")
         mask = (mask if mask.dtype == torch.bool else mask != 0).contiguous()
-    x = logits if len(lead) == 1 else logits.reshape(math.prod(lead), n, e) if lead else logits.unsqueeze(0)
-    if x.stride(2) != 1:
-        x = x.contiguous()
-    if use_native(x):
-        loss, counts = native().balance_loss(x, expert_ids, mask, top_k, z_coef, error_word(x.device))
-    else:
-        loss, counts = _balance_torch(x, None if expert_ids is None else expert_ids.view(*x.shape[:2], top_k),
-                                      None if mask is None else mask.view(x.shape[:2]), top_k, z_coef)
-    if len(lead) == 1:
-        return BalanceLoss(loss, counts)
+    x = logits.reshape(math.prod(lead), n, e)
+    loss, counts = _balance_torch(x, None if expert_ids is None else expert_ids.view(*x.shape[:2], top_k),
+                                  None if mask is None else mask.view(x.shape[:2]), top_k, z_coef)
     return BalanceLoss(loss.reshape(lead), counts.reshape(*lead, e))

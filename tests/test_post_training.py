@@ -169,6 +169,30 @@ def test_launch_checks_of_labels_ids_and_positions():
         v["qk_norm_rope"]((None, None, None, None, torch.zeros(4, 2), None, torch.tensor([[0, 4]]), 1e-6, None), {})
 
 
+@pytest.mark.gpu
+def test_operators_under_launch_checks():
+    """With checks on, good arguments pass and the first bad index is named before anything is launched."""
+    x = torch.randn(2, 3, 5, device="cuda", requires_grad=True)
+    y, zero = torch.tensor([[0, 4, -100], [1, 2, 3]], device="cuda"), torch.zeros(2, device="cuda")
+    q, w = torch.randn(2, 3, 1, 8, device="cuda"), torch.ones(8, device="cuda")
+    tables = torch.zeros(3, 4, device="cuda"), torch.ones(3, 4, device="cuda")
+    checks.set_checks(True)
+    try:
+        for bad in (False, True):
+            off = 5 if bad else 0
+            for call in (lambda: ops.preference_loss(x, y + off, zero), lambda: ops.policy_loss(x, y + off, zero),
+                         lambda: ops.router_balance_loss(x[0], 2, torch.full((3, 2), 1 + off, device="cuda")),
+                         lambda: ops.qk_norm_rope(q, q, w, w, *tables, torch.tensor([0, 1, 2 + off], device="cuda"))):
+                if bad:
+                    with pytest.raises(checks.LaunchCheckError):
+                        call()
+                else:
+                    call()
+        ops.check_device_errors()
+    finally:
+        checks.set_checks(False)
+
+
 @pytest.mark.parametrize("dev", DEVICES)
 def test_example_runs(dev):
     env = dict(os.environ, MASTER_PORT="29517")
