@@ -15,13 +15,14 @@
 // whose copy rate is 6.55 TB/s:
 //     statistics  read 1.58 GB            266 us   5.9 TB/s   (the exponential's unit is 75 % busy beside it)
 //     gradient    read 1.58, write 2.10   607 us   6.1 TB/s
-//     policy      the same bytes, once    679 us   5.4 TB/s   with its two small kernels (699 us a pass with the backward's scaling)
+//     policy      the same bytes, once    658 us   5.6 TB/s   with its two small kernels (686 us each of many passes, which
+//                                                             wait for one another's writes, with the backward's scaling)
 // The preference loss needs both passes over HBM, since a pair's coefficient needs every token of both sequences. The
 // policy's does not, and takes them in one kernel.
 // Tried and slower for the policy: the row in registers over a cluster of CTAs, joined through distributed shared memory
 // (1020 us: a row's chain of load, barrier and store is too long for the few CTAs that fit); persistent CTAs with an
-// asynchronous ring across rows (843 us: too few warps for the arithmetic); the kept part refilled with the next row's head
-// during the second pass (767 us). A polynomial on the FMA pipe for a quarter of the exponentials costs more issue slots
+// asynchronous ring across rows (843 us: too few warps for the arithmetic); persistent CTAs that refill the kept part with
+// the next row's head during the second pass (767 us). A polynomial on the FMA pipe for a quarter of the exponentials costs more issue slots
 // than it frees (statistics 266 -> 288 us).
 #include "logit_loss.cuh"
 
@@ -646,9 +647,28 @@ __global__ void __launch_bounds__(Place<kGroup>::kThreads, kMin) policy_row_kern
     row_grad<T, kGroup>(span, out, row_grad_of(span, out, y, base_of(m), 1.f / s, c, coef));
 }
 
-// Long rows, two CTAs of an SM: the first kKept vectors wait in shared memory for the second pass, where the thread that read
-// them finds them again, and only the rest is read again from L2. A step's loads are issued before the step in front is used.
+// Long rows, two CTAs of an SM: the first kKept vectors are all asked for at once, into shared memory, and stay there for the
+// second pass, which asks for the rest again (from L2) three steps ahead as places come free. A thread only reads the places
+// it filled itself.
 constexpr int kLongThreads = 512, kLongHold = kLongThreads * kUnroll, kKept = 3 * kLongHold;
+
+// The step of vectors from j0 on, on its way to the places of this thread from `to` on; nothing where the row has ended.
+template <typename T>
+__device__ __forceinline__ void keep_step(uint4* to, const RowSpan<T>& span, int j0) {
+  const int j = j0 + (int)threadIdx.x;
+  to += threadIdx.x;
+  if (span.inner(j0, kLongHold)) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to + u * kLongThreads)),
+                   "l"(span.vec(j + u * kLongThreads))
+                   : "memory");
+  } else if (j0 < span.nv) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) to[u * kLongThreads] = span.template load<false>(j + u * kLongThreads);
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kLongThreads, 2) policy_long_kernel(PolicyArgs a) {
@@ -664,22 +684,30 @@ __global__ void __launch_bounds__(kLongThreads, 2) policy_long_kernel(PolicyArgs
   }
   const T* x = row_ptr<T>(r, row);
   const RowSpan<T> span(x, r.V);
+  for (int j0 = 0; j0 < kKept; j0 += kLongHold) keep_step<T>(keep + j0, span, j0);
   const float c = kLog2e * r.inv_temp, xy = ElemOf<T>::up(x[y]), w = token_weight(a, b);
   const TokenIn in = token_in(a, row, b);
   uint4 v[kUnroll], ahead[kUnroll];
   const auto load = [&](int j0) {
     fetch<T, kLongThreads, false>(span, j0 + tid, span.inner(j0, kLongHold), ahead);
   };
-  load(0);
+  load(kKept);
   float m = -INFINITY, s = 0.f;
-  for (int j0 = 0; j0 < span.nv; j0 += kLongHold) {
+  const auto kept = [&](int j0) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) v[u] = keep[j0 + u * kLongThreads + tid];
+    take<T>(v, c, m, s);
+  };
+  asm volatile("cp.async.wait_group 2;" ::: "memory");
+  kept(0);
+  asm volatile("cp.async.wait_group 1;" ::: "memory");
+  kept(kLongHold);
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  kept(2 * kLongHold);
+  for (int j0 = kKept; j0 < span.nv; j0 += kLongHold) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) v[u] = ahead[u];
     if (j0 + kLongHold < span.nv) load(j0 + kLongHold);
-    if (j0 < kKept) {
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) keep[j0 + u * kLongThreads + tid] = v[u];
-    }
     take<T>(v, c, m, s);
   }
   merge_group<kLongThreads>(m, s, c, parts);
@@ -689,20 +717,13 @@ __global__ void __launch_bounds__(kLongThreads, 2) policy_long_kernel(PolicyArgs
     return;
   }
   const RowGrad g = row_grad_of(span, out, y, base_of(m), 1.f / s, c, coef);
-  const auto again = [&](int j0) {
-    if (j0 < kKept) {
+  for (int j0 = 0, at = 0; j0 < span.nv; j0 += kLongHold) {
+    asm volatile("cp.async.wait_group 2;" ::: "memory");
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) ahead[u] = keep[j0 + u * kLongThreads + tid];
-    } else {
-      fetch<T, kLongThreads, true>(span, j0 + tid, span.inner(j0, kLongHold), ahead);
-    }
-  };
-  again(0);
-  for (int j0 = 0; j0 < span.nv; j0 += kLongHold) {
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) v[u] = ahead[u];
-    if (j0 + kLongHold < span.nv) again(j0 + kLongHold);
+    for (int u = 0; u < kUnroll; ++u) v[u] = keep[at + u * kLongThreads + tid];
     put<T, kLongThreads>(span, out, j0 + tid, span.inner(j0, kLongHold), v, g);
+    keep_step<T>(keep + at, span, j0 + kKept);
+    at = at == kKept - kLongHold ? 0 : at + kLongHold;
   }
 }
 
@@ -740,7 +761,7 @@ unsigned grid_of(const LogitRows& r) {
 //     32768 x 4000            500   32: 70,  128: 83       32: 112, 128: 115      32: 136, 128: 178
 //     16384 x 16000          2000   32: 103, 128: 94       32: 191, 256: 175      32: 242, 128: 212, 256: 243
 //     1998 x 32003 (fp16)    4000   128: 46, 512: 49       256: 78, 512: 79       128: 92, 256: 86, long: 92
-//     8192 x 128256         16032   128: 266, 512: 280     256: 620, 512: 605     256: 842, long: 679
+//     8192 x 128256         16032   128: 266, 512: 280     256: 620, 512: 605     256: 842, long: 658
 constexpr int kShort = 768;
 
 template <typename T, int kGroup, int kMin>

@@ -3,7 +3,8 @@
 //
 // Their autograd functions are C++: a backward node written in Python takes the interpreter
 // lock from the engine's thread, which cost more than the kernels of a small call (forward and
-// backward of 96 logit rows on one B200: 111 us with Python nodes, 87 us with these, of which 48 us are the engine's).
+// backward of 96 logit rows on one B200: 111 us with Python nodes and checks, 87 us with these nodes, 70 us with the checks
+// here too; 45 us of it are the engine's).
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
