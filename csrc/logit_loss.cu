@@ -277,9 +277,8 @@ __device__ __forceinline__ void row_stats(const RowSpan<T>& span, float c, float
 }
 
 template <typename T, int kGroup>
-__global__ void __launch_bounds__(Place<kGroup>::kThreads, kGroup == 32 ? 10 : 12) row_stats_kernel(LogitRows r, float* __restrict__ logps,
-                                                                            RowStat* __restrict__ stats,
-                                                                            unsigned* __restrict__ ticket) {
+__global__ void __launch_bounds__(Place<kGroup>::kThreads, kGroup == 32 ? 10 : 12)
+    row_stats_kernel(LogitRows r, float* __restrict__ logps, RowStat* __restrict__ stats, unsigned* __restrict__ ticket) {
   __shared__ float2 parts[32];
   const long long row = Place<kGroup>::row();
   const int tid = Place<kGroup>::tid();
@@ -311,13 +310,14 @@ __device__ __forceinline__ void zero_row(T* out, int V) {
   for (int j = Place<kGroup>::tid(); j < span.nv; j += kGroup) store_vec<T>(out, V, span.first(j), make_uint4(0, 0, 0, 0), true);
 }
 
-// Writes coef (onehot - softmax) of kUnroll vectors. What a gradient needs of its row:
+// What the gradient of a row is made of.
 struct RowGrad {
   int y;
   float base, c, k, coef;  // k = -coef / s
   bool aligned;            // the gradient's row starts at the same place within 16 bytes
 };
 
+// Writes coef (onehot - softmax) of kUnroll vectors.
 template <typename T, int kStride>
 __device__ __forceinline__ void put(const RowSpan<T>& span, T* out, int j, bool whole, const uint4 (&v)[kUnroll],
                                     const RowGrad& g) {
@@ -495,8 +495,10 @@ __device__ __forceinline__ TokenTerms policy_token(const PolicyArgs& a, const To
   if (a.ref_logps != nullptr) {
     const float d = in.ref_logp - logp;
     t.kl = exp_excess(d);
-    t.loss += a.kl_coef * t.kl;
-    t.slope -= a.kl_coef * expm1f(d);
+    if (a.kl_coef != 0.f) {  // an infinite distance that is only reported leaves the loss alone
+      t.loss += a.kl_coef * t.kl;
+      t.slope -= a.kl_coef * expm1f(d);
+    }
   }
   return t;
 }

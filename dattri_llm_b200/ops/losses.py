@@ -170,7 +170,8 @@ def _policy_torch(logits, labels, adv, old, ref, lo, hi, kl_coef, temperature, r
     if ref is not None:
         d = (ref - logps).masked_fill(~valid, 0.0)
         kl = torch.expm1(d) - d
-        loss = loss + kl_coef * kl
+        if kl_coef:  # an infinite distance that is only reported leaves the loss alone
+            loss = loss + kl_coef * kl
     loss = loss.masked_fill(~valid, 0.0)
     n = valid.sum().clamp(min=1)
     if reduction == "token_mean":

@@ -420,6 +420,19 @@ def test_policy_small_kl_keeps_its_digits(dev):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+def test_policy_reports_an_infinite_distance_without_using_it(dev):
+    x = torch.randn(2, 3, 11, generator=_gen(0)).to(dev).requires_grad_()
+    y, adv = torch.zeros(2, 3, dtype=torch.long, device=dev), torch.ones(2, device=dev)
+    ref = torch.full((2, 3), -math.inf, device=dev)
+    got, want = ops.policy_loss(x, y, adv, ref_logps=ref), ops.policy_loss(x, y, adv)
+    assert float(got.kl) == math.inf and torch.equal(got.loss, want.loss)
+    assert torch.equal(torch.autograd.grad(got.loss, x)[0], torch.autograd.grad(want.loss, x)[0])
+    empty = ops.policy_loss(x[:, :0], y[:, :0], adv)
+    (grad,) = torch.autograd.grad(empty.loss, x)
+    assert float(empty.loss) == 0 and empty.logps.shape == (2, 0) and not grad.any()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 def test_policy_gradient_against_differences(dev):
     kw = dict(kl_coef=0.2, clip=(0.3, 0.3), temperature=0.9)
     got, x, _, x64, labels = _policy(dev, (2, 4, 23), torch.float32, has_ref=True, **kw)
