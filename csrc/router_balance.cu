@@ -234,9 +234,13 @@ __device__ __forceinline__ float exps(float (&f)[8], float m) {
   return group_sum<kLanes>(s.x + s.y);
 }
 
+// CTAs of an SM: both tokens' fp32 lists need the registers of two (three of them spill).
+template <typename T, int kTop>
+constexpr int kSelectCtas = sizeof(T) == 4 && kTop > 0 ? 2 : 3;
+
 // kTop: the length of the sorted lists, at least the number of choices; 0: the choices are given.
 template <typename T, int kTop, int kLog>
-__global__ void __launch_bounds__(kWarps * 32, 3) balance_fwd8_kernel(BalanceArgs a, int vec) {
+__global__ void __launch_bounds__(kWarps * 32, kSelectCtas<T, kTop>) balance_fwd8_kernel(BalanceArgs a, int vec) {
   __shared__ float sum_p[257];
   __shared__ int hist[257];
   const int g = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -766,7 +770,8 @@ void bwd_of(const BalanceGradArgs& b, cudaStream_t s) {
 
 int balance_chunks(const BalanceArgs& a) {
   const int log = a.E <= 256 ? log_of(a.E) : 5;
-  return chunks_of(a, 3, a.E <= 256 ? kWarps * 2 * (32 >> log) : kWarps);
+  const int per_sm = a.type == Elem::kF32 && a.ids == nullptr ? kSelectCtas<float, 8> : kSelectCtas<__half, 8>;
+  return chunks_of(a, per_sm, a.E <= 256 ? kWarps * 2 * (32 >> log) : kWarps);
 }
 
 void balance_fwd(const BalanceArgs& a, cudaStream_t s) {
