@@ -16,7 +16,7 @@
 //     statistics  read 1.58 GB            266 us   5.9 TB/s   (the exponential's unit is 75 % busy beside it)
 //     gradient    read 1.58, write 2.10   607 us   6.1 TB/s
 //     policy      the same bytes, once    658 us   5.6 TB/s   with its two small kernels (686 us each of many passes, which
-//                                                             wait for one another's writes, with the backward's scaling)
+//                                                             wait for one another's writes, with the backward's launch)
 // The preference loss needs both passes over HBM, since a pair's coefficient needs every token of both sequences. The
 // policy's does not, and takes them in one kernel.
 // Tried and slower for the policy: the row in registers over a cluster of CTAs, joined through distributed shared memory
@@ -357,15 +357,14 @@ __device__ __forceinline__ void row_grad(const RowSpan<T>& span, T* out, const R
   }
 }
 
-// coef (onehot - softmax) / temperature of every row. A zero coefficient (an ignored row, a clipped token)
-// writes zeros without reading the row. Rows run backwards: the last ones read before are the likeliest still in L2.
+// coef (onehot - softmax) / temperature of a row. A zero coefficient (an ignored row, a clipped token)
+// writes zeros without reading the row.
 template <typename T, int kGroup>
-__global__ void __launch_bounds__(Place<kGroup>::kThreads) logit_grad_kernel(LogitGradArgs a) {
+__device__ __forceinline__ void logit_grad_row(const LogitGradArgs& a, long long row) {
   const LogitRows& r = a.rows;
-  const long long row = (long long)r.B * r.T - 1 - Place<kGroup>::row();
-  if (row < 0) return;
   const long long b = row / r.T, t = row - b * r.T;
   const int y = row_label(r, row);
+  if (y < 0 && a.unit_grad) return;
   T* out = reinterpret_cast<T*>(a.out) + b * a.osb + t * a.ost;
   float coef = 0.f;
   if (y >= 0) {
@@ -382,6 +381,24 @@ __global__ void __launch_bounds__(Place<kGroup>::kThreads) logit_grad_kernel(Log
   const RowStat st = a.stats[row];
   const RowSpan<T> span(row_ptr<T>(r, row), r.V);
   row_grad<T, kGroup>(span, out, row_grad_of(span, out, y, st.m, st.inv_s, kLog2e * r.inv_temp, coef));
+}
+
+// Every row. They run backwards: the last ones read before are the likeliest still in L2.
+template <typename T, int kGroup>
+__global__ void __launch_bounds__(Place<kGroup>::kThreads) logit_grad_kernel(LogitGradArgs a) {
+  const long long row = (long long)a.rows.B * a.rows.T - 1 - Place<kGroup>::row();
+  if (row >= 0) logit_grad_row<T, kGroup>(a, row);
+}
+
+// Where `out` has the gradient for a loss gradient of 1 (a loss that ends the graph) it is done. For any other the rows
+// are computed again from the logits: the numbers in `out` are rounded, and what a scaled loss keeps within the range of
+// a 16-bit float is gone from them. As many CTAs as are resident, so that they leave at once where there is nothing to do.
+template <typename T, int kGroup>
+__global__ void __launch_bounds__(Place<kGroup>::kThreads) logit_regrad_kernel(LogitGradArgs a) {
+  if (*a.g_loss == 1.f) return;
+  const long long by = (long long)gridDim.x * Place<kGroup>::kRows;
+  for (long long row = (long long)a.rows.B * a.rows.T - 1 - Place<kGroup>::row(); row >= 0; row -= by)
+    logit_grad_row<T, kGroup>(a, row);
 }
 
 // ---------------------------------------------------------------- sums over tokens
@@ -729,28 +746,6 @@ __global__ void __launch_bounds__(kLongThreads, 2) policy_long_kernel(PolicyArgs
   }
 }
 
-// grad *= g unless g is 1, which is what a loss that ends the graph sends.
-template <typename T>
-__global__ void __launch_bounds__(512) logit_scale_kernel(LogitRows r, T* grad, long long sb, long long st,
-                                                          const float* __restrict__ g) {
-  constexpr int N = kVecOf<T>;
-  const float by = *g;
-  if (by == 1.f) return;
-  const long long rows = (long long)r.B * r.T;
-  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
-    const long long b = row / r.T;
-    T* out = grad + b * sb + (row - b * r.T) * st;
-    const RowSpan<T> span(out, r.V);
-    for (int j = threadIdx.x; j < span.nv; j += blockDim.x) {
-      float f[N];
-      raw_up<T>(span.template load<true>(j), f);
-#pragma unroll
-      for (int i = 0; i < N; ++i) f[i] *= by;
-      store_vec<T>(out, r.V, span.first(j), raw_down<T, uint4>(f), true);
-    }
-  }
-}
-
 template <int kGroup>
 unsigned grid_of(const LogitRows& r) {
   return (unsigned)(((long long)r.B * r.T + Place<kGroup>::kRows - 1) / Place<kGroup>::kRows);
@@ -790,15 +785,22 @@ void launch_stats(const LogitRows& r, float* logps, RowStat* stats, unsigned* ti
     row_stats_kernel<T, 128><<<grid_of<128>(r), 128, 0, s>>>(r, logps, stats, ticket);
 }
 
+template <typename T, int kGroup>
+void launch_grad_rows(const LogitGradArgs& a, cudaStream_t s) {
+  constexpr int kThreads = Place<kGroup>::kThreads;
+  const unsigned all = grid_of<kGroup>(a.rows), resident = 148 * 2048 / kThreads;
+  if (a.unit_grad)
+    logit_regrad_kernel<T, kGroup><<<all < resident ? all : resident, kThreads, 0, s>>>(a);
+  else
+    logit_grad_kernel<T, kGroup><<<all, kThreads, 0, s>>>(a);
+}
+
 template <typename T>
 void launch_grad(const LogitGradArgs& a, cudaStream_t s) {
   const int n = a.rows.V / kVecOf<T>;
-  if (n <= kShort)
-    logit_grad_kernel<T, 32><<<grid_of<32>(a.rows), Place<32>::kThreads, 0, s>>>(a);
-  else if (n <= 8192)
-    logit_grad_kernel<T, 256><<<grid_of<256>(a.rows), 256, 0, s>>>(a);
-  else
-    logit_grad_kernel<T, 512><<<grid_of<512>(a.rows), 512, 0, s>>>(a);
+  if (n <= kShort) return launch_grad_rows<T, 32>(a, s);
+  if (n <= 8192) return launch_grad_rows<T, 256>(a, s);
+  launch_grad_rows<T, 512>(a, s);
 }
 
 void stats_of(const LogitRows& r, float* logps, RowStat* stats, unsigned* ticket, cudaStream_t s) {
@@ -835,18 +837,6 @@ int policy_fwd(const PolicyArgs& a, cudaStream_t s) {
     rows_of<float>(a, s);
   policy_finish_kernel<<<a.rows.B, 256, 0, s>>>(a);
   return (a.grad == nullptr ? 4 : 3) + many;
-}
-
-void logit_scale(const LogitRows& r, void* grad, long long sb, long long st, const float* g, cudaStream_t s) {
-  const long long rows = (long long)r.B * r.T;
-  if (rows == 0) return;
-  const unsigned grid = (unsigned)(rows < 148 * 4 ? rows : 148 * 4);
-  if (r.type == Elem::kBF16)
-    logit_scale_kernel<<<grid, 512, 0, s>>>(r, reinterpret_cast<__nv_bfloat16*>(grad), sb, st, g);
-  else if (r.type == Elem::kF16)
-    logit_scale_kernel<<<grid, 512, 0, s>>>(r, reinterpret_cast<__half*>(grad), sb, st, g);
-  else
-    logit_scale_kernel<<<grid, 512, 0, s>>>(r, reinterpret_cast<float*>(grad), sb, st, g);
 }
 
 void logit_grad(const LogitGradArgs& a, cudaStream_t s) {

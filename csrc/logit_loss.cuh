@@ -77,13 +77,14 @@ struct LogitGradArgs {
   bool per_row;
   void* out;
   long long osb, ost;
+  // `out` has the gradient for g_loss = 1 already, with zeros in the rows that do not count: g_loss is one number, and
+  // there is no g_logps.
+  bool unit_grad;
 };
 
 void preference_fwd(const PreferenceArgs& a, cudaStream_t s);
 // Returns the kernels launched.
 int policy_fwd(const PolicyArgs& a, cudaStream_t s);
-// grad *= *g, unless *g is 1; rows as in `rows`.
-void logit_scale(const LogitRows& rows, void* grad, long long sb, long long st, const float* g, cudaStream_t s);
 void logit_grad(const LogitGradArgs& a, cudaStream_t s);
 
 }  // namespace bw

@@ -163,6 +163,7 @@ Tensor preference_bwd(const Tensor& logits, const Tensor& labels, const Tensor& 
   a.g_loss_mod = g_loss.has_value() && g_loss->dim() > 0 ? (int)(B / 2) : 0;
   a.g_logps = floats(g_logps);
   a.per_row = false;
+  a.unit_grad = false;
   a.out = out.data_ptr();
   a.osb = out.stride(0);
   a.ost = out.stride(1);
@@ -226,8 +227,9 @@ variable_list policy_fwd(const Tensor& logits, const Tensor& labels, const Tenso
   return {loss, logps, kl, clipped, ws, grad};
 }
 
+// unit_grad: the gradient for a loss gradient of 1, which is given out where that is what the loss has; undefined: none.
 Tensor policy_bwd(const Tensor& logits, const Tensor& labels, const Tensor& ws, const OptTensor& g_loss,
-                  const OptTensor& g_logps, double temperature, int64_t ignore, const Tensor& err) {
+                  const OptTensor& g_logps, double temperature, int64_t ignore, const Tensor& err, Tensor unit_grad) {
   const c10::cuda::CUDAGuard guard(logits.device());
   bw::LogitGradArgs a;
   a.rows = logit_rows(logits, labels, ignore, temperature, err);
@@ -242,7 +244,8 @@ Tensor policy_bwd(const Tensor& logits, const Tensor& labels, const Tensor& ws, 
     check_like(*g_logps, "logps gradient", torch::kFloat32, logits);
     TORCH_CHECK(g_logps->numel() == R, "logps gradient must be (B, T)");
   }
-  auto out = grad_like(logits);
+  a.unit_grad = unit_grad.defined() && g_loss.has_value() && !g_logps.has_value();
+  auto out = a.unit_grad ? std::move(unit_grad) : grad_like(logits);
   const float* w = ws.data_ptr<float>();
   a.stats = reinterpret_cast<const bw::RowStat*>(w);
   a.d = w + 2 * R;
@@ -474,24 +477,14 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     if (!g[0].defined() && !g[1].defined()) return out;
     const auto s = ctx->get_saved_variables();
     // The gradient written by the forward is given away once; another backward through the graph computes it again.
+    Tensor unit_grad;
     const auto kept = ctx->saved_data.find("grad");
     if (kept != ctx->saved_data.end()) {
-      Tensor grad = kept->second.toTensor();
+      unit_grad = kept->second.toTensor();
       ctx->saved_data.erase(kept);
-      if (!g[1].defined()) {
-        const c10::cuda::CUDAGuard guard(grad.device());
-        const auto by = *dense(g[0]);
-        check_like(by, "loss gradient", torch::kFloat32, grad);
-        bw::logit_scale(logit_rows(s[0], s[1], 0, 1.0, s[3]), grad.data_ptr(), grad.stride(0), grad.stride(1),
-                        by.data_ptr<float>(), at::cuda::getCurrentCUDAStream());
-        C10_CUDA_KERNEL_LAUNCH_CHECK();
-        ++launches;
-        out[0] = std::move(grad);
-        return once(std::move(out), "policy_loss");
-      }
     }
     out[0] = policy_bwd(s[0], s[1], s[2], dense(g[0]), dense(g[1]), ctx->saved_data["temperature"].toDouble(),
-                        ctx->saved_data["ignore"].toInt(), s[3]);
+                        ctx->saved_data["ignore"].toInt(), s[3], std::move(unit_grad));
     ++launches;
     return once(std::move(out), "policy_loss");
   }

@@ -195,8 +195,9 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, advantages: torch.Te
     ``-min(r A, clamp(r, 1 - clip[0], 1 + clip[1]) A) + kl_coef (exp(d) - d - 1)``.
 
     On the GPU the gradient is written along with the loss (memory of the logits' size from the
-    forward on, unless the logits need none) and scaled by the loss's own gradient in the
-    backward; a second backward through the graph computes it again.
+    forward on, unless the logits need none) and given out where the loss ends the graph; under
+    any other loss gradient (a scaled loss, accumulation) and in a second backward the backward
+    computes it from the logits, in 32 bits and rounded once.
 
     Args:
         logits: ``(B, T, V)``, any batch and token strides.

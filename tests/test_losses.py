@@ -771,3 +771,84 @@ def test_native_forms_are_the_ones_that_run():
     with torch.no_grad():
         got = ops.preference_loss(torch.zeros(2, 1, 4), torch.zeros(2, 1, dtype=torch.long), torch.zeros(2))
     assert not got.loss.requires_grad and abs(float(got.loss) - math.log(2.0)) < 1e-6
+
+
+# ---------------------------------------------------------------- gradients entry by entry
+# Slack that is the same for a whole row hides all of it but the label's entry: most entries are a coefficient times a
+# probability of 1e-5 and less.  So each entry has a bound of its own: 4e-5 of (probability + 1 at the label) times the
+# row's coefficient bound, which covers the probability's and the coefficient's own error, and one rounding to the type:
+# half a unit in the last place (2^-8 bf16, 2^-11 fp16), half the smallest step below fp16's normal range, and what 32
+# bits hold no more digits of (1e-36).
+
+HALF_UNIT = {torch.float32: 0.0, torch.bfloat16: 2**-8, torch.float16: 2**-11}
+HALF_STEP = {torch.float32: 1e-36, torch.bfloat16: 1e-36, torch.float16: 2**-25}
+
+
+def _check_entries(grad, want, x64, labels, row_bound, temperature=1.0):
+    """*row_bound*: ``(B, T)``, the size of the terms that a row's coefficient adds up, with all factors."""
+    keep = labels != -100
+    p = torch.softmax(x64.detach() / temperature, -1)
+    p.scatter_add_(2, labels.clamp(min=0)[..., None], torch.ones_like(labels, dtype=p.dtype)[..., None])
+    size = want.abs()
+    slack = 4e-5 * torch.where(keep, row_bound / temperature, 0.0)[..., None] * p
+    off = (grad.detach().double().cpu() - want).abs() - slack - HALF_UNIT[grad.dtype] * (size + slack)
+    off = torch.where(keep[..., None], off - HALF_STEP[grad.dtype], off)
+    assert float(off.max()) <= 0, (float(off.max()), int((off > 0).sum()), off.numel())
+    assert float(size[keep].gt(0).double().mean()) > 0.2  # enough of it is there to be compared
+
+
+def _policy_row_bound(x64, labels, adv, old, ref, kl_coef, temperature, weight):
+    logps = _logps64(x64.detach(), labels, temperature)[0]
+    adv = adv.double() if adv.dim() == 2 else adv.double()[:, None]
+    size = adv.abs() * (1.0 if old is None else (logps - old.double()).exp())
+    if kl_coef:
+        size = size + kl_coef * ((ref.double() - logps).exp() + 1)
+    return size * weight
+
+
+def _policy_entries(dev, size, dtype, layout, scale=1.0, adv_scale=1.0, reduction="token_mean", temperature=1.0, kl_coef=0.1):
+    b, t, v = size
+    labels, g = _labels(b, t, v, 1), _gen(3)
+    x = _logits(b, t, v, dtype, 0, layout, dev)
+    x64 = _double(x)
+    now = _logps64(x64.detach(), labels, temperature)[0]
+    adv = adv_scale * (0.5 + torch.rand(b, t, generator=g))
+    noise = 0.15 * (2 * torch.rand(b, t, generator=g) - 1)  # within the clip: every row that counts has a gradient
+    old, ref = (now - noise).float(), (now + 0.5 * torch.randn(b, t, generator=g)).float()
+    kw = dict(kl_coef=kl_coef, temperature=temperature, reduction=reduction)
+    got = ops.policy_loss(x, labels.to(dev), adv.to(dev), old.to(dev), ref.to(dev), **kw)
+    want = policy64(x64, labels, adv.double(), old.double(), ref.double(), **kw)
+    keep = labels != -100
+    weight = {"token_mean": (1 / keep.sum().clamp(min=1)).expand(b, t), "sum": torch.ones(b, t),
+              "sequence_mean": (1 / keep.sum(1, keepdim=True).clamp(min=1) / b).expand(b, t)}[reduction].double()
+    bound = _policy_row_bound(x64, labels, adv, old, ref, kl_coef, temperature, weight) * scale
+    (want64,) = torch.autograd.grad(want[0] * scale, x64)
+    return got, x, want64, x64, labels, bound, temperature
+
+
+ENTRY_SIZES = [(3, 17, 1001), (2, 4, 8192), (2, 3, 9001), (2, 9, 32003), (1, 3, 40003), (1, 2, 70001), (1, 2, 131072)]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("size", ENTRY_SIZES)
+@pytest.mark.parametrize("dtype,scale,adv_scale", [
+    (torch.float16, 65536.0, 1 / 6144),  # a scaled loss over 6144 tokens: unscaled, most entries are below fp16's range
+    (torch.float16, 2.0**-13, 65536.0 * 4),  # unscaled, the labels' entries are above it
+    (torch.bfloat16, 1 / 3, 1.0), (torch.float32, 1 / 3, 1.0)])  # accumulation over three micro-batches
+def test_policy_gradient_of_a_scaled_loss_is_rounded_once(dev, size, dtype, scale, adv_scale):
+    kl_coef = 0.1 * adv_scale
+    got, x, *want = _policy_entries(dev, size, dtype, "shifted", scale, adv_scale, "sum", kl_coef=kl_coef)
+    for keep in (True, False):  # the gradient kept by the forward, and the one computed again
+        (grad,) = torch.autograd.grad(got.loss * scale, x, retain_graph=keep)
+        _check_entries(grad, *want)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_policy_gradient_of_a_loss_times_nothing(dev):
+    """A loss gradient of 0 gives zeros, one of NaN reaches the rows that count and no other."""
+    got, x, _, _, labels, _, _ = _policy_entries(dev, (3, 17, 1001), torch.bfloat16, "shifted")
+    assert not torch.autograd.grad(got.loss * 0.0, x, retain_graph=True)[0].any()
+    got, x, *_ = _policy_entries(dev, (3, 17, 1001), torch.bfloat16, "shifted")
+    (grad,) = torch.autograd.grad(got.loss, x, torch.tensor(math.nan, device=dev))
+    keep = (labels != -100).to(dev)
+    assert grad[keep].isnan().all() and not grad[~keep].any()
