@@ -78,13 +78,16 @@ def _check_logits(logits: torch.Tensor, labels: torch.Tensor) -> tuple[torch.Ten
     return logits, labels.long().contiguous()
 
 
-def _token_logps(logits: torch.Tensor, labels: torch.Tensor, ignore: int) -> tuple[torch.Tensor, torch.Tensor]:
+def _token_logps(logits: torch.Tensor, labels: torch.Tensor, ignore: int,
+                 temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
     """``(log-probabilities of the labels, 0 where ignored, which tokens count)`` in PyTorch."""
     valid = labels != ignore
     if bool(((labels < 0) | (labels >= logits.shape[2]))[valid].any()):
         raise ValueError(f"labels must be {ignore} or in [0, {logits.shape[2]})")
     x = logits if logits.dtype == torch.float64 else logits.float()
     x = x.masked_fill(~valid.unsqueeze(-1), 0.0)  # an ignored row may hold anything
+    if temperature != 1.0:
+        x = x / temperature  # not in a half type, which would round the quotient
     logps = torch.log_softmax(x, -1).gather(2, labels.masked_fill(~valid, 0).unsqueeze(-1)).squeeze(-1)
     return logps.masked_fill(~valid, 0.0), valid
 
@@ -160,7 +163,7 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
 
 
 def _policy_torch(logits, labels, adv, old, ref, lo, hi, kl_coef, temperature, reduction, ignore) -> PolicyLoss:
-    logps, valid = _token_logps(logits if temperature == 1.0 else logits / temperature, labels, ignore)
+    logps, valid = _token_logps(logits, labels, ignore, temperature)
     adv = adv if adv.dim() == 2 else adv.unsqueeze(1)
     base = logps.detach() if old is None else old
     ratio = torch.exp((logps - base).masked_fill(~valid, 0.0))

@@ -852,3 +852,13 @@ def test_policy_gradient_of_a_loss_times_nothing(dev):
     (grad,) = torch.autograd.grad(got.loss, x, torch.tensor(math.nan, device=dev))
     keep = (labels != -100).to(dev)
     assert grad[keep].isnan().all() and not grad[~keep].any()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_policy_temperature_is_applied_in_32_bits(dev, dtype):
+    """Logits over a temperature that is no power of two: rounded to a half type they would be off by 2^-9 of 20."""
+    b, t, v = 2, 7, 301
+    labels, x = _labels(b, t, v, 1), _logits(b, t, v, dtype, 0, device=dev, spread=5.0).detach()
+    got = ops.policy_loss(x, labels.to(dev), torch.zeros(b, device=dev), temperature=0.7)
+    _close(got.logps, _logps64(_double(x).detach(), labels, 0.7)[0], 2**-22, 1e-5)
