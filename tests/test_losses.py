@@ -862,3 +862,21 @@ def test_policy_temperature_is_applied_in_32_bits(dev, dtype):
     labels, x = _labels(b, t, v, 1), _logits(b, t, v, dtype, 0, device=dev, spread=5.0).detach()
     got = ops.policy_loss(x, labels.to(dev), torch.zeros(b, device=dev), temperature=0.7)
     _close(got.logps, _logps64(_double(x).detach(), labels, 0.7)[0], 2**-22, 1e-5)
+
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("layout", ["plain", "shifted"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", ENTRY_SIZES)
+def test_policy_gradient_entry_by_entry(dev, layout, dtype, size):
+    got, x, *want = _policy_entries(dev, size, dtype, layout)
+    _check_entries(torch.autograd.grad(got.loss, x)[0], *want)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kw", [{"reduction": "sum"}, {"reduction": "sequence_mean"}, {"temperature": 0.5}, {"kl_coef": 0.0}])
+def test_policy_gradient_forms_entry_by_entry(dev, dtype, kw):
+    got, x, *want = _policy_entries(dev, (3, 17, 1001), dtype, "plain", **kw)
+    _check_entries(torch.autograd.grad(got.loss, x)[0], *want)
