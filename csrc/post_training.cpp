@@ -6,6 +6,7 @@
 // backward of 96 logit rows on one B200: 111 us with Python nodes and checks, 87 us with these nodes, 70 us with the checks
 // here too; 45 us of it are the engine's).
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -545,9 +546,23 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
 // Without a gradient to come there is no node.
 bool wants_grad(const Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
 
+// The kernels read memory and have no forward-mode derivative: a tensor of a functional transform, which has no memory, is
+// turned away, and so is one with a tangent, which would be lost without a word.
+void plain(const Tensor& t, const char* name) {
+  TORCH_CHECK_NOT_IMPLEMENTED(t.has_storage(), name, " has no memory of its own (a functional transform, a sparse tensor)");
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined() || !c10::AutogradState::get_tls_state().get_fw_grad_mode(),
+                              "forward-mode derivatives are not implemented on the GPU: ", name, " has a tangent");
+}
+
+void plain(const OptTensor& t, const char* name) {
+  if (t.has_value()) plain(*t, name);
+}
+
 bool whole_numbers(const Tensor& t) { return at::isIntegralType(t.scalar_type(), false); }
 
 void take_logits(Tensor& logits, Tensor& labels) {
+  plain(logits, "logits");
+  plain(labels, "labels");
   TORCH_CHECK_VALUE(logits.dim() == 3 && at::isFloatingType(logits.scalar_type()), "logits must be floating (B, T, V), got ",
                     logits.scalar_type());
   TORCH_CHECK_VALUE(labels.dim() == 2 && labels.size(0) == logits.size(0) && labels.size(1) == logits.size(1) &&
@@ -560,6 +575,7 @@ void take_logits(Tensor& logits, Tensor& labels) {
 }
 
 Tensor constant(const Tensor& t, const char* name) {
+  plain(t, name);
   TORCH_CHECK_VALUE(!t.requires_grad(), name, " is a constant of the loss: detach it");
   return t.to(torch::kFloat32).contiguous();
 }
@@ -622,6 +638,9 @@ variable_list policy_loss(Tensor logits, Tensor labels, Tensor adv, OptTensor ol
 }
 
 variable_list balance_loss(Tensor logits, OptTensor ids, OptTensor mask, int64_t top_k, double z_coef, Tensor err) {
+  plain(logits, "router logits");
+  plain(ids, "expert_ids");
+  plain(mask, "mask");
   TORCH_CHECK_VALUE(logits.dim() >= 2 && at::isFloatingType(logits.scalar_type()),
                     "router logits must be floating (..., N, E), got ", logits.scalar_type());
   const auto lead = logits.sizes().slice(0, logits.dim() - 2).vec();
@@ -659,6 +678,13 @@ variable_list balance_loss(Tensor logits, OptTensor ids, OptTensor mask, int64_t
 // A call by a decoder's every layer and token: its arguments are checked here, not in Python.
 variable_list qk_norm_rope(Tensor q, Tensor k, Tensor qw, Tensor kw, Tensor cos, Tensor sin, OptTensor positions,
                            double eps, Tensor err) {
+  plain(q, "q");
+  plain(k, "k");
+  plain(qw, "q_weight");
+  plain(kw, "k_weight");
+  plain(cos, "cos");
+  plain(sin, "sin");
+  plain(positions, "positions");
   TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && q.size(0) == k.size(0) && q.size(1) == k.size(1) &&
                         q.size(3) == k.size(3) && q.scalar_type() == k.scalar_type(),
                     "q and k must be (B, T, H, D) of one type with the same B, T and D");

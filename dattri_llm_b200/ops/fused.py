@@ -367,7 +367,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
             :func:`~dattri_llm_b200.ops.check_device_errors` (raised at once on CPU).
 
     Returns:
-        The new q and k, contiguous.  Gradients reach q, k and both weights.
+        The new q and k, contiguous.  Gradients reach q, k and both weights (forward-mode
+        derivatives: on CPU only, inputs with tangents are refused on the GPU).
     """
     if use_native(q):
         return tuple(native().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, error_word(q.device)))

@@ -9,8 +9,9 @@ Each takes logits and returns a loss that backpropagates into them:
   tokens each expert received.
 
 On sm_100 they run the kernels of ``csrc/logit_loss.cu`` and ``csrc/router_balance.cu``
-(bf16, fp16 or fp32 logits; fp32 softmax statistics, sums over tokens in fp64); the same
-formulas in PyTorch serve CPU tensors.  The reference has neither: its losses are the
+(bf16, fp16 or fp32 logits; fp32 softmax statistics, sums over tokens in fp64), which have
+no forward-mode derivatives and refuse inputs with tangents; the same formulas in PyTorch
+serve CPU tensors.  The reference has neither: its losses are the
 user's own.
 """
 

@@ -880,3 +880,59 @@ def test_policy_gradient_entry_by_entry(dev, layout, dtype, size):
 def test_policy_gradient_forms_entry_by_entry(dev, dtype, kw):
     got, x, *want = _policy_entries(dev, (3, 17, 1001), dtype, "plain", **kw)
     _check_entries(torch.autograd.grad(got.loss, x)[0], *want)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_forward_mode_derivatives_are_right_or_refused(dev):
+    """The kernels have none and say so, whether or not the primal needs a gradient; the CPU forms have them."""
+    import torch.autograd.forward_ad as fwd
+
+    g = _gen(0)
+    x, y, adv = torch.randn(2, 3, 5, generator=g).to(dev), torch.zeros(2, 3, dtype=torch.long, device=dev), torch.ones(2, device=dev)
+    w, (cos, sin) = torch.ones(4, device=dev), torch.ones(2, 3, 2, device=dev)
+    q, turn = torch.randn(1, 3, 2, 4, generator=g).to(dev), torch.randn(1, 3, 2, 4, generator=g).to(dev)
+    calls = [(lambda z: ops.preference_loss(z, y, adv).loss, x), (lambda z: ops.policy_loss(z, y, adv, adv[:, None] - torch.full_like(x[..., 0], 2.6), clip=(1.0, 1e9)).loss, x),
+             (lambda z: ops.router_balance_loss(z, 2).loss.sum(), x),
+             (lambda z: (ops.qk_norm_rope(z, q, w, w, cos, sin)[0] * turn).sum(), q),
+             (lambda z: (ops.qk_norm_rope(q, q, z, w, cos, sin)[0] * turn).sum(), w),
+             (lambda z: ops.policy_loss(x, y, z).loss, adv), (lambda z: ops.policy_loss(x, y, adv, None, z, kl_coef=1.0).loss, -x[..., 0].abs()),
+             (lambda z: ops.preference_loss(x, y, z).loss, adv)]
+    for call, at in calls:
+        for wants in (False, True):
+            if wants and call in [c for c, _ in calls[5:]]:
+                continue  # a constant that needs a gradient is refused anyway
+            way = torch.randn(at.shape, generator=g).to(dev)
+            with fwd.dual_level():
+                z = fwd.make_dual(at.detach().clone().requires_grad_(wants), way)
+                if dev == "cuda":
+                    with pytest.raises(NotImplementedError):
+                        call(z)
+                    call(at)  # no tangent, no refusal
+                    continue
+                got = fwd.unpack_dual(call(z)).tangent
+            h = 1e-3
+            ends = [float(call(at + s * h * way)) for s in (1, -1)]
+            # Central differences in 32 bits: 1e-6 of losses below 5 over 2 h, and h^2 of a third derivative below 20.
+            assert abs(float(got.detach()) - (ends[0] - ends[1]) / (2 * h)) < 5e-3
+
+
+def test_native_entry_points_refuse_tensors_without_memory():
+    """Tensors of functional transforms have none; they are turned away before anything is read."""
+    try:
+        native = ops.native()
+    except RuntimeError:
+        pytest.skip("the extension is not built")
+    x, y, err = torch.randn(2, 3, 5), torch.zeros(2, 3, dtype=torch.long), torch.zeros(1, dtype=torch.int32)
+    w = torch.ones(4)
+    tables = torch.ones(3, 2), torch.zeros(3, 2)
+    calls = [lambda z: native.preference_loss(z, y, torch.zeros(2), "sigmoid", 0.1, 0.0, False, "mean", -100, err)[0],
+             lambda z: native.policy_loss(z, y, torch.zeros(2), None, None, 0.2, 0.2, 0.0, 1.0, "sum", -100, err)[0],
+             lambda z: native.balance_loss(z, None, None, 2, 0.0, err)[0].sum(),
+             lambda z: native.qk_norm_rope(z[:, :, None, :4], z[:, :, None, :4], w, w, *tables, None, 1e-6, err)[0].sum()]
+    for call in calls:
+        with pytest.raises(NotImplementedError):
+            torch.func.jvp(call, (x,), (x,))
+        with pytest.raises(NotImplementedError):
+            torch.func.grad(call)(x)
+        with pytest.raises(NotImplementedError):
+            torch.func.vmap(call)(x[None])
