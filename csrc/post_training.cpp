@@ -437,6 +437,9 @@ variable_list qk_norm_bwd(const OptTensor& gq, const OptTensor& gk, const Tensor
 }
 
 // ---------------------------------------------------------------- autograd
+// The device's error word is no saved variable of a node: clearing it between a forward and its backward, which is what
+// reporting an error does, must not read as a change of the forward's inputs.
+Tensor error_word(AutogradContext* ctx) { return ctx->saved_data["err"].toTensor(); }
 
 struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& labels, const Tensor& ref,
@@ -445,7 +448,8 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
     auto out = preference_fwd(logits, labels, ref, kind, beta, smoothing, average, reduction, ignore, err);
     launches += 2;
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({logits, labels, out[2], err});
+    ctx->save_for_backward({logits, labels, out[2]});
+    ctx->saved_data["err"] = err;
     ctx->saved_data["ignore"] = ignore;
     return {out[0], out[1]};
   }
@@ -453,7 +457,7 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
     variable_list out(10);
     if (!g[0].defined() && !g[1].defined()) return out;
     const auto s = ctx->get_saved_variables();
-    out[0] = preference_bwd(s[0], s[1], s[2], dense(g[0]), dense(g[1]), ctx->saved_data["ignore"].toInt(), s[3]);
+    out[0] = preference_bwd(s[0], s[1], s[2], dense(g[0]), dense(g[1]), ctx->saved_data["ignore"].toInt(), error_word(ctx));
     ++launches;
     return once(std::move(out), "preference_loss");
   }
@@ -467,7 +471,8 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
                           ignore, err, true);
     ctx->set_materialize_grads(false);
     ctx->mark_non_differentiable({out[2], out[3]});
-    ctx->save_for_backward({logits, labels, out[4], err});
+    ctx->save_for_backward({logits, labels, out[4]});
+    ctx->saved_data["err"] = err;
     ctx->saved_data["ignore"] = ignore;
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["grad"] = out[5];
@@ -485,7 +490,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
       ctx->saved_data.erase(kept);
     }
     out[0] = policy_bwd(s[0], s[1], s[2], dense(g[0]), dense(g[1]), ctx->saved_data["temperature"].toDouble(),
-                        ctx->saved_data["ignore"].toInt(), s[3], std::move(unit_grad));
+                        ctx->saved_data["ignore"].toInt(), error_word(ctx), std::move(unit_grad));
     ++launches;
     return once(std::move(out), "policy_loss");
   }
@@ -498,7 +503,8 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
     launches += 2;
     ctx->set_materialize_grads(false);
     ctx->mark_non_differentiable({out[1]});
-    ctx->save_for_backward({logits, mask.value_or(Tensor()), out[2], err});
+    ctx->save_for_backward({logits, mask.value_or(Tensor()), out[2]});
+    ctx->saved_data["err"] = err;
     ctx->saved_data["top_k"] = top_k;
     ctx->saved_data["z"] = z_coef;
     return {out[0], out[1]};
@@ -508,7 +514,7 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
     if (!g[0].defined()) return out;
     const auto s = ctx->get_saved_variables();
     out[0] = balance_bwd(s[0], s[1].defined() ? OptTensor(s[1]) : std::nullopt, s[2], g[0],
-                         ctx->saved_data["top_k"].toInt(), ctx->saved_data["z"].toDouble(), s[3]);
+                         ctx->saved_data["top_k"].toInt(), ctx->saved_data["z"].toDouble(), error_word(ctx));
     ++launches;
     return once(std::move(out), "router_balance_loss");
   }
@@ -521,7 +527,8 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
     auto out = qk_norm_fwd(q, k, qw, kw, cos, sin, positions, eps, err);
     ++launches;
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({q, k, qw, kw, cos, sin, positions.value_or(Tensor()), err});
+    ctx->save_for_backward({q, k, qw, kw, cos, sin, positions.value_or(Tensor())});
+    ctx->saved_data["err"] = err;
     ctx->saved_data["eps"] = eps;
     return out;
   }
@@ -533,7 +540,7 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
       return !t.defined() ? OptTensor() : OptTensor(t.stride(-1) == 1 ? t : t.contiguous());
     };
     auto d = qk_norm_bwd(row(g[0]), row(g[1]), s[0], s[1], s[2], s[3], s[4], s[5],
-                         s[6].defined() ? OptTensor(s[6]) : std::nullopt, ctx->saved_data["eps"].toDouble(), s[7]);
+                         s[6].defined() ? OptTensor(s[6]) : std::nullopt, ctx->saved_data["eps"].toDouble(), error_word(ctx));
     launches += 2;
     std::copy(d.begin(), d.end(), out.begin());
     return once(std::move(out), "qk_norm_rope");

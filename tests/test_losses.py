@@ -936,3 +936,32 @@ def test_native_entry_points_refuse_tensors_without_memory():
             torch.func.grad(call)(x)
         with pytest.raises(NotImplementedError):
             torch.func.vmap(call)(x[None])
+
+
+def _four_losses(x, y, bad):
+    """One graph of each operator, with labels, ids or positions off the end where *bad*."""
+    w, tables = torch.ones(4, device="cuda", requires_grad=True), (torch.ones(3, 2, device="cuda"), torch.zeros(3, 2, device="cuda"))
+    ref, off = torch.zeros(2, device="cuda"), 99 if bad else 0
+    q = x[:, :, None, :4]
+    return [ops.preference_loss(x, y + off, ref).loss, ops.policy_loss(x, y + off, ref + 1).loss,
+            ops.policy_loss(x, y + off, ref + 1).logps.sum(),
+            ops.router_balance_loss(x, 1, y[..., None] + off, z_coef=0.1).loss.sum(),
+            ops.qk_norm_rope(q, q, w, w, *tables, torch.arange(3, device="cuda") + off)[0].sum()]
+
+
+@pytest.mark.gpu
+def test_a_reported_index_leaves_the_graphs_alone():
+    """A bad index is left out and reported; the backward of its graph and of the others on the device goes on."""
+    ops.check_device_errors()
+    x = torch.randn(2, 3, 5, device="cuda", requires_grad=True)
+    y = torch.zeros(2, 3, dtype=torch.long, device="cuda")
+    good, bad = _four_losses(x, y, False), _four_losses(x, y, True)
+    with pytest.raises(RuntimeError, match="error 5"):
+        ops.check_device_errors()
+    for loss in good:
+        (grad,) = torch.autograd.grad(loss, x)
+        assert torch.isfinite(grad).all() and grad.any()
+    for loss in bad:
+        assert torch.isfinite(torch.autograd.grad(loss, x)[0]).all()
+    with pytest.raises(RuntimeError, match="error 5"):  # the backward meets the same labels and positions
+        ops.check_device_errors()
