@@ -109,7 +109,8 @@ def error_word(device: torch.device | int) -> torch.Tensor:
         idx = torch.cuda.current_device()
     w = _err_words.get(idx)
     if w is None:
-        w = torch.zeros(1, dtype=torch.int32, device=f"cuda:{idx}")
+        with torch.inference_mode(False):  # cleared outside of inference mode too
+            w = torch.zeros(1, dtype=torch.int32, device=f"cuda:{idx}")
         _err_words[idx] = w
     return w
 

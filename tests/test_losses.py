@@ -965,3 +965,23 @@ def test_a_reported_index_leaves_the_graphs_alone():
         assert torch.isfinite(torch.autograd.grad(loss, x)[0]).all()
     with pytest.raises(RuntimeError, match="error 5"):  # the backward meets the same labels and positions
         ops.check_device_errors()
+
+
+@pytest.mark.gpu
+def test_a_device_first_used_in_inference_mode_trains_and_reports():
+    word = ops._err_words.pop(torch.cuda.current_device(), None)
+    try:
+        x = torch.randn(2, 3, 5, device="cuda", requires_grad=True)
+        y = torch.zeros(2, 3, dtype=torch.long, device="cuda")
+        with torch.inference_mode():
+            ops.policy_loss(x, y, torch.ones(2, device="cuda"))
+        for loss in _four_losses(x, y, False):
+            assert torch.autograd.grad(loss, x)[0].any()
+        ops.check_device_errors()
+        ops.policy_loss(x, y + 9, torch.ones(2, device="cuda"))
+        with pytest.raises(RuntimeError, match="error 5"):
+            ops.check_device_errors()
+        ops.check_device_errors()
+    finally:
+        if word is not None:
+            ops._err_words[torch.cuda.current_device()] = word
