@@ -416,7 +416,9 @@ __global__ void __launch_bounds__(kVecWarps * 32, 4) qk_norm_bwd_vec_kernel(QkNo
       }
       const float sq = group_sum<kLog>(ss.x + ss.y, log), dt = group_sum<kLog>(dot.x + dot.y, log);
       load(stage == 0 ? kStages - 1 : stage - 1);  // the stage used a step ago
-      const float r = rsqrt_of(fmaf(sq, inv_d, eps));
+      // Beyond the heads there is no norm: without eps the root of the ring's zeros would be infinite, and 0 times it a NaN
+      // in the weight's gradient.
+      const float r = h < end ? rsqrt_of(fmaf(sq, inv_d, eps)) : 0.f;
       const float pull = -r * r * (dt * r * inv_d);  // dx = r w dy + x pull
       const float2 rr = make_float2(r, r), pp = make_float2(pull, pull);
 #pragma unroll

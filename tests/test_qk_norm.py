@@ -258,3 +258,28 @@ def test_repeats_streams_and_graph_capture():
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("heads", [(1, 1), (4, 3), (9, 2)])
+@pytest.mark.parametrize("d", [30, 64, 96, 256])
+def test_weight_gradients_without_eps(dev, heads, d):
+    """With eps = 0 only a head of zeros has no norm: heads that fill no whole step of the kernel leave no NaN."""
+    q, k, qw, kw = _inputs((1, 3, *heads, d, d - d % 4), torch.float32, torch.float32, dev)
+    cos, sin = (x.to(dev) for x in _tables(3, d - d % 4))
+    outer = [torch.randn(1, 3, h, d, generator=_gen(7)) for h in heads]
+    out = ops.qk_norm_rope(q, k, qw, kw, cos, sin, eps=0.0)
+    torch.autograd.backward(out, [o.to(dev) for o in outer])
+    for x, w, y, o in zip((q, k), (qw, kw), out, outer):
+        x64, w64 = x.detach().cpu().double().requires_grad_(), w.detach().cpu().double().requires_grad_()
+        n = x64 / (x64 ** 2).mean(-1, keepdim=True).sqrt()
+        turn = torch.complex(cos.cpu().double(), sin.cpu().double())[None, :, None]
+        z, half = n * w64, cos.shape[1]
+        z2 = torch.complex(z[..., :half], z[..., half:2 * half]) * turn
+        want = torch.cat([z2.real, z2.imag, z[..., 2 * half:]], -1)
+        want.backward(o.double())
+        _close(y, want.detach(), 1e-6, 1e-6 * 8 * math.sqrt(d))
+        rms = float((x64.detach() ** 2).mean(-1).sqrt().min())
+        _close(x.grad, x64.grad, 1e-6, 4e-6 * 12 / rms * (1 + math.sqrt(d)))
+        size_of_sum = (n.detach().abs() * o.double().abs().amax(-1, keepdim=True) * 2).sum((0, 1, 2)).max()
+        _close(w.grad, w64.grad, 1e-6, 4e-6 * float(size_of_sum))
