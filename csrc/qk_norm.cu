@@ -229,8 +229,8 @@ __global__ void __launch_bounds__(kVecWarps * 32, 5) qk_norm_fwd_vec_kernel(QkNo
   const bool is_q = (int)blockIdx.x < q_blocks;
   const HeadTensor& X = is_q ? a.q : a.k;
   const unsigned block = is_q ? blockIdx.x : blockIdx.x - q_blocks, by = (is_q ? q_blocks : k_blocks) * kVecWarps;
-  const int parts = is_q ? q_tasks : k_tasks, H = X.H, step = 32 >> log;
-  const unsigned tasks = (unsigned)a.B * (unsigned)a.T * (unsigned)parts;
+  const int parts = max(is_q ? q_tasks : k_tasks, 1), H = X.H, step = 32 >> log;  // a tensor without heads has no tasks
+  const unsigned tasks = H > 0 ? (unsigned)a.B * (unsigned)a.T * (unsigned)parts : 0;
   const Lanes<VEC> L(a, log);
   const float inv_d = 1.f / a.D, eps = a.eps;
   const Stride stride(by, max(a.T, 1), parts);
@@ -333,10 +333,10 @@ __global__ void __launch_bounds__(kVecWarps * 32, 4) qk_norm_bwd_vec_kernel(QkNo
   const bool is_q = (int)blockIdx.x < g.q_blocks;
   const HeadTensor& X = is_q ? a.q : a.k;
   const unsigned block = is_q ? blockIdx.x : blockIdx.x - g.q_blocks, by = (is_q ? g.q_blocks : g.k_blocks) * kVecWarps;
-  const int parts = is_q ? q_tasks : k_tasks, H = X.H, step = 32 >> log, warp = threadIdx.x >> 5;
+  const int parts = max(is_q ? q_tasks : k_tasks, 1), H = X.H, step = 32 >> log, warp = threadIdx.x >> 5;
   const T* grad = reinterpret_cast<const T*>(is_q ? g.gq : g.gk);
   const long long gb = is_q ? g.gqb : g.gkb, gt = is_q ? g.gqt : g.gkt, gh = is_q ? g.gqh : g.gkh;
-  const unsigned tasks = (unsigned)a.B * (unsigned)a.T * (unsigned)parts;
+  const unsigned tasks = H > 0 ? (unsigned)a.B * (unsigned)a.T * (unsigned)parts : 0;
   const Lanes<VEC> L(a, log);
   const float inv_d = 1.f / a.D, eps = a.eps;
   const Stride stride(by, max(a.T, 1), parts);
@@ -656,7 +656,8 @@ Plan plan_of(const QkNormArgs& a, const QkNormGradArgs* g) {
 void blocks_of(const QkNormArgs& a, const Plan& p, long long most, int* q_blocks, int* k_blocks) {
   const long long tokens = (long long)a.B * a.T, per = p.vec ? kVecWarps : kWarps;
   const long long q = (tokens * p.q_tasks + per - 1) / per, k = (tokens * p.k_tasks + per - 1) / per;
-  long long qs = most * a.q.H / (a.q.H + a.k.H), ks;
+  const int heads = a.q.H + a.k.H;  // neither may have any
+  long long qs = most * a.q.H / (heads > 0 ? heads : 1), ks;
   qs = qs < 1 ? 1 : (qs > most - 1 ? most - 1 : qs);
   ks = most - qs;
   *q_blocks = (int)(q < qs ? (q < 1 ? 1 : q) : qs);

@@ -283,3 +283,17 @@ def test_weight_gradients_without_eps(dev, heads, d):
         _close(x.grad, x64.grad, 1e-6, 4e-6 * 12 / rms * (1 + math.sqrt(d)))
         size_of_sum = (n.detach().abs() * o.double().abs().amax(-1, keepdim=True) * 2).sum((0, 1, 2)).max()
         _close(w.grad, w64.grad, 1e-6, 4e-6 * float(size_of_sum))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("heads", [(0, 0), (0, 2), (3, 0)])
+def test_tensors_without_heads(dev, heads):
+    """Gradients of no heads at all, and of one tensor's heads beside none of the other's."""
+    q, k, qw, kw = _inputs((2, 3, *heads, 64, 64), torch.float32, torch.float32, dev)
+    cos, sin = (x.to(dev) for x in _tables(3, 64))
+    out = ops.qk_norm_rope(q, k, qw, kw, cos, sin, eps=EPS)
+    assert [y.shape[2] for y in out] == list(heads)
+    (out[0].sum() + out[1].sum()).backward()
+    for x, w, h in zip((q, k), (qw, kw), heads):
+        assert x.grad.shape == x.shape and torch.isfinite(w.grad).all()
+        assert bool(w.grad.any()) == (h > 0)
