@@ -3,7 +3,7 @@
 // Both need log p(y | row) = x_y - lse(x) of the labelled token of every row that counts, and
 // both send back coef (onehot(y) - softmax(x)). In base two with c = log2(e) / temperature and
 // m = max(x):
-//     s = sum_v 2^((x_v - m) c),   log p = ln 2 ((x_y - m) c - log2 s),   p_v = 2^((x_v - m) c) / s.
+//     s = sum_v 2^((x_v - m) c),   log p = (x_y - m) / temperature - ln 2 log2 s,   p_v = 2^((x_v - m) c) / s.
 // The maximum is taken off before the scaling: x_v c - m c in one step would overflow where a
 // mask put the type's lowest value. Sums are fp32 within a row (each thread its share) and fp64
 // over a sequence's tokens and over pairs.
@@ -106,6 +106,12 @@ __device__ __forceinline__ void store_vec(T* row, int V, int lo, const uint4& v,
 
 // What the terms of a part with maximum m are taken off: 0 where all of it is -inf, so that its terms are 0.
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
+
+// The label's log-probability. Its own logit goes without the factor log2(e), which would take the type's lowest value,
+// what a mask may have put there, to -inf.
+__device__ __forceinline__ float label_logp(float xy, float base, float inv_temp, float s) {
+  return (xy - base) * inv_temp - kLn2 * log2f(s);
+}
 
 // The larger of each element of two words; a NaN is passed over here and found again in the sum.
 __device__ __forceinline__ uint32_t word_max(uint32_t a, uint32_t b, __nv_bfloat16) {
@@ -298,7 +304,7 @@ __global__ void __launch_bounds__(Place<kGroup>::kThreads, kGroup == 32 ? 10 : 1
   row_stats<T, kGroup>(RowSpan<T>(x, r.V), c, m, s, parts);
   if (tid == 0) {
     const float base = base_of(m);
-    logps[row] = kLn2 * ((ElemOf<T>::up(x[y]) - base) * c - log2f(s));
+    logps[row] = label_logp(ElemOf<T>::up(x[y]), base, r.inv_temp, s);
     stats[row] = RowStat{base, 1.f / s};
   }
 }
@@ -611,8 +617,8 @@ __global__ void __launch_bounds__(256) policy_finish_kernel(PolicyArgs a) {
 
 // What of a row that counts goes out, from its maximum and sum; the gradient's coefficient, the same in every thread.
 __device__ __forceinline__ float policy_out(const PolicyArgs& a, long long row, const TokenIn& in, float w, float xy, float m,
-                                            float s, float c, bool first) {
-  const float base = base_of(m), logp = kLn2 * ((xy - base) * c - log2f(s));
+                                            float s, bool first) {
+  const float base = base_of(m), logp = label_logp(xy, base, a.rows.inv_temp, s);
   const TokenTerms k = policy_token(a, in, logp);
   if (first) {
     a.logps[row] = logp;
@@ -659,7 +665,7 @@ __global__ void __launch_bounds__(Place<kGroup>::kThreads, kMin) policy_row_kern
   const TokenIn in = token_in(a, row, b);
   float m, s;
   row_stats<T, kGroup>(span, c, m, s, parts);
-  const float coef = policy_out(a, row, in, w, xy, m, s, c, Place<kGroup>::tid() == 0);
+  const float coef = policy_out(a, row, in, w, xy, m, s, Place<kGroup>::tid() == 0);
   if (coef == 0.f)
     zero_row<T, kGroup>(out, r.V);
   else
@@ -730,7 +736,7 @@ __global__ void __launch_bounds__(kLongThreads, 2) policy_long_kernel(PolicyArgs
     take<T>(v, c, m, s);
   }
   merge_group<kLongThreads>(m, s, c, parts);
-  const float coef = policy_out(a, row, in, w, xy, m, s, c, tid == 0);
+  const float coef = policy_out(a, row, in, w, xy, m, s, tid == 0);
   if (coef == 0.f) {
     zero_row<T, kLongThreads>(out, r.V);
     return;

@@ -985,3 +985,23 @@ def test_a_device_first_used_in_inference_mode_trains_and_reports():
     finally:
         if word is not None:
             ops._err_words[torch.cuda.current_device()] = word
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_label_of_the_lowest_logit_keeps_a_finite_log_probability(dev, dtype):
+    """A mask that put the type's lowest value where a label points: its log-probability is that value, not -inf."""
+    low = torch.finfo(dtype).min
+    x = _logits(2, 3, 40, dtype, 0, device=dev).detach()
+    x[:, 1, 5] = low
+    labels = torch.full((2, 3), -100)
+    labels[:, 1] = 5
+    want = _logps64(_double(x).detach(), labels)[0]
+    assert torch.isfinite(want.float()).all()
+    got = ops.policy_loss(x, labels.to(dev), torch.ones(2, device=dev))
+    _close(got.logps, want, 2**-22, 1e-5)
+    got = ops.preference_loss(x.requires_grad_(), labels.to(dev), torch.zeros(2, device=dev))
+    want_loss, want = preference64(_double(x).detach(), labels, torch.zeros(2).double())
+    _close(got.logps, want, 2**-22, 1e-5)
+    assert torch.isfinite(got.loss)
+    _close(got.loss, want_loss, 1e-5, 0.1 * 2 * (1e-5 + 2**-22 * abs(low)))
