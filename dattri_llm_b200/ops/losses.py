@@ -55,13 +55,13 @@ class BalanceLoss(NamedTuple):
     counts: torch.Tensor
 
 
-def _constant(name: str, x: torch.Tensor | None) -> torch.Tensor | None:
-    """*x* as contiguous fp32, or an error if it would need a gradient."""
+def _constant(name: str, x: torch.Tensor | None, logits: torch.Tensor) -> torch.Tensor | None:
+    """*x* in 32 bits, or in the 64 of *logits*, or an error if it would need a gradient."""
     if x is None:
         return None
     if x.requires_grad:
         raise ValueError(f"{name} is a constant of the loss: detach it")
-    return x.to(torch.float32).contiguous()
+    return x.to(torch.promote_types(logits.dtype, torch.float32))
 
 
 def _check_logits(logits: torch.Tensor, labels: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -156,7 +156,7 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
         raise ValueError(f"label_smoothing must be in [0, 0.5), and 0 unless kind is 'sigmoid', got {label_smoothing}")
     if ref_logps.shape != (b,):
         raise ValueError(f"ref_logps must be ({b},), got {tuple(ref_logps.shape)}")
-    ref = _constant("ref_logps", ref_logps).to(torch.promote_types(logits.dtype, torch.float32))
+    ref = _constant("ref_logps", ref_logps, logits)
     return _preference_torch(logits, labels, ref, kind, beta, label_smoothing, average_logps, reduction, ignore_index)
 
 
@@ -240,10 +240,8 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, advantages: torch.Te
     if kl_coef and ref_logps is None:
         raise ValueError("a KL term needs ref_logps")
     lo, hi = 1.0 - clip[0], 1.0 + clip[1]
-    consts = tuple(_constant(n, x) for n, x in (("advantages", advantages), ("old_logps", old_logps),
-                                                 ("ref_logps", ref_logps)))
-    wide = torch.promote_types(logits.dtype, torch.float32)
-    consts = tuple(None if x is None else x.to(wide) for x in consts)
+    consts = (_constant(n, x, logits) for n, x in (("advantages", advantages), ("old_logps", old_logps),
+                                                   ("ref_logps", ref_logps)))
     return _policy_torch(logits, labels, *consts, lo, hi, kl_coef, temperature, reduction, ignore_index)
 
 

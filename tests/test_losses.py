@@ -1005,3 +1005,15 @@ def test_a_label_of_the_lowest_logit_keeps_a_finite_log_probability(dev, dtype):
     _close(got.logps, want, 2**-22, 1e-5)
     assert torch.isfinite(got.loss)
     _close(got.loss, want_loss, 1e-5, 0.1 * 2 * (1e-5 + 2**-22 * abs(low)))
+
+
+def test_constants_of_64_bit_logits_keep_their_digits():
+    x = torch.randn(2, 3, 11, generator=_gen(0), dtype=torch.float64)
+    y, g = torch.randint(0, 11, (2, 3), generator=_gen(1)), _gen(2)
+    ref = -2000 + torch.randn(2, generator=g, dtype=torch.float64)  # 32 bits hold these to 1e-4
+    _close(ops.preference_loss(x, y, ref).loss, preference64(x, y, ref)[0], 1e-12, 0)
+    now = _logps64(x, y)[0]
+    adv, old, ref = torch.randn(2, generator=g, dtype=torch.float64), now + 1 / 3, now - 1 / 7
+    got, want = ops.policy_loss(x, y, adv, old, ref, kl_coef=0.1), policy64(x, y, adv, old, ref, kl_coef=0.1)
+    for a, b in zip(got, want):
+        _close(a, b, 1e-12, 1e-15)
