@@ -595,8 +595,9 @@ class ExpertParallelMoE(nn.Module):
     any backend).
 
     With ``track_balance`` each forward leaves the router's balance loss and expert counts of
-    this rank's tokens in ``balance`` (:func:`dattri_llm_b200.ops.router_balance_loss`); add
-    :func:`balance_loss` of the model to a training loss."""
+    this rank's tokens, padding among them, in ``balance``
+    (:func:`dattri_llm_b200.ops.router_balance_loss`); add :func:`balance_loss` of the model to a
+    training loss before another forward of the model replaces it."""
 
     def __init__(self, hidden: int, intermediate: int, n_experts: int, top_k: int, *, max_tokens: int,
                  norm_topk_prob: bool = False, group=None, device: torch.device | None = None,
@@ -616,6 +617,7 @@ class ExpertParallelMoE(nn.Module):
         self.norm_topk_prob = norm_topk_prob
         self.track_balance = track_balance
         self.balance = None
+        self.balance_has_graph = False  # whether the forward that left it ran with gradients
         self.max_tokens = max_tokens
         self.capacity = self.world * max_tokens * top_k
         self.dtype = dtype
@@ -663,6 +665,7 @@ class ExpertParallelMoE(nn.Module):
         topv, topi = probs.topk(self.top_k, dim=-1)
         if self.track_balance:
             self.balance = router_balance_loss(logits.reshape(-1, self.n_experts), self.top_k, topi)
+            self.balance_has_graph = torch.is_grad_enabled()
         if self.norm_topk_prob:
             topv = topv / topv.sum(-1, keepdim=True)
         return topv, topi
@@ -757,13 +760,31 @@ def expert_parallelize(model: nn.Module, *, max_tokens: int, group=None, device:
     return replaced
 
 
+class _NoGraph(torch.autograd.Function):
+    """The value it is given; an error in the backward."""
+
+    @staticmethod
+    def forward(ctx, loss):
+        return loss.clone()
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError("the last forward of a tracking expert block ran without gradients (an evaluation, or a "
+                           "checkpointed block in its reentrant form): its balance loss has none; take balance_loss(model) "
+                           "right after the training forward, and checkpoint with use_reentrant=False")
+
+
 def balance_loss(model: nn.Module) -> torch.Tensor:
     """Mean of the balance losses that the last forward left in *model*'s tracking
-    :class:`ExpertParallelMoE` blocks."""
-    found = [m.balance.loss for m in model.modules() if isinstance(m, ExpertParallelMoE) and m.balance is not None]
-    if not found:
+    :class:`ExpertParallelMoE` blocks.  Where that forward ran without gradients the value is
+    right and a backward through it raises."""
+    blocks = [m for m in model.modules() if isinstance(m, ExpertParallelMoE) and m.balance is not None]
+    if not blocks:
         raise ValueError("no expert block of the model tracked its balance in a forward (track_balance=True)")
-    return torch.stack(found).mean()
+    loss = torch.stack([m.balance.loss for m in blocks]).mean()
+    if torch.is_grad_enabled() and not all(m.balance_has_graph for m in blocks):
+        return _NoGraph.apply(loss.detach().requires_grad_())
+    return loss
 
 
 def expert_parallel_buffers(model: nn.Module) -> list[str]:

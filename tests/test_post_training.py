@@ -203,3 +203,47 @@ def test_example_runs(dev):
     # Four pairs at the reference model itself: 4 log 2.
     assert first and abs(float(first.group(1)) - 2.7726) < (0.05 if dev == "cuda" else 1e-3)
     assert "nan" not in out.stdout
+
+
+def _tracked_block(**kw):
+    block = moe.ExpertParallelMoE(16, 8, 4, 2, max_tokens=32, device=torch.device("cpu"), dtype=torch.float32,
+                                  track_balance=True, **kw)
+    torch.nn.init.normal_(block.gate.weight, generator=torch.Generator().manual_seed(0))
+    return block, torch.randn(3, 5, 16, generator=torch.Generator().manual_seed(1))
+
+
+def test_a_balance_without_a_graph_is_no_training_loss():
+    """A forward without gradients after the training one (an evaluation, a checkpointed block in its reentrant form)
+    leaves a balance that would add nothing to the gradients: a backward through it says so."""
+    block, x = _tracked_block()
+    block.route(x)
+    want = float(moe.balance_loss(block).detach())
+    with torch.no_grad():
+        block.route(x)
+        assert float(moe.balance_loss(block)) == pytest.approx(want)
+    loss = moe.balance_loss(block)
+    assert loss.item() == pytest.approx(want)  # a number to log all the same
+    with pytest.raises(RuntimeError, match="without gradients"):
+        (loss * 0.01 + block.gate.weight.sum()).backward()
+    block.route(x)
+    moe.balance_loss(block).backward()
+    assert block.gate.weight.grad.abs().sum() > 0
+
+
+def test_the_balance_of_checkpointed_blocks():
+    from torch.utils.checkpoint import checkpoint
+
+    grads = []
+    for how in (None, False, True):
+        block, x = _tracked_block()
+        x.requires_grad_()
+        route = lambda z: block.route(z)[0].sum()  # noqa: E731
+        y = route(x) if how is None else checkpoint(route, x, use_reentrant=how)
+        total = y * 0.1 + moe.balance_loss(block)
+        if how:
+            with pytest.raises(RuntimeError, match="without gradients"):
+                total.backward()
+            continue
+        total.backward()
+        grads.append(block.gate.weight.grad)
+    assert torch.equal(*grads)
