@@ -637,6 +637,11 @@ class ExpertParallelMoE(nn.Module):
             self.capture_rows = bufs.capture_rows
         self.grouped_capture: EPGroupedCapture | None = None  # set by a capture manager
 
+    def __getstate__(self) -> dict:
+        """A copy (a reference model) or a saved block starts without the last batch's balance,
+        whose graph can be neither copied nor saved."""
+        return {**self.__dict__, "balance": None, "balance_has_graph": False}
+
     @property
     def dattri_experts(self) -> nn.ModuleList:
         """The per-expert ``{"gate_up", "down"}`` taps."""

@@ -247,3 +247,19 @@ def test_the_balance_of_checkpointed_blocks():
         total.backward()
         grads.append(block.gate.weight.grad)
     assert torch.equal(*grads)
+
+
+def test_a_block_with_a_balance_is_copied_and_saved(tmp_path):
+    """A reference model is a copy of the trained one; the balance of the last batch stays with the original."""
+    import copy
+
+    block, x = _tracked_block()
+    block.route(x)
+    twin = copy.deepcopy(block)
+    assert twin.track_balance and twin.balance is None and block.balance is not None
+    moe.balance_loss(block).backward()
+    assert block.gate.weight.grad.abs().sum() > 0 and twin.gate.weight.grad is None
+    twin.route(x)
+    assert torch.equal(twin.balance.counts, block.balance.counts)
+    torch.save(block, tmp_path / "block.pt")
+    assert torch.load(tmp_path / "block.pt", weights_only=False).balance is None
