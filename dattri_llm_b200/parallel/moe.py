@@ -665,6 +665,7 @@ class ExpertParallelMoE(nn.Module):
 
         The router runs on *x* in its own shape, so a capture hook on ``gate`` sees the
         ``(B, T, H)`` layout of the samples."""
+        self.balance = None  # the last forward's, whether or not it is tracked
         logits = self.gate(x)
         probs = torch.softmax(logits.float().reshape(-1, self.n_experts), dim=-1)
         topv, topi = probs.topk(self.top_k, dim=-1)

@@ -263,3 +263,13 @@ def test_a_block_with_a_balance_is_copied_and_saved(tmp_path):
     assert torch.equal(twin.balance.counts, block.balance.counts)
     torch.save(block, tmp_path / "block.pt")
     assert torch.load(tmp_path / "block.pt", weights_only=False).balance is None
+
+
+def test_a_forward_that_is_not_tracked_leaves_no_balance():
+    block, x = _tracked_block()
+    block.route(x)
+    block.track_balance = False
+    block.route(x)
+    assert block.balance is None
+    with pytest.raises(ValueError, match="track_balance"):
+        moe.balance_loss(block)
