@@ -175,12 +175,12 @@ class LlamaAttention(nn.Module):
 
     def _norm_and_rotate(self, q, k, cos, sin, half_tables):
         """Head norms and rotation of ``q, k (B, T, H, d)``, returned as ``(B, H, T, d)``: one
-        kernel, or the modules one by one where a hook watches a norm."""
+        kernel, or the modules one by one where a hook watches a norm or the heads are too wide."""
         from dattri_llm_b200.ops import fused
 
         watched = any(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks
                       for m in (self.q_norm, self.k_norm))
-        if half_tables is not None and fused.enabled(q) and not watched:
+        if half_tables is not None and fused.enabled(q) and self.head_dim <= fused.MAX_HEAD_DIM and not watched:
             q, k = fused.qk_norm_rope(q, k, self.q_norm.weight, self.k_norm.weight, *half_tables, eps=self.q_norm.eps)
             return q.transpose(1, 2), k.transpose(1, 2)
         return apply_rope(self.q_norm(q).transpose(1, 2), self.k_norm(k).transpose(1, 2), cos, sin)

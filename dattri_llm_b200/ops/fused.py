@@ -341,6 +341,9 @@ def causal_conv_silu(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor |
     return _CausalConvSiLU.apply(x, weight, bias)
 
 
+MAX_HEAD_DIM = 512  # of qk_norm_rope on the GPU (kMaxHeadDim of csrc/qk_norm.cuh)
+
+
 def _qk_norm_rope_torch(x, weight, cos, sin, eps):
     wide = torch.promote_types(x.dtype, torch.float32)
     half = cos.shape[-1]
@@ -358,7 +361,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
 
     Args:
         q, k: ``(B, T, Hq, D)`` and ``(B, T, Hk, D)`` of one type (bf16, fp16 or fp32 on the
-            GPU), ``D`` even and at most 512; any strides, e.g. slices of one projection's output.
+            GPU), ``D`` even and at most :data:`MAX_HEAD_DIM` there; any strides, e.g. slices of one projection's output.
         q_weight, k_weight: ``(D,)`` norm weights.
         cos, sin: ``(positions, R / 2)`` tables of the angles, ``R <= D``; element *i* is
             rotated with element ``i + R / 2``, elements from ``R`` on are not.

@@ -273,3 +273,14 @@ def test_a_forward_that_is_not_tracked_leaves_no_balance():
     assert block.balance is None
     with pytest.raises(ValueError, match="track_balance"):
         moe.balance_loss(block)
+
+
+@pytest.mark.gpu
+def test_head_norms_of_heads_wider_than_the_kernel_takes():
+    """Heads of more than 512 elements go through the modules, as on the CPU."""
+    model = LlamaForCausalLM(LlamaConfig.tiny(qk_norm=True, head_dim=528, num_attention_heads=2, num_key_value_heads=1))
+    model.reset_parameters(seed=0)
+    model, batch = model.to("cuda", torch.bfloat16), _batch("cuda", 2, 9)
+    got = model(**batch).logits
+    want = model.float()(**batch).logits  # the modules, in 32 bits
+    assert float((got.float() - want).norm()) <= 0.05 * float(want.norm())
