@@ -11,12 +11,18 @@
 // A row whose label is ignored is not read: whatever stands there, its log-probability is 0
 // and its gradient is 0.
 //
-// What bounds them: memory. Figures are of 8 x 1024 x 128256 bf16 logits, a quarter of the rows ignored, on one B200
-// whose copy rate is 6.55 TB/s:
-//     statistics  read 1.58 GB            266 us   5.9 TB/s   (the exponential's unit is 75 % busy beside it)
-//     gradient    read 1.58, write 2.10   607 us   6.1 TB/s
-//     policy      the same bytes, once    658 us   5.6 TB/s   with its two small kernels (686 us each of many passes, which
-//                                                             wait for one another's writes, with the backward's launch)
+// What bounds them. Long rows: memory. 8 x 1024 x 128256 bf16 logits, a quarter of the rows ignored, on one B200 whose copy
+// rate is 6.55 TB/s (launches one by one, the L2 flushed before each):
+//     statistics  read 1.58 GB            264 us   6.0 TB/s   (the exponential's unit is 68 % busy beside it)
+//     gradient    read 1.58, write 2.10   559 us   6.6 TB/s
+//     policy      the same bytes, once    641 us   5.7 TB/s   with its two small kernels
+//     gradient under a loss gradient that is not 1: read 1.58, write 1.58 (the ignored rows have their zeros) 510 us
+// Passes of a program one behind the other wait for one another's write-backs: 827..852 us for a preference step,
+// 644..700 us for a policy step, 1157 us for one whose loss gradient is not 1.
+// Short and middle rows: the chain of one row. A warp (or a small CTA) loads a row, takes its maximum, exponentials and
+// sums and leaves, with nothing of the next row on its way: 65536 x 1024 statistics 43 us where reading takes 15, with DRAM
+// 46 %, issue slots 64 % and the exponential's unit 55 % busy. Rows of 12 to 96 KB take the policy's second read from L2.
+// The table above kShort has them all with their floors.
 // The preference loss needs both passes over HBM, since a pair's coefficient needs every token of both sequences. The
 // policy's does not, and takes them in one kernel.
 // Tried and slower for the policy: the row in registers over a cluster of CTAs, joined through distributed shared memory
@@ -758,13 +764,15 @@ unsigned grid_of(const LogitRows& r) {
 }
 
 // The threads of a row by its vectors of 16 bytes. Short rows want warps (no barrier, four to a CTA), long ones threads
-// enough for their loads; measured in us on one B200, bf16, a quarter of the rows ignored, by threads of a row:
-//     rows x logits       vectors   statistics             gradient               policy
-//     65536 x 1024            128   32: 57,  128: 124      32: 76,  128: 123      32: 101, 128: 235
-//     32768 x 4000            500   32: 70,  128: 83       32: 112, 128: 115      32: 136, 128: 178
-//     16384 x 16000          2000   32: 103, 128: 94       32: 191, 256: 175      32: 242, 128: 212, 256: 243
-//     1998 x 32003 (fp16)    4000   128: 46, 512: 49       256: 78, 512: 79       128: 92, 256: 86, long: 92
-//     8192 x 128256         16032   128: 266, 512: 280     256: 620, 512: 605     256: 842, long: 658
+// enough for their loads; measured in us on one B200, bf16 (the fourth fp16), a quarter of the rows ignored, by threads of a
+// row, each launch by itself after a flush of the L2, with the loss's own small kernels (about 5 us). Before the bar: what
+// reading, or reading and writing, takes at the copy rate (writes of less than the L2's 126 MB need not wait for it):
+//     rows x logits   vectors   statistics                gradient                           policy
+//     65536 x 1024        128    15 | 32: 43,  128: 106    36 | 32: 37,  128: 86              36 | 32: 80,  128: 213
+//     32768 x 4000        500    30 | 32: 59,  128: 70     70 | 32: 68,  128: 76              70 | 32: 111, 128: 147
+//     16384 x 16000      2000    60 | 32: 96,  128: 88    140 | 32: 143, 128: 133, 256: 133  140 | 128: 190, 256: 219
+//     1998 x 32003       4000    15 | 128: 39, 512: 41     34 | 128: 37, 256: 33,  512: 41    34 | 128: 72, 256: 68
+//     8192 x 128256     16032   241 | 128: 264, 512: 266  561 | 256: 569, 512: 557           561 | 256: 813, long: 641
 constexpr int kShort = 768;
 
 template <typename T, int kGroup, int kMin>

@@ -68,7 +68,12 @@ def policy_token_terms(model: nn.Module, batch: dict, **options) -> PolicyLoss:
 def stacked_balance_loss(router_logits, top_k: int, attention_mask: torch.Tensor | None = None, *,
                          z_coef: float = 0.0) -> BalanceLoss:
     """Balance loss of every layer from the ``router_logits`` a Hugging Face expert model
-    returns (one ``(B * T, E)`` tensor for each layer), padded tokens left out."""
+    returns (one ``(B * T, E)`` tensor for each layer), padded tokens left out.
+
+    One loss for each layer; Hugging Face's own auxiliary loss joins the tokens of all layers
+    first.  The experts are chosen again from the logits, the lowest index where they tie: 16-bit
+    logits tie often and ``torch.topk`` promises no order, so the counts need not be those of
+    the model's routing (:func:`~dattri_llm_b200.ops.router_balance_loss` takes the model's ids)."""
     logits = torch.stack([x.reshape(-1, x.shape[-1]) for x in router_logits])
     mask = None
     if attention_mask is not None:
