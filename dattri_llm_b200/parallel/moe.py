@@ -665,13 +665,14 @@ class ExpertParallelMoE(nn.Module):
 
         The router runs on *x* in its own shape, so a capture hook on ``gate`` sees the
         ``(B, T, H)`` layout of the samples."""
-        self.balance = None  # the last forward's, whether or not it is tracked
         logits = self.gate(x)
         probs = torch.softmax(logits.float().reshape(-1, self.n_experts), dim=-1)
         topv, topi = probs.topk(self.top_k, dim=-1)
-        if self.track_balance:
+        if self.track_balance:  # assigned whole: a checkpoint's recomputation may stop within this call
             self.balance = router_balance_loss(logits.reshape(-1, self.n_experts), self.top_k, topi)
             self.balance_has_graph = torch.is_grad_enabled()
+        else:
+            self.balance = None  # not an earlier forward's
         if self.norm_topk_prob:
             topv = topv / topv.sum(-1, keepdim=True)
         return topv, topi

@@ -284,3 +284,14 @@ def test_head_norms_of_heads_wider_than_the_kernel_takes():
     got = model(**batch).logits
     want = model.float()(**batch).logits  # the modules, in 32 bits
     assert float((got.float() - want).norm()) <= 0.05 * float(want.norm())
+
+
+def test_the_balance_of_a_checkpointed_block_stays_after_its_backward():
+    """The recomputation stops once it has what the backward needs, which may be within the router."""
+    from torch.utils.checkpoint import checkpoint
+
+    block, x = _tracked_block()
+    y = checkpoint(lambda z: block.route(z)[0].sum(), x.requires_grad_(), use_reentrant=False)
+    counts = block.balance.counts
+    (y + moe.balance_loss(block)).backward()
+    assert torch.equal(block.balance.counts, counts)
