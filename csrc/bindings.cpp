@@ -31,6 +31,7 @@
 
 namespace bw {
 void register_post_training(pybind11::module_& m);  // post_training.cpp
+void register_trajectory(pybind11::module_& m);     // trajectory.cpp
 }
 
 namespace {
@@ -1388,4 +1389,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ce_bwd_inplace", &ce_bwd_inplace);
   bw::register_projector(m);
   bw::register_post_training(m);
+  bw::register_trajectory(m);
 }

@@ -36,6 +36,7 @@ from dattri_llm_b200.utils.hashing import hash_batch, hash_sample
 __version__ = "0.1.0"
 
 _LAZY_EXPORTS = {
+    "AdamW": "dattri_llm_b200.gradient.adamw",
     "GradientStreamer": "dattri_llm_b200.gradient.streaming",
     "DiskGradientSource": "dattri_llm_b200.gradient.streaming",
     "ReplayGradientSource": "dattri_llm_b200.gradient.streaming",

@@ -1,0 +1,101 @@
+"""AdamW over the multi-tensor kernel of :func:`dattri_llm_b200.ops.adamw_step`, moments in 32 or 8 bits.
+
+A trajectory's optimizer states outweigh its 16-bit weights four to one; in 8 bits they weigh
+as much as the weights.  The update rule is ``torch.optim.AdamW``'s, so everything that reads
+optimizer state (snapshots, preconditioned capture, the dynamics of AdamW-influence) follows
+it; :meth:`AdamW.moment` gives those readers the numbers that 8-bit states stand for.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from dattri_llm_b200.ops.optim import adamw_moments, adamw_state, adamw_step
+
+
+class AdamW(torch.optim.AdamW):
+    """``torch.optim.AdamW`` whose step is one launch for all tensors of a group and type.
+
+    Args:
+        state_bits: 32 (fp32 moments, whatever the parameters' type) or 8 (e4m3 codes with a
+            scale for every 256 elements); also a setting of a parameter group.
+
+    The update counts are kept on the host: a step is not captured into a CUDA graph, which
+    would repeat one count's bias correction.  Parameters sharded as DTensors (FSDP2) are not supported.
+    """
+
+    def __init__(self, params, lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, *, state_bits: int = 32, maximize: bool = False) -> None:
+        super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, maximize=maximize)
+        self.defaults["state_bits"] = state_bits
+        for group in self.param_groups:
+            self._settle(group)
+
+    def _settle(self, group: dict) -> None:
+        bits = group.setdefault("state_bits", self.defaults["state_bits"])
+        if bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {bits}")
+        for p in group["params"]:
+            if hasattr(p, "to_local") and hasattr(p, "placements"):
+                raise NotImplementedError("AdamW of this library steps whole tensors, not DTensors")
+
+    def add_param_group(self, param_group: dict) -> None:
+        super().add_param_group(param_group)
+        if "state_bits" in self.defaults:  # not while the base class is being made
+            self._settle(self.param_groups[-1])
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        """One update of every parameter that has a gradient."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("this optimizer counts its updates on the host: a captured step would repeat one count's "
+                               "bias correction")
+        for group in self.param_groups:
+            bits = group["state_bits"]
+            batches: dict[tuple, list[list]] = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                state = self.state[p]
+                if not state:
+                    state["step"] = torch.tensor(0.0)
+                    state["exp_avg"], state["exp_avg_sq"], scales = adamw_state(p, bits)
+                    if scales is not None:
+                        state["scales"] = scales
+                state["step"] += 1
+                lists = batches.setdefault((p.device, int(state["step"]), "scales" in state), [[], [], [], [], []])
+                for to, x in zip(lists, (p, p.grad, state["exp_avg"], state["exp_avg_sq"], state.get("scales")), strict=True):
+                    to.append(x)
+            for (_device, step, coded), (params, grads, m, v, scales) in batches.items():
+                adamw_step(params, grads, m, v, scales if coded else None, step=step, lr=float(group["lr"]),
+                           betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
+                           maximize=group["maximize"])
+        return loss
+
+    def moment(self, param: torch.Tensor, key: str) -> torch.Tensor | None:
+        """State *key* of *param* in the numbers it stands for; ``None`` before its first update."""
+        state = self.state.get(param, {})
+        if "scales" not in state or key not in ("exp_avg", "exp_avg_sq"):
+            return state.get(key)
+        m, v = adamw_moments(state["exp_avg"], state["exp_avg_sq"], state["scales"])
+        return m if key == "exp_avg" else v
+
+    def load_state_dict(self, state_dict: dict) -> None:
+        """As ``torch.optim``'s, without its cast of the states to the parameters' type."""
+        super().load_state_dict(state_dict)
+        saved = state_dict["state"]
+        ids = (i for group in state_dict["param_groups"] for i in group["params"])
+        params = (p for group in self.param_groups for p in group["params"])
+        for i, p in zip(ids, params, strict=True):
+            for key, value in saved.get(i, {}).items():
+                if isinstance(value, torch.Tensor) and value.dim() > 0:
+                    moved = value.detach().to(p.device, copy=True)
+                    if key != "scales" and moved.stride() != p.stride():  # codes and moments lie as the parameter does
+                        moved = torch.empty_like(p, dtype=value.dtype, requires_grad=False).copy_(moved)
+                    if key in ("exp_avg", "exp_avg_sq") and moved.dtype != torch.float8_e4m3fn:
+                        moved = moved.float()  # moments that another AdamW kept in the parameters' type
+                    self.state[p][key] = moved

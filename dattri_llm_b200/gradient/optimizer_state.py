@@ -98,6 +98,13 @@ def _all_reduce_sum(t: torch.Tensor) -> None:
         dist.all_reduce(t, op=dist.ReduceOp.SUM)
 
 
+def _state_value(optimizer: torch.optim.Optimizer, param: nn.Parameter, key: str):
+    """State *key* of *param*: through the optimizer's own reader where it holds states in
+    another form than their numbers (:meth:`dattri_llm_b200.gradient.adamw.AdamW.moment`)."""
+    reader = getattr(optimizer, "moment", None)
+    return reader(param, key) if callable(reader) else optimizer.state.get(param, {}).get(key)
+
+
 # ---------------------------------------------------------------------------------- sources
 @dataclass(frozen=True)
 class _Local:
@@ -110,7 +117,7 @@ class _Local:
         return tuple(self.param.shape)
 
     def read(self, optimizer, key):
-        return optimizer.state.get(self.param, {}).get(key)
+        return _state_value(optimizer, self.param, key)
 
 
 @dataclass(frozen=True)
@@ -143,7 +150,7 @@ class _FlatSlice:
         return self.full_shape
 
     def read(self, optimizer, key):
-        return optimizer.state.get(self.param, {}).get(key)
+        return _state_value(optimizer, self.param, key)
 
     def on_zeros(self, local: torch.Tensor | None, like: torch.Tensor) -> torch.Tensor:
         """This rank's piece of the full tensor, zeros elsewhere (summed over ranks later)."""
@@ -376,7 +383,7 @@ class OptimizerSnapshot:
             # every rank must take part in the sum, also one that holds none of this layer
             like = next((v for v in values.values() if v is not None), None)
             if like is None:
-                like = next((st[key] for st in self._optimizer.state.values() if key in st), None)
+                like = next((_state_value(self._optimizer, p, key) for p, st in self._optimizer.state.items() if key in st), None)
             if like is None:
                 return None
             if like.ndim == 0:

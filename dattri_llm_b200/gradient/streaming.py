@@ -704,8 +704,13 @@ class GradientStreamer(GradientSource):
             fused = bool(params) and all(p.is_cuda and p.is_floating_point() for p in params)
             opt = torch.optim.AdamW(groups, lr=a.learning_rate, betas=(a.adam_beta1, a.adam_beta2),
                                     eps=a.adam_epsilon, fused=True if fused else None)
+        elif a.optim in ("adamw_8bit", "adamw_bnb_8bit"):
+            from dattri_llm_b200.gradient.adamw import AdamW
+
+            opt = AdamW(groups, lr=a.learning_rate, betas=(a.adam_beta1, a.adam_beta2), eps=a.adam_epsilon, state_bits=8)
         else:
-            raise ValueError(f"optimizer {a.optim!r} is not supported by the streamer: use 'adamw_torch' or 'sgd'.")
+            raise ValueError(f"optimizer {a.optim!r} is not supported by the streamer: use 'adamw_torch', 'adamw_8bit' "
+                             "or 'sgd'.")
         updates = -(-len(self._loader) // self._window)
         return opt, _make_scheduler(a.lr_scheduler_type, opt, a.warmup_steps, updates)
 

@@ -11,13 +11,15 @@ from dattri_llm_b200.models.layers import TcLinear, tc_linearize
 from dattri_llm_b200.models.llama import LlamaConfig, LlamaForCausalLM, LlamaModel, token_sum_loss
 from dattri_llm_b200.models.mamba2 import accelerate_mamba2, ssd_chunked
 from dattri_llm_b200.models.post_training import (
+    entropy_regularized_loss,
     policy_token_loss,
     preference_pair_loss,
     shift_labels,
     stacked_balance_loss,
     token_logps,
+    token_quality,
 )
 
 __all__ = ["GPT2Config", "accelerate_mamba2", "ssd_chunked", "GPT2LMHeadModel", "LlamaConfig", "LlamaForCausalLM", "LlamaModel", "TcLinear",
-           "policy_token_loss", "preference_pair_loss", "shift_labels", "stacked_balance_loss", "tc_linearize", "token_logps",
+           "policy_token_loss", "preference_pair_loss", "shift_labels", "stacked_balance_loss", "tc_linearize", "token_logps", "token_quality", "entropy_regularized_loss",
            "token_sum_loss"]

@@ -16,6 +16,7 @@ import torch
 from torch import nn
 
 from dattri_llm_b200.ops.losses import BalanceLoss, PolicyLoss, PreferenceLoss, policy_loss, preference_loss, router_balance_loss
+from dattri_llm_b200.ops.scores import TokenScores, token_scores
 
 IGNORE = -100
 
@@ -38,6 +39,21 @@ def token_logps(model: nn.Module, batch: dict, *, temperature: float = 1.0) -> t
     labels = shift_labels(batch["labels"])
     zero = torch.zeros(labels.shape[0], device=labels.device)
     return policy_loss(_logits(model, batch), labels, zero, temperature=temperature, ignore_index=IGNORE).logps
+
+
+@torch.no_grad()
+def token_quality(model: nn.Module, batch: dict, *, top_k: int = 0, temperature: float = 1.0) -> TokenScores:
+    """:func:`~dattri_llm_b200.ops.token_scores` of the batch's labels under *model*, at the position that
+    predicts them: how likely and how uncertain the model finds each token, and what it would
+    have said instead (for choosing samples, or for reading an attribution)."""
+    return token_scores(_logits(model, batch), shift_labels(batch["labels"]), top_k=top_k, temperature=temperature,
+                        ignore_index=IGNORE)
+
+
+def entropy_regularized_loss(model: nn.Module, batch: dict, *, coef: float = 0.0, temperature: float = 1.0) -> torch.Tensor:
+    """Summed next-token loss less *coef* times the summed entropy of the predictions, in one pass over the logits."""
+    scores = token_scores(_logits(model, batch), shift_labels(batch["labels"]), temperature=temperature, ignore_index=IGNORE)
+    return -scores.logps.sum() - coef * scores.entropy.sum()
 
 
 def preference_pair_loss(model: nn.Module, batch: dict, *, reduction: str = "sum", **options) -> torch.Tensor:

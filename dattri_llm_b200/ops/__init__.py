@@ -32,7 +32,7 @@ def count_launch(n: int = 1) -> None:
 
 def launch_count() -> int:
     """Native kernels launched by this process so far."""
-    return _LAUNCHES[0] + (_C.post_training_launches() if _C is not None else 0)
+    return _LAUNCHES[0] + (_C.post_training_launches() + _C.trajectory_launches() if _C is not None else 0)
 
 
 _lock = threading.Lock()
@@ -172,8 +172,9 @@ from dattri_llm_b200.ops.losses import (  # noqa: E402
     router_balance_loss,
 )
 from dattri_llm_b200.ops.norm import embedding_dense_grad, norm_per_sample_grad  # noqa: E402
-from dattri_llm_b200.ops.optim import adam_direction  # noqa: E402
+from dattri_llm_b200.ops.optim import adam_direction, adamw_moments, adamw_state, adamw_step  # noqa: E402
 from dattri_llm_b200.ops.projection import projection_matrix_t  # noqa: E402
+from dattri_llm_b200.ops.scores import TokenScores, token_scores  # noqa: E402
 
 __all__ = [
     "BalanceLoss",
@@ -184,7 +185,11 @@ __all__ = [
     "STORE_BF16_T",
     "STORE_SQ_SUM_F32",
     "STORE_F32",
+    "TokenScores",
     "adam_direction",
+    "adamw_moments",
+    "adamw_state",
+    "adamw_step",
     "available",
     "check_device_errors",
     "count_launch",
@@ -209,5 +214,6 @@ __all__ = [
     "projection_matrix_t",
     "qk_norm_rope",
     "router_balance_loss",
+    "token_scores",
     "use_native",
 ]

@@ -1,0 +1,292 @@
+"""The AdamW step of many tensors and the optimizer over it, against the formula in 64 bits and ``torch.optim.AdamW``.
+
+Tolerances count roundings: a result is rounded once to its type (``eps / 2`` relative); before that come a handful of
+fp32 operations on values no larger than the terms of each sum (2^-21 of them covers eight). A code of 4 bits of
+significand is off by 2^-4 of its value, or by half a step of the smallest codes (2^-10 of the scale).
+"""
+
+import copy
+
+import pytest
+import torch
+
+import dattri_llm_b200 as bw
+from dattri_llm_b200 import ops
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+HYPER = {"lr": 3e-3, "betas": (0.9, 0.99), "eps": 1e-7, "weight_decay": 0.1}
+SLACK = 2.0 ** -21
+
+
+def make(shapes, dtype, device, *, bits, grad_dtype=None, seed=0, offset=0):
+    gen = torch.Generator().manual_seed(seed)
+    params, grads, m, v, scales = [], [], [], [], []
+    for i, shape in enumerate(shapes):
+        n = int(torch.tensor(shape).prod()) if shape else 1
+
+        def place(x, dt):  # at an odd place of a larger buffer, where the test asks for it
+            buf = torch.empty(n + offset, dtype=dt, device=device)
+            out = buf[offset:].view(shape)
+            out.copy_(x)
+            return out
+
+        p = place(torch.randn(shape, generator=gen), dtype)
+        g = place(torch.randn(shape, generator=gen) * 10.0 ** (-(i % 5)), grad_dtype or dtype)
+        if n > 6:
+            g.view(-1)[:3] = 0
+        m0 = torch.randn(shape, generator=gen).to(device) * 10.0 ** (-(i % 5))
+        v0 = (torch.randn(shape, generator=gen).to(device) * 10.0 ** (-(i % 5))).square()
+        if bits == 32:
+            m.append(place(m0, torch.float32))
+            v.append(place(v0, torch.float32))
+        else:
+            sc = torch.zeros(2, -(-n // 256), device=device)
+            for x, row, to in ((m0, 0, m), (v0.sqrt(), 1, v)):
+                flat = torch.nn.functional.pad(x.reshape(-1), (0, -n % 256)).view(-1, 256)
+                if n:
+                    sc[row] = flat.abs().amax(1) / 448
+                codes = (flat / sc[row][:, None].clamp(min=1e-30)).clamp(-448, 448).to(torch.float8_e4m3fn).view(-1)[:n]
+                to.append(place(torch.zeros(shape), torch.float8_e4m3fn))
+                to[-1].copy_(codes.view(shape))
+            scales.append(sc)
+        params.append(p)
+        grads.append(g)
+    return params, grads, m, v, scales or None
+
+
+def exact(p, g, m, v, step, maximize=False):
+    b1, b2 = HYPER["betas"]
+    p, g, m, v = (x.double() for x in (p, -g if maximize else g, m, v))
+    m = b1 * m + (1 - b1) * g
+    v = b2 * v + (1 - b2) * g * g
+    move = HYPER["lr"] * (m / (1 - b1 ** step)) / ((v / (1 - b2 ** step)).sqrt() + HYPER["eps"])
+    return p * (1 - HYPER["lr"] * HYPER["weight_decay"]) - move, m, v, move
+
+
+def check(shapes, dtype, device, bits, step, **kw):
+    maximize = kw.pop("maximize", False)
+    params, grads, m, v, scales = make(shapes, dtype, device, bits=bits, **kw)
+    start = []
+    for i, p in enumerate(params):
+        wide = ops.adamw_moments(m[i], v[i], None if scales is None else scales[i])
+        start.append((p.clone(), grads[i].clone(), wide[0].clone(), wide[1].clone()))
+    ops.adamw_step(params, grads, m, v, scales, step=step, maximize=maximize, **HYPER)
+    half = torch.finfo(dtype).eps / 2
+    for i, p in enumerate(params):
+        old, g, m0, v0 = start[i]
+        want, wm, wv, move = exact(old, g, m0, v0, step, maximize)
+        off = (p.double() - want).abs()
+        assert (off <= half * want.abs() + SLACK * (old.double().abs() + move.abs()) + torch.finfo(dtype).smallest_normal).all()
+        gm, gv = ops.adamw_moments(m[i], v[i], None if scales is None else scales[i])
+        terms_m = m0.double().abs() + g.double().abs()
+        terms_v = v0.double() + g.double().square()
+        if bits == 32:
+            assert ((gm.double() - wm).abs() <= SLACK * terms_m).all()
+            assert ((gv.double() - wv).abs() <= SLACK * terms_v + 1e-44).all()
+            continue
+        n = p.numel()
+        for got, true, row, smallest in ((gm, wm, 0, 2.0 ** -10), (gv.sqrt(), wv.sqrt(), 1, 2.0 ** -9)):
+            flat = torch.nn.functional.pad(true.reshape(-1), (0, -n % 256)).view(-1, 256)
+            scale = flat.abs().amax(1) / 448 if n else flat.new_zeros(0)
+            assert ((scales[i][row].double() - scale).abs() <= SLACK * (scale + terms_m.amax() / 448 if n else scale)).all()
+            each = scale.repeat_interleave(256)[:n].view(p.shape)
+            assert ((got.double() - true).abs() <= (2.0 ** -4 + SLACK) * true.abs() + (smallest + SLACK) * each).all()
+            if row == 1:
+                assert (got[true > 0] > 0).all()  # a root that is not zero keeps a code
+                assert (got[true == 0] == 0).all()
+
+
+SHAPES = [(3,), (256,), (257,), (0,), (1,), (17, 31), (8192,), (8200,), (3, 5, 7), (64, 256), ()]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("step", [1, 1000])
+def test_step_matches_the_formula(device, bits, dtype, step):
+    check(SHAPES, dtype, device, bits, step)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [8, 32])
+def test_tensors_that_start_anywhere_and_gradients_in_32_bits(device, bits):
+    check(SHAPES, torch.bfloat16, device, bits, 3, offset=1)
+    check(SHAPES, torch.bfloat16, device, bits, 3, grad_dtype=torch.float32, maximize=True)
+    check(SHAPES, torch.float16, device, bits, 3, grad_dtype=torch.float32, offset=3)
+    check(SHAPES, torch.float32, device, bits, 3, offset=2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
+def test_more_tensors_than_one_launch_takes_and_a_large_one(bits):
+    check([(1 + i % 700,) for i in range(1111)], torch.float32, "cuda", bits, 2)
+    check([(1037, 4099)], torch.bfloat16, "cuda", bits, 2)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [8, 32])
+def test_axes_in_any_order(device, bits):
+    """A transposed parameter and a gradient laid out otherwise: the same numbers as contiguous ones give."""
+    torch.manual_seed(0)
+    w = torch.randn(40, 33, device=device)
+    g = torch.randn(40, 33, device=device)
+    results = []
+    for p, grad in ((w.t().contiguous().t(), g.clone()), (w.clone(), g.t().contiguous().t())):
+        state = ops.adamw_state(p, bits)
+        ops.adamw_step([p], [grad], [state[0]], [state[1]], None if bits == 32 else [state[2]], step=1, **HYPER)
+        m, _ = ops.adamw_moments(*state)
+        assert m.stride() == p.stride()
+        results.append(p.clone())
+    assert torch.equal(results[0], results[1])  # the step uses the moments before they become codes
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_state_of_zeros_and_tiny_and_infinite_gradients(device):
+    p = torch.ones(600, device=device)
+    m, v, s = ops.adamw_state(p, 8)
+    ops.adamw_step([p], [torch.zeros(600, device=device)], [m], [v], [s], step=1, **HYPER)
+    assert torch.equal(s, torch.zeros_like(s)) and torch.isfinite(p).all()
+    g = torch.full((600,), 1e-30, device=device)
+    g[300:] = 0
+    ops.adamw_step([p], [g], [m], [v], [s], step=2, **HYPER)
+    assert torch.isfinite(p).all() and all(torch.isfinite(x).all() for x in ops.adamw_moments(m, v, s))
+    g = torch.zeros(600, device=device)
+    g[5] = float("nan")
+    g[300] = float("inf")
+    ops.adamw_step([p], [g], [m], [v], [s], step=3, **HYPER)
+    assert torch.isnan(p[5]) and torch.isnan(p[300])  # as every AdamW has it
+    assert torch.isfinite(p[512:]).all()  # their block is theirs alone
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals(device):
+    p = torch.randn(8, 4, device=device)
+    m, v, _ = ops.adamw_state(p)
+    g = torch.randn_like(p)
+    ok = {"step": 1, "lr": 0.1}
+    with pytest.raises(ValueError, match="twice"):
+        ops.adamw_step([p, p], [g, g], [m, m.clone()], [v, v.clone()], **ok)
+    with pytest.raises(ValueError, match="needs a gradient"):
+        ops.adamw_step([p], [], [m], [v], **ok)
+    with pytest.raises(ValueError, match="shape"):
+        ops.adamw_step([p], [g[:4]], [m], [v], **ok)
+    with pytest.raises(ValueError, match="strides"):
+        ops.adamw_step([p], [g], [m.t().contiguous().t()], [v], **ok)
+    with pytest.raises(TypeError):
+        ops.adamw_step([p], [g], [m.to(torch.bfloat16)], [v], **ok)
+    with pytest.raises(TypeError):
+        ops.adamw_step([p], [g], [m], [v], [torch.zeros(2, 1, device=device)], **ok)
+    with pytest.raises(ValueError, match="scales"):
+        m8, v8, s = ops.adamw_state(p, 8)
+        ops.adamw_step([p], [g], [m8], [v8], [torch.zeros(2, 3, device=device)], **ok)
+    with pytest.raises(NotImplementedError):
+        ops.adamw_step([p], [g.to_sparse()], [m], [v], **ok)
+    with pytest.raises(ValueError, match="step"):
+        ops.adamw_step([p], [g], [m], [v], step=0, lr=0.1)
+    with pytest.raises(ValueError):
+        ops.adamw_state(p, 4)
+    with pytest.raises(ValueError, match="state_bits"):
+        bw.AdamW([torch.nn.Parameter(p)], state_bits=16)
+
+
+def _steps(opt, p, grads):
+    for g in grads:
+        p.grad = g.clone()
+        opt.step()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_optimizer_follows_torch(device):
+    torch.manual_seed(1)
+    start = torch.randn(50, 70, device=device)
+    grads = [torch.randn(50, 70, device=device) for _ in range(12)]
+    mine, theirs, coded = (torch.nn.Parameter(start.clone()) for _ in range(3))
+    kw = {"lr": 1e-2, "betas": (0.9, 0.95), "weight_decay": 0.2}
+    a, b, c = bw.AdamW([mine], **kw), torch.optim.AdamW([theirs], **kw), bw.AdamW([coded], state_bits=8, **kw)
+    _steps(a, mine, grads)
+    _steps(b, theirs, grads)
+    _steps(c, coded, grads)
+    # 12 steps of at most lr (1 + small) each, every one of them off by some 2^-21 of its parts
+    assert (mine - theirs).abs().max() <= 12 * SLACK * (start.abs().max() + 1)
+    # a code is off by 2^-4 each step and a moment remembers 10 or 20 steps of it: well below the 0.12 the weights move
+    assert (coded - theirs).abs().max() <= 12 * kw["lr"] * 0.5
+    assert c.state[coded]["exp_avg"].dtype == torch.float8_e4m3fn
+    assert torch.equal(a.moment(mine, "exp_avg"), a.state[mine]["exp_avg"])
+    assert ((c.moment(coded, "exp_avg") - b.state[theirs]["exp_avg"]).abs() <= 0.5).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [8, 32])
+def test_saved_and_loaded_it_goes_on_as_before(device, bits):
+    torch.manual_seed(2)
+    start = torch.randn(300, device=device, dtype=torch.bfloat16)
+    grads = [torch.randn(300, device=device, dtype=torch.bfloat16) for _ in range(6)]
+    p = torch.nn.Parameter(start.clone())
+    opt = bw.AdamW([p], state_bits=bits)
+    _steps(opt, p, grads[:3])
+    saved, weights = copy.deepcopy(opt.state_dict()), p.detach().clone()
+    _steps(opt, p, grads[3:])
+    q = torch.nn.Parameter(weights)
+    other = bw.AdamW([q], state_bits=bits)
+    other.load_state_dict(saved)
+    assert other.state[q]["exp_avg"].dtype == (torch.float32 if bits == 32 else torch.float8_e4m3fn)  # not the weights' type
+    _steps(other, q, grads[3:])
+    assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_what_autograd_saved_is_seen_to_have_changed(device):
+    w = torch.nn.Parameter(torch.randn(4, 4, device=device))
+    x = torch.randn(4, 4, device=device, requires_grad=True)
+    y = (x @ w).sum()
+    w.grad = torch.ones_like(w)
+    bw.AdamW([w]).step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_snapshots_read_coded_states(device):
+    """The optimizer-state reader gives 8-bit moments as the numbers they stand for."""
+    from dattri_llm_b200.gradient.optimizer_state import OptimizerSnapshot, optimizer_from_state_dict
+
+    torch.manual_seed(3)
+    model = torch.nn.Sequential(torch.nn.Linear(9, 5)).to(device)
+    opt = bw.AdamW(model.parameters(), state_bits=8)
+    for _ in range(3):
+        model(torch.randn(4, 9, device=device)).square().sum().backward()
+        opt.step()
+        opt.zero_grad()
+    reader = OptimizerSnapshot(model, opt)
+    assert reader.optimizer_type == "AdamW" and reader.step_count("0") == 3
+    weight, bias = model[0].weight, model[0].bias
+    want = torch.cat([opt.moment(weight, "exp_avg_sq"), opt.moment(bias, "exp_avg_sq").unsqueeze(1)], 1).reshape(-1)
+    got = reader.state("0", "exp_avg_sq")
+    assert got.dtype == torch.float32 and torch.equal(got.reshape(-1).sort().values, want.sort().values)
+    direction = reader.precondition("0", torch.randn(2, got.numel(), device=device))
+    assert torch.isfinite(direction).all()
+    names = [n for n, _ in model.named_parameters()]
+    again = optimizer_from_state_dict(model, copy.deepcopy(opt.state_dict()), names, optimizer_cls=bw.AdamW)
+    assert torch.equal(OptimizerSnapshot(model, again).state("0", "exp_avg"), reader.state("0", "exp_avg"))
+
+
+@pytest.mark.gpu
+def test_another_stream_and_a_captured_step():
+    torch.manual_seed(4)
+    p, g = torch.randn(5000, device="cuda"), torch.randn(5000, device="cuda")
+    m, v, s = ops.adamw_state(p, 8)
+    want = p.clone()
+    wm, wv, ws = ops.adamw_state(p, 8)
+    for _ in range(3):
+        ops.adamw_step([want], [g], [wm], [wv], [ws], step=1, lr=0.1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.adamw_step([p], [g], [m], [v], [s], step=1, lr=0.1)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.adamw_step([p], [g], [m], [v], [s], step=1, lr=0.1)
+    graph.replay()
+    graph.replay()
+    assert torch.equal(p, want) and torch.equal(s, ws)
