@@ -1,4 +1,4 @@
-// Bindings of the operators of trajectory training: the AdamW step of many tensors and token scores. Arguments are
+// Bindings of the operators of trajectory training: the AdamW step of many tensors, token scores and the gated delta rule. Arguments are
 // checked here and autograd functions are C++ for the reasons that post_training.cpp gives.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
@@ -9,6 +9,7 @@
 #include <unordered_set>
 
 #include "adamw.cuh"
+#include "delta_rule.cuh"
 #include "entry.h"
 #include "token_scores.cuh"
 
@@ -196,6 +197,249 @@ variable_list token_scores(Tensor logits, Tensor labels, int64_t top, double tem
   return out;
 }
 
+// ---------------------------------------------------------------- gated delta rule
+struct DeltaIn {
+  Tensor q, k, v, a, b, a_log, dt_bias;
+};
+
+bw::HeadRows head_rows(const Tensor& t) {
+  return bw::HeadRows{t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)};
+}
+
+// Rows on 16-byte boundaries.
+bool rows_aligned(const Tensor& t) {
+  const int64_t n = 16 / t.element_size();
+  for (int i = 0; i < 3; ++i)
+    if (t.size(i) > 1 && t.stride(i) % n != 0) return false;
+  return at_multiple(t.data_ptr(), 16);
+}
+
+bw::DeltaDims delta_dims(const DeltaIn& x, double scale) {
+  bw::DeltaDims d;
+  d.B = (int)x.q.size(0);
+  d.T = (int)x.q.size(1);
+  d.Hk = (int)x.q.size(2);
+  d.dk = (int)x.q.size(3);
+  d.H = (int)x.v.size(2);
+  d.dv = (int)x.v.size(3);
+  d.chunks = (d.T + bw::kChunk - 1) / bw::kChunk;
+  d.type = elem_of(x.q, "q");
+  d.scale = (float)scale;
+  d.wide = rows_aligned(x.q) && rows_aligned(x.k) && rows_aligned(x.v);
+  return d;
+}
+
+bw::DeltaGates delta_gates(const DeltaIn& x) {
+  return bw::DeltaGates{head_rows(x.a), head_rows(x.b), x.a_log.data_ptr(), x.dt_bias.data_ptr(), elem_of(x.a_log, "a_log"),
+                        elem_of(x.dt_bias, "dt_bias")};
+}
+
+// Checks the arguments and brings them into a form that the kernels read; the scale.
+double take_delta(DeltaIn& x, const std::optional<double>& scale) {
+  for (const auto& [t, name] : {std::pair<const Tensor&, const char*>{x.q, "q"}, {x.k, "k"}, {x.v, "v"}, {x.a, "a"}, {x.b, "b"},
+                                {x.a_log, "a_log"}, {x.dt_bias, "dt_bias"}}) {
+    plain(t, name);
+    TORCH_CHECK_VALUE(t.device() == x.q.device(), name, " is on ", t.device(), ", q on ", x.q.device());
+  }
+  TORCH_CHECK_VALUE(x.q.dim() == 4 && x.q.sizes() == x.k.sizes() && x.v.dim() == 4 && x.v.size(0) == x.q.size(0) &&
+                        x.v.size(1) == x.q.size(1),
+                    "q and k must be (B, T, Hk, dk), v (B, T, H, dv) with the same B and T");
+  const int64_t B = x.q.size(0), T = x.q.size(1), Hk = x.q.size(2), H = x.v.size(2), dk = x.q.size(3), dv = x.v.size(3);
+  TORCH_CHECK_VALUE(Hk > 0 && H > 0 && H % Hk == 0 && H / Hk <= bw::kMostGroup, "v must have 1 to ", std::to_string(bw::kMostGroup),
+                    " heads for each head of q and k");
+  TORCH_CHECK_VALUE(dk >= 8 && dk % 8 == 0 && dk <= bw::kMostKeyDim, "heads of q and k must have 8 to ",
+                    std::to_string(bw::kMostKeyDim), " elements, a multiple of 8");
+  TORCH_CHECK_VALUE(dv >= 8 && dv % 8 == 0 && dv <= 1024, "heads of v must have 8 to 1024 elements, a multiple of 8");
+  for (const Tensor* t : {&x.a, &x.b})
+    TORCH_CHECK_VALUE(t->dim() == 3 && t->size(0) == B && t->size(1) == T && t->size(2) == H, "a and b must be (B, T, H)");
+  for (const Tensor* t : {&x.a_log, &x.dt_bias}) TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == H, "a_log and dt_bias must be (H,)");
+  for (const Tensor* t : {&x.k, &x.v, &x.a, &x.b})
+    TORCH_CHECK_TYPE(t->scalar_type() == x.q.scalar_type(), "q, k, v, a and b must be of one type, got ", x.q.scalar_type(), " and ",
+                     t->scalar_type());
+  // 2^31 - 1 blocks at most, of one value head's slice of 32 columns
+  TORCH_CHECK_VALUE(T < (int64_t(1) << 31) - 64 && B * H * ((T + 63) / 64 + 1) * ((dv + 31) / 32) < (int64_t(1) << 31),
+                    "the batch has too many tokens and heads for one call");
+  for (Tensor* t : {&x.q, &x.k, &x.v})
+    if (t->stride(3) != 1) *t = t->contiguous();
+  x.a_log = x.a_log.contiguous();
+  x.dt_bias = x.dt_bias.contiguous();
+  if (!scale.has_value()) return 1.0 / std::sqrt((double)dk);
+  TORCH_CHECK_VALUE(*scale > 0 && std::isfinite(*scale), "scale must be positive");
+  return *scale;
+}
+
+Tensor take_state(const Tensor& state, const DeltaIn& x, const char* name) {
+  plain(state, name);
+  const std::vector<int64_t> want{x.q.size(0), x.v.size(2), x.q.size(3), x.v.size(3)};
+  TORCH_CHECK_VALUE(state.device() == x.q.device() && state.sizes() == at::IntArrayRef(want), name,
+                    " must be (B, H, dk, dv) on the device of q");
+  TORCH_CHECK_TYPE(state.scalar_type() == torch::kFloat32, name, " must be float32, got ", state.scalar_type());
+  return state;
+}
+
+// The forward's workspace, kept for the backward where there is one.
+struct Kept {
+  Tensor halves, floats;  // 16-bit planes: solve, attend, writes, states; 32-bit: total, beta, rk, rq
+};
+
+// Elements of each part, each part on a 16-byte boundary.
+struct KeptSizes {
+  int64_t square, writes, states, tokens, rows;
+  explicit KeptSizes(const bw::DeltaDims& d) {
+    const int64_t n = (int64_t)d.B * d.H * d.chunks;
+    square = n * 2 * bw::kChunk * bw::kChunk;
+    writes = n * 2 * bw::kChunk * d.dv;
+    states = (int64_t)d.B * d.H * (d.chunks + 1) * 2 * d.dk * d.dv;
+    tokens = n * bw::kChunk;
+    rows = (int64_t)d.B * d.Hk * d.chunks * bw::kChunk;
+  }
+};
+
+Kept make_kept(const bw::DeltaDims& d, const Tensor& like) {
+  const KeptSizes z(d);
+  return Kept{torch::empty({2 * z.square + z.writes + z.states}, like.options().dtype(torch::kBFloat16)),
+              torch::empty({3 * z.tokens + 2 * z.rows}, like.options().dtype(torch::kFloat32))};
+}
+
+bw::DeltaKept kept_parts(const bw::DeltaDims& d, const Kept& k) {
+  const KeptSizes z(d);
+  auto* h = reinterpret_cast<__nv_bfloat16*>(k.halves.data_ptr());
+  float* f = k.floats.data_ptr<float>();
+  return bw::DeltaKept{h, h + z.square, h + 2 * z.square, h + 2 * z.square + z.writes, reinterpret_cast<float2*>(f),
+                       f + 2 * z.tokens, f + 3 * z.tokens, f + 3 * z.tokens + z.rows};
+}
+
+// {out, last state (or nothing)}; what it leaves in `kept`.
+std::pair<Tensor, Tensor> delta_fwd(const DeltaIn& x, const OptTensor& first, bool want_last, double scale, Kept& kept) {
+  const c10::cuda::CUDAGuard guard(x.q.device());
+  bw::DeltaFwd f;
+  f.d = delta_dims(x, scale);
+  f.q = head_rows(x.q);
+  f.k = head_rows(x.k);
+  f.v = head_rows(x.v);
+  f.g = delta_gates(x);
+  kept = make_kept(f.d, x.q);
+  f.keep = kept_parts(f.d, kept);
+  auto out = torch::empty({f.d.B, f.d.T, f.d.H, f.d.dv}, x.v.options());
+  Tensor last;
+  if (want_last) last = torch::empty({f.d.B, f.d.H, f.d.dk, f.d.dv}, x.q.options().dtype(torch::kFloat32));
+  f.first = floats(first);
+  f.last = want_last ? last.data_ptr<float>() : nullptr;
+  f.out = out.data_ptr();
+  launches += bw::delta_rule_fwd(f, at::cuda::getCurrentCUDAStream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {out, last};
+}
+
+struct GatedDelta : torch::autograd::Function<GatedDelta> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& a,
+                               const Tensor& b, const Tensor& a_log, const Tensor& dt_bias, const OptTensor& first, bool want_last,
+                               double scale) {
+    Kept kept;
+    auto [out, last] = delta_fwd(DeltaIn{q, k, v, a, b, a_log, dt_bias}, first, want_last, scale, kept);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({q, k, v, a, b, a_log, dt_bias, kept.halves, kept.floats});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["first"] = first.has_value();
+    if (!want_last) return {out};
+    return {out, last};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    variable_list grads(10);
+    const bool handed = g.size() > 1 && g[1].defined();
+    if (!g[0].defined() && !handed) return grads;
+    const auto s = ctx->get_saved_variables();
+    const DeltaIn x{s[0], s[1], s[2], s[3], s[4], s[5], s[6]};
+    const c10::cuda::CUDAGuard guard(x.q.device());
+    bw::DeltaBwd w;
+    w.d = delta_dims(x, ctx->saved_data["scale"].toDouble());
+    w.q = head_rows(x.q);
+    w.k = head_rows(x.k);
+    w.v = head_rows(x.v);
+    w.g = delta_gates(x);
+    w.keep = kept_parts(w.d, Kept{s[7], s[8]});
+    Tensor g_out = g[0].defined() ? g[0].contiguous() : torch::zeros({w.d.B, w.d.T, w.d.H, w.d.dv}, x.v.options());
+    if (!at_multiple(g_out.data_ptr(), 16)) g_out = g_out.clone();
+    w.g_out = g_out.data_ptr();
+    Tensor g_last;
+    if (handed) g_last = g[1].contiguous();
+    w.g_last = handed ? g_last.data_ptr<float>() : nullptr;
+    const int64_t n = (int64_t)w.d.B * w.d.H * w.d.chunks;
+    auto half = torch::empty({n * 2 * ((int64_t)w.d.dk + bw::kChunk) * w.d.dv}, x.q.options().dtype(torch::kBFloat16));
+    auto part = torch::empty({2 * n}, x.q.options().dtype(torch::kFloat32));
+    w.dstates = reinterpret_cast<__nv_bfloat16*>(half.data_ptr());
+    w.dreads = w.dstates + n * 2 * w.d.dk * w.d.dv;
+    w.part = part.data_ptr<float>();
+    for (int i = 0; i < 7; ++i) grads[i] = torch::empty(s[i].sizes(), s[i].options());
+    w.dq = grads[0].data_ptr();
+    w.dk = grads[1].data_ptr();
+    w.dv = grads[2].data_ptr();
+    w.da = grads[3].data_ptr();
+    w.db = grads[4].data_ptr();
+    w.da_log = grads[5].data_ptr();
+    w.ddt_bias = grads[6].data_ptr();
+    w.dfirst = nullptr;
+    if (ctx->saved_data["first"].toBool()) {
+      grads[7] = torch::empty({w.d.B, w.d.H, w.d.dk, w.d.dv}, x.q.options().dtype(torch::kFloat32));
+      w.dfirst = grads[7].data_ptr<float>();
+    }
+    launches += bw::delta_rule_bwd(w, at::cuda::getCurrentCUDAStream());
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    return once(std::move(grads), "gated_delta_rule");
+  }
+};
+
+std::pair<Tensor, OptTensor> gated_delta_rule(Tensor q, Tensor k, Tensor v, Tensor a, Tensor b, Tensor a_log, Tensor dt_bias,
+                                              OptTensor first, bool want_last, std::optional<double> scale) {
+  DeltaIn x{q, k, v, a, b, a_log, dt_bias};
+  const double by = take_delta(x, scale);
+  TORCH_CHECK_TYPE(x.q.scalar_type() == torch::kBFloat16 || x.q.scalar_type() == torch::kHalf,
+                   "q, k, v, a and b must be bfloat16 or float16 on the GPU, got ", x.q.scalar_type());
+  if (first.has_value()) first = take_state(*first, x, "initial_state").contiguous();
+  bool tracked = first.has_value() && wants_grad(*first);
+  for (const Tensor* t : {&x.q, &x.k, &x.v, &x.a, &x.b, &x.a_log, &x.dt_bias}) tracked = tracked || wants_grad(*t);
+  if (!tracked) {
+    Kept kept;
+    auto [out, last] = delta_fwd(x, first, want_last, by, kept);
+    return {out, want_last ? OptTensor(last) : std::nullopt};
+  }
+  auto out = GatedDelta::apply(x.q, x.k, x.v, x.a, x.b, x.a_log, x.dt_bias, first, want_last, by);
+  return {out[0], want_last ? OptTensor(out[1]) : std::nullopt};
+}
+
+Tensor gated_delta_step(Tensor q, Tensor k, Tensor v, Tensor a, Tensor b, Tensor a_log, Tensor dt_bias, Tensor state,
+                        std::optional<double> scale) {
+  DeltaIn x{q, k, v, a, b, a_log, dt_bias};
+  const double by = take_delta(x, scale);
+  elem_of(x.q, "q, k, v, a and b");
+  take_state(state, x, "state");
+  for (const Tensor* t : {&x.q, &x.k, &x.v, &x.a, &x.b, &x.a_log, &x.dt_bias, &state})
+    TORCH_CHECK(!wants_grad(*t), "gated_delta_step has no gradient: call it under torch.no_grad(), or gated_delta_rule");
+  const int64_t dk = x.q.size(3), dv = x.v.size(3);
+  TORCH_CHECK_VALUE((state.stride(3) == 1 && state.stride(2) == dv && state.stride(1) % 4 == 0 && state.stride(0) % 4 == 0 &&
+                     at_multiple(state.data_ptr(), 16)) || state.numel() == 0,
+                    "state must be contiguous along dk and dv, each head's on a 16-byte boundary");
+  TORCH_CHECK_VALUE(state.numel() == 0 || ((state.size(1) == 1 || state.stride(1) >= dk * dv) && (state.size(0) == 1 || state.stride(0) >= dk * dv)),
+                    "state: the heads must not overlap");
+  const c10::cuda::CUDAGuard guard(x.q.device());
+  bw::DeltaStep s;
+  s.d = delta_dims(x, by);
+  s.q = head_rows(x.q);
+  s.k = head_rows(x.k);
+  s.v = head_rows(x.v);
+  s.g = delta_gates(x);
+  auto out = torch::empty({s.d.B, s.d.T, s.d.H, s.d.dv}, x.v.options());
+  s.state = state.data_ptr<float>();
+  s.ssb = state.stride(0);
+  s.ssh = state.stride(1);
+  s.out = out.data_ptr();
+  bw::delta_step(s, at::cuda::getCurrentCUDAStream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  ++launches;
+  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
+  return out;
+}
+
 }  // namespace
 
 namespace bw {
@@ -203,6 +447,8 @@ namespace bw {
 void register_trajectory(pybind11::module_& m) {
   m.def("adamw_step", &::adamw_step, "AdamW step of many tensors, moments in 32 or 8 bits");
   m.def("token_scores", &::token_scores, "log-probabilities, entropies and best alternatives from logits");
+  m.def("gated_delta_rule", &::gated_delta_rule, "gated delta rule in chunks");
+  m.def("gated_delta_step", &::gated_delta_step, "gated delta rule token by token, the state updated in place");
   m.def("trajectory_launches", [] { return launches.load(); }, "kernels that these functions launched");
 }
 

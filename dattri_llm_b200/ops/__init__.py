@@ -142,6 +142,7 @@ def check_device_errors(device: torch.device | int | None = None) -> None:
             )
 
 
+from dattri_llm_b200.ops.delta import gated_delta_rule, gated_delta_step  # noqa: E402
 from dattri_llm_b200.ops.fused import qk_norm_rope  # noqa: E402
 from dattri_llm_b200.ops.gemm import (  # noqa: E402
     STORE_ATOMIC_F32,
@@ -194,6 +195,8 @@ __all__ = [
     "check_device_errors",
     "count_launch",
     "error_word",
+    "gated_delta_rule",
+    "gated_delta_step",
     "gemm_grouped",
     "gemm_tn",
     "gemm_tn_seg",
