@@ -15,7 +15,7 @@ namespace {
 constexpr int kCols = 32, kThreads = 256, kRowsOf = kMostKeyDim / 32;  // rows of a thread at most
 
 template <typename I>
-__global__ void __launch_bounds__(kThreads) step_kernel(const DeltaStep s) {
+__global__ void __launch_bounds__(kThreads, 4) step_kernel(const DeltaStep s) {
   __shared__ float rows[2][kMostKeyDim];  // q, k
   __shared__ float part[2][8][kCols];
   __shared__ float norm[2];

@@ -10,8 +10,10 @@
 //
 // Alternatives. In the pass each thread only keeps the maximum of its own elements (packed maxima, which the running
 // maximum needs anyway). The K-th largest of these maxima is a lower bound of the K-th largest logit, so that the K
-// best lie within the elements of the threads that reach it: K threads of the row's, plus ties. Warps read those
-// elements again, from the L2 for the most part, and keep a sorted list with one entry for each lane; one warp merges the lists.
+// best lie within the elements of the threads that reach it: K threads of the row's, plus ties. A search over the bits of
+// the maxima finds the bound; all threads read those elements again, from the L2 for the most part, and note the ones
+// that reach it, hardly more than K; each of those is ranked by counting the larger ones. Where ties make them more than
+// kNoted, one warp takes them into a sorted list with an entry for each lane instead.
 //
 // A row whose label is ignored is not read. A NaN in a row makes its numbers NaN; among the alternatives it is the
 // largest.
@@ -21,6 +23,8 @@
 
 namespace bw {
 namespace {
+
+using bf16 = __nv_bfloat16;
 
 // t below this adds nothing to s or w: 2^-200 is 0. It stands for -inf, which would make a NaN of 0 t.
 constexpr float kFar = -200.f;
@@ -36,29 +40,72 @@ __device__ __forceinline__ void rebase(Sums& a, float to, float c) {
   a.s *= f;
 }
 
-template <typename T, int K>
-__device__ __forceinline__ void take_scores(const uint4 (&v)[K], float c, float top, Sums& a) {
-  if (top > a.m) {
-    rebase(a, top, c);
-    a.m = top;
-  }
-  const float base = base_of(a.m);
+// Words of elements no smaller than `low`; a NaN stays.
+__device__ __forceinline__ uint32_t word_floor(uint32_t a, uint32_t low, bf16) {
+  const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&low));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t word_floor(uint32_t a, uint32_t low, __half) {
+  const __half2 m = __hmax2_nan(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&low));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t word_floor(uint32_t a, uint32_t low, float) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(__uint_as_float(a)), "f"(__uint_as_float(low)));
+  return __float_as_uint(m);
+}
+
+// The word that elements are raised to before t is taken: 250 / c or more below the base, where 2^t is 0 and t still a number.
+// Rounded down, so that no element that counts is raised. -inf, which raises none, where the type's range ends before.
+__device__ __forceinline__ uint32_t floor_of(float base, float reach, bf16) {
+  const bf16 f = __float2bfloat16_rd(__fsub_rd(base, reach));
+  const __nv_bfloat162 two = __halves2bfloat162(f, f);
+  return *reinterpret_cast<const uint32_t*>(&two);
+}
+__device__ __forceinline__ uint32_t floor_of(float base, float reach, __half) {
+  const __half f = __float2half_rd(__fsub_rd(base, reach));
+  const __half2 two = __halves2half2(f, f);
+  return *reinterpret_cast<const uint32_t*>(&two);
+}
+__device__ __forceinline__ uint32_t floor_of(float base, float reach, float) {
+  return __float_as_uint(__fsub_rd(base, reach));
+}
+
+// kRaise: by `low`. Otherwise, at the lower end of the type's range, t itself is held to what counts.
+template <typename T, bool kRaise, int K>
+__device__ __forceinline__ void add_scores(const uint4 (&v)[K], float c, float base, uint32_t low, Sums& a) {
   const float2 off = make_float2(-base, -base), cc = make_float2(c, c);
   float2 s = make_float2(0.f, 0.f), w = make_float2(0.f, 0.f);
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     float f[kVecOf<T>];
-    raw_up<T>(v[k], f);
+    uint4 r = v[k];
+    if (kRaise)
+      r = make_uint4(word_floor(r.x, low, T()), word_floor(r.y, low, T()), word_floor(r.z, low, T()), word_floor(r.w, low, T()));
+    raw_up<T>(r, f);
 #pragma unroll
     for (int i = 0; i < kVecOf<T> / 2; ++i) {
-      const float2 t = __fmul2_rn(__fadd2_rn(make_float2(f[2 * i], f[2 * i + 1]), off), cc);
+      float2 t = __fmul2_rn(__fadd2_rn(make_float2(f[2 * i], f[2 * i + 1]), off), cc);
       const float2 e = make_float2(ex2(t.x), ex2(t.y));
       s = __fadd2_rn(s, e);
-      w = __ffma2_rn(e, make_float2(fmaxf(t.x, kFar), fmaxf(t.y, kFar)), w);
+      if (!kRaise) t = make_float2(fmaxf(t.x, kFar), fmaxf(t.y, kFar));
+      w = __ffma2_rn(e, t, w);
     }
   }
   a.s += s.x + s.y;
   a.w += w.x + w.y;
+}
+
+template <typename T, int K>
+__device__ __forceinline__ void take_scores(const uint4 (&v)[K], float c, float reach, float top, Sums& a) {
+  if (top > a.m) {
+    rebase(a, top, c);
+    a.m = top;
+  }
+  const float base = base_of(a.m);
+  const uint32_t low = floor_of(base, reach, T());
+  if ((sizeof(T) == 2 ? low & 0xffffu : low) != ElemOf<T>::kNegInf) add_scores<T, true>(v, c, base, low, a);
+  else add_scores<T, false>(v, c, base, low, a);
 }
 
 __device__ __forceinline__ void merge_lanes(Sums& a, float c) {
@@ -100,83 +147,88 @@ __device__ __forceinline__ void insert(unsigned long long key, int K, unsigned l
   }
 }
 
+constexpr int kNoted = 96;  // elements of a row that reach the bound, for the quick way
+
 template <int kGroup>
 struct ScoreShared {
   static constexpr int kWarps = kGroup / 32;
   Sums parts[kWarps];
-  alignas(16) float tops[kGroup];
-  float bound;
-  unsigned long long lists[kWarps][32];
+  int owners[kGroup];  // the threads whose maxima reach the bound
+  int count[2];        // of the owners, of the elements noted
+  unsigned long long noted[kNoted];
 };
+
+template <int kGroup>
+__device__ __forceinline__ void group_sync() {
+  if (kGroup > 32) __syncthreads();
+  else __syncwarp();
+}
+
+template <int kGroup>
+__device__ __forceinline__ int group_count(bool x) {
+  return kGroup > 32 ? __syncthreads_count(x) : __popc(__ballot_sync(0xffffffffu, x));
+}
 
 // The row's alternatives. `mine`: the maximum of the calling thread's vectors (tid, tid + kGroup, ...).
 template <typename T, int kGroup>
 __device__ __forceinline__ void alternatives(const ScoreArgs& a, const RowSpan<T>& span, long long row, float mine, bool has_nan,
                                              float base, float log2_s, ScoreShared<kGroup>& sh) {
-  constexpr int kW = kGroup / 32, N = kVecOf<T>;
-  const int tid = Place<kGroup>::tid(), lane = threadIdx.x & 31, warp = kW > 1 ? threadIdx.x >> 5 : 0, K = a.top;
-  float bound = -INFINITY;
-  if constexpr (kW == 1) {
-    int above = 0, equal = 0;
-#pragma unroll
-    for (int o = 0; o < 32; ++o) {
-      const float x = __shfl_sync(0xffffffffu, mine, o);
-      above += x > mine;
-      equal += x >= mine;
-    }
-    const unsigned at = __ballot_sync(0xffffffffu, above < K && equal >= K);
-    if (at && !has_nan) bound = __shfl_sync(0xffffffffu, mine, __ffs(at) - 1);
-  } else {
-    sh.tops[tid] = mine;
-    if (tid == 0) sh.bound = -INFINITY;
-    __syncthreads();
-    int above = 0, equal = 0;
-    const float4* tops = reinterpret_cast<const float4*>(sh.tops);
-#pragma unroll 4
-    for (int o = 0; o < kGroup / 4; ++o) {
-      const float4 x = tops[o];
-      above += (x.x > mine) + (x.y > mine) + (x.z > mine) + (x.w > mine);
-      equal += (x.x >= mine) + (x.y >= mine) + (x.z >= mine) + (x.w >= mine);
-    }
-    if (above < K && equal >= K && !has_nan) sh.bound = mine;  // the same value from each that writes
-    __syncthreads();
-    bound = sh.bound;
+  constexpr int N = kVecOf<T>;
+  const int tid = Place<kGroup>::tid(), lane = threadIdx.x & 31, K = a.top;
+  // The largest number with 16 significant bits that K maxima reach, bit by bit. Small rows and rows with a NaN, which the
+  // maxima pass over, are looked at whole.
+  const uint32_t key = (uint32_t)(key_of(mine, 0) >> 32);
+  uint32_t bound = 0;
+  if (!has_nan) {
+#pragma unroll 1
+    for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1)
+      if (group_count<kGroup>(key >= (bound | bit)) >= K) bound |= bit;
   }
-  // The keys that count lie above `last`: at first all whose value is the bound at least.
-  unsigned long long list = 0, last = key_of(bound, 0) >> 32 << 32;
-  if (last) --last;
-  const auto scan = [&](int owner) {
-    for (int j0 = owner; j0 < span.nv; j0 += 32 * kGroup) {
-      const int j = j0 + lane * kGroup, lo = span.first(j);
-      float f[N];
-      raw_up<T>(span.template load<false>(j), f);
+  const bool owner = has_nan || key >= bound;
+  if (tid < 2) sh.count[tid] = 0;
+  group_sync<kGroup>();
+  if (owner) sh.owners[atomicAdd(&sh.count[0], 1)] = tid;
+  group_sync<kGroup>();
+  const int owners = sh.count[0], per = (span.nv + kGroup - 1) / kGroup;
+  for (int u = tid; u < owners * per; u += kGroup) {
+    const int j = sh.owners[u / per] + u % per * kGroup, lo = span.first(j);
+    if (j >= span.nv) continue;
+    float f[N];
+    raw_up<T>(span.template load<false>(j), f);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const bool in = j < span.nv && lo + i >= 0 && lo + i < span.V;
-        insert(in ? key_of(f[i], lo + i) : 0ull, K, list, last);
+    for (int i = 0; i < N; ++i) {
+      const unsigned long long x = key_of(f[i], lo + i);
+      if ((uint32_t)(x >> 32) >= bound && lo + i >= 0 && lo + i < span.V) {
+        const int at = atomicAdd(&sh.count[1], 1);
+        if (at < kNoted) sh.noted[at] = x;
       }
     }
-  };
-  if constexpr (kW == 1) {
-    unsigned todo = __ballot_sync(0xffffffffu, mine >= bound);
-    while (todo) {
-      scan(__ffs(todo) - 1);
-      todo &= todo - 1;
-    }
-  } else {
-    // The warps share the threads that reach the bound: each takes every kW-th of them.
-    int seen = 0;
-    for (int w = 0; w < kW; ++w) {
-      unsigned todo = __ballot_sync(0xffffffffu, sh.tops[w * 32 + lane] >= bound);
-      while (todo) {
-        if (seen++ % kW == warp) scan(w * 32 + __ffs(todo) - 1);
-        todo &= todo - 1;
+  }
+  group_sync<kGroup>();
+  const int found = sh.count[1];
+  if (found <= kNoted) {
+    for (int i = tid; i < found; i += kGroup) {
+      const unsigned long long x = sh.noted[i];
+      int rank = 0;
+      for (int o = 0; o < found; ++o) rank += sh.noted[o] > x;
+      if (rank < K) {
+        a.top_ids[row * K + rank] = (int)~(uint32_t)x;
+        a.top_logps[row * K + rank] = label_logp_of(value_of(x), base, a.rows.inv_temp, log2_s);
       }
     }
-    sh.lists[warp][lane] = list;
-    __syncthreads();
-    if (warp > 0) return;
-    for (int w = 1; w < kW; ++w) insert(sh.lists[w][lane], K, list, last);
+    return;
+  }
+  if (tid >= 32) return;
+  unsigned long long list = 0, last = bound ? ((unsigned long long)bound << 32) - 1 : 0;
+  for (int u0 = 0; u0 < owners * per; u0 += 32) {
+    const int u = u0 + lane, j = u < owners * per ? sh.owners[u / per] + u % per * kGroup : span.nv, lo = span.first(j);
+    float f[N];
+    raw_up<T>(span.template load<false>(j), f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const bool in = j < span.nv && lo + i >= 0 && lo + i < span.V;
+      insert(in ? key_of(f[i], lo + i) : 0ull, K, list, last);
+    }
   }
   if (lane < K) {
     a.top_ids[row * K + lane] = (int)~(uint32_t)list;
@@ -185,8 +237,8 @@ __device__ __forceinline__ void alternatives(const ScoreArgs& a, const RowSpan<T
 }
 
 template <typename T, int kGroup, bool kTop>
-__global__ void __launch_bounds__(Place<kGroup>::kThreads) scores_kernel(ScoreArgs a) {
-  __shared__ ScoreShared<kGroup> shared[kTop || kGroup > 32 ? Place<kGroup>::kRows : 1];
+__global__ void __launch_bounds__(Place<kGroup>::kThreads, kGroup == 32 ? 10 : 6) scores_kernel(ScoreArgs a) {
+  __shared__ ScoreShared<kGroup> shared[kTop ? Place<kGroup>::kRows : 1];
   constexpr int kW = kGroup / 32, kHold = kGroup * kUnroll;
   const LogitRows& r = a.rows;
   const long long row = Place<kGroup>::row();
@@ -209,12 +261,12 @@ __global__ void __launch_bounds__(Place<kGroup>::kThreads) scores_kernel(ScoreAr
   }
   const T* x = row_ptr<T>(r, row);
   const RowSpan<T> span(x, r.V);
-  const float c = kLog2e * r.inv_temp;
+  const float c = kLog2e * r.inv_temp, reach = 250.f / c;
   Sums sum{-INFINITY, 0.f, 0.f};
   for (int j = tid; j < span.nv; j += kHold) {
     uint4 v[kUnroll];
     fetch<T, kGroup, false>(span, j, span.inner(j - tid, kHold), v);
-    take_scores<T>(v, c, max_of<T>(v), sum);
+    take_scores<T>(v, c, reach, max_of<T>(v), sum);
   }
   const float mine = sum.m;
   merge_lanes(sum, c);

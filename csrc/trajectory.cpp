@@ -66,30 +66,33 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
     if (p.numel() > 0)
       TORCH_CHECK_VALUE(seen.insert(p.data_ptr()).second, "a parameter is given twice");
   }
-  bw::AdamwTable table;
-  table.beta1 = (float)beta1;
-  table.beta2 = (float)beta2;
-  table.one_beta1 = (float)(1 - beta1);
-  table.one_beta2 = (float)(1 - beta2);
-  table.keep = (float)(1 - lr * weight_decay);
-  table.size = (float)(lr / (1 - std::pow(beta1, (double)step)));
-  table.inv_root2 = (float)(1 / std::sqrt(1 - std::pow(beta2, (double)step)));
-  table.eps = (float)eps;
-  table.sign = maximize ? -1.f : 1.f;
+  bw::AdamwTable<bw::kAdamwMany> table;
+  table.s.beta1 = (float)beta1;
+  table.s.beta2 = (float)beta2;
+  table.s.one_beta1 = (float)(maximize ? beta1 - 1 : 1 - beta1);
+  table.s.one_beta2 = (float)(1 - beta2);
+  table.s.keep = (float)(1 - lr * weight_decay);
+  table.s.size = (float)(lr / (1 - std::pow(beta1, (double)step)));
+  table.s.inv_root2 = (float)(1 / std::sqrt(1 - std::pow(beta2, (double)step)));
+  table.s.eps = (float)eps;
   const c10::cuda::CUDAGuard guard(params[0].device());
   const auto stream = at::cuda::getCurrentCUDAStream();
   using bw::Elem;
   for (const auto& [pt, gt] : {std::pair<Elem, Elem>{Elem::kBF16, Elem::kBF16}, {Elem::kBF16, Elem::kF32},
                                {Elem::kF16, Elem::kF16}, {Elem::kF16, Elem::kF32}, {Elem::kF32, Elem::kF32}}) {
-    table.count = 0;
-    table.chunks = 0;
+    int64_t total = 0;
+    for (size_t i = 0; i < count; ++i)
+      if (elem_of(params[i], "") == pt && elem_of(grads[i], "") == gt) total += params[i].numel();
+    table.s.chunk = bw::adamw_chunk(total, bits8);
+    table.s.count = 0;
+    table.s.chunks = 0;
     const auto flush = [&] {
-      if (table.count == 0) return;
+      if (table.s.count == 0) return;
       bw::adamw_step(table, pt, gt, bits8, stream);
       C10_CUDA_KERNEL_LAUNCH_CHECK();
       ++launches;
-      table.count = 0;
-      table.chunks = 0;
+      table.s.count = 0;
+      table.s.chunks = 0;
     };
     for (size_t i = 0; i < count; ++i) {
       const Tensor& p = params[i];
@@ -100,15 +103,16 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
         g.copy_(grads[i].detach());
         held.push_back(g);
       }
-      bw::AdamwTensor& t = table.t[table.count];
-      t = bw::AdamwTensor{p.data_ptr(),  g.data_ptr(),
-                          exp_avgs[i].data_ptr(), exp_avg_sqs[i].data_ptr(),
-                          bits8 ? (*scales)[i].data_ptr<float>() : nullptr, p.numel(), table.chunks, 0u};
-      t.aligned = at_multiple(t.p, 16) && at_multiple(t.g, 16) && at_multiple(t.m, bits8 ? 8 : 16) && at_multiple(t.v, bits8 ? 8 : 16);
-      const int64_t chunks = (p.numel() + bw::kAdamwChunk - 1) / bw::kAdamwChunk;
-      TORCH_CHECK_VALUE(chunks < (int64_t(1) << 30), "a parameter has more than 2^43 elements");
-      table.chunks += (unsigned)chunks;
-      if (++table.count == bw::kAdamwTensors || table.chunks >= (1u << 30)) flush();
+      bw::AdamwTensor& t = table.t[table.s.count];
+      t = bw::AdamwTensor{p.data_ptr(), g.data_ptr(), exp_avgs[i].data_ptr(), exp_avg_sqs[i].data_ptr(),
+                          bits8 ? (*scales)[i].data_ptr<float>() : nullptr, p.numel()};
+      const size_t of_moments = bits8 ? 8 : 16;
+      if (!at_multiple(t.p, 16) || !at_multiple(t.g, 16) || !at_multiple(t.m, of_moments) || !at_multiple(t.v, of_moments)) t.n = -t.n;
+      table.first[table.s.count] = table.s.chunks;
+      const int64_t chunks = (p.numel() + table.s.chunk - 1) / table.s.chunk;
+      TORCH_CHECK_VALUE(chunks < (int64_t(1) << 30), "a parameter has 2^41 elements or more");
+      table.s.chunks += (unsigned)chunks;
+      if (++table.s.count == bw::kAdamwMany || table.s.chunks >= (1u << 30)) flush();
     }
     flush();
   }

@@ -30,7 +30,8 @@ def _scores_torch(logits, labels, top_k, temperature, ignore) -> TokenScores:
     if bool(((labels < 0) | (labels >= logits.shape[2]))[valid].any()):
         raise ValueError(f"labels must be {ignore} or in [0, {logits.shape[2]})")
     raw = (logits if logits.dtype == torch.float64 else logits.float()).masked_fill(~valid.unsqueeze(-1), 0.0)
-    logs = torch.log_softmax(raw / temperature, -1)
+    base = raw.detach().amax(-1, keepdim=True)  # off before the division, which would round it
+    logs = torch.log_softmax((raw - torch.where(torch.isfinite(base), base, 0.0)) / temperature, -1)
     p = logs.exp()
     # a token that cannot come (p = 0) adds nothing, though its log-probability may be -inf
     entropy = -torch.where(p > 0, p * torch.where(p > 0, logs, 0.0), p).sum(-1)

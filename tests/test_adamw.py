@@ -57,10 +57,11 @@ def make(shapes, dtype, device, *, bits, grad_dtype=None, seed=0, offset=0):
 def exact(p, g, m, v, step, maximize=False):
     b1, b2 = HYPER["betas"]
     p, g, m, v = (x.double() for x in (p, -g if maximize else g, m, v))
+    terms = b1 * m.abs() + (1 - b1) * g.abs()  # of m: where they cancel, their roundings do not
     m = b1 * m + (1 - b1) * g
     v = b2 * v + (1 - b2) * g * g
-    move = HYPER["lr"] * (m / (1 - b1 ** step)) / ((v / (1 - b2 ** step)).sqrt() + HYPER["eps"])
-    return p * (1 - HYPER["lr"] * HYPER["weight_decay"]) - move, m, v, move
+    by = HYPER["lr"] / (1 - b1 ** step) / ((v / (1 - b2 ** step)).sqrt() + HYPER["eps"])
+    return p * (1 - HYPER["lr"] * HYPER["weight_decay"]) - by * m, m, v, by * terms
 
 
 def check(shapes, dtype, device, bits, step, **kw):
@@ -290,3 +291,13 @@ def test_another_stream_and_a_captured_step():
     graph.replay()
     graph.replay()
     assert torch.equal(p, want) and torch.equal(s, ws)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [8, 32])
+def test_gradients_whose_squares_overflow_move_nothing(device, bits):
+    p, g = torch.ones(300, device=device), torch.zeros(300, device=device)
+    g[7] = 1e25
+    m, v, s = ops.adamw_state(p, bits)
+    ops.adamw_step([p], [g], [m], [v], None if s is None else [s], step=1, lr=0.1, weight_decay=0.0)
+    assert torch.equal(p, torch.ones_like(p))  # m / inf

@@ -242,3 +242,38 @@ def test_many_rows_and_long_ones_agree_with_themselves():
     for dtype in (torch.bfloat16, torch.float16, torch.float32):
         x, labels = make(1, 3, 131071, dtype, "cuda", spread=2.0)
         check(x, labels, top_k=32)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_logits_far_from_zero(device, dtype):
+    """Where neighbouring numbers of the type are further apart than any exponential reaches, and at the ends of its range."""
+    top = torch.finfo(dtype).max
+    x, labels = make(1, 6, 2051, dtype, device)
+    labels[:] = 5
+    for row, at in enumerate((1e4, -1e4, 6e4, top, -top, 300.0)):
+        x[0, row] = at
+        steps = torch.randint(0, 4, (2051,), generator=torch.Generator().manual_seed(row)).to(device)
+        for _ in range(3):  # one to three representable numbers below it, or above where it is the lowest
+            lower = torch.nextafter(x[0, row], torch.full_like(x[0, row], top if row == 4 else -top))
+            x[0, row] = torch.where(steps > 0, lower, x[0, row])
+            steps -= 1
+    check(x, labels, top_k=32, grad=False)
+    check(x, labels, top_k=0, temperature=7.0, grad=False)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_alternatives_crowded_into_few_places(device):
+    """The best logits next to one another, and more equal ones than a row's short list holds."""
+    for v in (600, 9001, 40000):
+        x, labels = make(1, 5, v, torch.bfloat16, device)
+        labels[:] = 0
+        x[0, 0, 8:48] = torch.arange(40, device=device, dtype=torch.bfloat16) + 20
+        x[0, 1, v // 2:] = 30.0
+        x[0, 2, ::3] = 25.0
+        x[0, 3, -33:] = 40.0
+        x[0, 4] = -math.inf
+        x[0, 4, 7] = 1.0
+        check(x[:, :4], labels[:, :4], top_k=32)
+        got = ops.token_scores(x[:, 4:], labels[:, 4:], top_k=5)
+        assert got.top_ids[0, 0].tolist() == [7, 0, 1, 2, 3] and got.entropy[0, 0] == 0
