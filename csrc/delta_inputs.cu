@@ -1,0 +1,426 @@
+// Gated delta rule in chunks, backward: the gradients of q, k and the gates (formulas in delta_state.cu).
+//
+// A CTA to each chunk of a value head; the value heads of one key head are a cluster, whose CTAs add their rows of dq and dk
+// over distributed shared memory in the order of the heads. Products, all with 128 lanes of tensor memory:
+//     [dO | dV] V'^T           dP in lanes 0..63, dL in 64..127: both gradients side by side as the rows of one operand
+//     S [dO | dV]^T, dS' V'^T  lanes are the elements of a key row, columns the tokens
+//     K^T W, K^T W', Q^T W     W = dP D rq_i rk_j and dL D rk_i rk_j: q and k go in as given, their lengths in the small matrix
+// so that all scalings of tokens are by columns, in fp32, when the sums leave tensor memory.
+//
+// What bounds it: 300 KB to read for each chunk of 128 x 128, 64 of them S and 64 dS', which share their place.
+#include <cooperative_groups.h>
+
+#include "delta_tiles.cuh"
+
+namespace bw {
+namespace {
+
+namespace cg = cooperative_groups;
+
+template <typename I, int DK, int DV>
+struct InputsMem {
+  static constexpr int kPanels = DK / 64, kPanelS = DV * 128, kPlaneS = kPanels * kPanelS, kPlaneX = DV * 128, kPlaneK = kPanels * kTok;
+  // S, then dS'; V'; the stack: dO and dV, the high halves before the low ones (dO in bf16 has none)
+  static constexpr int S = 0, V = S + 2 * kPlaneS, O = V + 2 * kPlaneX, G = O + kPlaneX,
+                       Ol = G + kPlaneX, Gl = Ol + (kParts<I> == 2 ? kPlaneX : 0), Q = Gl + kPlaneX, K = Q + kParts<I> * kPlaneK,
+                       W = K + kParts<I> * kPlaneK, N = W + 2 * kTok, kTiles = N + 2 * kTok;
+  static constexpr int ldF = DK + 4, kRows = 2 * kChunk * ldF * 4;  // in the end, from S on: this head's dq and dk
+  static constexpr int kBytes = kTiles > kRows ? kTiles : kRows;
+};
+
+enum InputsBar { kGotQK, kGotV, kGotS, kGotD, kMixDone, kReadS, kMixSet, kAllDone, kTaken, kInputsBars };
+
+struct InputsShared {
+  uint64_t bar[kInputsBars];
+  uint32_t tmem;
+  float2 G[kChunk];
+  float rk[kChunk], rq[kChunk], beta[kChunk], left[kChunk], grown[kChunk];
+  float dots[3][kChunk];  // V' . dV, v . dv, q . dq
+  float part[2][4][kChunk];
+  float handed[8];
+};
+
+// Adds 64 values of each of 32 lanes over the lanes: lane l ends with the sums of values 2 l and 2 l + 1 in x[0] and x[1].
+__device__ __forceinline__ void lanes_fold(float (&x)[64]) {
+#pragma unroll
+  for (int o = 16, n = 32; o > 0; o >>= 1, n >>= 1) {
+    const bool up = threadIdx.x & o;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float send = up ? x[i] : x[i + n], keep = up ? x[i + n] : x[i];
+      x[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+    }
+  }
+}
+
+template <typename I, int DK, int DV>
+__global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd a) {
+  using Mem = InputsMem<I, DK, DV>;
+  constexpr int P = kParts<I>, kVs = DV / 16;
+  extern __shared__ __align__(1024) unsigned char mem[];
+  InputsShared& sh = *reinterpret_cast<InputsShared*>(mem + Mem::kBytes);
+  const DeltaDims& d = a.d;
+  const int group = d.H / d.Hk, chunks = d.chunks, slices = d.slices;
+  // blockIdx.x = (batch * Hk + key head, chunk, head within the group): the last runs over the cluster
+  const int hg = blockIdx.x % group;
+  const long long rest = blockIdx.x / group, bk = rest / chunks;
+  const int c = (int)(rest % chunks), b = (int)(bk / d.Hk), hk = (int)(bk % d.Hk), h = hk * group + hg;
+  const long long head = (long long)b * d.H + h, n = head * chunks + c, m = bk * chunks + c;
+  const int t0 = c * kChunk, rows = min(kChunk, d.T - t0);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < kInputsBars; ++i) mbar_init(&sh.bar[i], i == kMixSet || i == kTaken ? kWorkers : 1);
+    fence_barrier_init();
+  }
+  if (warp == 8) tmem_alloc(&sh.tmem, 512);
+  if (tid < kChunk) {
+    const float2 G = a.keep.total[n * kChunk + tid], end = a.keep.total[n * kChunk + kChunk - 1];
+    sh.G[tid] = G;
+    sh.rk[tid] = a.keep.rk[m * kChunk + tid];
+    sh.rq[tid] = a.keep.rq[m * kChunk + tid];
+    sh.beta[tid] = a.keep.beta[n * kChunk + tid];
+    sh.left[tid] = decay_between(end, G);
+    sh.grown[tid] = __expf(G.x + G.y);
+    sh.dots[0][tid] = sh.dots[1][tid] = sh.dots[2][tid] = 0.f;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tm = sh.tmem;
+  constexpr uint32_t cMix = 0, cLow = 64, cS = 128, cD = 256, cQ = 320, cK = 384;
+  Waiter wait{a.err};
+  const auto state_at = [&](int chunk, int s) { return a.keep.states + ((head * (chunks + 1) + chunk) * slices + s) * 2 * Mem::kPlaneS; };
+  if (warp == 8) {
+    if (lane == 0) {
+      const uint32_t base = smem_u32(mem);
+      mbar_arrive_expect_tx(&sh.bar[kGotQK], 2 * P * Mem::kPlaneK);
+      const auto load_slice = [&](int s) {
+        const long long at = n * slices + s;
+        mbar_arrive_expect_tx(&sh.bar[kGotV], (4 + P) * Mem::kPlaneX);
+        bulk_load(mem + Mem::V, a.keep.writes + at * 2 * Mem::kPlaneX, 2 * Mem::kPlaneX, &sh.bar[kGotV]);
+        bulk_load(mem + Mem::O, a.douts + at * P * Mem::kPlaneX, Mem::kPlaneX, &sh.bar[kGotV]);
+        if (P == 2) bulk_load(mem + Mem::Ol, a.douts + (at * P + 1) * Mem::kPlaneX, Mem::kPlaneX, &sh.bar[kGotV]);
+        bulk_load(mem + Mem::G, a.dreads + at * 2 * Mem::kPlaneX, Mem::kPlaneX, &sh.bar[kGotV]);
+        bulk_load(mem + Mem::Gl, a.dreads + at * 2 * Mem::kPlaneX + Mem::kPlaneX, Mem::kPlaneX, &sh.bar[kGotV]);
+        mbar_arrive_expect_tx(&sh.bar[kGotS], 2 * Mem::kPlaneS);
+        bulk_load(mem + Mem::S, state_at(c, s), 2 * Mem::kPlaneS, &sh.bar[kGotS]);
+      };
+      load_slice(0);
+      bulk_load(mem + Mem::Q, a.keep.queries + m * P * Mem::kPlaneK, P * Mem::kPlaneK, &sh.bar[kGotQK]);
+      bulk_load(mem + Mem::K, a.keep.keys + m * P * Mem::kPlaneK, P * Mem::kPlaneK, &sh.bar[kGotQK]);
+      // The stack of high halves, and that of low ones; without a low half of dO the first 64 lanes of its product are not used.
+      const Operand high{base + Mem::O, Mem::G - Mem::O}, low{base + (P == 2 ? Mem::Ol : Mem::O), Mem::Gl - (P == 2 ? Mem::Ol : Mem::O)},
+          low_g{base + Mem::Gl, Mem::kPlaneX}, V{base + Mem::V, Mem::kPlaneX}, Vl{base + Mem::V + Mem::kPlaneX, Mem::kPlaneX},
+          S{base + Mem::S, Mem::kPanelS}, Sl{base + Mem::S + Mem::kPlaneS, Mem::kPanelS};
+      for (int s = 0; s < slices; ++s) {
+        const bool more = s > 0;
+        if (!wait(&sh.bar[kGotV], s)) break;
+        multiply<kVs, 64, true, true>(tm + cMix, high, V, more);
+        multiply<kVs, 64, true, true>(tm + cMix, high, Vl, true);
+        multiply<kVs, 64, true, true>(P == 2 ? tm + cMix : tm + cLow, low, V, P == 2 || more);
+        if (s == slices - 1) tc_commit(&sh.bar[kMixDone]);
+        if (!wait(&sh.bar[kGotS], s)) break;
+        multiply<kVs, 128, true, true>(tm + cS, S, high, more);
+        multiply<kVs, 128, true, true>(tm + cS, Sl, high, true);
+        if (P == 2) multiply<kVs, 128, true, true>(tm + cS, S, low, true);
+        else multiply<kVs, 64, true, true>(tm + cS + 64, S, low_g, true);
+        tc_commit(&sh.bar[kReadS]);
+        if (!wait(&sh.bar[kReadS], 2 * s)) break;
+        mbar_arrive_expect_tx(&sh.bar[kGotD], 2 * Mem::kPlaneS);
+        bulk_load(mem + Mem::S, a.dstates + (n * slices + s) * 2 * Mem::kPlaneS, 2 * Mem::kPlaneS, &sh.bar[kGotD]);
+        if (!wait(&sh.bar[kGotD], s)) break;
+        multiply<kVs, 64, true, true>(tm + cD, S, V, more);
+        multiply<kVs, 64, true, true>(tm + cD, Sl, V, true);
+        multiply<kVs, 64, true, true>(tm + cD, S, Vl, true);
+        tc_commit(&sh.bar[kReadS]);
+        if (s + 1 < slices) {  // the places are free once they are read, by the products and by the workers
+          if (!wait(&sh.bar[kReadS], 2 * s + 1) || !wait(&sh.bar[kTaken], s)) break;
+          load_slice(s + 1);
+        }
+      }
+      const Operand Q{base + Mem::Q, kTok}, K{base + Mem::K, kTok}, W{base + Mem::W, kTok}, N{base + Mem::N, kTok};
+      if (wait(&sh.bar[kGotQK], 0) && wait(&sh.bar[kMixSet], 0)) {
+        tc_fence_after();
+        multiply_parts<4, 64, true, false, P, 2>(tm + cQ, K, Mem::kPlaneK, W, kTok, false);
+        multiply_parts<4, 64, true, true, P, 2>(tm + cK, Q, Mem::kPlaneK, W, kTok, false);
+        multiply_parts<4, 64, true, false, P, 2>(tm + cK, K, Mem::kPlaneK, N, kTok, true);
+        multiply_parts<4, 64, true, true, P, 2>(tm + cK, K, Mem::kPlaneK, N, kTok, true);
+        tc_commit(&sh.bar[kAllDone]);
+        wait(&sh.bar[kAllDone], 0);
+      }
+    }
+  } else {
+    const int row = (warp & 3) * 32 + lane, half = warp >> 2;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+    float handed = 0.f;
+    for (int s = 0; s < slices; ++s) {
+      const int v0 = s * DV;
+      const bool in = row < min(DV, d.dv - v0);
+      // A lane holds an element of the values: V' . dV (the first four warps) and v . dv (the others) of all tokens.
+      float x[64];
+      if (half == 1) {
+        const I* v = head_at<I>(a.v, b, t0, h) + v0 + row;
+#pragma unroll
+        for (int i = 0; i < 64; ++i) x[i] = in && i < rows ? ElemOf<I>::up(v[i * a.v.st]) : 0.f;
+      }
+      if (!wait(&sh.bar[kGotV], s)) break;
+      const bool there = row < DV;
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
+        const int at = piece_at(there ? row : 0, p);
+        const uint4 gh = *reinterpret_cast<const uint4*>(mem + Mem::G + at), gl = *reinterpret_cast<const uint4*>(mem + Mem::Gl + at);
+        const float2 g[4] = {pair_sum(gh.x, gl.x), pair_sum(gh.y, gl.y), pair_sum(gh.z, gl.z), pair_sum(gh.w, gl.w)};
+        float2 w[4];
+        if (half == 0) {
+          const uint4 wh = *reinterpret_cast<const uint4*>(mem + Mem::V + at), wl = *reinterpret_cast<const uint4*>(mem + Mem::V + Mem::kPlaneX + at);
+          w[0] = pair_sum(wh.x, wl.x);
+          w[1] = pair_sum(wh.y, wl.y);
+          w[2] = pair_sum(wh.z, wl.z);
+          w[3] = pair_sum(wh.w, wl.w);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = make_float2(x[p * 8 + 2 * k], x[p * 8 + 2 * k + 1]);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          x[p * 8 + 2 * k] = in ? w[k].x * g[k].x : 0.f;
+          x[p * 8 + 2 * k + 1] = in ? w[k].y * g[k].y : 0.f;
+        }
+      }
+      lanes_fold(x);
+      // <dS', S'>: both tiles have their elements at the same places.
+      const uint4* after = reinterpret_cast<const uint4*>(state_at(c + 1, s));
+      constexpr int kPieces = Mem::kPlaneS / 16;
+      sh.part[half][warp & 3][2 * lane] = s ? sh.part[half][warp & 3][2 * lane] + x[0] : x[0];
+      sh.part[half][warp & 3][2 * lane + 1] = s ? sh.part[half][warp & 3][2 * lane + 1] + x[1] : x[1];
+      if (!wait(&sh.bar[kGotD], s)) break;
+#pragma unroll 2
+      for (int i = tid; i < kPieces; i += kWorkers) {
+        const uint4 ah = after[i], al = after[kPieces + i];
+        const uint4 dh = *reinterpret_cast<const uint4*>(mem + Mem::S + i * 16), dl = *reinterpret_cast<const uint4*>(mem + Mem::S + Mem::kPlaneS + i * 16);
+        const uint32_t u[4] = {ah.x, ah.y, ah.z, ah.w}, v[4] = {al.x, al.y, al.z, al.w}, y[4] = {dh.x, dh.y, dh.z, dh.w}, z[4] = {dl.x, dl.y, dl.z, dl.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 e = pair_sum(u[k], v[k]), f = pair_sum(y[k], z[k]);
+          handed = fmaf(e.x, f.x, fmaf(e.y, f.y, handed));
+        }
+      }
+      mbar_arrive(&sh.bar[kTaken]);
+    }
+    handed = lanes_sum(handed);
+    if (lane == 0) sh.handed[warp] = handed;
+    // The small matrices: row i of dP in lane i, of dL in lane 64 + i.
+    if (!wait.dead && wait(&sh.bar[kMixDone], 0)) {
+      tc_fence_after();
+      const int i = row & 63, j0 = half * 32;
+      const bool of_l = row >= 64;
+      float f[32];
+      tmem_row(tm + lanes + cMix + j0, f);
+      if (P == 1) {
+        float g[32];
+        tmem_row(tm + lanes + cLow + j0, g);
+        if (of_l)
+#pragma unroll
+          for (int k = 0; k < 32; ++k) f[k] += g[k];
+      }
+      const float by = of_l ? -sh.rk[i] : sh.rq[i];
+      const float2 Gi = sh.G[i];
+      unsigned char* to = mem + (of_l ? Mem::N : Mem::W);
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int j = j0 + p * 8 + k;
+          x[k] = j < i || (j == i && !of_l) ? f[p * 8 + k] * by * (decay_between(Gi, sh.G[j]) * sh.rk[j]) : 0.f;
+        }
+        const int at = piece_at(i, half * 4 + p);
+        put8(to + at, to + kTok + at, x);
+      }
+    }
+    hand_over(&sh.bar[kMixSet]);
+    wait(&sh.bar[kAllDone], 0);
+  }
+  // dq and dk of this head: r dq^ and r dk^ of the scaled rows, tokens as rows, where S and V' lay.
+  __syncthreads();
+  float* F = reinterpret_cast<float*>(mem);
+  if (warp < 8) {
+    const int row = (warp & 3) * 32 + lane, half = warp >> 2;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+    tc_fence_after();
+    float s[32], y[32];
+    tmem_row(tm + lanes + cS + half * 32, s);
+    tmem_row(tm + lanes + cQ + half * 32, y);
+    if (row < DK)
+#pragma unroll
+      for (int k = 0; k < 32; ++k) {
+        const int i = half * 32 + k;
+        F[i * Mem::ldF + row] = fmaf(sh.rq[i] * sh.grown[i], s[k], y[k]);
+      }
+    float z[32];
+    tmem_row(tm + lanes + cS + 64 + half * 32, s);
+    tmem_row(tm + lanes + cD + half * 32, z);
+    tmem_row(tm + lanes + cK + half * 32, y);
+    if (row < DK)
+#pragma unroll
+      for (int k = 0; k < 32; ++k) {
+        const int i = half * 32 + k;
+        F[(kChunk + i) * Mem::ldF + row] = fmaf(sh.rk[i], fmaf(sh.left[i], z[k], -sh.grown[i] * s[k]), y[k]);
+      }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tm, 512);
+  }
+  if (tid < kChunk) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      sh.dots[0][tid] += sh.part[0][w][tid];
+      sh.dots[1][tid] += sh.part[1][w][tid];
+    }
+  }
+  // q^ . dq^ = q . dq of this head's rows
+  for (int i = warp; i < rows; i += 9) {
+    const I* q = head_at<I>(a.q, b, t0 + i, hk);
+    float dot = 0.f;
+#pragma unroll
+    for (int k = 0; k < DK / 32; ++k) {
+      const int col = k * 32 + lane;
+      if (col < d.dk) dot = fmaf(ElemOf<I>::up(q[col]), F[i * Mem::ldF + col], dot);
+    }
+    dot = lanes_sum(dot);
+    if (lane == 0) sh.dots[2][i] = dot;
+  }
+  cg::cluster_group cluster = cg::this_cluster();
+  if (group > 1) cluster.sync();
+  else __syncthreads();
+  if (warp == 8) {  // the gates: sums from each token to the chunk's end, two tokens a lane
+    float after = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) after += sh.handed[w];
+    const float x = sh.dots[2][2 * lane] - sh.dots[1][2 * lane], y = sh.dots[2][2 * lane + 1] - sh.dots[1][2 * lane + 1];
+    float sum = x + y;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const float up = __shfl_down_sync(0xffffffffu, sum, o);
+      if (lane + o < 32) sum += up;
+    }
+    const float a_log = load_any(a.g.a_log, a.g.a_log_type, h), dt = load_any(a.g.dt_bias, a.g.dt_bias_type, h);
+    double sum_log = 0.0, sum_bias = 0.0;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int i = 2 * lane + k;
+      if (i >= rows) continue;
+      const Gate gate = gate_of(ElemOf<I>::up(*head_at<I>(a.g.a, b, t0 + i, h)), a_log, dt);
+      // Nothing passes a gate whose factor is 0 in fp32: what the sum holds then is its rounding.
+      const float dg = gate.log_decay < -104.f ? 0.f : (k ? sum - x : sum) + after;
+      const float da = -dg * gate.rate * gate.slope;
+      const float beta = sh.beta[i];
+      const float db = beta > 1e-20f ? (1.f - beta) * (sh.dots[0][i] / beta) : 0.f;  // V' = beta E; below, db is under 1e-20 dV . E
+      const long long to = ((long long)b * d.T + t0 + i) * d.H + h;
+      reinterpret_cast<I*>(a.da)[to] = ElemOf<I>::down(da);
+      reinterpret_cast<I*>(a.db)[to] = ElemOf<I>::down(db);
+      sum_log += (double)dg * gate.log_decay;
+      sum_bias += da;
+    }
+    sum_log = lanes_sum(sum_log);
+    sum_bias = lanes_sum(sum_bias);
+    if (lane == 0) {
+      a.part[n * 2] = (float)sum_log;
+      a.part[n * 2 + 1] = (float)sum_bias;
+    }
+  } else {
+    // Sums over the key head's value heads, the rows of both shared out over the cluster's warps, then back through the
+    // rows' scaling: with x a row, r its reciprocal length and y the sum, dx = y - x r^2 (x . y).
+    for (int r = hg * 8 + warp; r < 2 * kChunk; r += 8 * group) {
+      const int i = r % kChunk;
+      if (i >= rows) continue;
+      const bool of_k = r >= kChunk;
+      const I* x = of_k ? head_at<I>(a.k, b, t0 + i, hk) : head_at<I>(a.q, b, t0 + i, hk);
+      float y[DK / 32], v[DK / 32], dot = 0.f;
+#pragma unroll
+      for (int k = 0; k < DK / 32; ++k) {
+        const int col = k * 32 + lane;
+        y[k] = 0.f;
+        for (int o = 0; o < group; ++o) {
+          const float* f = group > 1 ? cluster.map_shared_rank(F, o) : F;
+          y[k] += f[r * Mem::ldF + col];
+        }
+        v[k] = col < d.dk ? ElemOf<I>::up(x[col]) : 0.f;
+        dot = fmaf(v[k], y[k], dot);
+      }
+      dot = lanes_sum(dot);
+      const float len = of_k ? sh.rk[i] : sh.rq[i] / d.scale;
+      I* to = reinterpret_cast<I*>(of_k ? a.dk : a.dq) + (((long long)b * d.T + t0 + i) * d.Hk + hk) * d.dk;
+#pragma unroll
+      for (int k = 0; k < DK / 32; ++k) {
+        const int col = k * 32 + lane;
+        if (col < d.dk) to[col] = ElemOf<I>::down(y[k] - v[k] * (len * len * dot));
+      }
+    }
+  }
+  if (group > 1) cluster.sync();  // no CTA leaves while its rows are read
+}
+
+// The chunks' sums for a_log and dt_bias of one head, in a fixed order.
+__global__ void __launch_bounds__(256) gates_kernel(const DeltaBwd a) {
+  __shared__ double red[2][8];
+  const DeltaDims& d = a.d;
+  const int h = blockIdx.x;
+  double s[2] = {0.0, 0.0};
+  for (long long i = threadIdx.x; i < (long long)d.B * d.chunks; i += blockDim.x) {
+    const long long n = (i / d.chunks * d.H + h) * d.chunks + i % d.chunks;
+    s[0] += a.part[2 * n];
+    s[1] += a.part[2 * n + 1];
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    s[k] = lanes_sum(s[k]);
+    if ((threadIdx.x & 31) == 0) red[k][threadIdx.x >> 5] = s[k];
+  }
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    double t = 0.0;
+    for (int w = 0; w < 8; ++w) t += red[threadIdx.x][w];
+    if (threadIdx.x == 0) store_any(a.da_log, a.g.a_log_type, h, (float)t);
+    else store_any(a.ddt_bias, a.g.dt_bias_type, h, (float)t);
+  }
+}
+
+template <typename I, int DK, int DV>
+void inputs(const DeltaBwd& a, cudaStream_t s) {
+  constexpr int bytes = InputsMem<I, DK, DV>::kBytes + (int)sizeof(InputsShared);
+  static_assert(bytes <= 227 * 1024, "shared memory");
+  cudaFuncSetAttribute(inputs_kernel<I, DK, DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(a.d.B * a.d.H) * a.d.chunks);
+  cfg.blockDim = dim3(kWorkers + 32);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = a.d.H / a.d.Hk;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, inputs_kernel<I, DK, DV>, a);
+}
+
+template <typename I>
+void inputs_of(const DeltaBwd& a, cudaStream_t s) {
+  if (a.d.slice == 64) return a.d.dk <= 64 ? inputs<I, 64, 64>(a, s) : inputs<I, 128, 64>(a, s);
+  if constexpr (kParts<I> == 1)
+    if (a.d.dk > 64) return inputs<I, 128, 128>(a, s);
+  inputs<I, 64, 128>(a, s);
+}
+
+}  // namespace
+
+void delta_inputs(const DeltaBwd& a, cudaStream_t s) {
+  if (a.d.B * a.d.chunks > 0) a.d.type == Elem::kBF16 ? inputs_of<bf16>(a, s) : inputs_of<__half>(a, s);
+  gates_kernel<<<a.d.H, 256, 0, s>>>(a);
+}
+
+}  // namespace bw

@@ -1,0 +1,575 @@
+// Gated delta rule in chunks of 64 tokens, forward and backward.
+//
+// For each sequence and value head, with rows of k scaled to length one and rows of q to length `scale`:
+//     S_t = exp(g_t) S_{t-1} + k_t beta_t (v_t - exp(g_t) S_{t-1}^T k_t)^T,      o_t = S_t^T q_t.
+// Within a chunk let G_i be the sum of g from its start, D_ij = exp(G_i - G_j) for i >= j, L = strictly lower part of
+// (K K^T) D, P = lower part of (Q K^T) D, S the state before the chunk and S' the one after it. Then
+//     (I + L diag(beta)) E = V - diag(exp G) K S,     V' = diag(beta) E,
+//     O = diag(exp G) Q S + P V',                     S' = exp(G_63) S + (diag(exp(G_63 - G)) K)^T V'.
+// Four kernels: `prepare` (every chunk by itself: gates, lengths, P, and the inverse of the triangular matrix by forward
+// substitution in fp32), `state` (chunk after chunk, columns of S split over CTAs: V' and S'), `output` (every chunk by itself).
+//
+// The backward goes the same way, from dO and dS':
+//     dV' = P^T dO + diag(exp(G_63 - G)) K dS',       dV = (inverse)^T diag(beta) dV',
+//     dS = exp(G_63) dS' + Q^T diag(exp G) dO - K^T diag(exp G) dV,                                    (`dstate`)
+//     dP = lower(dO V'^T),  dL = -strictly lower(dV V'^T),
+//     dQ = diag(exp G) dO S^T + (dP D) K,
+//     dK = -diag(exp G) dV S^T + diag(exp(G_63 - G)) V' dS'^T + (dP D)^T Q + (dL D + (dL D)^T) K,
+// and with b the logit of beta:  db_i = (1 - beta_i) dV_i . E_i.  Scaling S between two tokens scales everything that
+// flows through it, so the log-decay's gradient is what leaves less what enters: with <dS', S'> for what the chunk hands on,
+//     dg_t = sum_{i >= t} (q_i . dq_i - v_i . dv_i) + <dS', S'>.                                       (`inputs`)
+//
+// Matrix products run on 16-bit tensor instructions with fp32 sums. q, k and dO are bf16 as given, so they are exact; all
+// that is computed (S, V', the inverse, P and their gradients) goes in as two bf16 halves, which keep 16 bits of 24: two products
+// where one side is exact, three where both have halves (the product of the two low halves is below 2^-16 of the result).
+// One half alone would round each operand by 2^-8, as much as the output's own rounding, several times over. fp16 inputs
+// are two exact halves as well.
+#include "delta_tiles.cuh"
+
+namespace bw {
+namespace {
+
+// Where a worker sits: warp w of eight holds tensor memory's lanes 32 (w % 4) .. + 31, one each, and half of the columns.
+struct Seat {
+  int row, half;
+  uint32_t lanes;  // of a tensor memory address
+  __device__ Seat() {
+    const int warp = threadIdx.x >> 5;
+    row = (warp & 3) * 32 + (threadIdx.x & 31);
+    half = warp >> 2;
+    lanes = (uint32_t)(warp & 3) << 21;
+  }
+};
+
+// Of a chunk's tokens: what the products' columns are multiplied by.
+struct Factors {
+  float grown_k[kChunk];  // exp(G) rk
+  float grown_q[kChunk];  // exp(G) rq
+  float left_k[kChunk];   // exp(G_63 - G) rk
+  float beta[kChunk];
+};
+
+__device__ __forceinline__ void fill_factors(Factors& f, const DeltaKept& keep, long long n, long long m, int i) {
+  const float2 G = keep.total[n * kChunk + i], end = keep.total[n * kChunk + kChunk - 1];
+  const float rk = keep.rk[m * kChunk + i], grown = __expf(G.x + G.y);
+  f.grown_k[i] = grown * rk;
+  f.grown_q[i] = grown * keep.rq[m * kChunk + i];
+  f.left_k[i] = decay_between(end, G) * rk;
+  f.beta[i] = keep.beta[n * kChunk + i];
+}
+
+// 32 tokens' values of one column of head rows, from token t on; zeros behind the last token and for columns that are not there.
+template <typename I>
+__device__ __forceinline__ void column_of(const I* p, long long st, int t, int rows, bool in, I (&x)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) x[i] = in && t + i < rows ? p[(long long)(t + i) * st] : ElemOf<I>::down(0.f);
+}
+
+// The threads of a role meet on an mbarrier, so that a wait that gives up elsewhere leaves nobody behind.
+struct Meeting {
+  uint64_t* bar;
+  int round = 0;
+  __device__ __forceinline__ void operator()(Waiter& wait) {
+    mbar_arrive(bar);
+    wait(bar, round++);
+  }
+};
+
+// ---------------------------------------------------------------- state
+template <typename I, int DK, int DV>
+struct StateMem {
+  static constexpr int kPanels = DK / 64, kParts_ = kParts<I>, kPanelS = DV * 128, kPlaneS = kPanels * kPanelS, kPlaneX = DV * 128,
+                       kPlaneK = kPanels * kTok;
+  // With two parts of q and k one chunk's keys and inverse fit, with one those of the next chunk too.
+  static constexpr int kStages = kParts<I> == 1 ? 2 : 1;
+  static constexpr int S = 0, X = S + 2 * kPlaneS, W = X + 2 * kPlaneX, K = W + 2 * kPlaneX, T = K + kStages * kParts_ * kPlaneK,
+                       Q = T + kStages * 2 * kTok, P = Q + kParts_ * kPlaneK, kTiles = P + 2 * kTok;
+};
+
+enum StateBar { kLoadedK, kLoadedK2, kLoadedQ, kStateSet, kRhsSet, kWritesSet, kReadDone, kSolveDone, kStateDone, kOutDone, kMeet, kStateBars };
+
+struct StateShared {
+  uint64_t bar[kStateBars];
+  uint32_t tmem;
+  Factors f[2];
+};
+
+// One slice of a head's state, chunk after chunk. Tensor memory: S^T (128 x DK), K S, E, and twice Q S and P V'.
+template <typename I, int DK, int DV>
+__global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd a) {
+  using Mem = StateMem<I, DK, DV>;
+  constexpr int P = kParts<I>, kSteps = DK / 16, kStages = Mem::kStages;
+  extern __shared__ __align__(1024) unsigned char mem[];
+  StateShared& sh = *reinterpret_cast<StateShared*>(mem + Mem::kTiles);
+  const DeltaDims& d = a.d;
+  const int slices = d.slices, slice = blockIdx.x % slices, v0 = slice * DV, width = min(DV, d.dv - v0);
+  const long long head = blockIdx.x / slices;
+  const int b = (int)(head / d.H), h = (int)(head % d.H), hk = h / (d.H / d.Hk), chunks = d.chunks;
+  const long long n0 = head * chunks, m0 = ((long long)b * d.Hk + hk) * chunks;
+  const int tid = threadIdx.x, warp = tid >> 5;
+  if (tid == 0) {
+    for (int i = 0; i < kStateBars; ++i)
+      mbar_init(&sh.bar[i], i == kStateSet || i == kRhsSet || i == kWritesSet || i == kMeet ? kWorkers : 1);
+    fence_barrier_init();
+  }
+  if (warp == 8) tmem_alloc(&sh.tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tm = sh.tmem;
+  constexpr uint32_t cS = 0, cK = 128, cE = 192, cQ = 256, cP = 320;  // the last two again 128 columns on
+  Waiter wait{a.err};
+  if (warp == 8) {
+    if ((tid & 31) == 0 && chunks > 0) {
+      const auto load_k = [&](int c) {
+        const int st = c % kStages;
+        uint64_t* bar = &sh.bar[kStages == 2 && (c & 1) ? kLoadedK2 : kLoadedK];
+        mbar_arrive_expect_tx(bar, P * Mem::kPlaneK + 2 * kTok);
+        bulk_load(mem + Mem::K + st * P * Mem::kPlaneK, a.keep.keys + (m0 + c) * P * Mem::kPlaneK, P * Mem::kPlaneK, bar);
+        bulk_load(mem + Mem::T + st * 2 * kTok, a.keep.solve + (n0 + c) * 2 * kTok, 2 * kTok, bar);
+      };
+      const auto load_q = [&](int c) {
+        mbar_arrive_expect_tx(&sh.bar[kLoadedQ], P * Mem::kPlaneK + 2 * kTok);
+        bulk_load(mem + Mem::Q, a.keep.queries + (m0 + c) * P * Mem::kPlaneK, P * Mem::kPlaneK, &sh.bar[kLoadedQ]);
+        bulk_load(mem + Mem::P, a.keep.attend + (n0 + c) * 2 * kTok, 2 * kTok, &sh.bar[kLoadedQ]);
+      };
+      for (int c = 0; c < kStages && c < chunks; ++c) load_k(c);
+      load_q(0);
+      const uint32_t base = smem_u32(mem);
+      const Operand S{base + Mem::S, Mem::kPanelS}, X{base + Mem::X, Mem::kPlaneX}, W{base + Mem::W, Mem::kPlaneX},
+          Q{base + Mem::Q, kTok}, At{base + Mem::P, kTok};
+      for (int c = 0; c < chunks; ++c) {
+        const int st = c % kStages;
+        const uint32_t flip = (c & 1) * 128;
+        const Operand K{base + Mem::K + st * P * Mem::kPlaneK, kTok}, T{base + Mem::T + st * 2 * kTok, kTok};
+        if (!wait(&sh.bar[kStateSet], c)) break;
+        if (!wait(&sh.bar[kStages == 2 && (c & 1) ? kLoadedK2 : kLoadedK], kStages == 2 ? c >> 1 : c)) break;
+        tc_fence_after();
+        multiply_parts<kSteps, 64, false, false, 2, P>(tm + cK, S, Mem::kPlaneS, K, Mem::kPlaneK, false);
+        tc_commit(&sh.bar[kReadDone]);
+        if (!wait(&sh.bar[kLoadedQ], c)) break;
+        multiply_parts<kSteps, 64, false, false, 2, P>(tm + cQ + flip, S, Mem::kPlaneS, Q, Mem::kPlaneK, false);
+        if (!wait(&sh.bar[kRhsSet], c)) break;
+        tc_fence_after();
+        multiply_parts<4, 64, false, false, 2, 2>(tm + cE, X, Mem::kPlaneX, T, kTok, false);
+        tc_commit(&sh.bar[kSolveDone]);
+        if (!wait(&sh.bar[kWritesSet], c)) break;
+        tc_fence_after();
+        multiply_parts<4, DK, false, true, 2, P>(tm + cS, X, Mem::kPlaneX, K, Mem::kPlaneK, true);
+        tc_commit(&sh.bar[kStateDone]);
+        multiply_parts<4, 64, false, false, 2, 2>(tm + cP + flip, W, Mem::kPlaneX, At, kTok, false);
+        tc_commit(&sh.bar[kOutDone]);
+        if (!wait(&sh.bar[kStateDone], c)) break;
+        if (c + kStages < chunks) load_k(c + kStages);
+        if (!wait(&sh.bar[kOutDone], c)) break;
+        if (c + 1 < chunks) load_q(c + 1);
+      }
+    }
+  } else {
+    const Seat seat;
+    const bool there = seat.row < DV, in = seat.row < width;  // a lane of the slice; one with an element of the head
+    const int t32 = seat.half * 32;
+    Meeting meet{&sh.bar[kMeet]};
+    const I* v = head_at<I>(a.v, b, 0, h) + v0 + seat.row;
+    I* out = reinterpret_cast<I*>(a.out) + ((long long)b * d.T * d.H + h) * d.dv + v0 + seat.row;
+    constexpr int kCols = DK / 2;  // of a worker's half of a state's row
+    // Writes the state's row as halves into the tile, and scaled into tensor memory.
+    const auto set_state = [&](const float (&f)[32], int col, float left) {
+      if (there)
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          float x[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) x[k] = f[p * 8 + k];
+          unsigned char* to = mem + Mem::S + (col >> 6) * Mem::kPanelS + piece_at(seat.row, ((col >> 3) & 7) + p);
+          put8(to, to + Mem::kPlaneS, x);
+        }
+      uint32_t r[32];
+#pragma unroll
+      for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(f[k] * left);
+      tmem_st_32x32b_x32(tm + seat.lanes + cS + col, r);
+    };
+    const auto put_out = [&](int c) {  // the output of chunk c: Q S and P V' are done
+      const uint32_t flip = (c & 1) * 128;
+      float x[32], y[32];
+      tmem_row(tm + seat.lanes + cQ + flip + t32, x);
+      tmem_row(tm + seat.lanes + cP + flip + t32, y);
+      if (in) {
+        const int t0 = c * kChunk + t32;
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (t0 + i < d.T) out[(long long)(t0 + i) * d.H * d.dv] = ElemOf<I>::down(fmaf(sh.f[c & 1].grown_q[t32 + i], x[i], y[i]));
+      }
+    };
+    for (int c = 0; c <= chunks && !wait.dead; ++c) {
+      if (c > 0 && !wait(&sh.bar[kStateDone], c - 1)) break;
+      tc_fence_after();
+      if (tid == 0) bulk_read_done();  // of the tiles written below
+      if (c < chunks && tid < kChunk) fill_factors(sh.f[c & 1], a.keep, n0 + c, m0 + c, tid);
+      meet(wait);
+      if (wait.dead) break;
+      const float2 end = c < chunks ? a.keep.total[(n0 + c) * kChunk + kChunk - 1] : make_float2(0.f, 0.f);
+      const float left = __expf(end.x + end.y);
+      I x[32];
+      if (c < chunks) column_of(v + (long long)c * kChunk * a.v.st, a.v.st, t32, d.T - c * kChunk, in, x);
+#pragma unroll
+      for (int k = 0; k < kCols / 32; ++k) {
+        const int col = seat.half * kCols + k * 32;
+        float f[32];
+        if (c > 0) {
+          tmem_row(tm + seat.lanes + cS + col, f);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            f[i] = a.first != nullptr && in && col + i < d.dk ? a.first[(head * d.dk + col + i) * d.dv + v0 + seat.row] : 0.f;
+        }
+        if (c == chunks && a.last != nullptr && in) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (col + i < d.dk) a.last[(head * d.dk + col + i) * d.dv + v0 + seat.row] = f[i];
+        }
+        set_state(f, col, left);
+      }
+      tmem_st_wait();
+      hand_over(&sh.bar[kStateSet]);
+      if (a.keep.states != nullptr) {
+        meet(wait);
+        if (tid == 0 && !wait.dead) {
+          bulk_store(a.keep.states + ((head * (chunks + 1) + c) * slices + slice) * 2 * Mem::kPlaneS, mem + Mem::S, 2 * Mem::kPlaneS);
+          bulk_commit();
+        }
+      }
+      if (c > 0) {
+        if (!wait(&sh.bar[kOutDone], c - 1)) break;
+        tc_fence_after();
+        put_out(c - 1);
+      }
+      if (c == chunks) break;
+      const Factors& fac = sh.f[c & 1];
+      if (!wait(&sh.bar[kReadDone], c)) break;
+      tc_fence_after();
+      float f[32];
+      tmem_row(tm + seat.lanes + cK + t32, f);
+      if (there) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          float y[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) y[k] = fmaf(-fac.grown_k[t32 + p * 8 + k], f[p * 8 + k], ElemOf<I>::up(x[p * 8 + k]));
+          unsigned char* to = mem + Mem::X + piece_at(seat.row, seat.half * 4 + p);
+          put8(to, to + Mem::kPlaneX, y);
+        }
+      }
+      hand_over(&sh.bar[kRhsSet]);
+      if (!wait(&sh.bar[kSolveDone], c)) break;
+      tc_fence_after();
+      tmem_row(tm + seat.lanes + cE + t32, f);
+      if (there) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          float y[8];
+          const int at = piece_at(seat.row, seat.half * 4 + p);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) y[k] = fac.beta[t32 + p * 8 + k] * f[p * 8 + k];
+          put8(mem + Mem::W + at, mem + Mem::W + Mem::kPlaneX + at, y);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) y[k] *= fac.left_k[t32 + p * 8 + k];
+          put8(mem + Mem::X + at, mem + Mem::X + Mem::kPlaneX + at, y);
+        }
+      }
+      hand_over(&sh.bar[kWritesSet]);
+      if (a.keep.writes != nullptr) {
+        meet(wait);
+        if (tid == 0 && !wait.dead) {
+          bulk_store(a.keep.writes + ((n0 + c) * slices + slice) * 2 * Mem::kPlaneX, mem + Mem::W, 2 * Mem::kPlaneX);
+          bulk_commit();
+        }
+      }
+    }
+    if (tid == 0) bulk_done();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tm, 512);
+  }
+}
+
+// ---------------------------------------------------------------- dstate
+template <typename I, int DK, int DV>
+struct DstateMem {
+  static constexpr int kPanels = DK / 64, kParts_ = kParts<I>, kPanelS = DV * 128, kPlaneS = kPanels * kPanelS, kPlaneX = DV * 128,
+                       kPlaneK = kPanels * kTok;
+  static constexpr int kStages = kParts<I> == 1 ? 2 : 1;  // of the keys, which a chunk's first and last product read
+  // Y: diag(exp G rq) dO, then dV; O: dO
+  static constexpr int S = 0, X = S + 2 * kPlaneS, Y = X + 2 * kPlaneX, O = Y + 2 * kPlaneX, K = O + kParts_ * kPlaneX,
+                       Q = K + kStages * kParts_ * kPlaneK, P = Q + kParts_ * kPlaneK, T = P + 2 * kTok, kTiles = T + 2 * kTok;
+};
+
+enum DstateBar { kGotK, kGotK2, kGotQ, kGotT, kDstateSet, kOutsSet, kGradSet, kReadsSet, kMixDone, kOutsDone, kBackDone, kDstateDone, kMeet2, kDstateBars };
+
+struct DstateShared {
+  uint64_t bar[kDstateBars];
+  uint32_t tmem;
+  Factors f[2];
+};
+
+// One slice of the gradient of a head's state, from the last chunk to the first. Tensor memory: dS^T (128 x DK), K dS', P^T dO, dV.
+template <typename I, int DK, int DV>
+__global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd a) {
+  using Mem = DstateMem<I, DK, DV>;
+  constexpr int P = kParts<I>, kSteps = DK / 16, kStages = Mem::kStages;
+  extern __shared__ __align__(1024) unsigned char mem[];
+  DstateShared& sh = *reinterpret_cast<DstateShared*>(mem + Mem::kTiles);
+  const DeltaDims& d = a.d;
+  const int slices = d.slices, slice = blockIdx.x % slices, v0 = slice * DV, width = min(DV, d.dv - v0);
+  const long long head = blockIdx.x / slices;
+  const int b = (int)(head / d.H), h = (int)(head % d.H), hk = h / (d.H / d.Hk), chunks = d.chunks;
+  const long long n0 = head * chunks, m0 = ((long long)b * d.Hk + hk) * chunks;
+  const int tid = threadIdx.x, warp = tid >> 5;
+  if (tid == 0) {
+    for (int i = 0; i < kDstateBars; ++i)
+      mbar_init(&sh.bar[i], i == kDstateSet || i == kOutsSet || i == kGradSet || i == kReadsSet || i == kMeet2 ? kWorkers : 1);
+    fence_barrier_init();
+  }
+  if (warp == 8) tmem_alloc(&sh.tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tm = sh.tmem;
+  constexpr uint32_t cS = 0, cK = 128, cO = 192, cV = 256;
+  Waiter wait{a.err};
+  if (warp == 8) {
+    if ((tid & 31) == 0 && chunks > 0) {
+      const auto load_k = [&](int r) {  // round r: chunk chunks - 1 - r
+        uint64_t* bar = &sh.bar[kStages == 2 && (r & 1) ? kGotK2 : kGotK];
+        mbar_arrive_expect_tx(bar, P * Mem::kPlaneK);
+        bulk_load(mem + Mem::K + r % kStages * P * Mem::kPlaneK, a.keep.keys + (m0 + chunks - 1 - r) * P * Mem::kPlaneK, P * Mem::kPlaneK, bar);
+      };
+      const auto load_q = [&](int r) {
+        mbar_arrive_expect_tx(&sh.bar[kGotQ], P * Mem::kPlaneK + 2 * kTok);
+        bulk_load(mem + Mem::Q, a.keep.queries + (m0 + chunks - 1 - r) * P * Mem::kPlaneK, P * Mem::kPlaneK, &sh.bar[kGotQ]);
+        bulk_load(mem + Mem::P, a.keep.attend + (n0 + chunks - 1 - r) * 2 * kTok, 2 * kTok, &sh.bar[kGotQ]);
+      };
+      const auto load_t = [&](int r) {
+        mbar_arrive_expect_tx(&sh.bar[kGotT], 2 * kTok);
+        bulk_load(mem + Mem::T, a.keep.solve + (n0 + chunks - 1 - r) * 2 * kTok, 2 * kTok, &sh.bar[kGotT]);
+      };
+      for (int r = 0; r < kStages && r < chunks; ++r) load_k(r);
+      load_q(0);
+      load_t(0);
+      const uint32_t base = smem_u32(mem);
+      const Operand S{base + Mem::S, Mem::kPanelS}, X{base + Mem::X, Mem::kPlaneX}, Y{base + Mem::Y, Mem::kPlaneX},
+          O{base + Mem::O, Mem::kPlaneX}, Q{base + Mem::Q, kTok}, At{base + Mem::P, kTok}, T{base + Mem::T, kTok};
+      for (int r = 0; r < chunks; ++r) {
+        const Operand K{base + Mem::K + r % kStages * P * Mem::kPlaneK, kTok};
+        if (!wait(&sh.bar[kDstateSet], r)) break;
+        if (!wait(&sh.bar[kStages == 2 && (r & 1) ? kGotK2 : kGotK], kStages == 2 ? r >> 1 : r)) break;
+        tc_fence_after();
+        multiply_parts<kSteps, 64, false, false, 2, P>(tm + cK, S, Mem::kPlaneS, K, Mem::kPlaneK, false);
+        if (!wait(&sh.bar[kOutsSet], r)) break;
+        if (!wait(&sh.bar[kGotQ], r)) break;
+        tc_fence_after();
+        multiply_parts<4, 64, false, true, P, 2>(tm + cO, O, Mem::kPlaneX, At, kTok, false);
+        tc_commit(&sh.bar[kMixDone]);
+        multiply_parts<4, DK, false, true, 2, P>(tm + cS, Y, Mem::kPlaneX, Q, Mem::kPlaneK, true);
+        tc_commit(&sh.bar[kOutsDone]);
+        if (!wait(&sh.bar[kGradSet], r)) break;
+        if (!wait(&sh.bar[kGotT], r)) break;
+        tc_fence_after();
+        multiply_parts<4, 64, false, true, 2, 2>(tm + cV, X, Mem::kPlaneX, T, kTok, false);
+        tc_commit(&sh.bar[kBackDone]);
+        if (!wait(&sh.bar[kOutsDone], r)) break;
+        if (r + 1 < chunks) load_q(r + 1);
+        if (!wait(&sh.bar[kReadsSet], r)) break;
+        if (r + 1 < chunks) load_t(r + 1);
+        tc_fence_after();
+        multiply_parts<4, DK, false, true, 2, P>(tm + cS, X, Mem::kPlaneX, K, Mem::kPlaneK, true);
+        tc_commit(&sh.bar[kDstateDone]);
+        if (!wait(&sh.bar[kDstateDone], r)) break;
+        if (r + kStages < chunks) load_k(r + kStages);
+      }
+    }
+  } else {
+    const Seat seat;
+    const bool there = seat.row < DV, in = seat.row < width;
+    const int t32 = seat.half * 32;
+    Meeting meet{&sh.bar[kMeet2]};
+    const long long step = (long long)d.H * d.dv, at_head = ((long long)b * d.T * d.H + h) * d.dv + v0 + seat.row;
+    const I* go = reinterpret_cast<const I*>(a.g_out) + at_head;
+    I* dv = reinterpret_cast<I*>(a.dv) + at_head;
+    constexpr int kCols = DK / 2;
+    for (int r = 0; r <= chunks && !wait.dead; ++r) {
+      const int c = chunks - 1 - r;
+      if (r > 0 && !wait(&sh.bar[kDstateDone], r - 1)) break;
+      tc_fence_after();
+      if (tid == 0) bulk_read_done();
+      if (c >= 0 && tid < kChunk) fill_factors(sh.f[r & 1], a.keep, n0 + c, m0 + c, tid);
+      meet(wait);
+      if (wait.dead) break;
+      const float2 end = c >= 0 ? a.keep.total[(n0 + c) * kChunk + kChunk - 1] : make_float2(0.f, 0.f);
+      const float left = __expf(end.x + end.y);
+      I x[32];
+      if (c >= 0) column_of(go + (long long)c * kChunk * step, step, t32, d.T - c * kChunk, in, x);
+#pragma unroll
+      for (int k = 0; k < kCols / 32; ++k) {
+        const int col = seat.half * kCols + k * 32;
+        float f[32];
+        if (r > 0) {
+          tmem_row(tm + seat.lanes + cS + col, f);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            f[i] = a.g_last != nullptr && in && col + i < d.dk ? a.g_last[(head * d.dk + col + i) * d.dv + v0 + seat.row] : 0.f;
+        }
+        if (c < 0) {
+          if (a.dfirst != nullptr && in) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (col + i < d.dk) a.dfirst[(head * d.dk + col + i) * d.dv + v0 + seat.row] = f[i];
+          }
+          continue;
+        }
+        if (there) {
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = f[p * 8 + i];
+            unsigned char* to = mem + Mem::S + (col >> 6) * Mem::kPanelS + piece_at(seat.row, ((col >> 3) & 7) + p);
+            put8(to, to + Mem::kPlaneS, y);
+          }
+        }
+        uint32_t u[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(f[i] * left);
+        tmem_st_32x32b_x32(tm + seat.lanes + cS + col, u);
+      }
+      if (c < 0) break;
+      tmem_st_wait();
+      hand_over(&sh.bar[kDstateSet]);
+      const Factors& fac = sh.f[r & 1];
+      if (there) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          float y[8];
+          const int at = piece_at(seat.row, seat.half * 4 + p);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) y[k] = ElemOf<I>::up(x[p * 8 + k]);
+          if constexpr (P == 2) put8(mem + Mem::O + at, mem + Mem::O + Mem::kPlaneX + at, y);
+          else *reinterpret_cast<uint4*>(mem + Mem::O + at) = raw_down<I, uint4>(y);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) y[k] *= fac.grown_q[t32 + p * 8 + k];
+          put8(mem + Mem::Y + at, mem + Mem::Y + Mem::kPlaneX + at, y);
+        }
+      }
+      hand_over(&sh.bar[kOutsSet]);
+      meet(wait);
+      const long long at_n = (n0 + c) * slices + slice;
+      if (tid == 0 && !wait.dead) {
+        bulk_store(a.dstates + at_n * 2 * Mem::kPlaneS, mem + Mem::S, 2 * Mem::kPlaneS);
+        bulk_store(a.douts + at_n * P * Mem::kPlaneX, mem + Mem::O, P * Mem::kPlaneX);
+        bulk_commit();
+      }
+      if (!wait(&sh.bar[kMixDone], r)) break;
+      tc_fence_after();
+      float f[32], y32[32];
+      tmem_row(tm + seat.lanes + cK + t32, f);
+      tmem_row(tm + seat.lanes + cO + t32, y32);
+      if (there) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          float y[8];
+          const int at = piece_at(seat.row, seat.half * 4 + p);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int i = p * 8 + k;
+            y[k] = fac.beta[t32 + i] * fmaf(fac.left_k[t32 + i], f[i], y32[i]);
+          }
+          put8(mem + Mem::X + at, mem + Mem::X + Mem::kPlaneX + at, y);
+        }
+      }
+      hand_over(&sh.bar[kGradSet]);
+      if (!wait(&sh.bar[kBackDone], r) || !wait(&sh.bar[kOutsDone], r)) break;  // the solve, and Y read
+      tc_fence_after();
+      tmem_row(tm + seat.lanes + cV + t32, f);
+      if (there) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          float y[8];
+          const int at = piece_at(seat.row, seat.half * 4 + p);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) y[k] = f[p * 8 + k];
+          put8(mem + Mem::Y + at, mem + Mem::Y + Mem::kPlaneX + at, y);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) y[k] *= -fac.grown_k[t32 + p * 8 + k];
+          put8(mem + Mem::X + at, mem + Mem::X + Mem::kPlaneX + at, y);
+        }
+      }
+      hand_over(&sh.bar[kReadsSet]);
+      meet(wait);
+      if (tid == 0 && !wait.dead) {
+        bulk_store(a.dreads + at_n * 2 * Mem::kPlaneX, mem + Mem::Y, 2 * Mem::kPlaneX);
+        bulk_commit();
+      }
+      if (in) {
+        const int t0 = c * kChunk + t32;
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (t0 + i < d.T) dv[(long long)(t0 + i) * step] = ElemOf<I>::down(f[i]);
+      }
+    }
+    if (tid == 0) bulk_done();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tm, 512);
+  }
+}
+
+template <typename I, int DK, int DV>
+void state(const DeltaFwd& a, cudaStream_t s) {
+  constexpr int bytes = StateMem<I, DK, DV>::kTiles + (int)sizeof(StateShared);
+  static_assert(bytes <= 227 * 1024, "shared memory");
+  cudaFuncSetAttribute(state_kernel<I, DK, DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  state_kernel<I, DK, DV><<<(unsigned)(a.d.B * a.d.H * a.d.slices), kWorkers + 32, bytes, s>>>(a);
+}
+
+template <typename I, int DK, int DV>
+void dstate(const DeltaBwd& a, cudaStream_t s) {
+  constexpr int bytes = DstateMem<I, DK, DV>::kTiles + (int)sizeof(DstateShared);
+  static_assert(bytes <= 227 * 1024, "shared memory");
+  cudaFuncSetAttribute(dstate_kernel<I, DK, DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  dstate_kernel<I, DK, DV><<<(unsigned)(a.d.B * a.d.H * a.d.slices), kWorkers + 32, bytes, s>>>(a);
+}
+
+template <typename I>
+void state_of(const DeltaFwd& a, cudaStream_t s) {
+  if (a.d.slice == 64) return a.d.dk <= 64 ? state<I, 64, 64>(a, s) : state<I, 128, 64>(a, s);
+  if constexpr (kParts<I> == 1)
+    if (a.d.dk > 64) return state<I, 128, 128>(a, s);
+  state<I, 64, 128>(a, s);
+}
+
+template <typename I>
+void dstate_of(const DeltaBwd& a, cudaStream_t s) {
+  if (a.d.slice == 64) return a.d.dk <= 64 ? dstate<I, 64, 64>(a, s) : dstate<I, 128, 64>(a, s);
+  if constexpr (kParts<I> == 1)
+    if (a.d.dk > 64) return dstate<I, 128, 128>(a, s);
+  dstate<I, 64, 128>(a, s);
+}
+
+}  // namespace
+
+void delta_state(const DeltaFwd& a, cudaStream_t s) {
+  a.d.type == Elem::kBF16 ? state_of<bf16>(a, s) : state_of<__half>(a, s);
+}
+
+void delta_dstate(const DeltaBwd& a, cudaStream_t s) {
+  a.d.type == Elem::kBF16 ? dstate_of<bf16>(a, s) : dstate_of<__half>(a, s);
+}
+
+}  // namespace bw

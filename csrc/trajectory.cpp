@@ -229,7 +229,9 @@ bw::DeltaDims delta_dims(const DeltaIn& x, double scale) {
   d.chunks = (d.T + bw::kChunk - 1) / bw::kChunk;
   d.type = elem_of(x.q, "q");
   d.scale = (float)scale;
-  d.wide = rows_aligned(x.q) && rows_aligned(x.k) && rows_aligned(x.v);
+  d.wide = rows_aligned(x.q) && rows_aligned(x.k);
+  d.slice = d.dv <= 64 || (d.dk > 64 && d.type == bw::Elem::kF16) ? 64 : 128;
+  d.slices = (d.dv + d.slice - 1) / d.slice;
   return d;
 }
 
@@ -283,38 +285,52 @@ Tensor take_state(const Tensor& state, const DeltaIn& x, const char* name) {
 
 // The forward's workspace, kept for the backward where there is one.
 struct Kept {
-  Tensor halves, floats;  // 16-bit planes: solve, attend, writes, states; 32-bit: total, beta, rk, rq
+  Tensor tiles, floats;  // keys, queries, solve, attend, writes, states; total, beta, rk, rq
 };
 
-// Elements of each part, each part on a 16-byte boundary.
+// Bytes of the tiles and numbers of the floats of each part.
 struct KeptSizes {
-  int64_t square, writes, states, tokens, rows;
-  explicit KeptSizes(const bw::DeltaDims& d) {
-    const int64_t n = (int64_t)d.B * d.H * d.chunks;
-    square = n * 2 * bw::kChunk * bw::kChunk;
-    writes = n * 2 * bw::kChunk * d.dv;
-    states = (int64_t)d.B * d.H * (d.chunks + 1) * 2 * d.dk * d.dv;
-    tokens = n * bw::kChunk;
-    rows = (int64_t)d.B * d.Hk * d.chunks * bw::kChunk;
+  int64_t rows, square, column, state, n, m, keys, writes, states;
+  KeptSizes(const bw::DeltaDims& d, bool keep) {
+    const int64_t parts = d.type == bw::Elem::kF16 ? 2 : 1, panels = d.dk <= 64 ? 1 : 2;
+    rows = parts * panels * bw::kChunk * 128;  // q or k of a chunk
+    square = 2 * bw::kChunk * 128;
+    column = (int64_t)d.slices * d.slice * 128;  // a chunk's values, one half of them
+    state = 2 * column * panels;
+    n = (int64_t)d.B * d.H * d.chunks;
+    m = (int64_t)d.B * d.Hk * d.chunks;
+    keys = m * rows;
+    writes = keep ? n * 2 * column : 0;
+    states = keep ? (int64_t)d.B * d.H * (d.chunks + 1) * state : 0;
   }
 };
 
-Kept make_kept(const bw::DeltaDims& d, const Tensor& like) {
-  const KeptSizes z(d);
-  return Kept{torch::empty({2 * z.square + z.writes + z.states}, like.options().dtype(torch::kBFloat16)),
-              torch::empty({3 * z.tokens + 2 * z.rows}, like.options().dtype(torch::kFloat32))};
+Kept make_kept(const bw::DeltaDims& d, const Tensor& like, bool keep) {
+  const KeptSizes z(d, keep);
+  return Kept{torch::empty({2 * z.keys + 2 * z.n * z.square + z.writes + z.states}, like.options().dtype(torch::kUInt8)),
+              torch::empty({(3 * z.n + 2 * z.m) * bw::kChunk}, like.options().dtype(torch::kFloat32))};
 }
 
-bw::DeltaKept kept_parts(const bw::DeltaDims& d, const Kept& k) {
-  const KeptSizes z(d);
-  auto* h = reinterpret_cast<__nv_bfloat16*>(k.halves.data_ptr());
+bw::DeltaKept kept_parts(const bw::DeltaDims& d, const Kept& k, bool keep) {
+  const KeptSizes z(d, keep);
+  bw::DeltaKept p;
+  p.keys = k.tiles.data_ptr<uint8_t>();
+  p.queries = p.keys + z.keys;
+  p.solve = p.queries + z.keys;
+  p.attend = p.solve + z.n * z.square;
+  p.writes = keep ? p.attend + z.n * z.square : nullptr;
+  p.states = keep ? p.writes + z.writes : nullptr;
   float* f = k.floats.data_ptr<float>();
-  return bw::DeltaKept{h, h + z.square, h + 2 * z.square, h + 2 * z.square + z.writes, reinterpret_cast<float2*>(f),
-                       f + 2 * z.tokens, f + 3 * z.tokens, f + 3 * z.tokens + z.rows};
+  p.total = reinterpret_cast<float2*>(f);
+  p.beta = f + 2 * z.n * bw::kChunk;
+  p.rk = p.beta + z.n * bw::kChunk;
+  p.rq = p.rk + z.m * bw::kChunk;
+  return p;
 }
 
 // {out, last state (or nothing)}; what it leaves in `kept`.
-std::pair<Tensor, Tensor> delta_fwd(const DeltaIn& x, const OptTensor& first, bool want_last, double scale, Kept& kept) {
+std::pair<Tensor, Tensor> delta_fwd(const DeltaIn& x, const OptTensor& first, bool want_last, double scale, const Tensor& err,
+                                    bool keep, Kept& kept) {
   const c10::cuda::CUDAGuard guard(x.q.device());
   bw::DeltaFwd f;
   f.d = delta_dims(x, scale);
@@ -322,8 +338,10 @@ std::pair<Tensor, Tensor> delta_fwd(const DeltaIn& x, const OptTensor& first, bo
   f.k = head_rows(x.k);
   f.v = head_rows(x.v);
   f.g = delta_gates(x);
-  kept = make_kept(f.d, x.q);
-  f.keep = kept_parts(f.d, kept);
+  kept = make_kept(f.d, x.q, keep);
+  f.keep = kept_parts(f.d, kept, keep);
+  check_like(err, "err", torch::kInt32, x.q);
+  f.err = err.data_ptr<int>();
   auto out = torch::empty({f.d.B, f.d.T, f.d.H, f.d.dv}, x.v.options());
   Tensor last;
   if (want_last) last = torch::empty({f.d.B, f.d.H, f.d.dk, f.d.dv}, x.q.options().dtype(torch::kFloat32));
@@ -338,18 +356,19 @@ std::pair<Tensor, Tensor> delta_fwd(const DeltaIn& x, const OptTensor& first, bo
 struct GatedDelta : torch::autograd::Function<GatedDelta> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& a,
                                const Tensor& b, const Tensor& a_log, const Tensor& dt_bias, const OptTensor& first, bool want_last,
-                               double scale) {
+                               double scale, const Tensor& err) {
     Kept kept;
-    auto [out, last] = delta_fwd(DeltaIn{q, k, v, a, b, a_log, dt_bias}, first, want_last, scale, kept);
+    auto [out, last] = delta_fwd(DeltaIn{q, k, v, a, b, a_log, dt_bias}, first, want_last, scale, err, true, kept);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({q, k, v, a, b, a_log, dt_bias, kept.halves, kept.floats});
+    ctx->save_for_backward({q, k, v, a, b, a_log, dt_bias, kept.tiles, kept.floats});
+    ctx->saved_data["err"] = err;
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["first"] = first.has_value();
     if (!want_last) return {out};
     return {out, last};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    variable_list grads(10);
+    variable_list grads(11);
     const bool handed = g.size() > 1 && g[1].defined();
     if (!g[0].defined() && !handed) return grads;
     const auto s = ctx->get_saved_variables();
@@ -361,18 +380,21 @@ struct GatedDelta : torch::autograd::Function<GatedDelta> {
     w.k = head_rows(x.k);
     w.v = head_rows(x.v);
     w.g = delta_gates(x);
-    w.keep = kept_parts(w.d, Kept{s[7], s[8]});
-    Tensor g_out = g[0].defined() ? g[0].contiguous() : torch::zeros({w.d.B, w.d.T, w.d.H, w.d.dv}, x.v.options());
-    if (!at_multiple(g_out.data_ptr(), 16)) g_out = g_out.clone();
+    w.keep = kept_parts(w.d, Kept{s[7], s[8]}, true);
+    const Tensor err = error_word(ctx);
+    w.err = err.data_ptr<int>();
+    const Tensor g_out = g[0].defined() ? g[0].contiguous() : torch::zeros({w.d.B, w.d.T, w.d.H, w.d.dv}, x.v.options());
     w.g_out = g_out.data_ptr();
     Tensor g_last;
     if (handed) g_last = g[1].contiguous();
     w.g_last = handed ? g_last.data_ptr<float>() : nullptr;
-    const int64_t n = (int64_t)w.d.B * w.d.H * w.d.chunks;
-    auto half = torch::empty({n * 2 * ((int64_t)w.d.dk + bw::kChunk) * w.d.dv}, x.q.options().dtype(torch::kBFloat16));
-    auto part = torch::empty({2 * n}, x.q.options().dtype(torch::kFloat32));
-    w.dstates = reinterpret_cast<__nv_bfloat16*>(half.data_ptr());
-    w.dreads = w.dstates + n * 2 * w.d.dk * w.d.dv;
+    const KeptSizes z(w.d, true);
+    const int64_t parts = w.d.type == bw::Elem::kF16 ? 2 : 1;
+    auto tiles = torch::empty({z.n * (z.state + (2 + parts) * z.column)}, x.q.options().dtype(torch::kUInt8));
+    auto part = torch::empty({2 * z.n}, x.q.options().dtype(torch::kFloat32));
+    w.dstates = tiles.data_ptr<uint8_t>();
+    w.dreads = w.dstates + z.n * z.state;
+    w.douts = w.dreads + z.n * 2 * z.column;
     w.part = part.data_ptr<float>();
     for (int i = 0; i < 7; ++i) grads[i] = torch::empty(s[i].sizes(), s[i].options());
     w.dq = grads[0].data_ptr();
@@ -394,7 +416,7 @@ struct GatedDelta : torch::autograd::Function<GatedDelta> {
 };
 
 std::pair<Tensor, OptTensor> gated_delta_rule(Tensor q, Tensor k, Tensor v, Tensor a, Tensor b, Tensor a_log, Tensor dt_bias,
-                                              OptTensor first, bool want_last, std::optional<double> scale) {
+                                              OptTensor first, bool want_last, std::optional<double> scale, Tensor err) {
   DeltaIn x{q, k, v, a, b, a_log, dt_bias};
   const double by = take_delta(x, scale);
   TORCH_CHECK_TYPE(x.q.scalar_type() == torch::kBFloat16 || x.q.scalar_type() == torch::kHalf,
@@ -404,10 +426,10 @@ std::pair<Tensor, OptTensor> gated_delta_rule(Tensor q, Tensor k, Tensor v, Tens
   for (const Tensor* t : {&x.q, &x.k, &x.v, &x.a, &x.b, &x.a_log, &x.dt_bias}) tracked = tracked || wants_grad(*t);
   if (!tracked) {
     Kept kept;
-    auto [out, last] = delta_fwd(x, first, want_last, by, kept);
+    auto [out, last] = delta_fwd(x, first, want_last, by, err, false, kept);
     return {out, want_last ? OptTensor(last) : std::nullopt};
   }
-  auto out = GatedDelta::apply(x.q, x.k, x.v, x.a, x.b, x.a_log, x.dt_bias, first, want_last, by);
+  auto out = GatedDelta::apply(x.q, x.k, x.v, x.a, x.b, x.a_log, x.dt_bias, first, want_last, by, err);
   return {out[0], want_last ? OptTensor(out[1]) : std::nullopt};
 }
 

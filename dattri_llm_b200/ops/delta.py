@@ -18,7 +18,7 @@ import math
 import torch
 import torch.nn.functional as F
 
-from dattri_llm_b200.ops import native, use_native
+from dattri_llm_b200.ops import error_word, native, use_native
 
 CHUNK = 64
 MAX_KEY_DIM = 128  # of a head on the GPU (kMostKeyDim of csrc/delta_rule.cuh)
@@ -109,7 +109,8 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, a: torch
         with ``b = -inf`` writes nothing; one with ``a = +inf`` forgets everything before it.
     """
     if use_native(q):
-        return native().gated_delta_rule(q, k, v, a, b, a_log, dt_bias, initial_state, output_final_state, scale)
+        return native().gated_delta_rule(q, k, v, a, b, a_log, dt_bias, initial_state, output_final_state, scale,
+                                         error_word(q.device))
     scale = _check(q, k, v, a, b, a_log, dt_bias, scale)
     parts = _parts(q, k, v, a, b, a_log, dt_bias, scale)
     if initial_state is None:
