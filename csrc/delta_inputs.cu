@@ -158,10 +158,13 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
       const bool in = row < min(DV, d.dv - v0);
       // A lane holds an element of the values: V' . dV (the first four warps) and v . dv (the others) of all tokens.
       float x[64];
-      if (half == 1) {
-        const I* v = head_at<I>(a.v, b, t0, h) + v0 + row;
+      I v[2][32];
 #pragma unroll
-        for (int i = 0; i < 64; ++i) x[i] = in && i < rows ? ElemOf<I>::up(v[i * a.v.st]) : 0.f;
+      for (int i = 0; i < 64; ++i) v[i >> 5][i & 31] = ElemOf<I>::down(0.f);
+      if (half == 1 && in) {
+        const I* from = head_at<I>(a.v, b, t0, h) + v0 + row;
+        column_of(from, a.v.st, rows, v[0]);
+        column_of(from + 32 * a.v.st, a.v.st, rows - 32, v[1]);
       }
       if (!wait(&sh.bar[kGotV], s)) break;
       const bool there = row < DV;
@@ -179,7 +182,8 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
           w[3] = pair_sum(wh.w, wl.w);
         } else {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) w[k] = make_float2(x[p * 8 + 2 * k], x[p * 8 + 2 * k + 1]);
+          for (int k = 0; k < 4; ++k)
+            w[k] = make_float2(ElemOf<I>::up(v[p >> 2][(p & 3) * 8 + 2 * k]), ElemOf<I>::up(v[p >> 2][(p & 3) * 8 + 2 * k + 1]));
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -188,17 +192,25 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
         }
       }
       lanes_fold(x);
-      // <dS', S'>: both tiles have their elements at the same places.
-      const uint4* after = reinterpret_cast<const uint4*>(state_at(c + 1, s));
-      constexpr int kPieces = Mem::kPlaneS / 16;
       sh.part[half][warp & 3][2 * lane] = s ? sh.part[half][warp & 3][2 * lane] + x[0] : x[0];
       sh.part[half][warp & 3][2 * lane + 1] = s ? sh.part[half][warp & 3][2 * lane + 1] + x[1] : x[1];
+      // <dS', S'>: both tiles have their elements at the same places.
+      const uint4* after = reinterpret_cast<const uint4*>(state_at(c + 1, s));
+      constexpr int kPieces = Mem::kPlaneS / 16, kMine = kPieces / kWorkers;
+      static_assert(kPieces % kWorkers == 0, "whole rounds");
+      uint4 ah[kMine], al[kMine];
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        ah[i] = __ldcs(after + i * kWorkers + tid);
+        al[i] = __ldcs(after + kPieces + i * kWorkers + tid);
+      }
       if (!wait(&sh.bar[kGotD], s)) break;
-#pragma unroll 2
-      for (int i = tid; i < kPieces; i += kWorkers) {
-        const uint4 ah = after[i], al = after[kPieces + i];
-        const uint4 dh = *reinterpret_cast<const uint4*>(mem + Mem::S + i * 16), dl = *reinterpret_cast<const uint4*>(mem + Mem::S + Mem::kPlaneS + i * 16);
-        const uint32_t u[4] = {ah.x, ah.y, ah.z, ah.w}, v[4] = {al.x, al.y, al.z, al.w}, y[4] = {dh.x, dh.y, dh.z, dh.w}, z[4] = {dl.x, dl.y, dl.z, dl.w};
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const unsigned char* at = mem + Mem::S + (i * kWorkers + tid) * 16;
+        const uint4 dh = *reinterpret_cast<const uint4*>(at), dl = *reinterpret_cast<const uint4*>(at + Mem::kPlaneS);
+        const uint32_t u[4] = {ah[i].x, ah[i].y, ah[i].z, ah[i].w}, v[4] = {al[i].x, al[i].y, al[i].z, al[i].w},
+                       y[4] = {dh.x, dh.y, dh.z, dh.w}, z[4] = {dl.x, dl.y, dl.z, dl.w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const float2 e = pair_sum(u[k], v[k]), f = pair_sum(y[k], z[k]);
@@ -225,6 +237,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
       }
       const float by = of_l ? -sh.rk[i] : sh.rq[i];
       const float2 Gi = sh.G[i];
+      const int last = of_l ? i : i + 1;
       unsigned char* to = mem + (of_l ? Mem::N : Mem::W);
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
@@ -232,7 +245,8 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const int j = j0 + p * 8 + k;
-          x[k] = j < i || (j == i && !of_l) ? f[p * 8 + k] * by * (decay_between(Gi, sh.G[j]) * sh.rk[j]) : 0.f;
+          const float w = f[p * 8 + k] * by * (decay_between(Gi, sh.G[j]) * sh.rk[j]);
+          x[k] = j < last ? w : 0.f;
         }
         const int at = piece_at(i, half * 4 + p);
         put8(to + at, to + kTok + at, x);
@@ -281,17 +295,40 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
       sh.dots[1][tid] += sh.part[1][w][tid];
     }
   }
-  // q^ . dq^ = q . dq of this head's rows
-  for (int i = warp; i < rows; i += 9) {
-    const I* q = head_at<I>(a.q, b, t0 + i, hk);
-    float dot = 0.f;
-#pragma unroll
-    for (int k = 0; k < DK / 32; ++k) {
-      const int col = k * 32 + lane;
-      if (col < d.dk) dot = fmaf(ElemOf<I>::up(q[col]), F[i * Mem::ldF + col], dot);
+  // q^ . dq^ = q . dq of this head's rows, a row's elements side by side in a warp; the rows of q and k still lie as tiles.
+  constexpr int kE = DK / 32;  // elements of a lane
+  const auto row_of = [&](int tile, int i, float (&x)[kE]) {
+    const unsigned char* at = mem + tile + element_at(i, lane * kE, kTok);
+    float lo[kE];
+    if constexpr (kE == 4) {
+      raw_up<bf16>(*reinterpret_cast<const uint2*>(at), x);
+      if (P == 2) raw_up<bf16>(*reinterpret_cast<const uint2*>(at + Mem::kPlaneK), lo);
+    } else {
+      raw_up<bf16>(*reinterpret_cast<const uint32_t*>(at), x);
+      if (P == 2) raw_up<bf16>(*reinterpret_cast<const uint32_t*>(at + Mem::kPlaneK), lo);
     }
-    dot = lanes_sum(dot);
-    if (lane == 0) sh.dots[2][i] = dot;
+    if (P == 2)
+#pragma unroll
+      for (int k = 0; k < kE; ++k) x[k] += lo[k];
+  };
+  const auto sums_of = [&](const float* f, float (&y)[kE], bool add) {
+    float z[kE];
+    if constexpr (kE == 4) *reinterpret_cast<float4*>(z) = *reinterpret_cast<const float4*>(f + lane * kE);
+    else *reinterpret_cast<float2*>(z) = *reinterpret_cast<const float2*>(f + lane * kE);
+#pragma unroll
+    for (int k = 0; k < kE; ++k) y[k] = add ? y[k] + z[k] : z[k];
+  };
+  if (warp < 8) {
+#pragma unroll 4
+    for (int i = warp; i < kChunk; i += 8) {
+      float x[kE], y[kE], dot = 0.f;
+      row_of(Mem::Q, i, x);
+      sums_of(F + i * Mem::ldF, y, false);
+#pragma unroll
+      for (int k = 0; k < kE; ++k) dot = fmaf(x[k], y[k], dot);
+      dot = lanes_sum(dot);
+      if (lane == 0) sh.dots[2][i] = dot;
+    }
   }
   cg::cluster_group cluster = cg::this_cluster();
   if (group > 1) cluster.sync();
@@ -334,30 +371,36 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
   } else {
     // Sums over the key head's value heads, the rows of both shared out over the cluster's warps, then back through the
     // rows' scaling: with x a row, r its reciprocal length and y the sum, dx = y - x r^2 (x . y).
-    for (int r = hg * 8 + warp; r < 2 * kChunk; r += 8 * group) {
-      const int i = r % kChunk;
-      if (i >= rows) continue;
-      const bool of_k = r >= kChunk;
-      const I* x = of_k ? head_at<I>(a.k, b, t0 + i, hk) : head_at<I>(a.q, b, t0 + i, hk);
-      float y[DK / 32], v[DK / 32], dot = 0.f;
+    const float* from[kMostGroup];
 #pragma unroll
-      for (int k = 0; k < DK / 32; ++k) {
-        const int col = k * 32 + lane;
-        y[k] = 0.f;
-        for (int o = 0; o < group; ++o) {
-          const float* f = group > 1 ? cluster.map_shared_rank(F, o) : F;
-          y[k] += f[r * Mem::ldF + col];
-        }
-        v[k] = col < d.dk ? ElemOf<I>::up(x[col]) : 0.f;
-        dot = fmaf(v[k], y[k], dot);
+    for (int o = 0; o < kMostGroup; ++o) from[o] = group > 1 ? cluster.map_shared_rank(F, o < group ? o : 0) : F;
+    // Four rows at a time, so that their loads are on their way together.
+    for (int r0 = hg * 8 + warp; r0 < 2 * kChunk; r0 += 32 * group) {
+      float y[4][kE], x[4][kE], dot[4];
+#pragma unroll
+      for (int n4 = 0; n4 < 4; ++n4) {
+        const int r = min(r0 + n4 * 8 * group, 2 * kChunk - 1);
+        row_of(r >= kChunk ? Mem::K : Mem::Q, r % kChunk, x[n4]);
+#pragma unroll
+        for (int o = 0; o < kMostGroup; ++o)
+          if (o < group) sums_of(from[o] + r * Mem::ldF, y[n4], o > 0);
+        dot[n4] = 0.f;
+#pragma unroll
+        for (int k = 0; k < kE; ++k) dot[n4] = fmaf(x[n4][k], y[n4][k], dot[n4]);
       }
-      dot = lanes_sum(dot);
-      const float len = of_k ? sh.rk[i] : sh.rq[i] / d.scale;
-      I* to = reinterpret_cast<I*>(of_k ? a.dk : a.dq) + (((long long)b * d.T + t0 + i) * d.Hk + hk) * d.dk;
 #pragma unroll
-      for (int k = 0; k < DK / 32; ++k) {
-        const int col = k * 32 + lane;
-        if (col < d.dk) to[col] = ElemOf<I>::down(y[k] - v[k] * (len * len * dot));
+      for (int n4 = 0; n4 < 4; ++n4) dot[n4] = lanes_sum(dot[n4]);
+#pragma unroll
+      for (int n4 = 0; n4 < 4; ++n4) {
+        const int r = r0 + n4 * 8 * group, i = r % kChunk;
+        if (r >= 2 * kChunk || i >= rows || lane * kE >= d.dk) continue;
+        const bool of_k = r >= kChunk;
+        const float len = of_k ? sh.rk[i] : sh.rq[i] / d.scale, by = -len * len * dot[n4];
+#pragma unroll
+        for (int k = 0; k < kE; ++k) y[n4][k] = fmaf(by, x[n4][k], y[n4][k]);
+        I* to = reinterpret_cast<I*>(of_k ? a.dk : a.dq) + (((long long)b * d.T + t0 + i) * d.Hk + hk) * d.dk + lane * kE;
+        if constexpr (kE == 4) *reinterpret_cast<uint2*>(to) = raw_down<I, uint2>(y[n4]);
+        else *reinterpret_cast<uint32_t*>(to) = raw_down<I, uint32_t>(y[n4]);
       }
     }
   }

@@ -34,10 +34,11 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// acc (16 x 16 NP) += A (16 x K, from row m0) B (K x 16 NP, from column n0) of a warp. kAT: A is stored (K, M); kBT: B is
+// acc (16 x 16 NP) += A (16 x K, from row m0) B (K x 16 NP, from column n0) of a warp, of which only the first `some` blocks of
+// 16 columns are wanted. kAT: A is stored (K, M); kBT: B is
 // stored (N, K). kA and kB: parts of each.
 template <int NP, int K, bool kAT, bool kBT, int kA, int kB>
-__device__ __forceinline__ void product(float (&acc)[2 * NP][4], const Tile& A, int m0, const Tile& B, int n0) {
+__device__ __forceinline__ void product(float (&acc)[2 * NP][4], const Tile& A, int m0, const Tile& B, int n0, int some) {
   const int lane = threadIdx.x & 31;
   const bf16* a = kAT ? A.p + ((lane >> 4) * 8 + (lane & 7)) * A.ld + m0 + ((lane >> 3) & 1) * 8
                       : A.p + (m0 + (lane & 15)) * A.ld + (lane >> 4) * 8;
@@ -51,6 +52,7 @@ __device__ __forceinline__ void product(float (&acc)[2 * NP][4], const Tile& A, 
     if (kA == 2) ldmatrix4<kAT>(al, a + A.lo + k * step_a);
 #pragma unroll
     for (int n = 0; n < NP; ++n) {
+      if (n >= some) break;
       const bf16* bn = b + k * step_b + (kBT ? n * 16 * B.ld : n * 16);
       uint32_t bh[4], bl[4];
       ldmatrix4<!kBT>(bh, bn);
@@ -74,12 +76,6 @@ __device__ __forceinline__ void put2(bf16* p, int lo, float x, float y) {
   halves(x, y, h, l);
   *reinterpret_cast<uint32_t*>(p) = h;
   *reinterpret_cast<uint32_t*>(p + lo) = l;
-}
-
-__device__ __forceinline__ float2 get2(const bf16* p, int lo) {
-  const float2 h = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p));
-  const float2 l = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p + lo));
-  return make_float2(h.x + l.x, h.y + l.y);
 }
 
 // ---------------------------------------------------------------- loads
@@ -183,17 +179,25 @@ __global__ void __launch_bounds__(128) prepare_kernel(const DeltaFwd a) {
       a.keep.total[at.n * kChunk + 2 * lane + k] = g;
     }
   }
-  for (int r = warp; r < 2 * kChunk; r += 4) {  // lengths
-    const bf16* x = (r < kChunk ? K : Q) + (r % kChunk) * ld;
-    float sq = 0.f;
-    for (int i = lane * 2; i < DK; i += 64) {
-      float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(x + i));
-      if (kParts<I> == 2) v = get2(x + i, plane);
-      sq = fmaf(v.x, v.x, fmaf(v.y, v.y, sq));
+  {  // lengths: a row of k or q to each thread
+    const bf16* x = (tid < kChunk ? K : Q) + (tid & 63) * ld;
+    float sq[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < DK; i += 8) {
+      float f[8];
+      raw_up<bf16>(*reinterpret_cast<const uint4*>(x + i), f);
+      if (kParts<I> == 2) {
+        float lo[8];
+        raw_up<bf16>(*reinterpret_cast<const uint4*>(x + plane + i), lo);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] += lo[k];
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sq[k & 1] = fmaf(f[k], f[k], sq[k & 1]);
     }
-    sq = lanes_sum(sq);
-    const float len = rsqrtf(sq + 1e-6f);
-    if (lane == 0) (r < kChunk ? rk[r] : rq[r - kChunk]) = r < kChunk ? len : len * d.scale;
+    const float len = rsqrtf(sq[0] + sq[1] + 1e-6f);
+    if (tid < kChunk) rk[tid] = len;
+    else rq[tid - kChunk] = len * d.scale;
   }
   float kk[8][4], qk[8][4];
 #pragma unroll
@@ -201,8 +205,8 @@ __global__ void __launch_bounds__(128) prepare_kernel(const DeltaFwd a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) kk[i][j] = qk[i][j] = 0.f;
   const Tile tk{K, ld, plane}, tq{Q, ld, plane};
-  product<4, DK, false, true, kParts<I>, kParts<I>>(kk, tk, warp * 16, tk, 0);
-  product<4, DK, false, true, kParts<I>, kParts<I>>(qk, tq, warp * 16, tk, 0);
+  product<4, DK, false, true, kParts<I>, kParts<I>>(kk, tk, warp * 16, tk, 0, warp + 1);
+  product<4, DK, false, true, kParts<I>, kParts<I>>(qk, tq, warp * 16, tk, 0, warp + 1);
   __syncthreads();
   if (at.h % group == 0) {  // the rows as tiles, for the other kernels
     if (tid < kChunk) {

@@ -44,36 +44,48 @@ struct Seat {
 // Of a chunk's tokens: what the products' columns are multiplied by.
 struct Factors {
   float grown_k[kChunk];  // exp(G) rk
-  float grown_q[kChunk];  // exp(G) rq
   float left_k[kChunk];   // exp(G_63 - G) rk
   float beta[kChunk];
+  float left;             // exp(G_63)
 };
 
-__device__ __forceinline__ void fill_factors(Factors& f, const DeltaKept& keep, long long n, long long m, int i) {
-  const float2 G = keep.total[n * kChunk + i], end = keep.total[n * kChunk + kChunk - 1];
-  const float rk = keep.rk[m * kChunk + i], grown = __expf(G.x + G.y);
-  f.grown_k[i] = grown * rk;
-  f.grown_q[i] = grown * keep.rq[m * kChunk + i];
-  f.left_k[i] = decay_between(end, G) * rk;
-  f.beta[i] = keep.beta[n * kChunk + i];
-}
-
-// 32 tokens' values of one column of head rows, from token t on; zeros behind the last token and for columns that are not there.
-template <typename I>
-__device__ __forceinline__ void column_of(const I* p, long long st, int t, int rows, bool in, I (&x)[32]) {
-#pragma unroll
-  for (int i = 0; i < 32; ++i) x[i] = in && t + i < rows ? p[(long long)(t + i) * st] : ElemOf<I>::down(0.f);
-}
-
-// The threads of a role meet on an mbarrier, so that a wait that gives up elsewhere leaves nobody behind.
-struct Meeting {
-  uint64_t* bar;
-  int round = 0;
-  __device__ __forceinline__ void operator()(Waiter& wait) {
-    mbar_arrive(bar);
-    wait(bar, round++);
+// What they are made of, of one token: read a chunk ahead.
+struct FactorParts {
+  float2 G, end;
+  float rk, rq, beta;
+  __device__ __forceinline__ void read(const DeltaKept& keep, long long n, long long m, int i) {
+    G = keep.total[n * kChunk + i];
+    end = keep.total[n * kChunk + kChunk - 1];
+    rk = keep.rk[m * kChunk + i];
+    rq = keep.rq[m * kChunk + i];
+    beta = keep.beta[n * kChunk + i];
+  }
+  __device__ __forceinline__ void fill(Factors& f, float* grown_q, int i) const {
+    const float grown = __expf(G.x + G.y);
+    f.grown_k[i] = grown * rk;
+    grown_q[i] = grown * rq;
+    f.left_k[i] = decay_between(end, G) * rk;
+    f.beta[i] = beta;
+    if (i == kChunk - 1) f.left = grown;
   }
 };
+
+template <typename I>
+__device__ __forceinline__ void put_column(I* p, long long st, int rows, const float (&x)[32]) {
+  if (rows >= 32) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      *p = ElemOf<I>::down(x[i]);
+      p += st;
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    if (i < rows) *p = ElemOf<I>::down(x[i]);
+    p += st;
+  }
+}
 
 // ---------------------------------------------------------------- state
 template <typename I, int DK, int DV>
@@ -86,12 +98,13 @@ struct StateMem {
                        Q = T + kStages * 2 * kTok, P = Q + kParts_ * kPlaneK, kTiles = P + 2 * kTok;
 };
 
-enum StateBar { kLoadedK, kLoadedK2, kLoadedQ, kStateSet, kRhsSet, kWritesSet, kReadDone, kSolveDone, kStateDone, kOutDone, kMeet, kStateBars };
+enum StateBar { kLoadedK, kLoadedK2, kLoadedQ, kStateSet, kRhsSet, kWritesSet, kReadDone, kSolveDone, kStateDone, kOutDone, kFree, kStateBars };
 
 struct StateShared {
   uint64_t bar[kStateBars];
   uint32_t tmem;
   Factors f[2];
+  float grown_q[3][kChunk];  // exp(G) rq: an output is written a chunk later than the factors are read
 };
 
 // One slice of a head's state, chunk after chunk. Tensor memory: S^T (128 x DK), K S, E, and twice Q S and P V'.
@@ -109,10 +122,15 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
   const int tid = threadIdx.x, warp = tid >> 5;
   if (tid == 0) {
     for (int i = 0; i < kStateBars; ++i)
-      mbar_init(&sh.bar[i], i == kStateSet || i == kRhsSet || i == kWritesSet || i == kMeet ? kWorkers : 1);
+      mbar_init(&sh.bar[i], i == kStateSet || i == kRhsSet || i == kWritesSet ? kWorkers : 1);
     fence_barrier_init();
   }
   if (warp == 8) tmem_alloc(&sh.tmem, 512);
+  FactorParts parts;
+  if (tid < kChunk && chunks > 0) {
+    parts.read(a.keep, n0, m0, tid);
+    parts.fill(sh.f[0], sh.grown_q[0], tid);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -120,7 +138,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
   constexpr uint32_t cS = 0, cK = 128, cE = 192, cQ = 256, cP = 320;  // the last two again 128 columns on
   Waiter wait{a.err};
   if (warp == 8) {
-    if ((tid & 31) == 0 && chunks > 0) {
+    if ((tid & 31) == 0) {
       const auto load_k = [&](int c) {
         const int st = c % kStages;
         uint64_t* bar = &sh.bar[kStages == 2 && (c & 1) ? kLoadedK2 : kLoadedK];
@@ -134,11 +152,17 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
         bulk_load(mem + Mem::P, a.keep.attend + (n0 + c) * 2 * kTok, 2 * kTok, &sh.bar[kLoadedQ]);
       };
       for (int c = 0; c < kStages && c < chunks; ++c) load_k(c);
-      load_q(0);
+      if (chunks > 0) load_q(0);
       const uint32_t base = smem_u32(mem);
       const Operand S{base + Mem::S, Mem::kPanelS}, X{base + Mem::X, Mem::kPlaneX}, W{base + Mem::W, Mem::kPlaneX},
           Q{base + Mem::Q, kTok}, At{base + Mem::P, kTok};
-      for (int c = 0; c < chunks; ++c) {
+      const auto store_state = [&](int c) {
+        if (a.keep.states == nullptr) return;
+        bulk_store(a.keep.states + ((head * (chunks + 1) + c) * slices + slice) * 2 * Mem::kPlaneS, mem + Mem::S, 2 * Mem::kPlaneS);
+        bulk_commit();
+      };
+      int c = 0;
+      for (; c < chunks; ++c) {
         const int st = c % kStages;
         const uint32_t flip = (c & 1) * 128;
         const Operand K{base + Mem::K + st * P * Mem::kPlaneK, kTok}, T{base + Mem::T + st * 2 * kTok, kTok};
@@ -147,6 +171,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
         tc_fence_after();
         multiply_parts<kSteps, 64, false, false, 2, P>(tm + cK, S, Mem::kPlaneS, K, Mem::kPlaneK, false);
         tc_commit(&sh.bar[kReadDone]);
+        store_state(c);
         if (!wait(&sh.bar[kLoadedQ], c)) break;
         multiply_parts<kSteps, 64, false, false, 2, P>(tm + cQ + flip, S, Mem::kPlaneS, Q, Mem::kPlaneK, false);
         if (!wait(&sh.bar[kRhsSet], c)) break;
@@ -159,19 +184,27 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
         tc_commit(&sh.bar[kStateDone]);
         multiply_parts<4, 64, false, false, 2, 2>(tm + cP + flip, W, Mem::kPlaneX, At, kTok, false);
         tc_commit(&sh.bar[kOutDone]);
+        if (a.keep.writes != nullptr) {
+          bulk_store(a.keep.writes + ((n0 + c) * slices + slice) * 2 * Mem::kPlaneX, mem + Mem::W, 2 * Mem::kPlaneX);
+          bulk_commit();
+        }
+        bulk_read_done();  // the tiles may be written again, once their products are done too
+        mbar_arrive(&sh.bar[kFree]);
         if (!wait(&sh.bar[kStateDone], c)) break;
         if (c + kStages < chunks) load_k(c + kStages);
         if (!wait(&sh.bar[kOutDone], c)) break;
         if (c + 1 < chunks) load_q(c + 1);
       }
+      if (c == chunks && wait(&sh.bar[kStateSet], chunks)) store_state(chunks);
+      bulk_done();
     }
   } else {
     const Seat seat;
     const bool there = seat.row < DV, in = seat.row < width;  // a lane of the slice; one with an element of the head
     const int t32 = seat.half * 32;
-    Meeting meet{&sh.bar[kMeet]};
     const I* v = head_at<I>(a.v, b, 0, h) + v0 + seat.row;
     I* out = reinterpret_cast<I*>(a.out) + ((long long)b * d.T * d.H + h) * d.dv + v0 + seat.row;
+    const long long step = (long long)d.H * d.dv;
     constexpr int kCols = DK / 2;  // of a worker's half of a state's row
     // Writes the state's row as halves into the tile, and scaled into tensor memory.
     const auto set_state = [&](const float (&f)[32], int col, float left) {
@@ -194,24 +227,25 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
       float x[32], y[32];
       tmem_row(tm + seat.lanes + cQ + flip + t32, x);
       tmem_row(tm + seat.lanes + cP + flip + t32, y);
-      if (in) {
-        const int t0 = c * kChunk + t32;
+      if (!in) return;
+      const float* by = sh.grown_q[c % 3] + t32;
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (t0 + i < d.T) out[(long long)(t0 + i) * d.H * d.dv] = ElemOf<I>::down(fmaf(sh.f[c & 1].grown_q[t32 + i], x[i], y[i]));
-      }
+      for (int i = 0; i < 32; ++i) y[i] = fmaf(by[i], x[i], y[i]);
+      const int t = c * kChunk + t32;
+      put_column(out + t * step, step, d.T - t, y);
     };
-    for (int c = 0; c <= chunks && !wait.dead; ++c) {
-      if (c > 0 && !wait(&sh.bar[kStateDone], c - 1)) break;
+    I x[32];
+    const auto take_values = [&](int c) {
+      if (in) column_of(v + (long long)(c * kChunk + t32) * a.v.st, a.v.st, d.T - c * kChunk - t32, x);
+    };
+#pragma unroll
+    for (int i = 0; i < 32; ++i) x[i] = ElemOf<I>::down(0.f);
+    if (chunks > 0) take_values(0);
+    for (int c = 0; c <= chunks; ++c) {
+      if (c > 0 && (!wait(&sh.bar[kStateDone], c - 1) || !wait(&sh.bar[kFree], c - 1))) break;
       tc_fence_after();
-      if (tid == 0) bulk_read_done();  // of the tiles written below
-      if (c < chunks && tid < kChunk) fill_factors(sh.f[c & 1], a.keep, n0 + c, m0 + c, tid);
-      meet(wait);
-      if (wait.dead) break;
-      const float2 end = c < chunks ? a.keep.total[(n0 + c) * kChunk + kChunk - 1] : make_float2(0.f, 0.f);
-      const float left = __expf(end.x + end.y);
-      I x[32];
-      if (c < chunks) column_of(v + (long long)c * kChunk * a.v.st, a.v.st, t32, d.T - c * kChunk, in, x);
+      const Factors& fac = sh.f[c & 1];
+      const float left = c < chunks ? fac.left : 0.f;
 #pragma unroll
       for (int k = 0; k < kCols / 32; ++k) {
         const int col = seat.half * kCols + k * 32;
@@ -232,20 +266,12 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
       }
       tmem_st_wait();
       hand_over(&sh.bar[kStateSet]);
-      if (a.keep.states != nullptr) {
-        meet(wait);
-        if (tid == 0 && !wait.dead) {
-          bulk_store(a.keep.states + ((head * (chunks + 1) + c) * slices + slice) * 2 * Mem::kPlaneS, mem + Mem::S, 2 * Mem::kPlaneS);
-          bulk_commit();
-        }
-      }
       if (c > 0) {
         if (!wait(&sh.bar[kOutDone], c - 1)) break;
         tc_fence_after();
         put_out(c - 1);
       }
       if (c == chunks) break;
-      const Factors& fac = sh.f[c & 1];
       if (!wait(&sh.bar[kReadDone], c)) break;
       tc_fence_after();
       float f[32];
@@ -261,6 +287,10 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
         }
       }
       hand_over(&sh.bar[kRhsSet]);
+      if (c + 1 < chunks) {
+        take_values(c + 1);
+        if (tid < kChunk) parts.read(a.keep, n0 + c + 1, m0 + c + 1, tid);
+      }
       if (!wait(&sh.bar[kSolveDone], c)) break;
       tc_fence_after();
       tmem_row(tm + seat.lanes + cE + t32, f);
@@ -277,16 +307,9 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
           put8(mem + Mem::X + at, mem + Mem::X + Mem::kPlaneX + at, y);
         }
       }
+      if (c + 1 < chunks && tid < kChunk) parts.fill(sh.f[(c + 1) & 1], sh.grown_q[(c + 1) % 3], tid);
       hand_over(&sh.bar[kWritesSet]);
-      if (a.keep.writes != nullptr) {
-        meet(wait);
-        if (tid == 0 && !wait.dead) {
-          bulk_store(a.keep.writes + ((n0 + c) * slices + slice) * 2 * Mem::kPlaneX, mem + Mem::W, 2 * Mem::kPlaneX);
-          bulk_commit();
-        }
-      }
     }
-    if (tid == 0) bulk_done();
   }
   tc_fence_before();
   __syncthreads();
@@ -307,12 +330,13 @@ struct DstateMem {
                        Q = K + kStages * kParts_ * kPlaneK, P = Q + kParts_ * kPlaneK, T = P + 2 * kTok, kTiles = T + 2 * kTok;
 };
 
-enum DstateBar { kGotK, kGotK2, kGotQ, kGotT, kDstateSet, kOutsSet, kGradSet, kReadsSet, kMixDone, kOutsDone, kBackDone, kDstateDone, kMeet2, kDstateBars };
+enum DstateBar { kGotK, kGotK2, kGotQ, kGotT, kDstateSet, kOutsSet, kGradSet, kReadsSet, kMixDone, kOutsDone, kBackDone, kDstateDone, kTilesFree, kDstateBars };
 
 struct DstateShared {
   uint64_t bar[kDstateBars];
   uint32_t tmem;
   Factors f[2];
+  float grown_q[2][kChunk];  // exp(G) rq
 };
 
 // One slice of the gradient of a head's state, from the last chunk to the first. Tensor memory: dS^T (128 x DK), K dS', P^T dO, dV.
@@ -330,10 +354,15 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
   const int tid = threadIdx.x, warp = tid >> 5;
   if (tid == 0) {
     for (int i = 0; i < kDstateBars; ++i)
-      mbar_init(&sh.bar[i], i == kDstateSet || i == kOutsSet || i == kGradSet || i == kReadsSet || i == kMeet2 ? kWorkers : 1);
+      mbar_init(&sh.bar[i], i == kDstateSet || i == kOutsSet || i == kGradSet || i == kReadsSet ? kWorkers : 1);
     fence_barrier_init();
   }
   if (warp == 8) tmem_alloc(&sh.tmem, 512);
+  FactorParts parts;
+  if (tid < kChunk && chunks > 0) {
+    parts.read(a.keep, n0 + chunks - 1, m0 + chunks - 1, tid);
+    parts.fill(sh.f[0], sh.grown_q[0], tid);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -375,6 +404,10 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
         tc_commit(&sh.bar[kMixDone]);
         multiply_parts<4, DK, false, true, 2, P>(tm + cS, Y, Mem::kPlaneX, Q, Mem::kPlaneK, true);
         tc_commit(&sh.bar[kOutsDone]);
+        const long long at_n = (n0 + chunks - 1 - r) * slices + slice;
+        bulk_store(a.dstates + at_n * 2 * Mem::kPlaneS, mem + Mem::S, 2 * Mem::kPlaneS);
+        bulk_store(a.douts + at_n * P * Mem::kPlaneX, mem + Mem::O, P * Mem::kPlaneX);
+        bulk_commit();
         if (!wait(&sh.bar[kGradSet], r)) break;
         if (!wait(&sh.bar[kGotT], r)) break;
         tc_fence_after();
@@ -387,31 +420,36 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
         tc_fence_after();
         multiply_parts<4, DK, false, true, 2, P>(tm + cS, X, Mem::kPlaneX, K, Mem::kPlaneK, true);
         tc_commit(&sh.bar[kDstateDone]);
+        bulk_store(a.dreads + at_n * 2 * Mem::kPlaneX, mem + Mem::Y, 2 * Mem::kPlaneX);
+        bulk_commit();
+        bulk_read_done();  // the tiles may be written again, once their products are done too
+        mbar_arrive(&sh.bar[kTilesFree]);
         if (!wait(&sh.bar[kDstateDone], r)) break;
         if (r + kStages < chunks) load_k(r + kStages);
       }
+      bulk_done();
     }
   } else {
     const Seat seat;
     const bool there = seat.row < DV, in = seat.row < width;
     const int t32 = seat.half * 32;
-    Meeting meet{&sh.bar[kMeet2]};
     const long long step = (long long)d.H * d.dv, at_head = ((long long)b * d.T * d.H + h) * d.dv + v0 + seat.row;
     const I* go = reinterpret_cast<const I*>(a.g_out) + at_head;
     I* dv = reinterpret_cast<I*>(a.dv) + at_head;
     constexpr int kCols = DK / 2;
-    for (int r = 0; r <= chunks && !wait.dead; ++r) {
+    I x[32];
+    const auto take_outs = [&](int c) {
+      if (in) column_of(go + (c * kChunk + t32) * step, step, d.T - c * kChunk - t32, x);
+    };
+#pragma unroll
+    for (int i = 0; i < 32; ++i) x[i] = ElemOf<I>::down(0.f);
+    if (chunks > 0) take_outs(chunks - 1);
+    for (int r = 0; r <= chunks; ++r) {
       const int c = chunks - 1 - r;
-      if (r > 0 && !wait(&sh.bar[kDstateDone], r - 1)) break;
+      if (r > 0 && (!wait(&sh.bar[kDstateDone], r - 1) || !wait(&sh.bar[kTilesFree], r - 1))) break;
       tc_fence_after();
-      if (tid == 0) bulk_read_done();
-      if (c >= 0 && tid < kChunk) fill_factors(sh.f[r & 1], a.keep, n0 + c, m0 + c, tid);
-      meet(wait);
-      if (wait.dead) break;
-      const float2 end = c >= 0 ? a.keep.total[(n0 + c) * kChunk + kChunk - 1] : make_float2(0.f, 0.f);
-      const float left = __expf(end.x + end.y);
-      I x[32];
-      if (c >= 0) column_of(go + (long long)c * kChunk * step, step, t32, d.T - c * kChunk, in, x);
+      const Factors& fac = sh.f[r & 1];
+      const float left = c >= 0 ? fac.left : 0.f;
 #pragma unroll
       for (int k = 0; k < kCols / 32; ++k) {
         const int col = seat.half * kCols + k * 32;
@@ -449,7 +487,6 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
       if (c < 0) break;
       tmem_st_wait();
       hand_over(&sh.bar[kDstateSet]);
-      const Factors& fac = sh.f[r & 1];
       if (there) {
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
@@ -460,17 +497,14 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
           if constexpr (P == 2) put8(mem + Mem::O + at, mem + Mem::O + Mem::kPlaneX + at, y);
           else *reinterpret_cast<uint4*>(mem + Mem::O + at) = raw_down<I, uint4>(y);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) y[k] *= fac.grown_q[t32 + p * 8 + k];
+          for (int k = 0; k < 8; ++k) y[k] *= sh.grown_q[r & 1][t32 + p * 8 + k];
           put8(mem + Mem::Y + at, mem + Mem::Y + Mem::kPlaneX + at, y);
         }
       }
       hand_over(&sh.bar[kOutsSet]);
-      meet(wait);
-      const long long at_n = (n0 + c) * slices + slice;
-      if (tid == 0 && !wait.dead) {
-        bulk_store(a.dstates + at_n * 2 * Mem::kPlaneS, mem + Mem::S, 2 * Mem::kPlaneS);
-        bulk_store(a.douts + at_n * P * Mem::kPlaneX, mem + Mem::O, P * Mem::kPlaneX);
-        bulk_commit();
+      if (c > 0) {
+        take_outs(c - 1);
+        if (tid < kChunk) parts.read(a.keep, n0 + c - 1, m0 + c - 1, tid);
       }
       if (!wait(&sh.bar[kMixDone], r)) break;
       tc_fence_after();
@@ -507,20 +541,11 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
           put8(mem + Mem::X + at, mem + Mem::X + Mem::kPlaneX + at, y);
         }
       }
+      if (c > 0 && tid < kChunk) parts.fill(sh.f[(r + 1) & 1], sh.grown_q[(r + 1) & 1], tid);
       hand_over(&sh.bar[kReadsSet]);
-      meet(wait);
-      if (tid == 0 && !wait.dead) {
-        bulk_store(a.dreads + at_n * 2 * Mem::kPlaneX, mem + Mem::Y, 2 * Mem::kPlaneX);
-        bulk_commit();
-      }
-      if (in) {
-        const int t0 = c * kChunk + t32;
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (t0 + i < d.T) dv[(long long)(t0 + i) * step] = ElemOf<I>::down(f[i]);
-      }
+      const int t = c * kChunk + t32;
+      if (in) put_column(dv + t * step, step, d.T - t, f);
     }
-    if (tid == 0) bulk_done();
   }
   tc_fence_before();
   __syncthreads();

@@ -62,6 +62,25 @@ __device__ __forceinline__ const I* head_at(const HeadRows& x, int b, long long 
   return reinterpret_cast<const I*>(x.p) + b * x.sb + t * x.st + h * x.sh;
 }
 
+// 32 tokens' values of one column of head rows; zeros behind the last of `rows` tokens. Whole chunks without a condition: with
+// one for each load, they wait for one another.
+template <typename I>
+__device__ __forceinline__ void column_of(const I* p, long long st, int rows, I (&x)[32]) {
+  if (rows >= 32) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      x[i] = *p;
+      p += st;
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    x[i] = i < rows ? *p : ElemOf<I>::down(0.f);
+    p += st;
+  }
+}
+
 // exp(G_i - G_j) of sums held in two parts: the small part counts where the large ones nearly cancel.
 __device__ __forceinline__ float decay_between(float2 i, float2 j) { return __expf((i.x - j.x) + (i.y - j.y)); }
 
