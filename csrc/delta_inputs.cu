@@ -37,20 +37,21 @@ struct InputsShared {
   float rk[kChunk], rq[kChunk], beta[kChunk], left[kChunk], grown[kChunk];
   float dots[3][kChunk];  // V' . dV, v . dv, q . dq
   float part[2][4][kChunk];
-  float handed[8];
+  float handed[kControl];
 };
 
-// Adds 64 values of each of 32 lanes over the lanes: lane l ends with the sums of values 2 l and 2 l + 1 in x[0] and x[1].
-__device__ __forceinline__ void lanes_fold(float (&x)[64]) {
+// Adds 32 values of each of 32 lanes over the lanes: lane l ends with the sum of value l.
+__device__ __forceinline__ float lanes_fold(float (&x)[32]) {
 #pragma unroll
-  for (int o = 16, n = 32; o > 0; o >>= 1, n >>= 1) {
-    const bool up = threadIdx.x & o;
+  for (int n = 16; n > 0; n >>= 1) {
+    const bool up = threadIdx.x & n;
 #pragma unroll
     for (int i = 0; i < n; ++i) {
       const float send = up ? x[i] : x[i + n], keep = up ? x[i + n] : x[i];
-      x[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+      x[i] = keep + __shfl_xor_sync(0xffffffffu, send, n);
     }
   }
+  return x[0];
 }
 
 template <typename I, int DK, int DV>
@@ -72,7 +73,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
     for (int i = 0; i < kInputsBars; ++i) mbar_init(&sh.bar[i], i == kMixSet || i == kTaken ? kWorkers : 1);
     fence_barrier_init();
   }
-  if (warp == 8) tmem_alloc(&sh.tmem, 512);
+  if (warp == kControl) tmem_alloc(&sh.tmem, 512);
   if (tid < kChunk) {
     const float2 G = a.keep.total[n * kChunk + tid], end = a.keep.total[n * kChunk + kChunk - 1];
     sh.G[tid] = G;
@@ -87,10 +88,11 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
   __syncthreads();
   tc_fence_after();
   const uint32_t tm = sh.tmem;
+  const Seat seat;
   constexpr uint32_t cMix = 0, cLow = 64, cS = 128, cD = 256, cQ = 320, cK = 384;
   Waiter wait{a.err};
   const auto state_at = [&](int chunk, int s) { return a.keep.states + ((head * (chunks + 1) + chunk) * slices + s) * 2 * Mem::kPlaneS; };
-  if (warp == 8) {
+  if (warp == kControl) {
     if (lane == 0) {
       const uint32_t base = smem_u32(mem);
       mbar_arrive_expect_tx(&sh.bar[kGotQK], 2 * P * Mem::kPlaneK);
@@ -150,50 +152,50 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
       }
     }
   } else {
-    const int row = (warp & 3) * 32 + lane, half = warp >> 2;
-    const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     float handed = 0.f;
+    const bool of_v = seat.part >= 2;  // V' . dV is the first two quarters' part, v . dv the others'; each of half of the tokens
+    const int tt = (seat.part & 1) * 32;
     for (int s = 0; s < slices; ++s) {
       const int v0 = s * DV;
-      const bool in = row < min(DV, d.dv - v0);
-      // A lane holds an element of the values: V' . dV (the first four warps) and v . dv (the others) of all tokens.
-      float x[64];
-      I v[2][32];
+      const bool in = seat.row < min(DV, d.dv - v0);
+      I v[32];
 #pragma unroll
-      for (int i = 0; i < 64; ++i) v[i >> 5][i & 31] = ElemOf<I>::down(0.f);
-      if (half == 1 && in) {
-        const I* from = head_at<I>(a.v, b, t0, h) + v0 + row;
-        column_of(from, a.v.st, rows, v[0]);
-        column_of(from + 32 * a.v.st, a.v.st, rows - 32, v[1]);
-      }
-      if (!wait(&sh.bar[kGotV], s)) break;
-      const bool there = row < DV;
+      for (int i = 0; i < 32; ++i) v[i] = ElemOf<I>::down(0.f);
+      if (of_v && in) column_of(head_at<I>(a.v, b, t0 + tt, h) + v0 + seat.row, a.v.st, rows - tt, v);
+      // The small matrices first, for the products that wait for them: row i of dP in lane i, of dL in lane 64 + i.
+      if (s == slices - 1) {
+        if (!wait(&sh.bar[kMixDone], 0)) break;
+        tc_fence_after();
+        const int i = seat.row & 63, j0 = seat.part * 16;
+        const bool of_l = seat.row >= 64;
+        float f[16];
+        if (P == 1) {
+          float g[16];
+          tmem_rows(tm + seat.lanes + cMix + j0, f, tm + seat.lanes + cLow + j0, g);
+          if (of_l)
 #pragma unroll
-      for (int p = 0; p < 8; ++p) {
-        const int at = piece_at(there ? row : 0, p);
-        const uint4 gh = *reinterpret_cast<const uint4*>(mem + Mem::G + at), gl = *reinterpret_cast<const uint4*>(mem + Mem::Gl + at);
-        const float2 g[4] = {pair_sum(gh.x, gl.x), pair_sum(gh.y, gl.y), pair_sum(gh.z, gl.z), pair_sum(gh.w, gl.w)};
-        float2 w[4];
-        if (half == 0) {
-          const uint4 wh = *reinterpret_cast<const uint4*>(mem + Mem::V + at), wl = *reinterpret_cast<const uint4*>(mem + Mem::V + Mem::kPlaneX + at);
-          w[0] = pair_sum(wh.x, wl.x);
-          w[1] = pair_sum(wh.y, wl.y);
-          w[2] = pair_sum(wh.z, wl.z);
-          w[3] = pair_sum(wh.w, wl.w);
+            for (int k = 0; k < 16; ++k) f[k] += g[k];
         } else {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            w[k] = make_float2(ElemOf<I>::up(v[p >> 2][(p & 3) * 8 + 2 * k]), ElemOf<I>::up(v[p >> 2][(p & 3) * 8 + 2 * k + 1]));
+          tmem_row(tm + seat.lanes + cMix + j0, f);
         }
+        const float by = of_l ? -sh.rk[i] : sh.rq[i];
+        const float2 Gi = sh.G[i];
+        const int last = of_l ? i : i + 1;
+        unsigned char* to = mem + (of_l ? Mem::N : Mem::W);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          x[p * 8 + 2 * k] = in ? w[k].x * g[k].x : 0.f;
-          x[p * 8 + 2 * k + 1] = in ? w[k].y * g[k].y : 0.f;
+        for (int p = 0; p < 2; ++p) {
+          float x[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int j = j0 + p * 8 + k;
+            const float w = f[p * 8 + k] * by * (decay_between(Gi, sh.G[j]) * sh.rk[j]);
+            x[k] = j < last ? w : 0.f;
+          }
+          const int at = piece_at(i, seat.part * 2 + p);
+          put8(to + at, to + kTok + at, x);
         }
+        hand_over(&sh.bar[kMixSet]);
       }
-      lanes_fold(x);
-      sh.part[half][warp & 3][2 * lane] = s ? sh.part[half][warp & 3][2 * lane] + x[0] : x[0];
-      sh.part[half][warp & 3][2 * lane + 1] = s ? sh.part[half][warp & 3][2 * lane + 1] + x[1] : x[1];
       // <dS', S'>: both tiles have their elements at the same places.
       const uint4* after = reinterpret_cast<const uint4*>(state_at(c + 1, s));
       constexpr int kPieces = Mem::kPlaneS / 16, kMine = kPieces / kWorkers;
@@ -204,16 +206,44 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
         ah[i] = __ldcs(after + i * kWorkers + tid);
         al[i] = __ldcs(after + kPieces + i * kWorkers + tid);
       }
+      if (!wait(&sh.bar[kGotV], s)) break;
+      // A lane holds an element of the values: the sums over them, of each token.
+      float x[32];
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const int at = piece_at(in ? seat.row : 0, tt / 8 + p);
+        const uint4 gh = *reinterpret_cast<const uint4*>(mem + Mem::G + at), gl = *reinterpret_cast<const uint4*>(mem + Mem::Gl + at);
+        const float2 g[4] = {pair_sum(gh.x, gl.x), pair_sum(gh.y, gl.y), pair_sum(gh.z, gl.z), pair_sum(gh.w, gl.w)};
+        float2 w[4];
+        if (of_v) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = make_float2(ElemOf<I>::up(v[p * 8 + 2 * k]), ElemOf<I>::up(v[p * 8 + 2 * k + 1]));
+        } else {
+          const uint4 wh = *reinterpret_cast<const uint4*>(mem + Mem::V + at), wl = *reinterpret_cast<const uint4*>(mem + Mem::V + Mem::kPlaneX + at);
+          w[0] = pair_sum(wh.x, wl.x);
+          w[1] = pair_sum(wh.y, wl.y);
+          w[2] = pair_sum(wh.z, wl.z);
+          w[3] = pair_sum(wh.w, wl.w);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          x[p * 8 + 2 * k] = in ? w[k].x * g[k].x : 0.f;
+          x[p * 8 + 2 * k + 1] = in ? w[k].y * g[k].y : 0.f;
+        }
+      }
+      const float sum = lanes_fold(x);
+      float* part = &sh.part[of_v][warp & 3][tt + lane];
+      *part = s ? *part + sum : sum;
       if (!wait(&sh.bar[kGotD], s)) break;
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
         const unsigned char* at = mem + Mem::S + (i * kWorkers + tid) * 16;
         const uint4 dh = *reinterpret_cast<const uint4*>(at), dl = *reinterpret_cast<const uint4*>(at + Mem::kPlaneS);
-        const uint32_t u[4] = {ah[i].x, ah[i].y, ah[i].z, ah[i].w}, v[4] = {al[i].x, al[i].y, al[i].z, al[i].w},
+        const uint32_t u[4] = {ah[i].x, ah[i].y, ah[i].z, ah[i].w}, v4[4] = {al[i].x, al[i].y, al[i].z, al[i].w},
                        y[4] = {dh.x, dh.y, dh.z, dh.w}, z[4] = {dl.x, dl.y, dl.z, dl.w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const float2 e = pair_sum(u[k], v[k]), f = pair_sum(y[k], z[k]);
+          const float2 e = pair_sum(u[k], v4[k]), f = pair_sum(y[k], z[k]);
           handed = fmaf(e.x, f.x, fmaf(e.y, f.y, handed));
         }
       }
@@ -221,70 +251,29 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
     }
     handed = lanes_sum(handed);
     if (lane == 0) sh.handed[warp] = handed;
-    // The small matrices: row i of dP in lane i, of dL in lane 64 + i.
-    if (!wait.dead && wait(&sh.bar[kMixDone], 0)) {
-      tc_fence_after();
-      const int i = row & 63, j0 = half * 32;
-      const bool of_l = row >= 64;
-      float f[32];
-      tmem_row(tm + lanes + cMix + j0, f);
-      if (P == 1) {
-        float g[32];
-        tmem_row(tm + lanes + cLow + j0, g);
-        if (of_l)
-#pragma unroll
-          for (int k = 0; k < 32; ++k) f[k] += g[k];
-      }
-      const float by = of_l ? -sh.rk[i] : sh.rq[i];
-      const float2 Gi = sh.G[i];
-      const int last = of_l ? i : i + 1;
-      unsigned char* to = mem + (of_l ? Mem::N : Mem::W);
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        float x[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int j = j0 + p * 8 + k;
-          const float w = f[p * 8 + k] * by * (decay_between(Gi, sh.G[j]) * sh.rk[j]);
-          x[k] = j < last ? w : 0.f;
-        }
-        const int at = piece_at(i, half * 4 + p);
-        put8(to + at, to + kTok + at, x);
-      }
-    }
-    hand_over(&sh.bar[kMixSet]);
     wait(&sh.bar[kAllDone], 0);
   }
   // dq and dk of this head: r dq^ and r dk^ of the scaled rows, tokens as rows, where S and V' lay.
   __syncthreads();
   float* F = reinterpret_cast<float*>(mem);
-  if (warp < 8) {
-    const int row = (warp & 3) * 32 + lane, half = warp >> 2;
-    const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+  if (warp < kControl) {
     tc_fence_after();
-    float s[32], y[32];
-    tmem_row(tm + lanes + cS + half * 32, s);
-    tmem_row(tm + lanes + cQ + half * 32, y);
-    if (row < DK)
+    const int tt = seat.part * 16;
+    float s[16], y[16], z[16];
+    tmem_rows(tm + seat.lanes + cS + tt, s, tm + seat.lanes + cQ + tt, y);
+    if (seat.row < DK)
 #pragma unroll
-      for (int k = 0; k < 32; ++k) {
-        const int i = half * 32 + k;
-        F[i * Mem::ldF + row] = fmaf(sh.rq[i] * sh.grown[i], s[k], y[k]);
-      }
-    float z[32];
-    tmem_row(tm + lanes + cS + 64 + half * 32, s);
-    tmem_row(tm + lanes + cD + half * 32, z);
-    tmem_row(tm + lanes + cK + half * 32, y);
-    if (row < DK)
+      for (int k = 0; k < 16; ++k) F[(tt + k) * Mem::ldF + seat.row] = fmaf(sh.rq[tt + k] * sh.grown[tt + k], s[k], y[k]);
+    tmem_rows(tm + seat.lanes + cS + 64 + tt, s, tm + seat.lanes + cD + tt, z);
+    tmem_row(tm + seat.lanes + cK + tt, y);
+    if (seat.row < DK)
 #pragma unroll
-      for (int k = 0; k < 32; ++k) {
-        const int i = half * 32 + k;
-        F[(kChunk + i) * Mem::ldF + row] = fmaf(sh.rk[i], fmaf(sh.left[i], z[k], -sh.grown[i] * s[k]), y[k]);
-      }
+      for (int k = 0; k < 16; ++k)
+        F[(kChunk + tt + k) * Mem::ldF + seat.row] = fmaf(sh.rk[tt + k], fmaf(sh.left[tt + k], z[k], -sh.grown[tt + k] * s[k]), y[k]);
     tc_fence_before();
   }
   __syncthreads();
-  if (warp == 8) {
+  if (warp == kControl) {
     tc_fence_after();
     tmem_dealloc(tm, 512);
   }
@@ -318,25 +307,32 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
 #pragma unroll
     for (int k = 0; k < kE; ++k) y[k] = add ? y[k] + z[k] : z[k];
   };
-  if (warp < 8) {
-#pragma unroll 4
-    for (int i = warp; i < kChunk; i += 8) {
-      float x[kE], y[kE], dot = 0.f;
+  if (warp < kControl) {
+    float dot[4];
+#pragma unroll
+    for (int n4 = 0; n4 < 4; ++n4) {
+      const int i = n4 * kControl + warp;
+      float x[kE], y[kE];
       row_of(Mem::Q, i, x);
       sums_of(F + i * Mem::ldF, y, false);
+      dot[n4] = 0.f;
 #pragma unroll
-      for (int k = 0; k < kE; ++k) dot = fmaf(x[k], y[k], dot);
-      dot = lanes_sum(dot);
-      if (lane == 0) sh.dots[2][i] = dot;
+      for (int k = 0; k < kE; ++k) dot[n4] = fmaf(x[k], y[k], dot[n4]);
+    }
+#pragma unroll
+    for (int n4 = 0; n4 < 4; ++n4) {
+      dot[n4] = lanes_sum(dot[n4]);
+      if (lane == 0) sh.dots[2][n4 * kControl + warp] = dot[n4];
     }
   }
+  static_assert(4 * kControl == kChunk, "a row of q to each warp, four times");
   cg::cluster_group cluster = cg::this_cluster();
   if (group > 1) cluster.sync();
   else __syncthreads();
-  if (warp == 8) {  // the gates: sums from each token to the chunk's end, two tokens a lane
+  if (warp == kControl) {  // the gates: sums from each token to the chunk's end, two tokens a lane
     float after = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) after += sh.handed[w];
+    for (int w = 0; w < kControl; ++w) after += sh.handed[w];
     const float x = sh.dots[2][2 * lane] - sh.dots[1][2 * lane], y = sh.dots[2][2 * lane + 1] - sh.dots[1][2 * lane + 1];
     float sum = x + y;
 #pragma unroll
@@ -375,11 +371,11 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
 #pragma unroll
     for (int o = 0; o < kMostGroup; ++o) from[o] = group > 1 ? cluster.map_shared_rank(F, o < group ? o : 0) : F;
     // Four rows at a time, so that their loads are on their way together.
-    for (int r0 = hg * 8 + warp; r0 < 2 * kChunk; r0 += 32 * group) {
+    for (int r0 = hg * kControl + warp; r0 < 2 * kChunk; r0 += 4 * kControl * group) {
       float y[4][kE], x[4][kE], dot[4];
 #pragma unroll
       for (int n4 = 0; n4 < 4; ++n4) {
-        const int r = min(r0 + n4 * 8 * group, 2 * kChunk - 1);
+        const int r = min(r0 + n4 * kControl * group, 2 * kChunk - 1);
         row_of(r >= kChunk ? Mem::K : Mem::Q, r % kChunk, x[n4]);
 #pragma unroll
         for (int o = 0; o < kMostGroup; ++o)
@@ -392,7 +388,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
       for (int n4 = 0; n4 < 4; ++n4) dot[n4] = lanes_sum(dot[n4]);
 #pragma unroll
       for (int n4 = 0; n4 < 4; ++n4) {
-        const int r = r0 + n4 * 8 * group, i = r % kChunk;
+        const int r = r0 + n4 * kControl * group, i = r % kChunk;
         if (r >= 2 * kChunk || i >= rows || lane * kE >= d.dk) continue;
         const bool of_k = r >= kChunk;
         const float len = of_k ? sh.rk[i] : sh.rq[i] / d.scale, by = -len * len * dot[n4];

@@ -29,18 +29,6 @@
 namespace bw {
 namespace {
 
-// Where a worker sits: warp w of eight holds tensor memory's lanes 32 (w % 4) .. + 31, one each, and half of the columns.
-struct Seat {
-  int row, half;
-  uint32_t lanes;  // of a tensor memory address
-  __device__ Seat() {
-    const int warp = threadIdx.x >> 5;
-    row = (warp & 3) * 32 + (threadIdx.x & 31);
-    half = warp >> 2;
-    lanes = (uint32_t)(warp & 3) << 21;
-  }
-};
-
 // Of a chunk's tokens: what the products' columns are multiplied by.
 struct Factors {
   float grown_k[kChunk];  // exp(G) rk
@@ -70,18 +58,18 @@ struct FactorParts {
   }
 };
 
-template <typename I>
-__device__ __forceinline__ void put_column(I* p, long long st, int rows, const float (&x)[32]) {
-  if (rows >= 32) {
+template <typename I, int N>
+__device__ __forceinline__ void put_column(I* p, long long st, int rows, const float (&x)[N]) {
+  if (rows >= N) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
+    for (int i = 0; i < N; ++i) {
       *p = ElemOf<I>::down(x[i]);
       p += st;
     }
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
+  for (int i = 0; i < N; ++i) {
     if (i < rows) *p = ElemOf<I>::down(x[i]);
     p += st;
   }
@@ -90,15 +78,14 @@ __device__ __forceinline__ void put_column(I* p, long long st, int rows, const f
 // ---------------------------------------------------------------- state
 template <typename I, int DK, int DV>
 struct StateMem {
-  static constexpr int kPanels = DK / 64, kParts_ = kParts<I>, kPanelS = DV * 128, kPlaneS = kPanels * kPanelS, kPlaneX = DV * 128,
-                       kPlaneK = kPanels * kTok;
-  // With two parts of q and k one chunk's keys and inverse fit, with one those of the next chunk too.
-  static constexpr int kStages = kParts<I> == 1 ? 2 : 1;
-  static constexpr int S = 0, X = S + 2 * kPlaneS, W = X + 2 * kPlaneX, K = W + 2 * kPlaneX, T = K + kStages * kParts_ * kPlaneK,
-                       Q = T + kStages * 2 * kTok, P = Q + kParts_ * kPlaneK, kTiles = P + 2 * kTok;
+  static constexpr int kPanels = DK / 64, kPanelS = DV * 128, kPlaneS = kPanels * kPanelS, kPlaneX = DV * 128;
+  // Keys and queries: 64 rows of each to a panel, so that one operand of 128 rows has both.
+  static constexpr int kPanelKQ = 2 * kTok, kPlaneKQ = kPanels * kPanelKQ, kStageKQ = kParts<I> * kPlaneKQ;
+  static constexpr int S = 0, X = S + 2 * kPlaneS, W = X + 2 * kPlaneX, KQ = W + 2 * kPlaneX, T = KQ + 2 * kStageKQ, P = T + 2 * kTok,
+                       kTiles = P + 2 * kTok;
 };
 
-enum StateBar { kLoadedK, kLoadedK2, kLoadedQ, kStateSet, kRhsSet, kWritesSet, kReadDone, kSolveDone, kStateDone, kOutDone, kFree, kStateBars };
+enum StateBar { kGotKQ, kGotKQ2, kLoadedT, kLoadedP, kStateSet, kRhsSet, kWritesSet, kReadDone, kSolveDone, kStateDone, kOutDone, kFactorsSet, kStateBars };
 
 struct StateShared {
   uint64_t bar[kStateBars];
@@ -107,11 +94,11 @@ struct StateShared {
   float grown_q[3][kChunk];  // exp(G) rq: an output is written a chunk later than the factors are read
 };
 
-// One slice of a head's state, chunk after chunk. Tensor memory: S^T (128 x DK), K S, E, and twice Q S and P V'.
+// One slice of a head's state, chunk after chunk. Tensor memory: S^T (128 x DK), twice K S and Q S, E, P V'.
 template <typename I, int DK, int DV>
 __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd a) {
   using Mem = StateMem<I, DK, DV>;
-  constexpr int P = kParts<I>, kSteps = DK / 16, kStages = Mem::kStages;
+  constexpr int P = kParts<I>, kSteps = DK / 16;
   extern __shared__ __align__(1024) unsigned char mem[];
   StateShared& sh = *reinterpret_cast<StateShared*>(mem + Mem::kTiles);
   const DeltaDims& d = a.d;
@@ -125,7 +112,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
       mbar_init(&sh.bar[i], i == kStateSet || i == kRhsSet || i == kWritesSet ? kWorkers : 1);
     fence_barrier_init();
   }
-  if (warp == 8) tmem_alloc(&sh.tmem, 512);
+  if (warp == kControl) tmem_alloc(&sh.tmem, 512);
   FactorParts parts;
   if (tid < kChunk && chunks > 0) {
     parts.read(a.keep, n0, m0, tid);
@@ -135,27 +122,33 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
   __syncthreads();
   tc_fence_after();
   const uint32_t tm = sh.tmem;
-  constexpr uint32_t cS = 0, cK = 128, cE = 192, cQ = 256, cP = 320;  // the last two again 128 columns on
+  constexpr uint32_t cS = 0, cK = 128, cQ = 192, cE = 384, cP = 448;  // cK and cQ again 128 columns on
   Waiter wait{a.err};
-  if (warp == 8) {
+  if (warp == kControl) {
     if ((tid & 31) == 0) {
-      const auto load_k = [&](int c) {
-        const int st = c % kStages;
-        uint64_t* bar = &sh.bar[kStages == 2 && (c & 1) ? kLoadedK2 : kLoadedK];
-        mbar_arrive_expect_tx(bar, P * Mem::kPlaneK + 2 * kTok);
-        bulk_load(mem + Mem::K + st * P * Mem::kPlaneK, a.keep.keys + (m0 + c) * P * Mem::kPlaneK, P * Mem::kPlaneK, bar);
-        bulk_load(mem + Mem::T + st * 2 * kTok, a.keep.solve + (n0 + c) * 2 * kTok, 2 * kTok, bar);
+      const auto load_kq = [&](int c) {
+        uint64_t* bar = &sh.bar[c & 1 ? kGotKQ2 : kGotKQ];
+        mbar_arrive_expect_tx(bar, Mem::kStageKQ);
+        unsigned char* to = mem + Mem::KQ + (c & 1) * Mem::kStageKQ;
+        const long long from = (m0 + c) * (Mem::kStageKQ / 2);
+#pragma unroll
+        for (int i = 0; i < P * Mem::kPanels; ++i) {
+          bulk_load(to + i * Mem::kPanelKQ, a.keep.keys + from + i * kTok, kTok, bar);
+          bulk_load(to + i * Mem::kPanelKQ + kTok, a.keep.queries + from + i * kTok, kTok, bar);
+        }
       };
-      const auto load_q = [&](int c) {
-        mbar_arrive_expect_tx(&sh.bar[kLoadedQ], P * Mem::kPlaneK + 2 * kTok);
-        bulk_load(mem + Mem::Q, a.keep.queries + (m0 + c) * P * Mem::kPlaneK, P * Mem::kPlaneK, &sh.bar[kLoadedQ]);
-        bulk_load(mem + Mem::P, a.keep.attend + (n0 + c) * 2 * kTok, 2 * kTok, &sh.bar[kLoadedQ]);
+      const auto load_square = [&](int to, const unsigned char* from, int c, uint64_t* bar) {
+        mbar_arrive_expect_tx(bar, 2 * kTok);
+        bulk_load(mem + to, from + (n0 + c) * 2 * kTok, 2 * kTok, bar);
       };
-      for (int c = 0; c < kStages && c < chunks; ++c) load_k(c);
-      if (chunks > 0) load_q(0);
+      for (int c = 0; c < 2 && c < chunks; ++c) load_kq(c);
+      if (chunks > 0) {
+        load_square(Mem::T, a.keep.solve, 0, &sh.bar[kLoadedT]);
+        load_square(Mem::P, a.keep.attend, 0, &sh.bar[kLoadedP]);
+      }
       const uint32_t base = smem_u32(mem);
-      const Operand S{base + Mem::S, Mem::kPanelS}, X{base + Mem::X, Mem::kPlaneX}, W{base + Mem::W, Mem::kPlaneX},
-          Q{base + Mem::Q, kTok}, At{base + Mem::P, kTok};
+      const Operand S{base + Mem::S, Mem::kPanelS}, X{base + Mem::X, Mem::kPlaneX}, W{base + Mem::W, Mem::kPlaneX}, T{base + Mem::T, kTok},
+          At{base + Mem::P, kTok};
       const auto store_state = [&](int c) {
         if (a.keep.states == nullptr) return;
         bulk_store(a.keep.states + ((head * (chunks + 1) + c) * slices + slice) * 2 * Mem::kPlaneS, mem + Mem::S, 2 * Mem::kPlaneS);
@@ -163,37 +156,37 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
       };
       int c = 0;
       for (; c < chunks; ++c) {
-        const int st = c % kStages;
-        const uint32_t flip = (c & 1) * 128;
-        const Operand K{base + Mem::K + st * P * Mem::kPlaneK, kTok}, T{base + Mem::T + st * 2 * kTok, kTok};
+        const Operand KQ{base + Mem::KQ + (c & 1) * Mem::kStageKQ, Mem::kPanelKQ};
         if (!wait(&sh.bar[kStateSet], c)) break;
-        if (!wait(&sh.bar[kStages == 2 && (c & 1) ? kLoadedK2 : kLoadedK], kStages == 2 ? c >> 1 : c)) break;
+        if (!wait(&sh.bar[c & 1 ? kGotKQ2 : kGotKQ], c >> 1)) break;
         tc_fence_after();
-        multiply_parts<kSteps, 64, false, false, 2, P>(tm + cK, S, Mem::kPlaneS, K, Mem::kPlaneK, false);
+        multiply_parts<kSteps, 128, false, false, 2, P>(tm + cK + (c & 1) * 128, S, Mem::kPlaneS, KQ, Mem::kPlaneKQ, false);
         tc_commit(&sh.bar[kReadDone]);
         store_state(c);
-        if (!wait(&sh.bar[kLoadedQ], c)) break;
-        multiply_parts<kSteps, 64, false, false, 2, P>(tm + cQ + flip, S, Mem::kPlaneS, Q, Mem::kPlaneK, false);
         if (!wait(&sh.bar[kRhsSet], c)) break;
+        if (!wait(&sh.bar[kLoadedT], c)) break;
         tc_fence_after();
         multiply_parts<4, 64, false, false, 2, 2>(tm + cE, X, Mem::kPlaneX, T, kTok, false);
+        bulk_read_one_left();  // the last chunk's writes are copied: their place may be written once this product is done
         tc_commit(&sh.bar[kSolveDone]);
         if (!wait(&sh.bar[kWritesSet], c)) break;
+        if (c + 1 < chunks) load_square(Mem::T, a.keep.solve, c + 1, &sh.bar[kLoadedT]);
         tc_fence_after();
-        multiply_parts<4, DK, false, true, 2, P>(tm + cS, X, Mem::kPlaneX, K, Mem::kPlaneK, true);
+        multiply_parts<4, DK, false, true, 2, P>(tm + cS, X, Mem::kPlaneX, KQ, Mem::kPlaneKQ, true);
+        bulk_read_done();  // so is the state
         tc_commit(&sh.bar[kStateDone]);
-        multiply_parts<4, 64, false, false, 2, 2>(tm + cP + flip, W, Mem::kPlaneX, At, kTok, false);
+        mbar_arrive(&sh.bar[kFactorsSet]);
+        if (!wait(&sh.bar[kLoadedP], c)) break;
+        multiply_parts<4, 64, false, false, 2, 2>(tm + cP, W, Mem::kPlaneX, At, kTok, false);
         tc_commit(&sh.bar[kOutDone]);
         if (a.keep.writes != nullptr) {
           bulk_store(a.keep.writes + ((n0 + c) * slices + slice) * 2 * Mem::kPlaneX, mem + Mem::W, 2 * Mem::kPlaneX);
           bulk_commit();
         }
-        bulk_read_done();  // the tiles may be written again, once their products are done too
-        mbar_arrive(&sh.bar[kFree]);
         if (!wait(&sh.bar[kStateDone], c)) break;
-        if (c + kStages < chunks) load_k(c + kStages);
+        if (c + 2 < chunks) load_kq(c + 2);
         if (!wait(&sh.bar[kOutDone], c)) break;
-        if (c + 1 < chunks) load_q(c + 1);
+        if (c + 1 < chunks) load_square(Mem::P, a.keep.attend, c + 1, &sh.bar[kLoadedP]);
       }
       if (c == chunks && wait(&sh.bar[kStateSet], chunks)) store_state(chunks);
       bulk_done();
@@ -201,65 +194,64 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
   } else {
     const Seat seat;
     const bool there = seat.row < DV, in = seat.row < width;  // a lane of the slice; one with an element of the head
-    const int t32 = seat.half * 32;
+    const int tt = seat.part * 16;
     const I* v = head_at<I>(a.v, b, 0, h) + v0 + seat.row;
     I* out = reinterpret_cast<I*>(a.out) + ((long long)b * d.T * d.H + h) * d.dv + v0 + seat.row;
     const long long step = (long long)d.H * d.dv;
-    constexpr int kCols = DK / 2;  // of a worker's half of a state's row
+    constexpr int kCols = DK / 4;  // of a worker's quarter of a state's row
     // Writes the state's row as halves into the tile, and scaled into tensor memory.
-    const auto set_state = [&](const float (&f)[32], int col, float left) {
+    const auto set_state = [&](const float (&f)[16], int col, float left) {
       if (there)
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
+        for (int p = 0; p < 2; ++p) {
           float x[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k) x[k] = f[p * 8 + k];
           unsigned char* to = mem + Mem::S + (col >> 6) * Mem::kPanelS + piece_at(seat.row, ((col >> 3) & 7) + p);
           put8(to, to + Mem::kPlaneS, x);
         }
-      uint32_t r[32];
+      uint32_t r[16];
 #pragma unroll
-      for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(f[k] * left);
-      tmem_st_32x32b_x32(tm + seat.lanes + cS + col, r);
+      for (int k = 0; k < 16; ++k) r[k] = __float_as_uint(f[k] * left);
+      tmem_st_32x32b_x16(tm + seat.lanes + cS + col, r);
     };
     const auto put_out = [&](int c) {  // the output of chunk c: Q S and P V' are done
       const uint32_t flip = (c & 1) * 128;
-      float x[32], y[32];
-      tmem_row(tm + seat.lanes + cQ + flip + t32, x);
-      tmem_row(tm + seat.lanes + cP + flip + t32, y);
+      float x[16], y[16];
+      tmem_rows(tm + seat.lanes + cQ + flip + tt, x, tm + seat.lanes + cP + tt, y);
       if (!in) return;
-      const float* by = sh.grown_q[c % 3] + t32;
+      const float* by = sh.grown_q[c % 3] + tt;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) y[i] = fmaf(by[i], x[i], y[i]);
-      const int t = c * kChunk + t32;
+      for (int i = 0; i < 16; ++i) y[i] = fmaf(by[i], x[i], y[i]);
+      const int t = c * kChunk + tt;
       put_column(out + t * step, step, d.T - t, y);
     };
-    I x[32];
+    I x[16];
     const auto take_values = [&](int c) {
-      if (in) column_of(v + (long long)(c * kChunk + t32) * a.v.st, a.v.st, d.T - c * kChunk - t32, x);
+      if (in) column_of(v + (long long)(c * kChunk + tt) * a.v.st, a.v.st, d.T - c * kChunk - tt, x);
     };
 #pragma unroll
-    for (int i = 0; i < 32; ++i) x[i] = ElemOf<I>::down(0.f);
+    for (int i = 0; i < 16; ++i) x[i] = ElemOf<I>::down(0.f);
     if (chunks > 0) take_values(0);
     for (int c = 0; c <= chunks; ++c) {
-      if (c > 0 && (!wait(&sh.bar[kStateDone], c - 1) || !wait(&sh.bar[kFree], c - 1))) break;
+      if (c > 0 && (!wait(&sh.bar[kStateDone], c - 1) || !wait(&sh.bar[kFactorsSet], c - 1))) break;
       tc_fence_after();
       const Factors& fac = sh.f[c & 1];
       const float left = c < chunks ? fac.left : 0.f;
 #pragma unroll
-      for (int k = 0; k < kCols / 32; ++k) {
-        const int col = seat.half * kCols + k * 32;
-        float f[32];
+      for (int k = 0; k < kCols / 16; ++k) {
+        const int col = seat.part * kCols + k * 16;
+        float f[16];
         if (c > 0) {
           tmem_row(tm + seat.lanes + cS + col, f);
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
+          for (int i = 0; i < 16; ++i)
             f[i] = a.first != nullptr && in && col + i < d.dk ? a.first[(head * d.dk + col + i) * d.dv + v0 + seat.row] : 0.f;
         }
         if (c == chunks && a.last != nullptr && in) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
+          for (int i = 0; i < 16; ++i)
             if (col + i < d.dk) a.last[(head * d.dk + col + i) * d.dv + v0 + seat.row] = f[i];
         }
         set_state(f, col, left);
@@ -274,15 +266,15 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
       if (c == chunks) break;
       if (!wait(&sh.bar[kReadDone], c)) break;
       tc_fence_after();
-      float f[32];
-      tmem_row(tm + seat.lanes + cK + t32, f);
+      float f[16];
+      tmem_row(tm + seat.lanes + cK + (c & 1) * 128 + tt, f);
       if (there) {
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
+        for (int p = 0; p < 2; ++p) {
           float y[8];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) y[k] = fmaf(-fac.grown_k[t32 + p * 8 + k], f[p * 8 + k], ElemOf<I>::up(x[p * 8 + k]));
-          unsigned char* to = mem + Mem::X + piece_at(seat.row, seat.half * 4 + p);
+          for (int k = 0; k < 8; ++k) y[k] = fmaf(-fac.grown_k[tt + p * 8 + k], f[p * 8 + k], ElemOf<I>::up(x[p * 8 + k]));
+          unsigned char* to = mem + Mem::X + piece_at(seat.row, seat.part * 2 + p);
           put8(to, to + Mem::kPlaneX, y);
         }
       }
@@ -293,17 +285,17 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
       }
       if (!wait(&sh.bar[kSolveDone], c)) break;
       tc_fence_after();
-      tmem_row(tm + seat.lanes + cE + t32, f);
+      tmem_row(tm + seat.lanes + cE + tt, f);
       if (there) {
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
+        for (int p = 0; p < 2; ++p) {
           float y[8];
-          const int at = piece_at(seat.row, seat.half * 4 + p);
+          const int at = piece_at(seat.row, seat.part * 2 + p);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) y[k] = fac.beta[t32 + p * 8 + k] * f[p * 8 + k];
+          for (int k = 0; k < 8; ++k) y[k] = fac.beta[tt + p * 8 + k] * f[p * 8 + k];
           put8(mem + Mem::W + at, mem + Mem::W + Mem::kPlaneX + at, y);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) y[k] *= fac.left_k[t32 + p * 8 + k];
+          for (int k = 0; k < 8; ++k) y[k] *= fac.left_k[tt + p * 8 + k];
           put8(mem + Mem::X + at, mem + Mem::X + Mem::kPlaneX + at, y);
         }
       }
@@ -313,7 +305,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == kControl) {
     tc_fence_after();
     tmem_dealloc(tm, 512);
   }
@@ -330,7 +322,7 @@ struct DstateMem {
                        Q = K + kStages * kParts_ * kPlaneK, P = Q + kParts_ * kPlaneK, T = P + 2 * kTok, kTiles = T + 2 * kTok;
 };
 
-enum DstateBar { kGotK, kGotK2, kGotQ, kGotT, kDstateSet, kOutsSet, kGradSet, kReadsSet, kMixDone, kOutsDone, kBackDone, kDstateDone, kTilesFree, kDstateBars };
+enum DstateBar { kGotK, kGotK2, kGotQ, kGotT, kDstateSet, kOutsSet, kGradSet, kReadsSet, kMixDone, kOutsDone, kBackDone, kDstateDone, kTilesFree, kPartsSet, kDstateBars };
 
 struct DstateShared {
   uint64_t bar[kDstateBars];
@@ -357,7 +349,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
       mbar_init(&sh.bar[i], i == kDstateSet || i == kOutsSet || i == kGradSet || i == kReadsSet ? kWorkers : 1);
     fence_barrier_init();
   }
-  if (warp == 8) tmem_alloc(&sh.tmem, 512);
+  if (warp == kControl) tmem_alloc(&sh.tmem, 512);
   FactorParts parts;
   if (tid < kChunk && chunks > 0) {
     parts.read(a.keep, n0 + chunks - 1, m0 + chunks - 1, tid);
@@ -369,7 +361,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
   const uint32_t tm = sh.tmem;
   constexpr uint32_t cS = 0, cK = 128, cO = 192, cV = 256;
   Waiter wait{a.err};
-  if (warp == 8) {
+  if (warp == kControl) {
     if ((tid & 31) == 0 && chunks > 0) {
       const auto load_k = [&](int r) {  // round r: chunk chunks - 1 - r
         uint64_t* bar = &sh.bar[kStages == 2 && (r & 1) ? kGotK2 : kGotK];
@@ -419,10 +411,12 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
         if (r + 1 < chunks) load_t(r + 1);
         tc_fence_after();
         multiply_parts<4, DK, false, true, 2, P>(tm + cS, X, Mem::kPlaneX, K, Mem::kPlaneK, true);
+        bulk_read_done();  // dS' and dO are copied: their places may be written once this product is done
         tc_commit(&sh.bar[kDstateDone]);
+        mbar_arrive(&sh.bar[kPartsSet]);
         bulk_store(a.dreads + at_n * 2 * Mem::kPlaneX, mem + Mem::Y, 2 * Mem::kPlaneX);
         bulk_commit();
-        bulk_read_done();  // the tiles may be written again, once their products are done too
+        bulk_read_done();
         mbar_arrive(&sh.bar[kTilesFree]);
         if (!wait(&sh.bar[kDstateDone], r)) break;
         if (r + kStages < chunks) load_k(r + kStages);
@@ -432,46 +426,46 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
   } else {
     const Seat seat;
     const bool there = seat.row < DV, in = seat.row < width;
-    const int t32 = seat.half * 32;
+    const int tt = seat.part * 16;
     const long long step = (long long)d.H * d.dv, at_head = ((long long)b * d.T * d.H + h) * d.dv + v0 + seat.row;
     const I* go = reinterpret_cast<const I*>(a.g_out) + at_head;
     I* dv = reinterpret_cast<I*>(a.dv) + at_head;
-    constexpr int kCols = DK / 2;
-    I x[32];
+    constexpr int kCols = DK / 4;
+    I x[16];
     const auto take_outs = [&](int c) {
-      if (in) column_of(go + (c * kChunk + t32) * step, step, d.T - c * kChunk - t32, x);
+      if (in) column_of(go + (c * kChunk + tt) * step, step, d.T - c * kChunk - tt, x);
     };
 #pragma unroll
-    for (int i = 0; i < 32; ++i) x[i] = ElemOf<I>::down(0.f);
+    for (int i = 0; i < 16; ++i) x[i] = ElemOf<I>::down(0.f);
     if (chunks > 0) take_outs(chunks - 1);
     for (int r = 0; r <= chunks; ++r) {
       const int c = chunks - 1 - r;
-      if (r > 0 && (!wait(&sh.bar[kDstateDone], r - 1) || !wait(&sh.bar[kTilesFree], r - 1))) break;
+      if (r > 0 && (!wait(&sh.bar[kDstateDone], r - 1) || !wait(&sh.bar[kPartsSet], r - 1))) break;
       tc_fence_after();
       const Factors& fac = sh.f[r & 1];
       const float left = c >= 0 ? fac.left : 0.f;
 #pragma unroll
-      for (int k = 0; k < kCols / 32; ++k) {
-        const int col = seat.half * kCols + k * 32;
-        float f[32];
+      for (int k = 0; k < kCols / 16; ++k) {
+        const int col = seat.part * kCols + k * 16;
+        float f[16];
         if (r > 0) {
           tmem_row(tm + seat.lanes + cS + col, f);
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
+          for (int i = 0; i < 16; ++i)
             f[i] = a.g_last != nullptr && in && col + i < d.dk ? a.g_last[(head * d.dk + col + i) * d.dv + v0 + seat.row] : 0.f;
         }
         if (c < 0) {
           if (a.dfirst != nullptr && in) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
+            for (int i = 0; i < 16; ++i)
               if (col + i < d.dk) a.dfirst[(head * d.dk + col + i) * d.dv + v0 + seat.row] = f[i];
           }
           continue;
         }
         if (there) {
 #pragma unroll
-          for (int p = 0; p < 4; ++p) {
+          for (int p = 0; p < 2; ++p) {
             float y[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] = f[p * 8 + i];
@@ -479,25 +473,26 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
             put8(to, to + Mem::kPlaneS, y);
           }
         }
-        uint32_t u[32];
+        uint32_t u[16];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(f[i] * left);
-        tmem_st_32x32b_x32(tm + seat.lanes + cS + col, u);
+        for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(f[i] * left);
+        tmem_st_32x32b_x16(tm + seat.lanes + cS + col, u);
       }
       if (c < 0) break;
       tmem_st_wait();
       hand_over(&sh.bar[kDstateSet]);
+      if (r > 0 && !wait(&sh.bar[kTilesFree], r - 1)) break;  // dV is copied
       if (there) {
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
+        for (int p = 0; p < 2; ++p) {
           float y[8];
-          const int at = piece_at(seat.row, seat.half * 4 + p);
+          const int at = piece_at(seat.row, seat.part * 2 + p);
 #pragma unroll
           for (int k = 0; k < 8; ++k) y[k] = ElemOf<I>::up(x[p * 8 + k]);
           if constexpr (P == 2) put8(mem + Mem::O + at, mem + Mem::O + Mem::kPlaneX + at, y);
           else *reinterpret_cast<uint4*>(mem + Mem::O + at) = raw_down<I, uint4>(y);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) y[k] *= sh.grown_q[r & 1][t32 + p * 8 + k];
+          for (int k = 0; k < 8; ++k) y[k] *= sh.grown_q[r & 1][tt + p * 8 + k];
           put8(mem + Mem::Y + at, mem + Mem::Y + Mem::kPlaneX + at, y);
         }
       }
@@ -508,18 +503,17 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
       }
       if (!wait(&sh.bar[kMixDone], r)) break;
       tc_fence_after();
-      float f[32], y32[32];
-      tmem_row(tm + seat.lanes + cK + t32, f);
-      tmem_row(tm + seat.lanes + cO + t32, y32);
+      float f[16], y16[16];
+      tmem_rows(tm + seat.lanes + cK + tt, f, tm + seat.lanes + cO + tt, y16);
       if (there) {
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
+        for (int p = 0; p < 2; ++p) {
           float y[8];
-          const int at = piece_at(seat.row, seat.half * 4 + p);
+          const int at = piece_at(seat.row, seat.part * 2 + p);
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const int i = p * 8 + k;
-            y[k] = fac.beta[t32 + i] * fmaf(fac.left_k[t32 + i], f[i], y32[i]);
+            y[k] = fac.beta[tt + i] * fmaf(fac.left_k[tt + i], f[i], y16[i]);
           }
           put8(mem + Mem::X + at, mem + Mem::X + Mem::kPlaneX + at, y);
         }
@@ -527,29 +521,29 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
       hand_over(&sh.bar[kGradSet]);
       if (!wait(&sh.bar[kBackDone], r) || !wait(&sh.bar[kOutsDone], r)) break;  // the solve, and Y read
       tc_fence_after();
-      tmem_row(tm + seat.lanes + cV + t32, f);
+      tmem_row(tm + seat.lanes + cV + tt, f);
       if (there) {
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
+        for (int p = 0; p < 2; ++p) {
           float y[8];
-          const int at = piece_at(seat.row, seat.half * 4 + p);
+          const int at = piece_at(seat.row, seat.part * 2 + p);
 #pragma unroll
           for (int k = 0; k < 8; ++k) y[k] = f[p * 8 + k];
           put8(mem + Mem::Y + at, mem + Mem::Y + Mem::kPlaneX + at, y);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) y[k] *= -fac.grown_k[t32 + p * 8 + k];
+          for (int k = 0; k < 8; ++k) y[k] *= -fac.grown_k[tt + p * 8 + k];
           put8(mem + Mem::X + at, mem + Mem::X + Mem::kPlaneX + at, y);
         }
       }
       if (c > 0 && tid < kChunk) parts.fill(sh.f[(r + 1) & 1], sh.grown_q[(r + 1) & 1], tid);
       hand_over(&sh.bar[kReadsSet]);
-      const int t = c * kChunk + t32;
+      const int t = c * kChunk + tt;
       if (in) put_column(dv + t * step, step, d.T - t, f);
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == kControl) {
     tc_fence_after();
     tmem_dealloc(tm, 512);
   }

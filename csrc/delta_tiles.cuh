@@ -62,20 +62,20 @@ __device__ __forceinline__ const I* head_at(const HeadRows& x, int b, long long 
   return reinterpret_cast<const I*>(x.p) + b * x.sb + t * x.st + h * x.sh;
 }
 
-// 32 tokens' values of one column of head rows; zeros behind the last of `rows` tokens. Whole chunks without a condition: with
+// N tokens' values of one column of head rows; zeros behind the last of `rows` tokens. Whole chunks without a condition: with
 // one for each load, they wait for one another.
-template <typename I>
-__device__ __forceinline__ void column_of(const I* p, long long st, int rows, I (&x)[32]) {
-  if (rows >= 32) {
+template <typename I, int N>
+__device__ __forceinline__ void column_of(const I* p, long long st, int rows, I (&x)[N]) {
+  if (rows >= N) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
+    for (int i = 0; i < N; ++i) {
       x[i] = *p;
       p += st;
     }
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
+  for (int i = 0; i < N; ++i) {
     x[i] = i < rows ? *p : ElemOf<I>::down(0.f);
     p += st;
   }
@@ -130,29 +130,62 @@ __device__ __forceinline__ void bulk_store(void* to, const void* from, uint32_t 
 }
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void bulk_read_done() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_read_one_left() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
 __device__ __forceinline__ void bulk_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 // ---------------------------------------------------------------- tensor memory
-__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32],"
-      " {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
-      "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
-      "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
-      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr));
-}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ void tmem_row(uint32_t taddr, float (&f)[32]) {
-  uint32_t r[32];
-  tmem_ld_32x32b_x32(taddr, r);
-  tmem_ld_wait();
-#pragma unroll
-  for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr));
 }
 
-constexpr int kWorkers = 256;  // threads of the eight warps that convert; a ninth warp's first lane copies and multiplies
+// 16 columns of the lane's row.
+__device__ __forceinline__ void tmem_row(uint32_t taddr, float (&f)[16]) {
+  uint32_t r[16];
+  tmem_ld_32x32b_x16(taddr, r);
+  tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(r[i]);
+}
+// Of two matrices at once.
+__device__ __forceinline__ void tmem_rows(uint32_t at, float (&f)[16], uint32_t bt, float (&g)[16]) {
+  uint32_t r[16], s[16];
+  tmem_ld_32x32b_x16(at, r);
+  tmem_ld_32x32b_x16(bt, s);
+  tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    f[i] = __uint_as_float(r[i]);
+    g[i] = __uint_as_float(s[i]);
+  }
+}
+
+// Where a worker sits: warp w of sixteen holds tensor memory's lanes 32 (w % 4) .. + 31, one each, and a quarter of the columns.
+struct Seat {
+  int row, part;
+  uint32_t lanes;  // of a tensor memory address
+  __device__ Seat() {
+    const int warp = threadIdx.x >> 5;
+    row = (warp & 3) * 32 + (threadIdx.x & 31);
+    part = warp >> 2;
+    lanes = (uint32_t)(warp & 3) << 21;
+  }
+};
+
+// Threads of the sixteen warps that convert (eight leave half of the issue slots empty: a training pass took 1085 us with them);
+// another warp's first lane copies and multiplies.
+constexpr int kWorkers = 512, kControl = kWorkers / 32;
 
 // A barrier that completes once in every round of a loop, and its waits. After a wait that gave up the kernel leaves: every
 // later wait of the thread returns at once.
