@@ -24,7 +24,7 @@ struct InputsMem {
   static constexpr int S = 0, V = S + 2 * kPlaneS, O = V + 2 * kPlaneX, G = O + kPlaneX,
                        Ol = G + kPlaneX, Gl = Ol + (kParts<I> == 2 ? kPlaneX : 0), Q = Gl + kPlaneX, K = Q + kParts<I> * kPlaneK,
                        W = K + kParts<I> * kPlaneK, N = W + 2 * kTok, kTiles = N + 2 * kTok;
-  static constexpr int ldF = DK + 4, kRows = 2 * kChunk * ldF * 4;  // in the end, from S on: this head's dq and dk
+  static constexpr int ldF = DK + 4, kRows = (2 * kChunk + kMostGroup) * ldF * 4;  // in the end, from S on: all heads' parts of the owned rows
   static constexpr int kBytes = kTiles > kRows ? kTiles : kRows;
 };
 
@@ -35,8 +35,8 @@ struct InputsShared {
   uint32_t tmem;
   float2 G[kChunk];
   float rk[kChunk], rq[kChunk], beta[kChunk], left[kChunk], grown[kChunk];
-  float dots[3][kChunk];  // V' . dV, v . dv, q . dq
-  float part[2][4][kChunk];
+  float part[2][4][kChunk];  // V' . dV and v . dv, of each quarter of a slice
+  float qdots[4][kChunk];    // q . dq, of each quarter of a key head
   float handed[kControl];
 };
 
@@ -44,6 +44,20 @@ struct InputsShared {
 __device__ __forceinline__ float lanes_fold(float (&x)[32]) {
 #pragma unroll
   for (int n = 16; n > 0; n >>= 1) {
+    const bool up = threadIdx.x & n;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float send = up ? x[i] : x[i + n], keep = up ? x[i + n] : x[i];
+      x[i] = keep + __shfl_xor_sync(0xffffffffu, send, n);
+    }
+  }
+  return x[0];
+}
+
+// Adds 16 values of each of 16 lanes (the other 16 hold the same): lane l ends with the sum of value l % 16.
+__device__ __forceinline__ float lanes_fold16(float (&x)[16]) {
+#pragma unroll
+  for (int n = 8; n > 0; n >>= 1) {
     const bool up = threadIdx.x & n;
 #pragma unroll
     for (int i = 0; i < n; ++i) {
@@ -69,10 +83,30 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
   const long long head = (long long)b * d.H + h, n = head * chunks + c, m = bk * chunks + c;
   const int t0 = c * kChunk, rows = min(kChunk, d.T - t0);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (tid == 0) {
+  const auto state_at = [&](int chunk, int s) { return a.keep.states + ((head * (chunks + 1) + chunk) * slices + s) * 2 * Mem::kPlaneS; };
+  const auto load_slice = [&](int s) {
+    const long long at = n * slices + s;
+    mbar_arrive_expect_tx(&sh.bar[kGotV], (4 + P) * Mem::kPlaneX);
+    bulk_load(mem + Mem::V, a.keep.writes + at * 2 * Mem::kPlaneX, 2 * Mem::kPlaneX, &sh.bar[kGotV]);
+    bulk_load(mem + Mem::O, a.douts + at * P * Mem::kPlaneX, Mem::kPlaneX, &sh.bar[kGotV]);
+    if (P == 2) bulk_load(mem + Mem::Ol, a.douts + (at * P + 1) * Mem::kPlaneX, Mem::kPlaneX, &sh.bar[kGotV]);
+    bulk_load(mem + Mem::G, a.dreads + at * 2 * Mem::kPlaneX, Mem::kPlaneX, &sh.bar[kGotV]);
+    bulk_load(mem + Mem::Gl, a.dreads + at * 2 * Mem::kPlaneX + Mem::kPlaneX, Mem::kPlaneX, &sh.bar[kGotV]);
+    mbar_arrive_expect_tx(&sh.bar[kGotS], 2 * Mem::kPlaneS);
+    bulk_load(mem + Mem::S, state_at(c, s), 2 * Mem::kPlaneS, &sh.bar[kGotS]);
+    bulk_prefetch(a.dstates + at * 2 * Mem::kPlaneS, 2 * Mem::kPlaneS);
+    bulk_prefetch(state_at(c + 1, s), 2 * Mem::kPlaneS);
+  };
+  if (tid == kWorkers) {
     for (int i = 0; i < kInputsBars; ++i) mbar_init(&sh.bar[i], i == kMixSet || i == kTaken ? kWorkers : 1);
     fence_barrier_init();
+    fence_proxy_async_smem();
+    load_slice(0);
+    mbar_arrive_expect_tx(&sh.bar[kGotQK], 2 * P * Mem::kPlaneK);
+    bulk_load(mem + Mem::Q, a.keep.queries + m * P * Mem::kPlaneK, P * Mem::kPlaneK, &sh.bar[kGotQK]);
+    bulk_load(mem + Mem::K, a.keep.keys + m * P * Mem::kPlaneK, P * Mem::kPlaneK, &sh.bar[kGotQK]);
   }
+  __syncwarp();
   if (warp == kControl) tmem_alloc(&sh.tmem, 512);
   if (tid < kChunk) {
     const float2 G = a.keep.total[n * kChunk + tid], end = a.keep.total[n * kChunk + kChunk - 1];
@@ -82,43 +116,26 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
     sh.beta[tid] = a.keep.beta[n * kChunk + tid];
     sh.left[tid] = decay_between(end, G);
     sh.grown[tid] = __expf(G.x + G.y);
-    sh.dots[0][tid] = sh.dots[1][tid] = sh.dots[2][tid] = 0.f;
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tm = sh.tmem;
   const Seat seat;
-  constexpr uint32_t cMix = 0, cLow = 64, cS = 128, cD = 256, cQ = 320, cK = 384;
+  // The last two come when the small matrices' products, in the same place, are read.
+  constexpr uint32_t cS = 0, cD = 128, cMix = 256, cLow = 384, cQ = 256, cK = 384;
   Waiter wait{a.err};
-  const auto state_at = [&](int chunk, int s) { return a.keep.states + ((head * (chunks + 1) + chunk) * slices + s) * 2 * Mem::kPlaneS; };
   if (warp == kControl) {
     if (lane == 0) {
       const uint32_t base = smem_u32(mem);
-      mbar_arrive_expect_tx(&sh.bar[kGotQK], 2 * P * Mem::kPlaneK);
-      const auto load_slice = [&](int s) {
-        const long long at = n * slices + s;
-        mbar_arrive_expect_tx(&sh.bar[kGotV], (4 + P) * Mem::kPlaneX);
-        bulk_load(mem + Mem::V, a.keep.writes + at * 2 * Mem::kPlaneX, 2 * Mem::kPlaneX, &sh.bar[kGotV]);
-        bulk_load(mem + Mem::O, a.douts + at * P * Mem::kPlaneX, Mem::kPlaneX, &sh.bar[kGotV]);
-        if (P == 2) bulk_load(mem + Mem::Ol, a.douts + (at * P + 1) * Mem::kPlaneX, Mem::kPlaneX, &sh.bar[kGotV]);
-        bulk_load(mem + Mem::G, a.dreads + at * 2 * Mem::kPlaneX, Mem::kPlaneX, &sh.bar[kGotV]);
-        bulk_load(mem + Mem::Gl, a.dreads + at * 2 * Mem::kPlaneX + Mem::kPlaneX, Mem::kPlaneX, &sh.bar[kGotV]);
-        mbar_arrive_expect_tx(&sh.bar[kGotS], 2 * Mem::kPlaneS);
-        bulk_load(mem + Mem::S, state_at(c, s), 2 * Mem::kPlaneS, &sh.bar[kGotS]);
-      };
-      load_slice(0);
-      bulk_load(mem + Mem::Q, a.keep.queries + m * P * Mem::kPlaneK, P * Mem::kPlaneK, &sh.bar[kGotQK]);
-      bulk_load(mem + Mem::K, a.keep.keys + m * P * Mem::kPlaneK, P * Mem::kPlaneK, &sh.bar[kGotQK]);
       // The stack of high halves, and that of low ones; without a low half of dO the first 64 lanes of its product are not used.
       const Operand high{base + Mem::O, Mem::G - Mem::O}, low{base + (P == 2 ? Mem::Ol : Mem::O), Mem::Gl - (P == 2 ? Mem::Ol : Mem::O)},
-          low_g{base + Mem::Gl, Mem::kPlaneX}, V{base + Mem::V, Mem::kPlaneX}, Vl{base + Mem::V + Mem::kPlaneX, Mem::kPlaneX},
+          low_g{base + Mem::Gl, Mem::kPlaneX}, V{base + Mem::V, Mem::kPlaneX},
           S{base + Mem::S, Mem::kPanelS}, Sl{base + Mem::S + Mem::kPlaneS, Mem::kPanelS};
       for (int s = 0; s < slices; ++s) {
         const bool more = s > 0;
         if (!wait(&sh.bar[kGotV], s)) break;
-        multiply<kVs, 64, true, true>(tm + cMix, high, V, more);
-        multiply<kVs, 64, true, true>(tm + cMix, high, Vl, true);
+        multiply<kVs, 128, true, true>(tm + cMix, high, V, more);  // both halves of V' side by side
         multiply<kVs, 64, true, true>(P == 2 ? tm + cMix : tm + cLow, low, V, P == 2 || more);
         if (s == slices - 1) tc_commit(&sh.bar[kMixDone]);
         if (!wait(&sh.bar[kGotS], s)) break;
@@ -131,9 +148,8 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
         mbar_arrive_expect_tx(&sh.bar[kGotD], 2 * Mem::kPlaneS);
         bulk_load(mem + Mem::S, a.dstates + (n * slices + s) * 2 * Mem::kPlaneS, 2 * Mem::kPlaneS, &sh.bar[kGotD]);
         if (!wait(&sh.bar[kGotD], s)) break;
-        multiply<kVs, 64, true, true>(tm + cD, S, V, more);
+        multiply<kVs, 128, true, true>(tm + cD, S, V, more);
         multiply<kVs, 64, true, true>(tm + cD, Sl, V, true);
-        multiply<kVs, 64, true, true>(tm + cD, S, Vl, true);
         tc_commit(&sh.bar[kReadS]);
         if (s + 1 < slices) {  // the places are free once they are read, by the products and by the workers
           if (!wait(&sh.bar[kReadS], 2 * s + 1) || !wait(&sh.bar[kTaken], s)) break;
@@ -143,10 +159,10 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
       const Operand Q{base + Mem::Q, kTok}, K{base + Mem::K, kTok}, W{base + Mem::W, kTok}, N{base + Mem::N, kTok};
       if (wait(&sh.bar[kGotQK], 0) && wait(&sh.bar[kMixSet], 0)) {
         tc_fence_after();
-        multiply_parts<4, 64, true, false, P, 2>(tm + cQ, K, Mem::kPlaneK, W, kTok, false);
-        multiply_parts<4, 64, true, true, P, 2>(tm + cK, Q, Mem::kPlaneK, W, kTok, false);
-        multiply_parts<4, 64, true, false, P, 2>(tm + cK, K, Mem::kPlaneK, N, kTok, true);
-        multiply_parts<4, 64, true, true, P, 2>(tm + cK, K, Mem::kPlaneK, N, kTok, true);
+        multiply_wide<4, 128, true, false, P>(tm + cQ, K, Mem::kPlaneK, W, false);
+        multiply_wide<4, 128, true, true, P>(tm + cK, Q, Mem::kPlaneK, W, false);
+        multiply_wide<4, 128, true, false, P>(tm + cK, K, Mem::kPlaneK, N, true);
+        multiply_wide<4, 128, true, true, P>(tm + cK, K, Mem::kPlaneK, N, true);
         tc_commit(&sh.bar[kAllDone]);
         wait(&sh.bar[kAllDone], 0);
       }
@@ -169,14 +185,13 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
         const int i = seat.row & 63, j0 = seat.part * 16;
         const bool of_l = seat.row >= 64;
         float f[16];
+        tmem_sum(tm + seat.lanes + cMix + j0, tm + seat.lanes + cMix + 64 + j0, f);
         if (P == 1) {
           float g[16];
-          tmem_rows(tm + seat.lanes + cMix + j0, f, tm + seat.lanes + cLow + j0, g);
+          tmem_row(tm + seat.lanes + cLow + j0, g);
           if (of_l)
 #pragma unroll
             for (int k = 0; k < 16; ++k) f[k] += g[k];
-        } else {
-          tmem_row(tm + seat.lanes + cMix + j0, f);
         }
         const float by = of_l ? -sh.rk[i] : sh.rq[i];
         const float2 Gi = sh.G[i];
@@ -253,38 +268,111 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
     if (lane == 0) sh.handed[warp] = handed;
     wait(&sh.bar[kAllDone], 0);
   }
-  // dq and dk of this head: r dq^ and r dk^ of the scaled rows, tokens as rows, where S and V' lay.
-  __syncthreads();
+  // dq and dk of this head: r dq^ and r dk^ of the scaled rows. Each CTA of the cluster owns every group-th row of both and
+  // gets them from all heads, where its S and V' lay: row r at place r / group of the sender's part.
+  cg::cluster_group cluster = cg::this_cluster();
+  if (group > 1) cluster.sync();  // all are done with their products
+  else __syncthreads();
   float* F = reinterpret_cast<float*>(mem);
+  const int own = (2 * kChunk + group - 1) / group;  // rows of an owner, at most
   if (warp < kControl) {
     tc_fence_after();
     const int tt = seat.part * 16;
-    float s[16], y[16], z[16];
-    tmem_rows(tm + seat.lanes + cS + tt, s, tm + seat.lanes + cQ + tt, y);
-    if (seat.row < DK)
+    float x[16], y[16], z[16];
+    const auto put = [&](int r0, const float (&v)[16]) {
+      int owner = r0 % group;
+      float* f = F + (hg * own + r0 / group) * Mem::ldF + seat.row;
 #pragma unroll
-      for (int k = 0; k < 16; ++k) F[(tt + k) * Mem::ldF + seat.row] = fmaf(sh.rq[tt + k] * sh.grown[tt + k], s[k], y[k]);
-    tmem_rows(tm + seat.lanes + cS + 64 + tt, s, tm + seat.lanes + cD + tt, z);
-    tmem_row(tm + seat.lanes + cK + tt, y);
-    if (seat.row < DK)
+      for (int k = 0; k < 16; ++k) {
+        *(group > 1 ? cluster.map_shared_rank(f, owner) : f) = v[k];
+        if (++owner == group) {
+          owner = 0;
+          f += Mem::ldF;
+        }
+      }
+    };
+    tmem_sum(tm + seat.lanes + cQ + tt, tm + seat.lanes + cQ + 64 + tt, y);
+    tmem_row(tm + seat.lanes + cS + tt, x);
 #pragma unroll
-      for (int k = 0; k < 16; ++k)
-        F[(kChunk + tt + k) * Mem::ldF + seat.row] = fmaf(sh.rk[tt + k], fmaf(sh.left[tt + k], z[k], -sh.grown[tt + k] * s[k]), y[k]);
+    for (int k = 0; k < 16; ++k) y[k] = fmaf(sh.rq[tt + k] * sh.grown[tt + k], x[k], y[k]);
+    if (seat.row < DK) put(tt, y);
+    // q^ . dq^ = q . dq: over the lanes here, over the warps of a column later. The rows of q still lie as a tile.
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      float q = 0.f;
+      if (seat.row < DK) {
+        const unsigned char* at = mem + Mem::Q + element_at(tt + k, seat.row, kTok);
+        q = __bfloat162float(*reinterpret_cast<const bf16*>(at));
+        if (P == 2) q += __bfloat162float(*reinterpret_cast<const bf16*>(at + Mem::kPlaneK));
+      }
+      x[k] = seat.row < DK ? q * y[k] : 0.f;
+      x[k] += __shfl_xor_sync(0xffffffffu, x[k], 16);
+    }
+    const float dot = lanes_fold16(x);
+    if (lane < 16) sh.qdots[warp & 3][tt + lane] = dot;
+    tmem_sum(tm + seat.lanes + cD + tt, tm + seat.lanes + cD + 64 + tt, z);
+    tmem_row(tm + seat.lanes + cS + 64 + tt, x);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) z[k] = sh.rk[tt + k] * fmaf(sh.left[tt + k], z[k], -sh.grown[tt + k] * x[k]);
+    tmem_sum(tm + seat.lanes + cK + tt, tm + seat.lanes + cK + 64 + tt, y);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) y[k] += z[k];
+    if (seat.row < DK) put(kChunk + tt, y);
     tc_fence_before();
   }
-  __syncthreads();
+  if (group > 1) cluster.sync();
+  else __syncthreads();
   if (warp == kControl) {
     tc_fence_after();
     tmem_dealloc(tm, 512);
-  }
-  if (tid < kChunk) {
+    // The gates: sums from each token to the chunk's end, two tokens a lane.
+    float after = 0.f, ends[2], writes[2];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      sh.dots[0][tid] += sh.part[0][w][tid];
-      sh.dots[1][tid] += sh.part[1][w][tid];
+    for (int w = 0; w < kControl; ++w) after += sh.handed[w];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int i = 2 * lane + k;
+      ends[k] = writes[k] = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        ends[k] += sh.qdots[w][i] - sh.part[1][w][i];
+        writes[k] += sh.part[0][w][i];
+      }
     }
+    float sum = ends[0] + ends[1];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const float up = __shfl_down_sync(0xffffffffu, sum, o);
+      if (lane + o < 32) sum += up;
+    }
+    const float a_log = load_any(a.g.a_log, a.g.a_log_type, h), dt = load_any(a.g.dt_bias, a.g.dt_bias_type, h);
+    double sum_log = 0.0, sum_bias = 0.0;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int i = 2 * lane + k;
+      if (i >= rows) continue;
+      const Gate gate = gate_of(ElemOf<I>::up(*head_at<I>(a.g.a, b, t0 + i, h)), a_log, dt);
+      // Nothing passes a gate whose factor is 0 in fp32: what the sum holds then is its rounding.
+      const float dg = gate.log_decay < -104.f ? 0.f : (k ? sum - ends[0] : sum) + after;
+      const float da = -dg * gate.rate * gate.slope;
+      const float beta = sh.beta[i];
+      const float db = beta > 1e-20f ? (1.f - beta) * (writes[k] / beta) : 0.f;  // V' = beta E; below, db is under 1e-20 dV . E
+      const long long to = ((long long)b * d.T + t0 + i) * d.H + h;
+      reinterpret_cast<I*>(a.da)[to] = ElemOf<I>::down(da);
+      reinterpret_cast<I*>(a.db)[to] = ElemOf<I>::down(db);
+      sum_log += (double)dg * gate.log_decay;
+      sum_bias += da;
+    }
+    sum_log = lanes_sum(sum_log);
+    sum_bias = lanes_sum(sum_bias);
+    if (lane == 0) {
+      a.part[n * 2] = (float)sum_log;
+      a.part[n * 2 + 1] = (float)sum_bias;
+    }
+    return;
   }
-  // q^ . dq^ = q . dq of this head's rows, a row's elements side by side in a warp; the rows of q and k still lie as tiles.
+  // The owned rows' sums over the heads in their order, a row's elements side by side in a warp, then back through the rows'
+  // scaling: with x a row, r its reciprocal length and y the sum, dx = y - x r^2 (x . y). Four rows at a time.
   constexpr int kE = DK / 32;  // elements of a lane
   const auto row_of = [&](int tile, int i, float (&x)[kE]) {
     const unsigned char* at = mem + tile + element_at(i, lane * kE, kTok);
@@ -300,107 +388,42 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
 #pragma unroll
       for (int k = 0; k < kE; ++k) x[k] += lo[k];
   };
-  const auto sums_of = [&](const float* f, float (&y)[kE], bool add) {
-    float z[kE];
-    if constexpr (kE == 4) *reinterpret_cast<float4*>(z) = *reinterpret_cast<const float4*>(f + lane * kE);
-    else *reinterpret_cast<float2*>(z) = *reinterpret_cast<const float2*>(f + lane * kE);
-#pragma unroll
-    for (int k = 0; k < kE; ++k) y[k] = add ? y[k] + z[k] : z[k];
-  };
-  if (warp < kControl) {
-    float dot[4];
+  for (int p0 = warp; p0 < own; p0 += 4 * kControl) {
+    float y[4][kE], x[4][kE], dot[4];
 #pragma unroll
     for (int n4 = 0; n4 < 4; ++n4) {
-      const int i = n4 * kControl + warp;
-      float x[kE], y[kE];
-      row_of(Mem::Q, i, x);
-      sums_of(F + i * Mem::ldF, y, false);
+      const int place = min(p0 + n4 * kControl, own - 1), r = min(place * group + hg, 2 * kChunk - 1);
+      row_of(r >= kChunk ? Mem::K : Mem::Q, r % kChunk, x[n4]);
+#pragma unroll
+      for (int k = 0; k < kE; ++k) y[n4][k] = 0.f;
+      for (int o = 0; o < group; ++o) {
+        const float* f = F + (o * own + place) * Mem::ldF + lane * kE;
+#pragma unroll
+        for (int k = 0; k < kE; k += 2) {
+          const float2 z = *reinterpret_cast<const float2*>(f + k);
+          y[n4][k] += z.x;
+          y[n4][k + 1] += z.y;
+        }
+      }
       dot[n4] = 0.f;
 #pragma unroll
-      for (int k = 0; k < kE; ++k) dot[n4] = fmaf(x[k], y[k], dot[n4]);
+      for (int k = 0; k < kE; ++k) dot[n4] = fmaf(x[n4][k], y[n4][k], dot[n4]);
     }
+#pragma unroll
+    for (int n4 = 0; n4 < 4; ++n4) dot[n4] = lanes_sum(dot[n4]);
 #pragma unroll
     for (int n4 = 0; n4 < 4; ++n4) {
-      dot[n4] = lanes_sum(dot[n4]);
-      if (lane == 0) sh.dots[2][n4 * kControl + warp] = dot[n4];
+      const int place = p0 + n4 * kControl, r = place * group + hg, i = r % kChunk;
+      if (place >= own || r >= 2 * kChunk || i >= rows || lane * kE >= d.dk) continue;
+      const bool of_k = r >= kChunk;
+      const float len = of_k ? sh.rk[i] : sh.rq[i] / d.scale, by = -len * len * dot[n4];
+#pragma unroll
+      for (int k = 0; k < kE; ++k) y[n4][k] = fmaf(by, x[n4][k], y[n4][k]);
+      I* to = reinterpret_cast<I*>(of_k ? a.dk : a.dq) + (((long long)b * d.T + t0 + i) * d.Hk + hk) * d.dk + lane * kE;
+      if constexpr (kE == 4) *reinterpret_cast<uint2*>(to) = raw_down<I, uint2>(y[n4]);
+      else *reinterpret_cast<uint32_t*>(to) = raw_down<I, uint32_t>(y[n4]);
     }
   }
-  static_assert(4 * kControl == kChunk, "a row of q to each warp, four times");
-  cg::cluster_group cluster = cg::this_cluster();
-  if (group > 1) cluster.sync();
-  else __syncthreads();
-  if (warp == kControl) {  // the gates: sums from each token to the chunk's end, two tokens a lane
-    float after = 0.f;
-#pragma unroll
-    for (int w = 0; w < kControl; ++w) after += sh.handed[w];
-    const float x = sh.dots[2][2 * lane] - sh.dots[1][2 * lane], y = sh.dots[2][2 * lane + 1] - sh.dots[1][2 * lane + 1];
-    float sum = x + y;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const float up = __shfl_down_sync(0xffffffffu, sum, o);
-      if (lane + o < 32) sum += up;
-    }
-    const float a_log = load_any(a.g.a_log, a.g.a_log_type, h), dt = load_any(a.g.dt_bias, a.g.dt_bias_type, h);
-    double sum_log = 0.0, sum_bias = 0.0;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int i = 2 * lane + k;
-      if (i >= rows) continue;
-      const Gate gate = gate_of(ElemOf<I>::up(*head_at<I>(a.g.a, b, t0 + i, h)), a_log, dt);
-      // Nothing passes a gate whose factor is 0 in fp32: what the sum holds then is its rounding.
-      const float dg = gate.log_decay < -104.f ? 0.f : (k ? sum - x : sum) + after;
-      const float da = -dg * gate.rate * gate.slope;
-      const float beta = sh.beta[i];
-      const float db = beta > 1e-20f ? (1.f - beta) * (sh.dots[0][i] / beta) : 0.f;  // V' = beta E; below, db is under 1e-20 dV . E
-      const long long to = ((long long)b * d.T + t0 + i) * d.H + h;
-      reinterpret_cast<I*>(a.da)[to] = ElemOf<I>::down(da);
-      reinterpret_cast<I*>(a.db)[to] = ElemOf<I>::down(db);
-      sum_log += (double)dg * gate.log_decay;
-      sum_bias += da;
-    }
-    sum_log = lanes_sum(sum_log);
-    sum_bias = lanes_sum(sum_bias);
-    if (lane == 0) {
-      a.part[n * 2] = (float)sum_log;
-      a.part[n * 2 + 1] = (float)sum_bias;
-    }
-  } else {
-    // Sums over the key head's value heads, the rows of both shared out over the cluster's warps, then back through the
-    // rows' scaling: with x a row, r its reciprocal length and y the sum, dx = y - x r^2 (x . y).
-    const float* from[kMostGroup];
-#pragma unroll
-    for (int o = 0; o < kMostGroup; ++o) from[o] = group > 1 ? cluster.map_shared_rank(F, o < group ? o : 0) : F;
-    // Four rows at a time, so that their loads are on their way together.
-    for (int r0 = hg * kControl + warp; r0 < 2 * kChunk; r0 += 4 * kControl * group) {
-      float y[4][kE], x[4][kE], dot[4];
-#pragma unroll
-      for (int n4 = 0; n4 < 4; ++n4) {
-        const int r = min(r0 + n4 * kControl * group, 2 * kChunk - 1);
-        row_of(r >= kChunk ? Mem::K : Mem::Q, r % kChunk, x[n4]);
-#pragma unroll
-        for (int o = 0; o < kMostGroup; ++o)
-          if (o < group) sums_of(from[o] + r * Mem::ldF, y[n4], o > 0);
-        dot[n4] = 0.f;
-#pragma unroll
-        for (int k = 0; k < kE; ++k) dot[n4] = fmaf(x[n4][k], y[n4][k], dot[n4]);
-      }
-#pragma unroll
-      for (int n4 = 0; n4 < 4; ++n4) dot[n4] = lanes_sum(dot[n4]);
-#pragma unroll
-      for (int n4 = 0; n4 < 4; ++n4) {
-        const int r = r0 + n4 * kControl * group, i = r % kChunk;
-        if (r >= 2 * kChunk || i >= rows || lane * kE >= d.dk) continue;
-        const bool of_k = r >= kChunk;
-        const float len = of_k ? sh.rk[i] : sh.rq[i] / d.scale, by = -len * len * dot[n4];
-#pragma unroll
-        for (int k = 0; k < kE; ++k) y[n4][k] = fmaf(by, x[n4][k], y[n4][k]);
-        I* to = reinterpret_cast<I*>(of_k ? a.dk : a.dq) + (((long long)b * d.T + t0 + i) * d.Hk + hk) * d.dk + lane * kE;
-        if constexpr (kE == 4) *reinterpret_cast<uint2*>(to) = raw_down<I, uint2>(y[n4]);
-        else *reinterpret_cast<uint32_t*>(to) = raw_down<I, uint32_t>(y[n4]);
-      }
-    }
-  }
-  if (group > 1) cluster.sync();  // no CTA leaves while its rows are read
 }
 
 // The chunks' sums for a_log and dt_bias of one head, in a fixed order.

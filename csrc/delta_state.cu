@@ -94,7 +94,8 @@ struct StateShared {
   float grown_q[3][kChunk];  // exp(G) rq: an output is written a chunk later than the factors are read
 };
 
-// One slice of a head's state, chunk after chunk. Tensor memory: S^T (128 x DK), twice K S and Q S, E, P V'.
+// One slice of a head's state, chunk after chunk. Tensor memory: S^T (128 x DK), twice K S and Q S, then E and
+// after it P V', each in two halves.
 template <typename I, int DK, int DV>
 __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd a) {
   using Mem = StateMem<I, DK, DV>;
@@ -122,7 +123,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
   __syncthreads();
   tc_fence_after();
   const uint32_t tm = sh.tmem;
-  constexpr uint32_t cS = 0, cK = 128, cQ = 192, cE = 384, cP = 448;  // cK and cQ again 128 columns on
+  constexpr uint32_t cS = 0, cK = 128, cQ = 192, cE = 384, cP = cE;  // cK and cQ again 128 columns on; E is read before P V' comes
   Waiter wait{a.err};
   if (warp == kControl) {
     if ((tid & 31) == 0) {
@@ -166,7 +167,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
         if (!wait(&sh.bar[kRhsSet], c)) break;
         if (!wait(&sh.bar[kLoadedT], c)) break;
         tc_fence_after();
-        multiply_parts<4, 64, false, false, 2, 2>(tm + cE, X, Mem::kPlaneX, T, kTok, false);
+        multiply_wide<4, 128, false, false, 2>(tm + cE, X, Mem::kPlaneX, T, false);
         bulk_read_one_left();  // the last chunk's writes are copied: their place may be written once this product is done
         tc_commit(&sh.bar[kSolveDone]);
         if (!wait(&sh.bar[kWritesSet], c)) break;
@@ -177,7 +178,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
         tc_commit(&sh.bar[kStateDone]);
         mbar_arrive(&sh.bar[kFactorsSet]);
         if (!wait(&sh.bar[kLoadedP], c)) break;
-        multiply_parts<4, 64, false, false, 2, 2>(tm + cP, W, Mem::kPlaneX, At, kTok, false);
+        multiply_wide<4, 128, false, false, 2>(tm + cP, W, Mem::kPlaneX, At, false);
         tc_commit(&sh.bar[kOutDone]);
         if (a.keep.writes != nullptr) {
           bulk_store(a.keep.writes + ((n0 + c) * slices + slice) * 2 * Mem::kPlaneX, mem + Mem::W, 2 * Mem::kPlaneX);
@@ -218,7 +219,8 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
     const auto put_out = [&](int c) {  // the output of chunk c: Q S and P V' are done
       const uint32_t flip = (c & 1) * 128;
       float x[16], y[16];
-      tmem_rows(tm + seat.lanes + cQ + flip + tt, x, tm + seat.lanes + cP + tt, y);
+      tmem_sum(tm + seat.lanes + cP + tt, tm + seat.lanes + cP + 64 + tt, y);
+      tmem_row(tm + seat.lanes + cQ + flip + tt, x);
       if (!in) return;
       const float* by = sh.grown_q[c % 3] + tt;
 #pragma unroll
@@ -285,7 +287,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
       }
       if (!wait(&sh.bar[kSolveDone], c)) break;
       tc_fence_after();
-      tmem_row(tm + seat.lanes + cE + tt, f);
+      tmem_sum(tm + seat.lanes + cE + tt, tm + seat.lanes + cE + 64 + tt, f);
       if (there) {
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
@@ -331,7 +333,8 @@ struct DstateShared {
   float grown_q[2][kChunk];  // exp(G) rq
 };
 
-// One slice of the gradient of a head's state, from the last chunk to the first. Tensor memory: dS^T (128 x DK), K dS', P^T dO, dV.
+// One slice of the gradient of a head's state, from the last chunk to the first. Tensor memory: dS^T (128 x DK), K dS',
+// P^T dO and dV in two halves each.
 template <typename I, int DK, int DV>
 __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd a) {
   using Mem = DstateMem<I, DK, DV>;
@@ -359,7 +362,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
   __syncthreads();
   tc_fence_after();
   const uint32_t tm = sh.tmem;
-  constexpr uint32_t cS = 0, cK = 128, cO = 192, cV = 256;
+  constexpr uint32_t cS = 0, cK = 128, cO = 192, cV = 320;
   Waiter wait{a.err};
   if (warp == kControl) {
     if ((tid & 31) == 0 && chunks > 0) {
@@ -392,7 +395,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
         if (!wait(&sh.bar[kOutsSet], r)) break;
         if (!wait(&sh.bar[kGotQ], r)) break;
         tc_fence_after();
-        multiply_parts<4, 64, false, true, P, 2>(tm + cO, O, Mem::kPlaneX, At, kTok, false);
+        multiply_wide<4, 128, false, true, P>(tm + cO, O, Mem::kPlaneX, At, false);
         tc_commit(&sh.bar[kMixDone]);
         multiply_parts<4, DK, false, true, 2, P>(tm + cS, Y, Mem::kPlaneX, Q, Mem::kPlaneK, true);
         tc_commit(&sh.bar[kOutsDone]);
@@ -403,7 +406,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
         if (!wait(&sh.bar[kGradSet], r)) break;
         if (!wait(&sh.bar[kGotT], r)) break;
         tc_fence_after();
-        multiply_parts<4, 64, false, true, 2, 2>(tm + cV, X, Mem::kPlaneX, T, kTok, false);
+        multiply_wide<4, 128, false, true, 2>(tm + cV, X, Mem::kPlaneX, T, false);
         tc_commit(&sh.bar[kBackDone]);
         if (!wait(&sh.bar[kOutsDone], r)) break;
         if (r + 1 < chunks) load_q(r + 1);
@@ -504,7 +507,8 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
       if (!wait(&sh.bar[kMixDone], r)) break;
       tc_fence_after();
       float f[16], y16[16];
-      tmem_rows(tm + seat.lanes + cK + tt, f, tm + seat.lanes + cO + tt, y16);
+      tmem_sum(tm + seat.lanes + cO + tt, tm + seat.lanes + cO + 64 + tt, y16);
+      tmem_row(tm + seat.lanes + cK + tt, f);
       if (there) {
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
@@ -521,7 +525,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
       hand_over(&sh.bar[kGradSet]);
       if (!wait(&sh.bar[kBackDone], r) || !wait(&sh.bar[kOutsDone], r)) break;  // the solve, and Y read
       tc_fence_after();
-      tmem_row(tm + seat.lanes + cV + tt, f);
+      tmem_sum(tm + seat.lanes + cV + tt, tm + seat.lanes + cV + 64 + tt, f);
       if (there) {
 #pragma unroll
         for (int p = 0; p < 2; ++p) {

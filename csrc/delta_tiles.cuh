@@ -119,7 +119,19 @@ __device__ __forceinline__ void multiply_parts(uint32_t d, Operand A, int lo_a, 
   if (kB == 2) multiply<kSteps, N, kAmn, kBmn>(d, A, Operand{B.addr + lo_b, B.panel}, true);
 }
 
+// The same with B's halves side by side as one operand of twice the columns (they lie `B.panel` apart, or one behind the other):
+// D has A's products with either half in N / 2 columns each. An operand A is then read half as often, which is what
+// a product of 64 columns waits for.
+template <int kSteps, int N, bool kAmn, bool kBmn, int kA>
+__device__ __forceinline__ void multiply_wide(uint32_t d, Operand A, int lo_a, Operand B, bool accumulate) {
+  multiply<kSteps, N, kAmn, kBmn>(d, A, B, accumulate);
+  if (kA == 2) multiply<kSteps, N / 2, kAmn, kBmn>(d, Operand{A.addr + lo_a, A.panel}, B, true);
+}
+
 // ---------------------------------------------------------------- copies
+__device__ __forceinline__ void bulk_prefetch(const void* from, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void bulk_load(void* to, const void* from, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(to)),
                "l"(from), "r"(bytes), "r"(smem_u32(bar))
@@ -169,6 +181,14 @@ __device__ __forceinline__ void tmem_rows(uint32_t at, float (&f)[16], uint32_t 
     f[i] = __uint_as_float(r[i]);
     g[i] = __uint_as_float(s[i]);
   }
+}
+
+// The sum of two matrices' columns.
+__device__ __forceinline__ void tmem_sum(uint32_t at, uint32_t bt, float (&f)[16]) {
+  float g[16];
+  tmem_rows(at, f, bt, g);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) f[i] += g[i];
 }
 
 // Where a worker sits: warp w of sixteen holds tensor memory's lanes 32 (w % 4) .. + 31, one each, and a quarter of the columns.
