@@ -118,69 +118,37 @@ __device__ __forceinline__ void load_rows(bf16* to, int ld, int lo, const I* fro
   }
 }
 
-struct Place3 {
-  int b, h, c;
-  long long bh, n;
-  __device__ Place3(const DeltaDims& d, long long head, int chunk) : c(chunk), bh(head), n(head * d.chunks + chunk) {
-    b = (int)(head / d.H);
-    h = (int)(head % d.H);
-  }
+// ---------------------------------------------------------------- prepare
+// One chunk of one key head: 4 warps, 16 tokens' rows of both products each, which all its value heads share; those two at a time.
+// The inverse of I + A, A strictly lower: the two diagonal blocks of 32 by forward substitution, a column to each thread
+// of a warp, then the block below them as -T22 A21 T11; all in fp32.
+template <typename I, int DK>
+struct PrepareMem {
+  static constexpr int ld = DK + kPad, plane = kChunk * ld, ldA = kChunk + 4, ldU = 36;
+  static constexpr int kRowBytes = 2 * kParts<I> * plane * 2, kPairBytes = 2 * kChunk * ldA * 4;  // A lies where q and k were
+  static constexpr int kFirst = kRowBytes > kPairBytes ? kRowBytes : kPairBytes, kBytes = kFirst + 2 * 32 * ldU * 4;
 };
 
-// ---------------------------------------------------------------- prepare
-// One chunk of one value head: 4 warps, 16 tokens' rows of both products each. The inverse of I + A, A strictly lower: the two
-// diagonal blocks of 32 by forward substitution, a column to each of 64 threads, then the block below them as
-// -T22 A21 T11 by all; all in fp32.
 template <typename I, int DK>
-__global__ void __launch_bounds__(128) prepare_kernel(const DeltaFwd a) {
-  constexpr int ld = DK + kPad, plane = kChunk * ld, ldA = kChunk + 4, ldU = 36;
+__global__ void __launch_bounds__(128, kParts<I> == 1 ? 4 : 3) prepare_kernel(const DeltaFwd a) {
+  using Mem = PrepareMem<I, DK>;
+  constexpr int ld = Mem::ld, plane = Mem::plane, ldA = Mem::ldA, ldU = Mem::ldU;
   extern __shared__ __align__(16) unsigned char raw[];
   bf16* Q = reinterpret_cast<bf16*>(raw);
   bf16* K = Q + kParts<I> * plane;
-  float* A = reinterpret_cast<float*>(K + kParts<I> * plane);  // (64, ldA): L diag(beta), then the inverse
-  float* U = A + kChunk * ldA;                                 // (32, ldU): A21 T11
-  __shared__ float2 G[kChunk];
-  __shared__ float beta[kChunk], rk[kChunk], rq[kChunk], logs[kChunk];
+  __shared__ float2 G[2][kChunk];
+  __shared__ float beta[2][kChunk], rk[kChunk], rq[kChunk], logs[2][kChunk];
   const DeltaDims& d = a.d;
-  const Place3 at(d, blockIdx.x / d.chunks, blockIdx.x % d.chunks);
-  const int group = d.H / d.Hk, hk = at.h / group;
-  const int t0 = at.c * kChunk, rows = min(kChunk, d.T - t0);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const long long m = ((long long)at.b * d.Hk + hk) * d.chunks + at.c;
-  load_rows<I, DK>(Q, ld, plane, head_at<I>(a.q, at.b, t0, hk), a.q.st, rows, d.dk, d.wide);
-  load_rows<I, DK>(K, ld, plane, head_at<I>(a.k, at.b, t0, hk), a.k.st, rows, d.dk, d.wide);
-  if (tid < kChunk) {
-    float g = 0.f, w = 0.f;
-    if (tid < rows) {
-      g = gate_of(ElemOf<I>::up(*head_at<I>(a.g.a, at.b, t0 + tid, at.h)), load_any(a.g.a_log, a.g.a_log_type, at.h),
-                  load_any(a.g.dt_bias, a.g.dt_bias_type, at.h)).log_decay;
-      w = sigmoid(ElemOf<I>::up(*head_at<I>(a.g.b, at.b, t0 + tid, at.h)));
-    }
-    logs[tid] = g;
-    beta[tid] = w;
-    a.keep.beta[at.n * kChunk + tid] = w;
-  }
+  const int group = d.H / d.Hk, c = blockIdx.x % d.chunks, b = blockIdx.x / d.chunks / d.Hk, hk = blockIdx.x / d.chunks % d.Hk;
+  const int t0 = c * kChunk, rows = min(kChunk, d.T - t0);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, which = tid >> 6, tok = tid & 63;
+  const long long m = blockIdx.x;  // (batch * Hk + key head) * chunks + chunk
+  load_rows<I, DK>(Q, ld, plane, head_at<I>(a.q, b, t0, hk), a.q.st, rows, d.dk, d.wide);
+  load_rows<I, DK>(K, ld, plane, head_at<I>(a.k, b, t0, hk), a.k.st, rows, d.dk, d.wide);
   copies_done();
   __syncthreads();
-  if (warp == 0) {  // sums of log-decays in 64 bits, kept as two floats
-    const double x = logs[2 * lane], y = logs[2 * lane + 1];
-    double sum = x + y;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double up = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += up;
-    }
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const double v = k ? sum : sum - y;
-      const float hi = (float)v;
-      const float2 g = make_float2(hi, (float)(v - hi));
-      G[2 * lane + k] = g;
-      a.keep.total[at.n * kChunk + 2 * lane + k] = g;
-    }
-  }
   {  // lengths: a row of k or q to each thread
-    const bf16* x = (tid < kChunk ? K : Q) + (tid & 63) * ld;
+    const bf16* x = (which ? Q : K) + tok * ld;
     float sq[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < DK; i += 8) {
@@ -195,9 +163,18 @@ __global__ void __launch_bounds__(128) prepare_kernel(const DeltaFwd a) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) sq[k & 1] = fmaf(f[k], f[k], sq[k & 1]);
     }
-    const float len = rsqrtf(sq[0] + sq[1] + 1e-6f);
-    if (tid < kChunk) rk[tid] = len;
-    else rq[tid - kChunk] = len * d.scale;
+    const float len = rsqrtf(sq[0] + sq[1] + 1e-6f) * (which ? d.scale : 1.f);
+    (which ? rq : rk)[tok] = len;
+    (which ? a.keep.rq : a.keep.rk)[m * kChunk + tok] = len;
+  }
+  // The rows as tiles, for the other kernels.
+  constexpr int kV = DK / 8;
+#pragma unroll 4
+  for (int i = tid; i < 2 * kParts<I> * kChunk * kV; i += 128) {
+    const int of_k = i / (kParts<I> * kChunk * kV), part = i / (kChunk * kV) % kParts<I>, r = i / kV % kChunk, p = i % kV;
+    unsigned char* to = (of_k ? a.keep.keys : a.keep.queries) + (m * kParts<I> + part) * (DK / 64) * kTok;
+    *reinterpret_cast<uint4*>(to + (p >> 3) * kTok + piece_at(r, p & 7)) =
+        *reinterpret_cast<const uint4*>((of_k ? K : Q) + part * plane + r * ld + p * 8);
   }
   float kk[8][4], qk[8][4];
 #pragma unroll
@@ -207,98 +184,138 @@ __global__ void __launch_bounds__(128) prepare_kernel(const DeltaFwd a) {
   const Tile tk{K, ld, plane}, tq{Q, ld, plane};
   product<4, DK, false, true, kParts<I>, kParts<I>>(kk, tk, warp * 16, tk, 0, warp + 1);
   product<4, DK, false, true, kParts<I>, kParts<I>>(qk, tq, warp * 16, tk, 0, warp + 1);
-  __syncthreads();
-  if (at.h % group == 0) {  // the rows as tiles, for the other kernels
-    if (tid < kChunk) {
-      a.keep.rk[m * kChunk + tid] = rk[tid];
-      a.keep.rq[m * kChunk + tid] = rq[tid];
-    }
-    constexpr int kV = DK / 8;
-    for (int i = tid; i < 2 * kParts<I> * kChunk * kV; i += 128) {
-      const int which = i / (kParts<I> * kChunk * kV), part = i / (kChunk * kV) % kParts<I>, r = i / kV % kChunk, c = i % kV;
-      unsigned char* to = (which ? a.keep.keys : a.keep.queries) + (m * kParts<I> + part) * (DK / 64) * kTok;
-      *reinterpret_cast<uint4*>(to + (c >> 3) * kTok + piece_at(r, c & 7)) =
-          *reinterpret_cast<const uint4*>((which ? K : Q) + part * plane + r * ld + c * 8);
-    }
-  }
-  unsigned char* P = a.keep.attend + at.n * 2 * kTok;
-#pragma unroll
-  for (int n = 0; n < 8; ++n)
-#pragma unroll
-    for (int e = 0; e < 4; e += 2) {
-      const int i = warp * 16 + (lane >> 2) + (e ? 8 : 0), j = n * 8 + (lane & 3) * 2;
-      float p[2], l[2];
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const float w = j + x <= i ? decay_between(G[i], G[j + x]) * rk[j + x] : 0.f;
-        p[x] = j + x <= i ? qk[n][e + x] * rq[i] * w : 0.f;
-        l[x] = j + x < i ? kk[n][e + x] * rk[i] * w * beta[j + x] : 0.f;
+  for (int g0 = 0; g0 < group; g0 += 2) {
+    const int pair = min(2, group - g0);
+    const long long n0 = ((long long)b * d.H + hk * group + g0) * d.chunks + c;  // the next value head is `chunks` further
+    if (which < pair) {
+      const int h = hk * group + g0 + which;
+      float g = 0.f, w = 0.f;
+      if (tok < rows) {
+        g = gate_of(ElemOf<I>::up(*head_at<I>(a.g.a, b, t0 + tok, h)), load_any(a.g.a_log, a.g.a_log_type, h),
+                    load_any(a.g.dt_bias, a.g.dt_bias_type, h)).log_decay;
+        w = sigmoid(ElemOf<I>::up(*head_at<I>(a.g.b, b, t0 + tok, h)));
       }
-      uint32_t hi, lo;
-      halves(p[0], p[1], hi, lo);
-      *reinterpret_cast<uint32_t*>(P + element_at(i, j, 0)) = hi;
-      *reinterpret_cast<uint32_t*>(P + kTok + element_at(i, j, 0)) = lo;
-      *reinterpret_cast<float2*>(A + i * ldA + j) = make_float2(l[0], l[1]);
+      logs[which][tok] = g;
+      beta[which][tok] = w;
+      a.keep.beta[(n0 + which * d.chunks) * kChunk + tok] = w;
     }
-  __syncthreads();
-  float x[32];
-  const int block = (tid >> 5) * 32, col = tid & 31;
-  if (tid < kChunk) {  // x_i = [i = column] - sum_{m < i} A_im x_m
-    const float* B = A + block * ldA + block;
+    __syncthreads();  // q and k are read, too
+    if (warp < pair) {  // sums of log-decays in 64 bits, kept as two floats
+      const double x = logs[warp][2 * lane], y = logs[warp][2 * lane + 1];
+      double sum = x + y;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      float s[4] = {i == col ? 1.f : 0.f, 0.f, 0.f, 0.f};
+      for (int o = 1; o < 32; o <<= 1) {
+        const double up = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += up;
+      }
 #pragma unroll
-      for (int k = 0; k < i; ++k) s[k & 3] = fmaf(-B[i * ldA + k], x[k], s[k & 3]);
-      x[i] = (s[0] + s[1]) + (s[2] + s[3]);
+      for (int k = 0; k < 2; ++k) {
+        const double v = k ? sum : sum - y;
+        const float hi = (float)v;
+        const float2 g = make_float2(hi, (float)(v - hi));
+        G[warp][2 * lane + k] = g;
+        a.keep.total[(n0 + warp * d.chunks) * kChunk + 2 * lane + k] = g;
+      }
     }
-    __syncwarp();  // the block belongs to this warp
+    __syncthreads();
+    for (int e2 = 0; e2 < pair; ++e2) {
+      unsigned char* P = a.keep.attend + (n0 + e2 * d.chunks) * 2 * kTok;
+      float* A = reinterpret_cast<float*>(raw) + e2 * kChunk * ldA;  // L diag(beta), then the inverse
 #pragma unroll
-    for (int i = 0; i < 32; ++i) A[(block + i) * ldA + block + col] = x[i];
-  }
-  __syncthreads();
-  const int row = tid >> 2, c8 = (tid & 3) * 8;
-  const auto rows_times = [&](const float* X, const float* Y, int ldY, float (&s)[8]) {  // (row of X) Y, 32 terms
+      for (int e = 0; e < 4; e += 2) {
+        const int i = warp * 16 + (lane >> 2) + (e ? 8 : 0);
+        const float2 Gi = G[e2][i];
+        const float qi = rq[i], ki = rk[i];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) s[k] = 0.f;
-#pragma unroll 8
-    for (int k = 0; k < 32; ++k) {
-      const float f = X[row * ldA + k];
-      const float4 y0 = *reinterpret_cast<const float4*>(Y + k * ldY + c8), y1 = *reinterpret_cast<const float4*>(Y + k * ldY + c8 + 4);
-      s[0] = fmaf(f, y0.x, s[0]);
-      s[1] = fmaf(f, y0.y, s[1]);
-      s[2] = fmaf(f, y0.z, s[2]);
-      s[3] = fmaf(f, y0.w, s[3]);
-      s[4] = fmaf(f, y1.x, s[4]);
-      s[5] = fmaf(f, y1.y, s[5]);
-      s[6] = fmaf(f, y1.z, s[6]);
-      s[7] = fmaf(f, y1.w, s[7]);
+        for (int n = 0; n < 8; ++n) {
+          const int j = n * 8 + (lane & 3) * 2;
+          uint32_t hi = 0, lo = 0;
+          float2 l = make_float2(0.f, 0.f);
+          if (n < 2 * (warp + 1)) {  // else above the diagonal
+            const float w0 = decay_between(Gi, G[e2][j]) * rk[j], w1 = decay_between(Gi, G[e2][j + 1]) * rk[j + 1];
+            const float p0 = qk[n][e] * qi * w0, p1 = qk[n][e + 1] * qi * w1;
+            const float l0 = kk[n][e] * ki * w0 * beta[e2][j], l1 = kk[n][e + 1] * ki * w1 * beta[e2][j + 1];
+            halves(j <= i ? p0 : 0.f, j + 1 <= i ? p1 : 0.f, hi, lo);
+            l = make_float2(j < i ? l0 : 0.f, j + 1 < i ? l1 : 0.f);
+          }
+          *reinterpret_cast<uint32_t*>(P + element_at(i, j, 0)) = hi;
+          *reinterpret_cast<uint32_t*>(P + kTok + element_at(i, j, 0)) = lo;
+          *reinterpret_cast<float2*>(A + i * ldA + j) = l;
+        }
+      }
     }
-  };
-  float s[8];
-  rows_times(A + 32 * ldA, A, ldA, s);
-  *reinterpret_cast<float4*>(U + row * ldU + c8) = make_float4(s[0], s[1], s[2], s[3]);
-  *reinterpret_cast<float4*>(U + row * ldU + c8 + 4) = make_float4(s[4], s[5], s[6], s[7]);
-  __syncthreads();
-  rows_times(A + 32 * ldA + 32, U, ldU, s);
-  *reinterpret_cast<float4*>(A + (32 + row) * ldA + c8) = make_float4(-s[0], -s[1], -s[2], -s[3]);
-  *reinterpret_cast<float4*>(A + (32 + row) * ldA + c8 + 4) = make_float4(-s[4], -s[5], -s[6], -s[7]);
-  __syncthreads();
-  unsigned char* T = a.keep.solve + at.n * 2 * kTok;
-  for (int i = tid; i < kChunk * 8; i += 128) {
-    const int r = i >> 3, p = i & 7;
-    float f[8];
+    __syncthreads();
+    const int mine = warp >> 1;  // two warps to a head
+    float* A = reinterpret_cast<float*>(raw) + mine * kChunk * ldA;
+    float* U = reinterpret_cast<float*>(raw + Mem::kFirst) + mine * 32 * ldU;  // A21 T11
+    const int block = (warp & 1) * 32;
+    if (mine < pair) {  // x_i = [i = column] - sum_{m < i} A_im x_m
+      const float* B = A + block * ldA + block;
+      float x[32];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = p * 8 + k <= r ? A[r * ldA + p * 8 + k] : 0.f;
-    put8(T + piece_at(r, p), T + kTok + piece_at(r, p), f);
+      for (int i = 0; i < 32; ++i) {
+        float s[4] = {i == lane ? 1.f : 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < i; ++k) s[k & 3] = fmaf(-B[i * ldA + k], x[k], s[k & 3]);
+        x[i] = (s[0] + s[1]) + (s[2] + s[3]);
+      }
+      __syncwarp();  // the block belongs to this warp
+#pragma unroll
+      for (int i = 0; i < 32; ++i) A[(block + i) * ldA + block + lane] = x[i];
+    }
+    __syncthreads();
+    const int row = (warp & 1) * 16 + (lane >> 1), c16 = (lane & 1) * 16;
+    const auto rows_times = [&](const float* X, const float* Y, int ldY, float (&s)[16]) {  // (row of X) Y, 32 terms
+#pragma unroll
+      for (int k = 0; k < 16; ++k) s[k] = 0.f;
+#pragma unroll 4
+      for (int k = 0; k < 32; ++k) {
+        const float f = X[row * ldA + k];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float4 y = *reinterpret_cast<const float4*>(Y + k * ldY + c16 + 4 * e);
+          s[4 * e] = fmaf(f, y.x, s[4 * e]);
+          s[4 * e + 1] = fmaf(f, y.y, s[4 * e + 1]);
+          s[4 * e + 2] = fmaf(f, y.z, s[4 * e + 2]);
+          s[4 * e + 3] = fmaf(f, y.w, s[4 * e + 3]);
+        }
+      }
+    };
+    float s[16];
+    if (mine < pair) {
+      rows_times(A + 32 * ldA, A, ldA, s);
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(U + row * ldU + c16 + e) = make_float4(s[e], s[e + 1], s[e + 2], s[e + 3]);
+    }
+    __syncthreads();
+    if (mine < pair) {
+      rows_times(A + 32 * ldA + 32, U, ldU, s);
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        *reinterpret_cast<float4*>(A + (32 + row) * ldA + c16 + e) = make_float4(-s[e], -s[e + 1], -s[e + 2], -s[e + 3]);
+    }
+    __syncthreads();
+    if (which < pair) {
+      unsigned char* T = a.keep.solve + (n0 + which * d.chunks) * 2 * kTok;
+      const float* X = reinterpret_cast<const float*>(raw) + which * kChunk * ldA;
+#pragma unroll 4
+      for (int i = tok; i < kChunk * 8; i += 64) {
+        const int r = i >> 3, p = i & 7;
+        float f[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] = p * 8 + k <= r ? X[r * ldA + p * 8 + k] : 0.f;
+        put8(T + piece_at(r, p), T + kTok + piece_at(r, p), f);
+      }
+    }
+    __syncthreads();
   }
 }
 
 template <typename I, int DK>
 void prepare(const DeltaFwd& a, cudaStream_t s) {
-  const size_t bytes = 2 * kParts<I> * sizeof(bf16) * kChunk * (DK + kPad) + sizeof(float) * (kChunk * (kChunk + 4) + 32 * 36);
-  cudaFuncSetAttribute(prepare_kernel<I, DK>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  prepare_kernel<I, DK><<<(unsigned)(a.d.B * a.d.H) * a.d.chunks, 128, bytes, s>>>(a);
+  constexpr int bytes = PrepareMem<I, DK>::kBytes;
+  cudaFuncSetAttribute(prepare_kernel<I, DK>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  prepare_kernel<I, DK><<<(unsigned)(a.d.B * a.d.Hk) * a.d.chunks, 128, bytes, s>>>(a);
 }
 
 }  // namespace
