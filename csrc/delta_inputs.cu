@@ -7,7 +7,7 @@
 //     K^T W, K^T W', Q^T W     W = dP D rq_i rk_j and dL D rk_i rk_j: q and k go in as given, their lengths in the small matrix
 // so that all scalings of tokens are by columns, in fp32, when the sums leave tensor memory.
 //
-// What bounds it: 300 KB to read for each chunk of 128 x 128, 64 of them S and 64 dS', which share their place.
+// What bounds it: 300 KB to read for each chunk of 128 x 128.
 #include <cooperative_groups.h>
 
 #include "delta_tiles.cuh"
@@ -20,15 +20,22 @@ namespace cg = cooperative_groups;
 template <typename I, int DK, int DV>
 struct InputsMem {
   static constexpr int kPanels = DK / 64, kPanelS = DV * 128, kPlaneS = kPanels * kPanelS, kPlaneX = DV * 128, kPlaneK = kPanels * kTok;
-  // S, then dS'; V'; the stack: dO and dV, the high halves before the low ones (dO in bf16 has none)
-  static constexpr int S = 0, V = S + 2 * kPlaneS, O = V + 2 * kPlaneX, G = O + kPlaneX,
-                       Ol = G + kPlaneX, Gl = Ol + (kParts<I> == 2 ? kPlaneX : 0), Q = Gl + kPlaneX, K = Q + kParts<I> * kPlaneK,
-                       W = K + kParts<I> * kPlaneK, N = W + 2 * kTok, kTiles = N + 2 * kTok;
-  static constexpr int ldF = DK + 4, kRows = (2 * kChunk + kMostGroup) * ldF * 4;  // in the end, from S on: all heads' parts of the owned rows
+  // dS'; V'; S; the stack: dO and dV, the high halves before the low ones (dO in bf16 has none); q and k; the small matrices.
+  // The largest state takes all there is: q, k and the small matrices then come where S was.
+  static constexpr int kKeys = 2 * kParts<I> * kPlaneK, kSquares = 4 * kTok;
+  static constexpr int D = 0, V = D + 2 * kPlaneS, O = V + 2 * kPlaneX, G = O + kPlaneX, Ol = G + kPlaneX,
+                       Gl = Ol + (kParts<I> == 2 ? kPlaneX : 0), S = Gl + kPlaneX, kEnd = S + 2 * kPlaneS;
+  static constexpr bool kShared = kEnd + kKeys + kSquares > 220 * 1024;
+  static constexpr bool kAllShared = kShared && kKeys + kSquares <= 2 * kPlaneS;
+  static constexpr int Q = kShared ? S : kEnd, K = Q + kParts<I> * kPlaneK, W = kShared && !kAllShared ? kEnd : Q + kKeys, N = W + 2 * kTok,
+                       kTiles = kAllShared ? kEnd : N + 2 * kTok;
+  static_assert(!kShared || kKeys <= 2 * kPlaneS, "room where S was");
+  static constexpr int ldF = DK + 4, kRows = (2 * kChunk + kMostGroup) * ldF * 4;  // in the end, from the start on: all heads' parts of the owned rows
+  static_assert(kRows <= (kShared ? S : kEnd), "the rows of q and k stay");
   static constexpr int kBytes = kTiles > kRows ? kTiles : kRows;
 };
 
-enum InputsBar { kGotQK, kGotV, kGotS, kGotD, kMixDone, kReadS, kMixSet, kAllDone, kTaken, kInputsBars };
+enum InputsBar { kGotQK, kGotV, kGotS, kGotD, kMixDone, kReadS, kReadD, kMixSet, kAllDone, kTaken, kInputsBars };
 
 struct InputsShared {
   uint64_t bar[kInputsBars];
@@ -94,17 +101,26 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
     bulk_load(mem + Mem::Gl, a.dreads + at * 2 * Mem::kPlaneX + Mem::kPlaneX, Mem::kPlaneX, &sh.bar[kGotV]);
     mbar_arrive_expect_tx(&sh.bar[kGotS], 2 * Mem::kPlaneS);
     bulk_load(mem + Mem::S, state_at(c, s), 2 * Mem::kPlaneS, &sh.bar[kGotS]);
-    bulk_prefetch(a.dstates + at * 2 * Mem::kPlaneS, 2 * Mem::kPlaneS);
+    mbar_arrive_expect_tx(&sh.bar[kGotD], 2 * Mem::kPlaneS);
+    bulk_load(mem + Mem::D, a.dstates + at * 2 * Mem::kPlaneS, 2 * Mem::kPlaneS, &sh.bar[kGotD]);
     bulk_prefetch(state_at(c + 1, s), 2 * Mem::kPlaneS);
+  };
+  const auto load_keys = [&] {
+    mbar_arrive_expect_tx(&sh.bar[kGotQK], 2 * P * Mem::kPlaneK);
+    bulk_load(mem + Mem::Q, a.keep.queries + m * P * Mem::kPlaneK, P * Mem::kPlaneK, &sh.bar[kGotQK]);
+    bulk_load(mem + Mem::K, a.keep.keys + m * P * Mem::kPlaneK, P * Mem::kPlaneK, &sh.bar[kGotQK]);
   };
   if (tid == kWorkers) {
     for (int i = 0; i < kInputsBars; ++i) mbar_init(&sh.bar[i], i == kMixSet || i == kTaken ? kWorkers : 1);
     fence_barrier_init();
     fence_proxy_async_smem();
     load_slice(0);
-    mbar_arrive_expect_tx(&sh.bar[kGotQK], 2 * P * Mem::kPlaneK);
-    bulk_load(mem + Mem::Q, a.keep.queries + m * P * Mem::kPlaneK, P * Mem::kPlaneK, &sh.bar[kGotQK]);
-    bulk_load(mem + Mem::K, a.keep.keys + m * P * Mem::kPlaneK, P * Mem::kPlaneK, &sh.bar[kGotQK]);
+    if (Mem::kShared) {
+      bulk_prefetch(a.keep.queries + m * P * Mem::kPlaneK, P * Mem::kPlaneK);
+      bulk_prefetch(a.keep.keys + m * P * Mem::kPlaneK, P * Mem::kPlaneK);
+    } else {
+      load_keys();
+    }
   }
   __syncwarp();
   if (warp == kControl) tmem_alloc(&sh.tmem, 512);
@@ -131,7 +147,8 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
       // The stack of high halves, and that of low ones; without a low half of dO the first 64 lanes of its product are not used.
       const Operand high{base + Mem::O, Mem::G - Mem::O}, low{base + (P == 2 ? Mem::Ol : Mem::O), Mem::Gl - (P == 2 ? Mem::Ol : Mem::O)},
           low_g{base + Mem::Gl, Mem::kPlaneX}, V{base + Mem::V, Mem::kPlaneX},
-          S{base + Mem::S, Mem::kPanelS}, Sl{base + Mem::S + Mem::kPlaneS, Mem::kPanelS};
+          S{base + Mem::S, Mem::kPanelS}, Sl{base + Mem::S + Mem::kPlaneS, Mem::kPanelS}, D{base + Mem::D, Mem::kPanelS},
+          Dl{base + Mem::D + Mem::kPlaneS, Mem::kPanelS};
       for (int s = 0; s < slices; ++s) {
         const bool more = s > 0;
         if (!wait(&sh.bar[kGotV], s)) break;
@@ -144,15 +161,16 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
         if (P == 2) multiply<kVs, 128, true, true>(tm + cS, S, low, true);
         else multiply<kVs, 64, true, true>(tm + cS + 64, S, low_g, true);
         tc_commit(&sh.bar[kReadS]);
-        if (!wait(&sh.bar[kReadS], 2 * s)) break;
-        mbar_arrive_expect_tx(&sh.bar[kGotD], 2 * Mem::kPlaneS);
-        bulk_load(mem + Mem::S, a.dstates + (n * slices + s) * 2 * Mem::kPlaneS, 2 * Mem::kPlaneS, &sh.bar[kGotD]);
         if (!wait(&sh.bar[kGotD], s)) break;
-        multiply<kVs, 128, true, true>(tm + cD, S, V, more);
-        multiply<kVs, 64, true, true>(tm + cD, Sl, V, true);
-        tc_commit(&sh.bar[kReadS]);
+        multiply<kVs, 128, true, true>(tm + cD, D, V, more);
+        multiply<kVs, 64, true, true>(tm + cD, Dl, V, true);
+        if (Mem::kShared && s == slices - 1) {
+          if (!wait(&sh.bar[kReadS], s)) break;
+          load_keys();
+        }
         if (s + 1 < slices) {  // the places are free once they are read, by the products and by the workers
-          if (!wait(&sh.bar[kReadS], 2 * s + 1) || !wait(&sh.bar[kTaken], s)) break;
+          tc_commit(&sh.bar[kReadD]);
+          if (!wait(&sh.bar[kReadS], s) || !wait(&sh.bar[kReadD], s) || !wait(&sh.bar[kTaken], s)) break;
           load_slice(s + 1);
         }
       }
@@ -197,6 +215,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
         const float2 Gi = sh.G[i];
         const int last = of_l ? i : i + 1;
         unsigned char* to = mem + (of_l ? Mem::N : Mem::W);
+        if (Mem::kAllShared && !wait(&sh.bar[kReadS], s)) break;
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
           float x[8];
@@ -252,7 +271,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
       if (!wait(&sh.bar[kGotD], s)) break;
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
-        const unsigned char* at = mem + Mem::S + (i * kWorkers + tid) * 16;
+        const unsigned char* at = mem + Mem::D + (i * kWorkers + tid) * 16;
         const uint4 dh = *reinterpret_cast<const uint4*>(at), dl = *reinterpret_cast<const uint4*>(at + Mem::kPlaneS);
         const uint32_t u[4] = {ah[i].x, ah[i].y, ah[i].z, ah[i].w}, v4[4] = {al[i].x, al[i].y, al[i].z, al[i].w},
                        y[4] = {dh.x, dh.y, dh.z, dh.w}, z[4] = {dl.x, dl.y, dl.z, dl.w};
