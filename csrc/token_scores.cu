@@ -9,11 +9,13 @@
 // one fused multiply-add more than that of a softmax.
 //
 // Alternatives. In the pass each thread only keeps the maximum of its own elements (packed maxima, which the running
-// maximum needs anyway). The K-th largest of these maxima is a lower bound of the K-th largest logit, so that the K
-// best lie within the elements of the threads that reach it: K threads of the row's, plus ties. A search over the bits of
-// the maxima finds the bound; all threads read those elements again, from the L2 for the most part, and note the ones
-// that reach it, hardly more than K; each of those is ranked by counting the larger ones. Where ties make them more than
-// kNoted, one warp takes them into a sorted list with an entry for each lane instead.
+// maximum needs anyway), the step that it came in, and the maximum of its other steps. The K-th largest of the threads'
+// maxima is a lower bound of the K-th largest logit, so that the K best lie within the elements of the threads that
+// reach it: K threads of the row's, plus ties, and of each the one step unless another step reaches it too. A search over the
+// bits of the maxima finds the bound; all threads read those steps again (some 2 % of a row; all steps of the K threads were
+// 35 % more bytes from memory) and note the elements that reach it, hardly more than K; each of those is ranked by counting the
+// larger ones. Where ties make steps or elements more than is noted, all elements of the threads are read, and one warp
+// takes them into a sorted list with an entry for each lane.
 //
 // A row whose label is ignored is not read. A NaN in a row makes its numbers NaN; among the alternatives it is the
 // largest.
@@ -147,14 +149,15 @@ __device__ __forceinline__ void insert(unsigned long long key, int K, unsigned l
   }
 }
 
-constexpr int kNoted = 96;  // elements of a row that reach the bound, for the quick way
+constexpr int kNoted = 96, kSteps = 256;  // elements of a row that reach the bound, and steps that have them, for the quick way
 
 template <int kGroup>
 struct ScoreShared {
   static constexpr int kWarps = kGroup / 32;
   Sums parts[kWarps];
   int owners[kGroup];  // the threads whose maxima reach the bound
-  int count[2];        // of the owners, of the elements noted
+  int steps[kSteps];   // their steps that do: thread + step * kGroup
+  int count[3];        // of the owners, of the elements noted, of the steps
   unsigned long long noted[kNoted];
 };
 
@@ -169,15 +172,30 @@ __device__ __forceinline__ int group_count(bool x) {
   return kGroup > 32 ? __syncthreads_count(x) : __popc(__ballot_sync(0xffffffffu, x));
 }
 
-// The row's alternatives. `mine`: the maximum of the calling thread's vectors (tid, tid + kGroup, ...).
+// The maximum of a thread's elements, the step it came in, and the maximum of its other steps.
+struct Best {
+  float most = -INFINITY, other = -INFINITY;
+  int step = 0;
+  __device__ __forceinline__ void take(float top, int at) {
+    if (top > most) {
+      other = most;
+      most = top;
+      step = at;
+    } else {
+      other = fmaxf(other, top);
+    }
+  }
+};
+
+// The row's alternatives. `mine`: of the calling thread's vectors (tid, tid + kGroup, ...), kUnroll of them a step.
 template <typename T, int kGroup>
-__device__ __forceinline__ void alternatives(const ScoreArgs& a, const RowSpan<T>& span, long long row, float mine, bool has_nan,
+__device__ __forceinline__ void alternatives(const ScoreArgs& a, const RowSpan<T>& span, long long row, const Best& mine, bool has_nan,
                                              float base, float log2_s, ScoreShared<kGroup>& sh) {
   constexpr int N = kVecOf<T>;
   const int tid = Place<kGroup>::tid(), lane = threadIdx.x & 31, K = a.top;
   // The largest number with 16 significant bits that K maxima reach, bit by bit. Small rows and rows with a NaN, which the
   // maxima pass over, are looked at whole.
-  const uint32_t key = (uint32_t)(key_of(mine, 0) >> 32);
+  const uint32_t key = (uint32_t)(key_of(mine.most, 0) >> 32);
   uint32_t bound = 0;
   if (!has_nan) {
 #pragma unroll 1
@@ -185,13 +203,21 @@ __device__ __forceinline__ void alternatives(const ScoreArgs& a, const RowSpan<T
       if (group_count<kGroup>(key >= (bound | bit)) >= K) bound |= bit;
   }
   const bool owner = has_nan || key >= bound;
-  if (tid < 2) sh.count[tid] = 0;
+  if (tid < 3) sh.count[tid] = 0;
   group_sync<kGroup>();
-  if (owner) sh.owners[atomicAdd(&sh.count[0], 1)] = tid;
+  constexpr int kHold = kGroup * kUnroll;
+  const int all_steps = (span.nv + kHold - 1) / kHold;
+  if (owner) {
+    sh.owners[atomicAdd(&sh.count[0], 1)] = tid;
+    const bool more = has_nan || (uint32_t)(key_of(mine.other, 0) >> 32) >= bound;
+    const int n = more ? all_steps : 1, at = atomicAdd(&sh.count[2], n);
+    for (int i = 0; i < n && at + i < kSteps; ++i) sh.steps[at + i] = tid + (more ? i : mine.step) * kGroup;
+  }
   group_sync<kGroup>();
-  const int owners = sh.count[0], per = (span.nv + kGroup - 1) / kGroup;
-  for (int u = tid; u < owners * per; u += kGroup) {
-    const int j = sh.owners[u / per] + u % per * kGroup, lo = span.first(j);
+  const bool few = sh.count[2] <= kSteps;
+  const int owners = sh.count[0], per = all_steps * kUnroll;
+  for (int u = tid; few && u < sh.count[2] * kUnroll; u += kGroup) {
+    const int unit = sh.steps[u / kUnroll], j = unit % kGroup + unit / kGroup * kHold + u % kUnroll * kGroup, lo = span.first(j);
     if (j >= span.nv) continue;
     float f[N];
     raw_up<T>(span.template load<false>(j), f);
@@ -206,7 +232,7 @@ __device__ __forceinline__ void alternatives(const ScoreArgs& a, const RowSpan<T
   }
   group_sync<kGroup>();
   const int found = sh.count[1];
-  if (found <= kNoted) {
+  if (few && found <= kNoted) {
     for (int i = tid; i < found; i += kGroup) {
       const unsigned long long x = sh.noted[i];
       int rank = 0;
@@ -237,7 +263,7 @@ __device__ __forceinline__ void alternatives(const ScoreArgs& a, const RowSpan<T
 }
 
 template <typename T, int kGroup, bool kTop>
-__global__ void __launch_bounds__(Place<kGroup>::kThreads, kGroup == 32 ? 10 : 6) scores_kernel(ScoreArgs a) {
+__global__ void __launch_bounds__(Place<kGroup>::kThreads, kGroup == 32 ? 10 : 1536 / kGroup) scores_kernel(ScoreArgs a) {
   __shared__ ScoreShared<kGroup> shared[kTop ? Place<kGroup>::kRows : 1];
   constexpr int kW = kGroup / 32, kHold = kGroup * kUnroll;
   const LogitRows& r = a.rows;
@@ -263,12 +289,14 @@ __global__ void __launch_bounds__(Place<kGroup>::kThreads, kGroup == 32 ? 10 : 6
   const RowSpan<T> span(x, r.V);
   const float c = kLog2e * r.inv_temp, reach = 250.f / c;
   Sums sum{-INFINITY, 0.f, 0.f};
+  Best mine;
   for (int j = tid; j < span.nv; j += kHold) {
     uint4 v[kUnroll];
     fetch<T, kGroup, false>(span, j, span.inner(j - tid, kHold), v);
-    take_scores<T>(v, c, reach, max_of<T>(v), sum);
+    const float top = max_of<T>(v);
+    take_scores<T>(v, c, reach, top, sum);
+    if constexpr (kTop) mine.take(top, j / kHold);
   }
-  const float mine = sum.m;
   merge_lanes(sum, c);
   if constexpr (kW > 1) {
     const int lane = threadIdx.x & 31;
