@@ -83,6 +83,7 @@ struct DeltaStep {
   float* state;  // (B, H, dk, dv)
   long long ssb, ssh;
   void* out;  // (B, T, H, dv)
+  int* err;
 };
 
 void delta_prepare(const DeltaFwd& a, cudaStream_t s);

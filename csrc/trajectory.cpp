@@ -434,7 +434,7 @@ std::pair<Tensor, OptTensor> gated_delta_rule(Tensor q, Tensor k, Tensor v, Tens
 }
 
 Tensor gated_delta_step(Tensor q, Tensor k, Tensor v, Tensor a, Tensor b, Tensor a_log, Tensor dt_bias, Tensor state,
-                        std::optional<double> scale) {
+                        std::optional<double> scale, Tensor err) {
   DeltaIn x{q, k, v, a, b, a_log, dt_bias};
   const double by = take_delta(x, scale);
   elem_of(x.q, "q, k, v, a and b");
@@ -459,6 +459,8 @@ Tensor gated_delta_step(Tensor q, Tensor k, Tensor v, Tensor a, Tensor b, Tensor
   s.ssb = state.stride(0);
   s.ssh = state.stride(1);
   s.out = out.data_ptr();
+  check_like(err, "err", torch::kInt32, x.q);
+  s.err = err.data_ptr<int>();
   bw::delta_step(s, at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   ++launches;

@@ -131,7 +131,7 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, a: torch
     launch that reads and writes the state once whatever the number of tokens.
     """
     if use_native(q):
-        return native().gated_delta_step(q, k, v, a, b, a_log, dt_bias, state, scale)
+        return native().gated_delta_step(q, k, v, a, b, a_log, dt_bias, state, scale, error_word(q.device))
     scale = _check(q, k, v, a, b, a_log, dt_bias, scale)
     _check_state("state", state, q, v)
     if torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, v, a, b, a_log, dt_bias, state)):

@@ -217,6 +217,22 @@ def test_token_by_token(device, dtype, shape):
         close("state", state, want_last, torch.float32, 2.0 ** -18)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape", [(40, 1, 4, 8, 128, 128), (100, 3, 1, 3, 72, 40), (37, 2, 8, 16, 32, 104), (75, 1, 2, 4, 128, 136)])
+def test_token_by_token_of_many_sequences(dtype, shape):
+    """More heads than two for each SM; the state's heads further apart than they are large."""
+    x, state = make(*shape, dtype, "cuda", state=True, layout="odd")
+    b, h = state.shape[:2]
+    held = torch.full((b, h + 1, *state.shape[2:]), 7.0, device="cuda")
+    held[:, :h] = state
+    want, want_last = recurrence({n: y.double() for n, y in x.items()}, state.double())
+    out = ops.gated_delta_step(*(x[n] for n in NAMES), held[:, :h])
+    close("out", out, want.cpu(), dtype, 2.0 ** -18)
+    close("state", held[:, :h], want_last.cpu(), torch.float32, 2.0 ** -18)
+    assert (held[:, h:] == 7).all()
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_prefill_then_decode(device):
     """A prompt in chunks and new tokens one at a time give what the whole sequence gives; the state may be a slice."""
