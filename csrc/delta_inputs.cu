@@ -25,9 +25,11 @@ struct InputsMem {
   static constexpr int kKeys = 2 * kParts<I> * kPlaneK, kSquares = 4 * kTok;
   static constexpr int D = 0, V = D + 2 * kPlaneS, O = V + 2 * kPlaneX, G = O + kPlaneX, Ol = G + kPlaneX,
                        Gl = Ol + (kParts<I> == 2 ? kPlaneX : 0), S = Gl + kPlaneX, kEnd = S + 2 * kPlaneS;
+  // Panels of q and of k take turns, so that their rows are one operand's 128; parts are kPart apart.
+  static constexpr int kPanelK = 2 * kTok, kPart = kPanels * kPanelK;
   static constexpr bool kShared = kEnd + kKeys + kSquares > 220 * 1024;
   static constexpr bool kAllShared = kShared && kKeys + kSquares <= 2 * kPlaneS;
-  static constexpr int Q = kShared ? S : kEnd, K = Q + kParts<I> * kPlaneK, W = kShared && !kAllShared ? kEnd : Q + kKeys, N = W + 2 * kTok,
+  static constexpr int Q = kShared ? S : kEnd, K = Q + kTok, W = kShared && !kAllShared ? kEnd : Q + kKeys, N = W + 2 * kTok,
                        kTiles = kAllShared ? kEnd : N + 2 * kTok;
   static_assert(!kShared || kKeys <= 2 * kPlaneS, "room where S was");
   static constexpr int ldF = DK + 4, kRows = (2 * kChunk + kMostGroup) * ldF * 4;  // in the end, from the start on: all heads' parts of the owned rows
@@ -35,34 +37,26 @@ struct InputsMem {
   static constexpr int kBytes = kTiles > kRows ? kTiles : kRows;
 };
 
-enum InputsBar { kGotQK, kGotV, kGotS, kGotD, kMixDone, kReadS, kReadD, kMixSet, kAllDone, kTaken, kInputsBars };
+enum InputsBar { kGotQK, kGotV, kGotS, kGotD, kMixDone, kReadS, kReadD, kMixSet, kGramDone, kGramRead, kAllDone, kTaken, kInputsBars };
 
 struct InputsShared {
   uint64_t bar[kInputsBars];
   uint32_t tmem;
   float2 G[kChunk];
   float rk[kChunk], rq[kChunk], beta[kChunk], left[kChunk], grown[kChunk];
-  float part[2][4][kChunk];  // V' . dV and v . dv, of each quarter of a slice
-  float qdots[4][kChunk];    // q . dq, of each quarter of a key head
-  float handed[kControl];
+  float written[4][kChunk];         // V' . dV, of each quarter of a slice
+  float read[4][kChunk];            // what S gives to a token, of each quarter of a key head
+  float left_over[4][kChunk];       // what a token gives to S'
+  float near[4][kChunk];            // what the tokens of t's sixteen before t give to t and those behind it: of half of P, of L each
+  float far[kChunk / 16][2 * kChunk];  // what each sixteen tokens give to a later one: P, L
+  float handed[kControl];           // S to S'
+
 };
 
-// Adds 32 values of each of 32 lanes over the lanes: lane l ends with the sum of value l.
-__device__ __forceinline__ float lanes_fold(float (&x)[32]) {
-#pragma unroll
-  for (int n = 16; n > 0; n >>= 1) {
-    const bool up = threadIdx.x & n;
-#pragma unroll
-    for (int i = 0; i < n; ++i) {
-      const float send = up ? x[i] : x[i + n], keep = up ? x[i + n] : x[i];
-      x[i] = keep + __shfl_xor_sync(0xffffffffu, send, n);
-    }
-  }
-  return x[0];
-}
-
-// Adds 16 values of each of 16 lanes (the other 16 hold the same): lane l ends with the sum of value l % 16.
+// Adds 16 values of each of 32 lanes over the lanes: lane l ends with the sum of value l % 16.
 __device__ __forceinline__ float lanes_fold16(float (&x)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] += __shfl_xor_sync(0xffffffffu, x[i], 16);
 #pragma unroll
   for (int n = 8; n > 0; n >>= 1) {
     const bool up = threadIdx.x & n;
@@ -103,15 +97,17 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
     bulk_load(mem + Mem::S, state_at(c, s), 2 * Mem::kPlaneS, &sh.bar[kGotS]);
     mbar_arrive_expect_tx(&sh.bar[kGotD], 2 * Mem::kPlaneS);
     bulk_load(mem + Mem::D, a.dstates + at * 2 * Mem::kPlaneS, 2 * Mem::kPlaneS, &sh.bar[kGotD]);
-    bulk_prefetch(state_at(c + 1, s), 2 * Mem::kPlaneS);
   };
   const auto load_keys = [&] {
     mbar_arrive_expect_tx(&sh.bar[kGotQK], 2 * P * Mem::kPlaneK);
-    bulk_load(mem + Mem::Q, a.keep.queries + m * P * Mem::kPlaneK, P * Mem::kPlaneK, &sh.bar[kGotQK]);
-    bulk_load(mem + Mem::K, a.keep.keys + m * P * Mem::kPlaneK, P * Mem::kPlaneK, &sh.bar[kGotQK]);
+#pragma unroll
+    for (int i = 0; i < P * Mem::kPanels; ++i) {
+      bulk_load(mem + Mem::Q + i * Mem::kPanelK, a.keep.queries + m * P * Mem::kPlaneK + i * kTok, kTok, &sh.bar[kGotQK]);
+      bulk_load(mem + Mem::K + i * Mem::kPanelK, a.keep.keys + m * P * Mem::kPlaneK + i * kTok, kTok, &sh.bar[kGotQK]);
+    }
   };
   if (tid == kWorkers) {
-    for (int i = 0; i < kInputsBars; ++i) mbar_init(&sh.bar[i], i == kMixSet || i == kTaken ? kWorkers : 1);
+    for (int i = 0; i < kInputsBars; ++i) mbar_init(&sh.bar[i], i == kMixSet || i == kGramRead || i == kTaken ? kWorkers : 1);
     fence_barrier_init();
     fence_proxy_async_smem();
     load_slice(0);
@@ -139,7 +135,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
   const uint32_t tm = sh.tmem;
   const Seat seat;
   // The last two come when the small matrices' products, in the same place, are read.
-  constexpr uint32_t cS = 0, cD = 128, cMix = 256, cLow = 384, cQ = 256, cK = 384;
+  constexpr uint32_t cS = 0, cD = 128, cMix = 256, cLow = 384, cGram = 448, cQ = 256, cK = 384;
   Waiter wait{a.err};
   if (warp == kControl) {
     if (lane == 0) {
@@ -174,28 +170,30 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
           load_slice(s + 1);
         }
       }
-      const Operand Q{base + Mem::Q, kTok}, K{base + Mem::K, kTok}, W{base + Mem::W, kTok}, N{base + Mem::N, kTok};
-      if (wait(&sh.bar[kGotQK], 0) && wait(&sh.bar[kMixSet], 0)) {
-        tc_fence_after();
-        multiply_wide<4, 128, true, false, P>(tm + cQ, K, Mem::kPlaneK, W, false);
-        multiply_wide<4, 128, true, true, P>(tm + cK, Q, Mem::kPlaneK, W, false);
-        multiply_wide<4, 128, true, false, P>(tm + cK, K, Mem::kPlaneK, N, true);
-        multiply_wide<4, 128, true, true, P>(tm + cK, K, Mem::kPlaneK, N, true);
-        tc_commit(&sh.bar[kAllDone]);
-        wait(&sh.bar[kAllDone], 0);
+      const Operand Q{base + Mem::Q, Mem::kPanelK}, K{base + Mem::K, Mem::kPanelK}, W{base + Mem::W, kTok}, N{base + Mem::N, kTok};
+      if (wait(&sh.bar[kGotQK], 0)) {
+        multiply_parts<DK / 16, 64, false, false, P, P>(tm + cGram, Q, Mem::kPart, K, Mem::kPart, false);  // [q | k] k^T
+        tc_commit(&sh.bar[kGramDone]);
+        if (wait(&sh.bar[kMixSet], 0)) {
+          tc_fence_after();
+          multiply_wide<4, 128, true, false, P>(tm + cQ, K, Mem::kPart, W, false);
+          if (wait(&sh.bar[kGramRead], 0)) {
+            tc_fence_after();
+            multiply_wide<4, 128, true, true, P>(tm + cK, Q, Mem::kPart, W, false);
+            multiply_wide<4, 128, true, false, P>(tm + cK, K, Mem::kPart, N, true);
+            multiply_wide<4, 128, true, true, P>(tm + cK, K, Mem::kPart, N, true);
+            tc_commit(&sh.bar[kAllDone]);
+            wait(&sh.bar[kAllDone], 0);
+          }
+        }
       }
     }
   } else {
     float handed = 0.f;
-    const bool of_v = seat.part >= 2;  // V' . dV is the first two quarters' part, v . dv the others'; each of half of the tokens
-    const int tt = (seat.part & 1) * 32;
+    const int tt = seat.part * 16;  // its tokens
+    float mix[16];
     for (int s = 0; s < slices; ++s) {
-      const int v0 = s * DV;
-      const bool in = seat.row < min(DV, d.dv - v0);
-      I v[32];
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = ElemOf<I>::down(0.f);
-      if (of_v && in) column_of(head_at<I>(a.v, b, t0 + tt, h) + v0 + seat.row, a.v.st, rows - tt, v);
+      const bool in = seat.row < min(DV, d.dv - s * DV);
       // The small matrices first, for the products that wait for them: row i of dP in lane i, of dL in lane 64 + i.
       if (s == slices - 1) {
         if (!wait(&sh.bar[kMixDone], 0)) break;
@@ -223,51 +221,63 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
           for (int k = 0; k < 8; ++k) {
             const int j = j0 + p * 8 + k;
             const float w = f[p * 8 + k] * by * (decay_between(Gi, sh.G[j]) * sh.rk[j]);
-            x[k] = j < last ? w : 0.f;
+            mix[p * 8 + k] = x[k] = j < last ? w : 0.f;
           }
           const int at = piece_at(i, seat.part * 2 + p);
           put8(to + at, to + kTok + at, x);
         }
         hand_over(&sh.bar[kMixSet]);
       }
-      // <dS', S'>: both tiles have their elements at the same places.
-      const uint4* after = reinterpret_cast<const uint4*>(state_at(c + 1, s));
+      // <dS', S>: both tiles have their elements at the same places. S may be gone from shared memory by then, but not from L2.
+      const uint4* before = reinterpret_cast<const uint4*>(state_at(c, s));
       constexpr int kPieces = Mem::kPlaneS / 16, kMine = kPieces / kWorkers;
       static_assert(kPieces % kWorkers == 0, "whole rounds");
       uint4 ah[kMine], al[kMine];
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
-        ah[i] = __ldcs(after + i * kWorkers + tid);
-        al[i] = __ldcs(after + kPieces + i * kWorkers + tid);
+        ah[i] = __ldcs(before + i * kWorkers + tid);
+        al[i] = __ldcs(before + kPieces + i * kWorkers + tid);
       }
       if (!wait(&sh.bar[kGotV], s)) break;
       // A lane holds an element of the values: the sums over them, of each token.
-      float x[32];
+      float x[16];
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
+      for (int p = 0; p < 2; ++p) {
         const int at = piece_at(in ? seat.row : 0, tt / 8 + p);
         const uint4 gh = *reinterpret_cast<const uint4*>(mem + Mem::G + at), gl = *reinterpret_cast<const uint4*>(mem + Mem::Gl + at);
-        const float2 g[4] = {pair_sum(gh.x, gl.x), pair_sum(gh.y, gl.y), pair_sum(gh.z, gl.z), pair_sum(gh.w, gl.w)};
-        float2 w[4];
-        if (of_v) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) w[k] = make_float2(ElemOf<I>::up(v[p * 8 + 2 * k]), ElemOf<I>::up(v[p * 8 + 2 * k + 1]));
-        } else {
-          const uint4 wh = *reinterpret_cast<const uint4*>(mem + Mem::V + at), wl = *reinterpret_cast<const uint4*>(mem + Mem::V + Mem::kPlaneX + at);
-          w[0] = pair_sum(wh.x, wl.x);
-          w[1] = pair_sum(wh.y, wl.y);
-          w[2] = pair_sum(wh.z, wl.z);
-          w[3] = pair_sum(wh.w, wl.w);
-        }
+        const uint4 wh = *reinterpret_cast<const uint4*>(mem + Mem::V + at), wl = *reinterpret_cast<const uint4*>(mem + Mem::V + Mem::kPlaneX + at);
+        const float2 g[4] = {pair_sum(gh.x, gl.x), pair_sum(gh.y, gl.y), pair_sum(gh.z, gl.z), pair_sum(gh.w, gl.w)},
+                     w[4] = {pair_sum(wh.x, wl.x), pair_sum(wh.y, wl.y), pair_sum(wh.z, wl.z), pair_sum(wh.w, wl.w)};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           x[p * 8 + 2 * k] = in ? w[k].x * g[k].x : 0.f;
           x[p * 8 + 2 * k + 1] = in ? w[k].y * g[k].y : 0.f;
         }
       }
-      const float sum = lanes_fold(x);
-      float* part = &sh.part[of_v][warp & 3][tt + lane];
-      *part = s ? *part + sum : sum;
+      const float sum = lanes_fold16(x);
+      if (lane < 16) {
+        float* to = &sh.written[warp & 3][tt + lane];
+        *to = s ? *to + sum : sum;
+      }
+      // What passes the gate of token t within the chunk: from the tokens of its sixteen before t here, from earlier sixteens by
+      // the sums of their columns.
+      if (s == slices - 1) {
+        if (!wait(&sh.bar[kGramDone], 0)) break;
+        tc_fence_after();
+        tmem_row(tm + seat.lanes + cGram + tt, x);
+        tc_fence_before();
+        mbar_arrive(&sh.bar[kGramRead]);
+        float run = 0.f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const float next = fmaf(mix[k], x[k], run);
+          x[k] = (seat.row & 63) >= tt + k ? run : 0.f;
+          run = next;
+        }
+        sh.far[seat.part][seat.row] = run;
+        const float near = lanes_fold16(x);
+        if (lane < 16) sh.near[warp & 3][tt + lane] = near;
+      }
       if (!wait(&sh.bar[kGotD], s)) break;
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
@@ -315,24 +325,30 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
 #pragma unroll
     for (int k = 0; k < 16; ++k) y[k] = fmaf(sh.rq[tt + k] * sh.grown[tt + k], x[k], y[k]);
     if (seat.row < DK) put(tt, y);
-    // q^ . dq^ = q . dq: over the lanes here, over the warps of a column later. The rows of q still lie as a tile.
+    // What S gives to a token and what a token gives to S': over the lanes here, over the warps of a column later. The rows of q
+    // and k still lie as tiles.
+    const auto element = [&](int tile, int i) {
+      const unsigned char* at = mem + tile + element_at(i, seat.row, Mem::kPanelK);
+      float v = __bfloat162float(*reinterpret_cast<const bf16*>(at));
+      if (P == 2) v += __bfloat162float(*reinterpret_cast<const bf16*>(at + Mem::kPart));
+      return seat.row < DK ? v : 0.f;
+    };
+    float g[16];
+    tmem_sum(tm + seat.lanes + cD + tt, tm + seat.lanes + cD + 64 + tt, z);
+    tmem_row(tm + seat.lanes + cS + 64 + tt, g);
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
-      float q = 0.f;
-      if (seat.row < DK) {
-        const unsigned char* at = mem + Mem::Q + element_at(tt + k, seat.row, kTok);
-        q = __bfloat162float(*reinterpret_cast<const bf16*>(at));
-        if (P == 2) q += __bfloat162float(*reinterpret_cast<const bf16*>(at + Mem::kPlaneK));
-      }
-      x[k] = seat.row < DK ? q * y[k] : 0.f;
-      x[k] += __shfl_xor_sync(0xffffffffu, x[k], 16);
+      const float key = element(Mem::K, tt + k), query = element(Mem::Q, tt + k), reads = -sh.rk[tt + k] * sh.grown[tt + k] * g[k],
+                  gives = sh.rk[tt + k] * sh.left[tt + k] * z[k];
+      x[k] = seat.row < DK ? fmaf(query, sh.rq[tt + k] * sh.grown[tt + k] * x[k], key * reads) : 0.f;
+      g[k] = seat.row < DK ? key * gives : 0.f;
+      z[k] = reads + gives;
     }
-    const float dot = lanes_fold16(x);
-    if (lane < 16) sh.qdots[warp & 3][tt + lane] = dot;
-    tmem_sum(tm + seat.lanes + cD + tt, tm + seat.lanes + cD + 64 + tt, z);
-    tmem_row(tm + seat.lanes + cS + 64 + tt, x);
-#pragma unroll
-    for (int k = 0; k < 16; ++k) z[k] = sh.rk[tt + k] * fmaf(sh.left[tt + k], z[k], -sh.grown[tt + k] * x[k]);
+    const float read = lanes_fold16(x), left_over = lanes_fold16(g);
+    if (lane < 16) {
+      sh.read[warp & 3][tt + lane] = read;
+      sh.left_over[warp & 3][tt + lane] = left_over;
+    }
     tmem_sum(tm + seat.lanes + cK + tt, tm + seat.lanes + cK + 64 + tt, y);
 #pragma unroll
     for (int k = 0; k < 16; ++k) y[k] += z[k];
@@ -344,26 +360,57 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
   if (warp == kControl) {
     tc_fence_after();
     tmem_dealloc(tm, 512);
-    // The gates: sums from each token to the chunk's end, two tokens a lane.
-    float after = 0.f, ends[2], writes[2];
+    // The gates, two tokens a lane: from S to tokens from t on, from tokens before t to S', from tokens before t to those from t on.
+    float handed = 0.f, dg[2], near[2], far[2] = {0.f, 0.f}, reads[2], gives[2], writes[2];
 #pragma unroll
-    for (int w = 0; w < kControl; ++w) after += sh.handed[w];
+    for (int w = 0; w < kControl; ++w) handed += sh.handed[w];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int i = 2 * lane + k;
-      ends[k] = writes[k] = 0.f;
+      near[k] = reads[k] = gives[k] = writes[k] = 0.f;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        ends[k] += sh.qdots[w][i] - sh.part[1][w][i];
-        writes[k] += sh.part[0][w][i];
+        near[k] += sh.near[w][i];
+        reads[k] += sh.read[w][i];
+        gives[k] += sh.left_over[w][i];
+        writes[k] += sh.written[w][i];
       }
     }
-    float sum = ends[0] + ends[1];
+    // Adds to the second of two tokens, and to the first, what a lane and those behind it have.
+    const auto from_here = [&](const float (&x)[2], float (&y)[2]) {
+      float sum = x[0] + x[1];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const float up = __shfl_down_sync(0xffffffffu, sum, o);
+        if (lane + o < 32) sum += up;
+      }
+      const float behind = __shfl_down_sync(0xffffffffu, sum, 1);
+      y[1] = (lane < 31 ? behind : 0.f) + x[1];
+      y[0] = y[1] + x[0];
+    };
+    from_here(reads, dg);
+    float before = gives[0] + gives[1];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const float up = __shfl_down_sync(0xffffffffu, sum, o);
-      if (lane + o < 32) sum += up;
+      const float down = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += down;
     }
+    before = __shfl_up_sync(0xffffffffu, before, 1);
+    if (lane == 0) before = 0.f;
+    dg[0] += before;
+    dg[1] += before + gives[0];
+#pragma unroll
+    for (int q = 1; q < kChunk / 16; ++q) {
+      float y[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) far[k] += sh.far[q - 1][2 * lane + k] + sh.far[q - 1][kChunk + 2 * lane + k];
+      from_here(far, y);
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (lane / 8 == q) dg[k] += y[k];
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) dg[k] += near[k] + sh.grown[kChunk - 1] * handed;
     const float a_log = load_any(a.g.a_log, a.g.a_log_type, h), dt = load_any(a.g.dt_bias, a.g.dt_bias_type, h);
     double sum_log = 0.0, sum_bias = 0.0;
 #pragma unroll
@@ -371,15 +418,13 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
       const int i = 2 * lane + k;
       if (i >= rows) continue;
       const Gate gate = gate_of(ElemOf<I>::up(*head_at<I>(a.g.a, b, t0 + i, h)), a_log, dt);
-      // Nothing passes a gate whose factor is 0 in fp32: what the sum holds then is its rounding.
-      const float dg = gate.log_decay < -104.f ? 0.f : (k ? sum - ends[0] : sum) + after;
-      const float da = -dg * gate.rate * gate.slope;
+      const float da = -dg[k] * gate.rate * gate.slope;
       const float beta = sh.beta[i];
       const float db = beta > 1e-20f ? (1.f - beta) * (writes[k] / beta) : 0.f;  // V' = beta E; below, db is under 1e-20 dV . E
       const long long to = ((long long)b * d.T + t0 + i) * d.H + h;
       reinterpret_cast<I*>(a.da)[to] = ElemOf<I>::down(da);
       reinterpret_cast<I*>(a.db)[to] = ElemOf<I>::down(db);
-      sum_log += (double)dg * gate.log_decay;
+      sum_log += (double)dg[k] * gate.log_decay;
       sum_bias += da;
     }
     sum_log = lanes_sum(sum_log);
@@ -394,14 +439,14 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
   // scaling: with x a row, r its reciprocal length and y the sum, dx = y - x r^2 (x . y). Four rows at a time.
   constexpr int kE = DK / 32;  // elements of a lane
   const auto row_of = [&](int tile, int i, float (&x)[kE]) {
-    const unsigned char* at = mem + tile + element_at(i, lane * kE, kTok);
+    const unsigned char* at = mem + tile + element_at(i, lane * kE, Mem::kPanelK);
     float lo[kE];
     if constexpr (kE == 4) {
       raw_up<bf16>(*reinterpret_cast<const uint2*>(at), x);
-      if (P == 2) raw_up<bf16>(*reinterpret_cast<const uint2*>(at + Mem::kPlaneK), lo);
+      if (P == 2) raw_up<bf16>(*reinterpret_cast<const uint2*>(at + Mem::kPart), lo);
     } else {
       raw_up<bf16>(*reinterpret_cast<const uint32_t*>(at), x);
-      if (P == 2) raw_up<bf16>(*reinterpret_cast<const uint32_t*>(at + Mem::kPlaneK), lo);
+      if (P == 2) raw_up<bf16>(*reinterpret_cast<const uint32_t*>(at + Mem::kPart), lo);
     }
     if (P == 2)
 #pragma unroll

@@ -60,16 +60,12 @@ def recurrence(x, first, scale=None):
     return torch.stack(outs, 1), state
 
 
-def gate_terms(x, out, g_out, dv):
-    """The log-decay's gradient at a token is a sum over the rest of its chunk of q . dq - v . dv, whose terms cancel: up to 64
-    of them with errors of random sign, 8 times one's. Those errors' size for each gate's gradient."""
-    wide = {n: x[n].detach().double().cpu() for n in ("a", "a_log", "dt_bias", "v")}
-    each = (out * g_out.double().cpu()).sum(-1).abs() + (wide["v"] * dv).sum(-1).abs()
-    dt = wide["a"] + wide["dt_bias"]
-    da = 8 * each.square().mean((0, 1)).sqrt() * wide["a_log"].exp() * torch.sigmoid(dt).square().mean((0, 1)).sqrt()
-    n = each[..., 0].numel() ** 0.5
-    ratio = (torch.nn.functional.softplus(dt) / torch.sigmoid(dt)).square().mean((0, 1)).sqrt()
-    return {"a": da.detach(), "dt_bias": (da * n).detach(), "a_log": (da * n * ratio).detach()}
+def gate_sums(x, da):
+    """The gradients of a_log and dt_bias are sums of all tokens' shares, of either sign, each with errors of its own size: what such
+    a sum comes to where signs are random, whatever they happen to cancel to in one head."""
+    dt = (x["a"].detach().double() + x["dt_bias"].detach().double()).cpu()
+    ratio = torch.nn.functional.softplus(dt) / torch.sigmoid(dt)  # of a token's share for a_log to that for dt_bias
+    return {"dt_bias": da.square().sum((0, 1)).sqrt(), "a_log": (da * ratio).square().sum((0, 1)).sqrt()}
 
 
 def close(name, got, want, dtype, slack, terms=0.0):
@@ -115,7 +111,7 @@ def check(shape, dtype, device, *, state=False, layout="sliced", g_state=False, 
     cpu = device == "cpu"
     close("out", out, want, dtype, terms * 2.0 ** (-18 if cpu else -9))
     close("state", last, want_last, torch.float32, terms * 2.0 ** (-18 if cpu else -12))
-    sums = gate_terms(x, want.detach(), g_out, grads["v"])
+    sums = gate_sums(x, grads["a"])
     for n, g in zip((*NAMES, "state"), got, strict=False):
         close("d" + n, g, grads[n], g.dtype, terms * 2.0 ** (-16 if cpu else -9), sums.get(n, 0.0))
 
@@ -130,6 +126,32 @@ SHAPES = [  # batch, tokens, key heads, value heads, key dim, value dim
 @pytest.mark.parametrize("shape", SHAPES)
 def test_forward_and_gradients(device, shape):
     check(shape, torch.float32 if device == "cpu" else torch.bfloat16, device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_gradients_of_gates_that_nearly_close(device):
+    """Heads that keep e^-1 to e^-40 of a state in a token, each measured by itself: what passes a gate is summed as such, not as
+    a difference of what a token takes and gives, so that a head's gradient has its own size's errors."""
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    x, _ = make(2, 150, 2, 4, 64, 64, dtype, device)
+    x["a_log"] = torch.tensor([1.0, 2.0, 4.0, 16.0], device=device).log()
+    x["dt_bias"] = torch.full((4,), 1.0, device=device)
+    for y in x.values():
+        y.requires_grad_(True)
+    out, _ = ops.gated_delta_rule(*(x[n] for n in NAMES))
+    g_out = torch.randn(out.shape, generator=torch.Generator().manual_seed(3)).to(dtype).to(device)
+    _, _, grads = exact(x, None, g_out, None)
+    got = torch.autograd.grad(out, [x["a"], x["a_log"], x["dt_bias"]], g_out)
+    wide = {n: x[n].detach().double().cpu() for n in ("a", "a_log", "dt_bias")}
+    dt = wide["a"] + wide["dt_bias"]
+    ratio = torch.nn.functional.softplus(dt) / torch.sigmoid(dt)  # of a token's shares in the gradients of a_log and a
+    for h in range(4):
+        da = grads["a"][..., h]
+        each = {"a": da, "dt_bias": da, "a_log": da * ratio[..., h]}
+        for n, g in zip(("a", "a_log", "dt_bias"), got, strict=True):
+            size = each[n].square().mean().sqrt() * (1.0 if n == "a" else each[n].numel() ** 0.5)
+            off, want = (g[..., h].double().cpu() - grads[n][..., h]).abs(), grads[n][..., h].abs()
+            assert (off <= (torch.finfo(g.dtype).eps / 2 + 2.0 ** -9) * want + 2.0 ** -9 * size + 1e-37).all(), (n, h, (off / size).max())
 
 
 @pytest.mark.gpu
