@@ -19,12 +19,15 @@ namespace cg = cooperative_groups;
 
 template <typename I, int DK, int DV>
 struct InputsMem {
-  static constexpr int kPanels = DK / 64, kPanelS = DV * 128, kPlaneS = kPanels * kPanelS, kPlaneX = DV * 128, kPlaneK = kPanels * kTok;
-  // dS'; V'; S; the stack: dO and dV, the high halves before the low ones (dO in bf16 has none); q and k; the small matrices.
-  // The largest state takes all there is: q, k and the small matrices then come where S was.
-  static constexpr int kKeys = 2 * kParts<I> * kPlaneK, kSquares = 4 * kTok;
+  static constexpr int kPanels = DK / 64, kPanelS = DV * 128, kPlaneS = kPanels * kPanelS, kPlaneX = DV * 128;
+  // dS'; V'; the stack: dO and dV, the high halves before the low ones (dO in bf16 has none); S; q and k; the small matrices.
+  // The largest state takes all there is: q, k and the small matrices then come where S was. In the end, from the start on: all
+  // heads' parts of the owned rows, a multiple of 16 (at most 32 from each of seven heads).
+  static constexpr int ldF = DK + 4, kRows = 7 * 32 * ldF * 4;
+  static constexpr int kKeys = 2 * kParts<I> * kPanels * kTok, kSquares = 4 * kTok;
   static constexpr int D = 0, V = D + 2 * kPlaneS, O = V + 2 * kPlaneX, G = O + kPlaneX, Ol = G + kPlaneX,
-                       Gl = Ol + (kParts<I> == 2 ? kPlaneX : 0), S = Gl + kPlaneX, kEnd = S + 2 * kPlaneS;
+                       Gl = Ol + (kParts<I> == 2 ? kPlaneX : 0), S = Gl + kPlaneX, kUsed = S + 2 * kPlaneS,
+                       kEnd = kUsed > kRows ? kUsed : align1k(kRows);
   // Panels of q and of k take turns, so that their rows are one operand's 128; parts are kPart apart.
   static constexpr int kPanelK = 2 * kTok, kPart = kPanels * kPanelK;
   static constexpr bool kShared = kEnd + kKeys + kSquares > 220 * 1024;
@@ -32,9 +35,8 @@ struct InputsMem {
   static constexpr int Q = kShared ? S : kEnd, K = Q + kTok, W = kShared && !kAllShared ? kEnd : Q + kKeys, N = W + 2 * kTok,
                        kTiles = kAllShared ? kEnd : N + 2 * kTok;
   static_assert(!kShared || kKeys <= 2 * kPlaneS, "room where S was");
-  static constexpr int ldF = DK + 4, kRows = (2 * kChunk + kMostGroup) * ldF * 4;  // in the end, from the start on: all heads' parts of the owned rows
-  static_assert(kRows <= (kShared ? S : kEnd), "the rows of q and k stay");
-  static constexpr int kBytes = kTiles > kRows ? kTiles : kRows;
+  static_assert(kRows <= Q, "the rows of q and k stay");
+  static constexpr int kBytes = kTiles;
 };
 
 enum InputsBar { kGotQK, kGotV, kGotS, kGotD, kMixDone, kReadS, kReadD, kMixSet, kGramDone, kGramRead, kAllDone, kTaken, kInputsBars };
@@ -43,8 +45,10 @@ struct InputsShared {
   uint64_t bar[kInputsBars];
   uint32_t tmem;
   float2 G[kChunk];
-  float rk[kChunk], rq[kChunk], beta[kChunk], left[kChunk], grown[kChunk];
-  float written[4][kChunk];         // V' . dV, of each quarter of a slice
+  float rk[kChunk], rq[kChunk], beta[kChunk];
+  float4 by[kChunk];                // what a token's sums are multiplied by: its query's read, its key's read and its write
+  float kept;                       // exp(G_63)
+  float written[kChunk];            // V' . dV
   float read[4][kChunk];            // what S gives to a token, of each quarter of a key head
   float left_over[4][kChunk];       // what a token gives to S'
   float near[4][kChunk];            // what the tokens of t's sixteen before t give to t and those behind it: of half of P, of L each
@@ -53,10 +57,41 @@ struct InputsShared {
 
 };
 
+// Adds to the sums of lane (i, i / 2 % 4) the products of bf16 pairs that lie in the same places of two matrices, each in halves:
+// a 16 x 8 product of which only the diagonals are wanted, a lane's words with the same lane's, takes a sixth of the
+// instructions that unpack and multiply them.
+__device__ __forceinline__ void dot_halves(float (&c)[4], uint32_t h0, uint32_t l0, uint32_t h1, uint32_t l1, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(h0), "r"(l0), "r"(h1), "r"(l1), "r"(b0), "r"(b1));
+}
+
+// Stores to the shared memory of a CTA of the cluster.
+__device__ __forceinline__ uint32_t rank_addr(uint32_t at, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void store_at(uint32_t at, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+}
+
+// Adds 32 values of each of 32 lanes over the lanes: lane l ends with the sum of value l.
+__device__ __forceinline__ float lanes_fold(float (&x)[32]) {
+#pragma unroll
+  for (int n = 16; n > 0; n >>= 1) {
+    const bool up = threadIdx.x & n;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float send = up ? x[i] : x[i + n], keep = up ? x[i + n] : x[i];
+      x[i] = keep + __shfl_xor_sync(0xffffffffu, send, n);
+    }
+  }
+  return x[0];
+}
+
 // Adds 16 values of each of 32 lanes over the lanes: lane l ends with the sum of value l % 16.
 __device__ __forceinline__ float lanes_fold16(float (&x)[16]) {
-#pragma unroll
-  for (int i = 0; i < 16; ++i) x[i] += __shfl_xor_sync(0xffffffffu, x[i], 16);
 #pragma unroll
   for (int n = 8; n > 0; n >>= 1) {
     const bool up = threadIdx.x & n;
@@ -66,7 +101,7 @@ __device__ __forceinline__ float lanes_fold16(float (&x)[16]) {
       x[i] = keep + __shfl_xor_sync(0xffffffffu, send, n);
     }
   }
-  return x[0];
+  return x[0] + __shfl_xor_sync(0xffffffffu, x[0], 16);
 }
 
 template <typename I, int DK, int DV>
@@ -99,11 +134,11 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
     bulk_load(mem + Mem::D, a.dstates + at * 2 * Mem::kPlaneS, 2 * Mem::kPlaneS, &sh.bar[kGotD]);
   };
   const auto load_keys = [&] {
-    mbar_arrive_expect_tx(&sh.bar[kGotQK], 2 * P * Mem::kPlaneK);
+    mbar_arrive_expect_tx(&sh.bar[kGotQK], 2 * P * Mem::kPanels * kTok);
 #pragma unroll
     for (int i = 0; i < P * Mem::kPanels; ++i) {
-      bulk_load(mem + Mem::Q + i * Mem::kPanelK, a.keep.queries + m * P * Mem::kPlaneK + i * kTok, kTok, &sh.bar[kGotQK]);
-      bulk_load(mem + Mem::K + i * Mem::kPanelK, a.keep.keys + m * P * Mem::kPlaneK + i * kTok, kTok, &sh.bar[kGotQK]);
+      bulk_load(mem + Mem::Q + i * Mem::kPanelK, a.keep.queries + m * P * Mem::kPanels * kTok + i * kTok, kTok, &sh.bar[kGotQK]);
+      bulk_load(mem + Mem::K + i * Mem::kPanelK, a.keep.keys + m * P * Mem::kPanels * kTok + i * kTok, kTok, &sh.bar[kGotQK]);
     }
   };
   if (tid == kWorkers) {
@@ -112,8 +147,8 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
     fence_proxy_async_smem();
     load_slice(0);
     if (Mem::kShared) {
-      bulk_prefetch(a.keep.queries + m * P * Mem::kPlaneK, P * Mem::kPlaneK);
-      bulk_prefetch(a.keep.keys + m * P * Mem::kPlaneK, P * Mem::kPlaneK);
+      bulk_prefetch(a.keep.queries + m * P * Mem::kPanels * kTok, P * Mem::kPanels * kTok);
+      bulk_prefetch(a.keep.keys + m * P * Mem::kPanels * kTok, P * Mem::kPanels * kTok);
     } else {
       load_keys();
     }
@@ -126,8 +161,9 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
     sh.rk[tid] = a.keep.rk[m * kChunk + tid];
     sh.rq[tid] = a.keep.rq[m * kChunk + tid];
     sh.beta[tid] = a.keep.beta[n * kChunk + tid];
-    sh.left[tid] = decay_between(end, G);
-    sh.grown[tid] = __expf(G.x + G.y);
+    const float grown = __expf(G.x + G.y);
+    sh.by[tid] = make_float4(sh.rq[tid] * grown, -sh.rk[tid] * grown, sh.rk[tid] * decay_between(end, G), 0.f);
+    if (tid == kChunk - 1) sh.kept = grown;
   }
   tc_fence_before();
   __syncthreads();
@@ -148,22 +184,22 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
       for (int s = 0; s < slices; ++s) {
         const bool more = s > 0;
         if (!wait(&sh.bar[kGotV], s)) break;
-        multiply<kVs, 128, true, true>(tm + cMix, high, V, more);  // both halves of V' side by side
-        multiply<kVs, 64, true, true>(P == 2 ? tm + cMix : tm + cLow, low, V, P == 2 || more);
-        if (s == slices - 1) tc_commit(&sh.bar[kMixDone]);
         if (!wait(&sh.bar[kGotS], s)) break;
         multiply<kVs, 128, true, true>(tm + cS, S, high, more);
         multiply<kVs, 128, true, true>(tm + cS, Sl, high, true);
         if (P == 2) multiply<kVs, 128, true, true>(tm + cS, S, low, true);
         else multiply<kVs, 64, true, true>(tm + cS + 64, S, low_g, true);
         tc_commit(&sh.bar[kReadS]);
-        if (!wait(&sh.bar[kGotD], s)) break;
-        multiply<kVs, 128, true, true>(tm + cD, D, V, more);
-        multiply<kVs, 64, true, true>(tm + cD, Dl, V, true);
+        multiply<kVs, 128, true, true>(tm + cMix, high, V, more);  // both halves of V' side by side
+        multiply<kVs, 64, true, true>(P == 2 ? tm + cMix : tm + cLow, low, V, P == 2 || more);
+        if (s == slices - 1) tc_commit(&sh.bar[kMixDone]);
         if (Mem::kShared && s == slices - 1) {
           if (!wait(&sh.bar[kReadS], s)) break;
           load_keys();
         }
+        if (!wait(&sh.bar[kGotD], s)) break;
+        multiply<kVs, 128, true, true>(tm + cD, D, V, more);
+        multiply<kVs, 64, true, true>(tm + cD, Dl, V, true);
         if (s + 1 < slices) {  // the places are free once they are read, by the products and by the workers
           tc_commit(&sh.bar[kReadD]);
           if (!wait(&sh.bar[kReadS], s) || !wait(&sh.bar[kReadD], s) || !wait(&sh.bar[kTaken], s)) break;
@@ -189,7 +225,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
       }
     }
   } else {
-    float handed = 0.f;
+    float handed[4] = {0.f, 0.f, 0.f, 0.f};
     const int tt = seat.part * 16;  // its tokens
     float mix[16];
     for (int s = 0; s < slices; ++s) {
@@ -222,6 +258,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
             const int j = j0 + p * 8 + k;
             const float w = f[p * 8 + k] * by * (decay_between(Gi, sh.G[j]) * sh.rk[j]);
             mix[p * 8 + k] = x[k] = j < last ? w : 0.f;
+            if (of_l && j == i) sh.written[i] = f[p * 8 + k];
           }
           const int at = piece_at(i, seat.part * 2 + p);
           put8(to + at, to + kTok + at, x);
@@ -238,30 +275,10 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
         ah[i] = __ldcs(before + i * kWorkers + tid);
         al[i] = __ldcs(before + kPieces + i * kWorkers + tid);
       }
-      if (!wait(&sh.bar[kGotV], s)) break;
-      // A lane holds an element of the values: the sums over them, of each token.
-      float x[16];
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const int at = piece_at(in ? seat.row : 0, tt / 8 + p);
-        const uint4 gh = *reinterpret_cast<const uint4*>(mem + Mem::G + at), gl = *reinterpret_cast<const uint4*>(mem + Mem::Gl + at);
-        const uint4 wh = *reinterpret_cast<const uint4*>(mem + Mem::V + at), wl = *reinterpret_cast<const uint4*>(mem + Mem::V + Mem::kPlaneX + at);
-        const float2 g[4] = {pair_sum(gh.x, gl.x), pair_sum(gh.y, gl.y), pair_sum(gh.z, gl.z), pair_sum(gh.w, gl.w)},
-                     w[4] = {pair_sum(wh.x, wl.x), pair_sum(wh.y, wl.y), pair_sum(wh.z, wl.z), pair_sum(wh.w, wl.w)};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          x[p * 8 + 2 * k] = in ? w[k].x * g[k].x : 0.f;
-          x[p * 8 + 2 * k + 1] = in ? w[k].y * g[k].y : 0.f;
-        }
-      }
-      const float sum = lanes_fold16(x);
-      if (lane < 16) {
-        float* to = &sh.written[warp & 3][tt + lane];
-        *to = s ? *to + sum : sum;
-      }
       // What passes the gate of token t within the chunk: from the tokens of its sixteen before t here, from earlier sixteens by
       // the sums of their columns.
       if (s == slices - 1) {
+        float x[16];
         if (!wait(&sh.bar[kGramDone], 0)) break;
         tc_fence_after();
         tmem_row(tm + seat.lanes + cGram + tt, x);
@@ -283,78 +300,81 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
       for (int i = 0; i < kMine; ++i) {
         const unsigned char* at = mem + Mem::D + (i * kWorkers + tid) * 16;
         const uint4 dh = *reinterpret_cast<const uint4*>(at), dl = *reinterpret_cast<const uint4*>(at + Mem::kPlaneS);
-        const uint32_t u[4] = {ah[i].x, ah[i].y, ah[i].z, ah[i].w}, v4[4] = {al[i].x, al[i].y, al[i].z, al[i].w},
-                       y[4] = {dh.x, dh.y, dh.z, dh.w}, z[4] = {dl.x, dl.y, dl.z, dl.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 e = pair_sum(u[k], v4[k]), f = pair_sum(y[k], z[k]);
-          handed = fmaf(e.x, f.x, fmaf(e.y, f.y, handed));
-        }
+        dot_halves(handed, dh.x, dl.x, dh.y, dl.y, ah[i].x, ah[i].y);
+        dot_halves(handed, dh.x, dl.x, dh.y, dl.y, al[i].x, al[i].y);
+        dot_halves(handed, dh.z, dl.z, dh.w, dl.w, ah[i].z, ah[i].w);
+        dot_halves(handed, dh.z, dl.z, dh.w, dl.w, al[i].z, al[i].w);
       }
       mbar_arrive(&sh.bar[kTaken]);
     }
-    handed = lanes_sum(handed);
-    if (lane == 0) sh.handed[warp] = handed;
+    // The diagonals of rows 0..7 and 8..15: row r, column 2 (lane % 4) + j of lane 4 r + lane % 4.
+    const int r = lane >> 2;
+    const float mine = lanes_sum((lane & 3) != r >> 1 ? 0.f : r & 1 ? handed[1] + handed[3] : handed[0] + handed[2]);
+    if (lane == 0) sh.handed[warp] = mine;
     wait(&sh.bar[kAllDone], 0);
   }
-  // dq and dk of this head: r dq^ and r dk^ of the scaled rows. Each CTA of the cluster owns every group-th row of both and
-  // gets them from all heads, where its S and V' lay: row r at place r / group of the sender's part.
+  // dq and dk of this head: r dq^ and r dk^ of the scaled rows. The CTAs of the cluster own a part of the rows of both each and
+  // get them from all heads, where dS' and V' lay.
   cg::cluster_group cluster = cg::this_cluster();
-  if (group > 1) cluster.sync();  // all are done with their products
-  else __syncthreads();
+  __syncwarp();
+  if (group > 1) cluster.barrier_arrive();  // this one is done with its products
   float* F = reinterpret_cast<float*>(mem);
-  const int own = (2 * kChunk + group - 1) / group;  // rows of an owner, at most
+  const int own = (2 * kChunk / 16 + group - 1) / group * 16;  // rows of an owner: one for the 16 tokens of a worker
+  float y[16], z[16];
   if (warp < kControl) {
     tc_fence_after();
     const int tt = seat.part * 16;
-    float x[16], y[16], z[16];
-    const auto put = [&](int r0, const float (&v)[16]) {
-      int owner = r0 % group;
-      float* f = F + (hg * own + r0 / group) * Mem::ldF + seat.row;
-#pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        *(group > 1 ? cluster.map_shared_rank(f, owner) : f) = v[k];
-        if (++owner == group) {
-          owner = 0;
-          f += Mem::ldF;
-        }
-      }
-    };
-    tmem_sum(tm + seat.lanes + cQ + tt, tm + seat.lanes + cQ + 64 + tt, y);
-    tmem_row(tm + seat.lanes + cS + tt, x);
-#pragma unroll
-    for (int k = 0; k < 16; ++k) y[k] = fmaf(sh.rq[tt + k] * sh.grown[tt + k], x[k], y[k]);
-    if (seat.row < DK) put(tt, y);
+    float x[32], g[16];
+    tmem_sum(tm + seat.lanes + cD + tt, tm + seat.lanes + cD + 64 + tt, z);
+    tmem_rows(tm + seat.lanes + cS + tt, y, tm + seat.lanes + cS + 64 + tt, g);
     // What S gives to a token and what a token gives to S': over the lanes here, over the warps of a column later. The rows of q
     // and k still lie as tiles.
     const auto element = [&](int tile, int i) {
       const unsigned char* at = mem + tile + element_at(i, seat.row, Mem::kPanelK);
       float v = __bfloat162float(*reinterpret_cast<const bf16*>(at));
       if (P == 2) v += __bfloat162float(*reinterpret_cast<const bf16*>(at + Mem::kPart));
-      return seat.row < DK ? v : 0.f;
+      return v;
     };
-    float g[16];
-    tmem_sum(tm + seat.lanes + cD + tt, tm + seat.lanes + cD + 64 + tt, z);
-    tmem_row(tm + seat.lanes + cS + 64 + tt, g);
+    const bool in = seat.row < DK;
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
-      const float key = element(Mem::K, tt + k), query = element(Mem::Q, tt + k), reads = -sh.rk[tt + k] * sh.grown[tt + k] * g[k],
-                  gives = sh.rk[tt + k] * sh.left[tt + k] * z[k];
-      x[k] = seat.row < DK ? fmaf(query, sh.rq[tt + k] * sh.grown[tt + k] * x[k], key * reads) : 0.f;
-      g[k] = seat.row < DK ? key * gives : 0.f;
+      const float key = in ? element(Mem::K, tt + k) : 0.f, query = in ? element(Mem::Q, tt + k) : 0.f;
+      const float4 by = sh.by[tt + k];
+      const float gives = by.z * z[k], reads = by.y * g[k];
+      y[k] *= by.x;
+      x[k] = in ? fmaf(query, y[k], key * reads) : 0.f;
+      x[16 + k] = in ? key * gives : 0.f;
       z[k] = reads + gives;
     }
-    const float read = lanes_fold16(x), left_over = lanes_fold16(g);
-    if (lane < 16) {
-      sh.read[warp & 3][tt + lane] = read;
-      sh.left_over[warp & 3][tt + lane] = left_over;
-    }
-    tmem_sum(tm + seat.lanes + cK + tt, tm + seat.lanes + cK + 64 + tt, y);
+    const float sum = lanes_fold(x);
+    (lane < 16 ? sh.read : sh.left_over)[warp & 3][tt + (lane & 15)] = sum;
+    tmem_sum(tm + seat.lanes + cQ + tt, tm + seat.lanes + cQ + 64 + tt, g);
 #pragma unroll
-    for (int k = 0; k < 16; ++k) y[k] += z[k];
-    if (seat.row < DK) put(kChunk + tt, y);
+    for (int k = 0; k < 16; ++k) y[k] += g[k];
+    tmem_sum(tm + seat.lanes + cK + tt, tm + seat.lanes + cK + 64 + tt, g);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) z[k] += g[k];
     tc_fence_before();
   }
+  if (group > 1) cluster.barrier_wait();
+  else __syncthreads();
+  if (warp < kControl && seat.row < DK) {
+    const auto put = [&](int r0, const float (&v)[16]) {
+      const int owner = r0 / own;
+      float* f = F + (hg * own + r0 % own) * Mem::ldF + seat.row;
+      if (owner == hg) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) f[k * Mem::ldF] = v[k];
+      } else {
+        const uint32_t at = rank_addr(smem_u32(f), owner);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) store_at(at + k * Mem::ldF * 4, v[k]);
+      }
+    };
+    put(seat.part * 16, y);
+    put(kChunk + seat.part * 16, z);
+  }
+  __syncwarp();
   if (group > 1) cluster.sync();
   else __syncthreads();
   if (warp == kControl) {
@@ -367,14 +387,14 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int i = 2 * lane + k;
-      near[k] = reads[k] = gives[k] = writes[k] = 0.f;
+      near[k] = reads[k] = gives[k] = 0.f;
+      writes[k] = sh.written[i];
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         near[k] += sh.near[w][i];
         reads[k] += sh.read[w][i];
         gives[k] += sh.left_over[w][i];
-        writes[k] += sh.written[w][i];
-      }
+              }
     }
     // Adds to the second of two tokens, and to the first, what a lane and those behind it have.
     const auto from_here = [&](const float (&x)[2], float (&y)[2]) {
@@ -410,7 +430,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
         if (lane / 8 == q) dg[k] += y[k];
     }
 #pragma unroll
-    for (int k = 0; k < 2; ++k) dg[k] += near[k] + sh.grown[kChunk - 1] * handed;
+    for (int k = 0; k < 2; ++k) dg[k] += near[k] + sh.kept * handed;
     const float a_log = load_any(a.g.a_log, a.g.a_log_type, h), dt = load_any(a.g.dt_bias, a.g.dt_bias_type, h);
     double sum_log = 0.0, sum_bias = 0.0;
 #pragma unroll
@@ -452,23 +472,36 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
 #pragma unroll
       for (int k = 0; k < kE; ++k) x[k] += lo[k];
   };
-  for (int p0 = warp; p0 < own; p0 += 4 * kControl) {
+  const long long width = (long long)d.Hk * d.dk, start = ((long long)b * d.T + t0) * width + (long long)hk * d.dk + lane * kE;
+  const float shorter = 1.f / d.scale;
+  const bool in = lane * kE < d.dk;
+  for (int p0 = warp; p0 < own && hg * own + p0 < 2 * kChunk; p0 += 4 * kControl) {
     float y[4][kE], x[4][kE], dot[4];
+    // The rows of a warp are 16 apart, an owner's a multiple of 16: all or none of each sixteen. Rows behind the last are read as the first.
+    const int most = min(own, 2 * kChunk - hg * own);
+    int place[4];
 #pragma unroll
     for (int n4 = 0; n4 < 4; ++n4) {
-      const int place = min(p0 + n4 * kControl, own - 1), r = min(place * group + hg, 2 * kChunk - 1);
+      place[n4] = p0 + n4 * kControl < most ? p0 + n4 * kControl : p0;
+      const int r = hg * own + place[n4];
       row_of(r >= kChunk ? Mem::K : Mem::Q, r % kChunk, x[n4]);
 #pragma unroll
       for (int k = 0; k < kE; ++k) y[n4][k] = 0.f;
-      for (int o = 0; o < group; ++o) {
-        const float* f = F + (o * own + place) * Mem::ldF + lane * kE;
+    }
+    for (int o = 0; o < group; ++o)
 #pragma unroll
-        for (int k = 0; k < kE; k += 2) {
-          const float2 z = *reinterpret_cast<const float2*>(f + k);
-          y[n4][k] += z.x;
-          y[n4][k + 1] += z.y;
+      for (int n4 = 0; n4 < 4; ++n4) {
+        using Vec = std::conditional_t<kE == 4, float4, float2>;
+        const Vec z = *reinterpret_cast<const Vec*>(F + (o * own + place[n4]) * Mem::ldF + lane * kE);
+        y[n4][0] += z.x;
+        y[n4][1] += z.y;
+        if constexpr (kE == 4) {
+          y[n4][2] += z.z;
+          y[n4][3] += z.w;
         }
       }
+#pragma unroll
+    for (int n4 = 0; n4 < 4; ++n4) {
       dot[n4] = 0.f;
 #pragma unroll
       for (int k = 0; k < kE; ++k) dot[n4] = fmaf(x[n4][k], y[n4][k], dot[n4]);
@@ -477,13 +510,13 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
     for (int n4 = 0; n4 < 4; ++n4) dot[n4] = lanes_sum(dot[n4]);
 #pragma unroll
     for (int n4 = 0; n4 < 4; ++n4) {
-      const int place = p0 + n4 * kControl, r = place * group + hg, i = r % kChunk;
-      if (place >= own || r >= 2 * kChunk || i >= rows || lane * kE >= d.dk) continue;
+      const int r = hg * own + place[n4], i = r % kChunk;
+      if (p0 + n4 * kControl >= most || i >= rows || !in) continue;
       const bool of_k = r >= kChunk;
-      const float len = of_k ? sh.rk[i] : sh.rq[i] / d.scale, by = -len * len * dot[n4];
+      const float len = of_k ? sh.rk[i] : sh.rq[i] * shorter, by = -len * len * dot[n4];
 #pragma unroll
       for (int k = 0; k < kE; ++k) y[n4][k] = fmaf(by, x[n4][k], y[n4][k]);
-      I* to = reinterpret_cast<I*>(of_k ? a.dk : a.dq) + (((long long)b * d.T + t0 + i) * d.Hk + hk) * d.dk + lane * kE;
+      I* to = reinterpret_cast<I*>(of_k ? a.dk : a.dq) + (start + i * width);
       if constexpr (kE == 4) *reinterpret_cast<uint2*>(to) = raw_down<I, uint2>(y[n4]);
       else *reinterpret_cast<uint32_t*>(to) = raw_down<I, uint32_t>(y[n4]);
     }
