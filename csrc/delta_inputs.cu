@@ -48,6 +48,7 @@ struct InputsShared {
   float rk[kChunk], rq[kChunk], beta[kChunk];
   float4 by[kChunk];                // what a token's sums are multiplied by: its query's read, its key's read and its write
   float kept;                       // exp(G_63)
+  float2 gate[kChunk];              // log-decay, and its derivative by a
   float written[kChunk];            // V' . dV
   float read[4][kChunk];            // what S gives to a token, of each quarter of a key head
   float left_over[4][kChunk];       // what a token gives to S'
@@ -228,6 +229,12 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
     float handed[4] = {0.f, 0.f, 0.f, 0.f};
     const int tt = seat.part * 16;  // its tokens
     float mix[16];
+    // While the first tiles are on their way. Left to the warp that sums the gates' gradients, this held the CTA back (433 us, 391 with it here).
+    if (tid < rows) {
+      const Gate gate = gate_of(ElemOf<I>::up(*head_at<I>(a.g.a, b, t0 + tid, h)), load_any(a.g.a_log, a.g.a_log_type, h),
+                                load_any(a.g.dt_bias, a.g.dt_bias_type, h));
+      sh.gate[tid] = make_float2(gate.log_decay, -gate.rate * gate.slope);
+    }
     for (int s = 0; s < slices; ++s) {
       const bool in = seat.row < min(DV, d.dv - s * DV);
       // The small matrices first, for the products that wait for them: row i of dP in lane i, of dL in lane 64 + i.
@@ -380,78 +387,56 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) inputs_kernel(const DeltaBwd
   if (warp == kControl) {
     tc_fence_after();
     tmem_dealloc(tm, 512);
-    // The gates, two tokens a lane: from S to tokens from t on, from tokens before t to S', from tokens before t to those from t on.
-    float handed = 0.f, dg[2], near[2], far[2] = {0.f, 0.f}, reads[2], gives[2], writes[2];
-#pragma unroll
-    for (int w = 0; w < kControl; ++w) handed += sh.handed[w];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int i = 2 * lane + k;
-      near[k] = reads[k] = gives[k] = 0.f;
-      writes[k] = sh.written[i];
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        near[k] += sh.near[w][i];
-        reads[k] += sh.read[w][i];
-        gives[k] += sh.left_over[w][i];
-              }
-    }
-    // Adds to the second of two tokens, and to the first, what a lane and those behind it have.
-    const auto from_here = [&](const float (&x)[2], float (&y)[2]) {
-      float sum = x[0] + x[1];
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const float up = __shfl_down_sync(0xffffffffu, sum, o);
-        if (lane + o < 32) sum += up;
+    // The gates, two tokens a lane: from S to tokens from t on, from tokens of earlier sixteens, of t's own, before t to those from
+    // t on, from tokens before t to S', and from S to S'. Rolled up: one warp waits for its instructions far longer than for these sums.
+    const float handed = lanes_sum(lane < kControl ? sh.handed[lane] : 0.f);
+    float dg[2] = {sh.kept * handed, sh.kept * handed}, far[2] = {0.f, 0.f};
+#pragma unroll 1
+    for (int q = 0; q <= kChunk / 16; ++q) {
+      const bool reads = q == 0, gives = q == kChunk / 16;
+      const int step = gives ? -1 : 1;
+      float x[2] = {0.f, 0.f};
+      for (int k = 0; k < 2; ++k) {
+        const int i = 2 * lane + k;
+        if (reads || gives) {
+          for (int w = 0; w < 4; ++w) x[k] += reads ? sh.read[w][i] : sh.left_over[w][i];
+        } else {
+          x[k] = far[k] += sh.far[q - 1][i] + sh.far[q - 1][kChunk + i];
+        }
       }
-      const float behind = __shfl_down_sync(0xffffffffu, sum, 1);
-      y[1] = (lane < 31 ? behind : 0.f) + x[1];
-      y[0] = y[1] + x[0];
-    };
-    from_here(reads, dg);
-    float before = gives[0] + gives[1];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const float down = __shfl_up_sync(0xffffffffu, before, o);
-      if (lane >= o) before += down;
+      float sum = x[0] + x[1];
+#pragma unroll 1
+      for (int o = 1; o < 32; o <<= 1) {
+        const int from = lane + step * o;
+        const float more = __shfl_sync(0xffffffffu, sum, from & 31);
+        if ((from & 31) == from) sum += more;
+      }
+      const float next = __shfl_sync(0xffffffffu, sum, (lane + step) & 31);
+      const float rest = lane == (gives ? 0 : 31) ? 0.f : next;
+      if (reads || gives || lane / 8 == q) {
+        dg[0] += gives ? rest : rest + x[1] + x[0];
+        dg[1] += gives ? rest + x[0] : rest + x[1];
+      }
     }
-    before = __shfl_up_sync(0xffffffffu, before, 1);
-    if (lane == 0) before = 0.f;
-    dg[0] += before;
-    dg[1] += before + gives[0];
-#pragma unroll
-    for (int q = 1; q < kChunk / 16; ++q) {
-      float y[2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) far[k] += sh.far[q - 1][2 * lane + k] + sh.far[q - 1][kChunk + 2 * lane + k];
-      from_here(far, y);
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        if (lane / 8 == q) dg[k] += y[k];
-    }
-#pragma unroll
-    for (int k = 0; k < 2; ++k) dg[k] += near[k] + sh.kept * handed;
-    const float a_log = load_any(a.g.a_log, a.g.a_log_type, h), dt = load_any(a.g.dt_bias, a.g.dt_bias_type, h);
-    double sum_log = 0.0, sum_bias = 0.0;
-#pragma unroll
+    float sum_log = 0.f, sum_bias = 0.f;
     for (int k = 0; k < 2; ++k) {
       const int i = 2 * lane + k;
       if (i >= rows) continue;
-      const Gate gate = gate_of(ElemOf<I>::up(*head_at<I>(a.g.a, b, t0 + i, h)), a_log, dt);
-      const float da = -dg[k] * gate.rate * gate.slope;
+      for (int w = 0; w < 4; ++w) dg[k] += sh.near[w][i];
+      const float da = dg[k] * sh.gate[i].y;
       const float beta = sh.beta[i];
-      const float db = beta > 1e-20f ? (1.f - beta) * (writes[k] / beta) : 0.f;  // V' = beta E; below, db is under 1e-20 dV . E
+      const float db = beta > 1e-20f ? (1.f - beta) * (sh.written[i] / beta) : 0.f;  // V' = beta E; below, db is under 1e-20 dV . E
       const long long to = ((long long)b * d.T + t0 + i) * d.H + h;
       reinterpret_cast<I*>(a.da)[to] = ElemOf<I>::down(da);
       reinterpret_cast<I*>(a.db)[to] = ElemOf<I>::down(db);
-      sum_log += (double)dg[k] * gate.log_decay;
+      sum_log = fmaf(dg[k], sh.gate[i].x, sum_log);
       sum_bias += da;
     }
     sum_log = lanes_sum(sum_log);
     sum_bias = lanes_sum(sum_bias);
     if (lane == 0) {
-      a.part[n * 2] = (float)sum_log;
-      a.part[n * 2 + 1] = (float)sum_bias;
+      a.part[n * 2] = sum_log;
+      a.part[n * 2 + 1] = sum_bias;
     }
     return;
   }
