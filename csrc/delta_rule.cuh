@@ -1,4 +1,4 @@
-// Gated delta rule, chunked (training, prefill) and token by token (decoding): delta_rule.cu, delta_step.cu.
+// Gated delta rule, chunked (training, prefill) and token by token (decoding): delta_prepare.cu, delta_state.cu and delta_inputs.cu; delta_step.cu.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -43,7 +43,7 @@ struct DeltaKept {
   unsigned char* solve;           // (n): [64][64], the inverse of I + L diag(beta)
   unsigned char* attend;          // (n): [64][64], P
   unsigned char* writes;          // (n, slice): [slice][tokens], V'^T; null without a backward
-  unsigned char* states;          // (batch * H + head, chunks + 1, slice): [slice][kp], S^T before each chunk, and the last; null likewise
+  unsigned char* states;          // (n, slice): [slice][kp], S^T before each chunk; null likewise
   float2* total;                  // (n, 64): sum of log-decays from the chunk's start, in two parts
   float* beta;                    // (n, 64)
   float *rk, *rq;                 // (m, 64): reciprocal lengths, that of q times scale

@@ -6,8 +6,8 @@
 // (K K^T) D, P = lower part of (Q K^T) D, S the state before the chunk and S' the one after it. Then
 //     (I + L diag(beta)) E = V - diag(exp G) K S,     V' = diag(beta) E,
 //     O = diag(exp G) Q S + P V',                     S' = exp(G_63) S + (diag(exp(G_63 - G)) K)^T V'.
-// Four kernels: `prepare` (every chunk by itself: gates, lengths, P, and the inverse of the triangular matrix by forward
-// substitution in fp32), `state` (chunk after chunk, columns of S split over CTAs: V' and S'), `output` (every chunk by itself).
+// Kernels: `prepare` (every chunk by itself: lengths, decays, P and the inverse of the triangular matrix, in fp32), then `state`
+// here (chunk after chunk: V', O and S').
 //
 // The backward goes the same way, from dO and dS':
 //     dV' = P^T dO + diag(exp(G_63 - G)) K dS',       dV = (inverse)^T diag(beta) dV',
@@ -15,15 +15,28 @@
 //     dP = lower(dO V'^T),  dL = -strictly lower(dV V'^T),
 //     dQ = diag(exp G) dO S^T + (dP D) K,
 //     dK = -diag(exp G) dV S^T + diag(exp(G_63 - G)) V' dS'^T + (dP D)^T Q + (dL D + (dL D)^T) K,
-// and with b the logit of beta:  db_i = (1 - beta_i) dV_i . E_i.  Scaling S between two tokens scales everything that
-// flows through it, so the log-decay's gradient is what leaves less what enters: with <dS', S'> for what the chunk hands on,
-//     dg_t = sum_{i >= t} (q_i . dq_i - v_i . dv_i) + <dS', S'>.                                       (`inputs`)
+// and with b the logit of beta:  db_i = (1 - beta_i) dV_i . E_i. The log-decay's gradient at t is all that passes from before t to
+// t or behind it: with M = dP P + dL L element by element and r the lengths' scaling left out,
+//     dg_t = sum_{i >= t > j} M_ij + sum_{i >= t} exp(G_i) (q_i . S dO_i - k_i . S dV_i)
+//          + sum_{j < t} exp(G_63 - G_j) k_j . dS' V'_j + exp(G_63) <dS', S>.                            (`inputs`)
+// The same sum as the difference of what tokens take and give, q . dq - v . dv, needs fewer products, but its terms stay where a
+// gate closes and what passes goes to nothing: half of a percent off over heads that keep e^-1 to e^-16 of a state.
 //
 // Matrix products run on 16-bit tensor instructions with fp32 sums. q, k and dO are bf16 as given, so they are exact; all
 // that is computed (S, V', the inverse, P and their gradients) goes in as two bf16 halves, which keep 16 bits of 24: two products
 // where one side is exact, three where both have halves (the product of the two low halves is below 2^-16 of the result).
 // One half alone would round each operand by 2^-8, as much as the output's own rounding, several times over. fp16 inputs
-// are two exact halves as well.
+// are two exact halves as well. The state itself stays in tensor memory in fp32 from the first chunk to the last; a final
+// state is 1e-6 to 6e-6 of its norm off.
+//
+// Layout: a CTA has up to 128 value elements of a head, one a lane of tensor memory, so that all of a token's factors are by columns
+// and the state's rows are the lanes: S^T, its reads by keys and queries, E and the outputs. The last warp's first lane copies and
+// multiplies; sixteen warps turn sums into halves.
+//
+// What bounds it: a chunk's chain of three products and three conversions, each waiting for the one before. 4 x 2048 tokens, 32
+// heads of 128 x 128, bf16 (128 CTAs, 32 chunks each): state 172 us, dstate 164 us, 5.3 us a chunk, while the bytes (0.85
+// GB each) would take 130 us. On instructions of single warps (state and outputs as kernels of their own):
+// 354 + 195 us and 594 us. Eight converting warps instead of sixteen: a training pass 1085 us instead of 1000.
 #include "delta_tiles.cuh"
 
 namespace bw {
@@ -152,7 +165,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
           At{base + Mem::P, kTok};
       const auto store_state = [&](int c) {
         if (a.keep.states == nullptr) return;
-        bulk_store(a.keep.states + ((head * (chunks + 1) + c) * slices + slice) * 2 * Mem::kPlaneS, mem + Mem::S, 2 * Mem::kPlaneS);
+        bulk_store(a.keep.states + ((head * chunks + c) * slices + slice) * 2 * Mem::kPlaneS, mem + Mem::S, 2 * Mem::kPlaneS);
         bulk_commit();
       };
       int c = 0;
@@ -189,7 +202,6 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
         if (!wait(&sh.bar[kOutDone], c)) break;
         if (c + 1 < chunks) load_square(Mem::P, a.keep.attend, c + 1, &sh.bar[kLoadedP]);
       }
-      if (c == chunks && wait(&sh.bar[kStateSet], chunks)) store_state(chunks);
       bulk_done();
     }
   } else {

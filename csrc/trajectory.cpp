@@ -301,7 +301,7 @@ struct KeptSizes {
     m = (int64_t)d.B * d.Hk * d.chunks;
     keys = m * rows;
     writes = keep ? n * 2 * column : 0;
-    states = keep ? (int64_t)d.B * d.H * (d.chunks + 1) * state : 0;
+    states = keep ? (int64_t)d.B * d.H * d.chunks * state : 0;
   }
 };
 

@@ -167,6 +167,11 @@ def _v_policy_loss(args, kwargs):
     check_labels("policy_loss", args[1], int(args[0].shape[-1]), int(args[10]))
 
 
+def _v_token_scores(args, kwargs):
+    # (logits, labels, top_k, temperature, ignore, err)
+    check_labels("token_scores", args[1], int(args[0].shape[-1]), int(args[4]))
+
+
 def _v_balance_loss(args, kwargs):
     # (logits, ids, mask, top_k, z_coef, err)
     if args[1] is not None:
@@ -189,6 +194,7 @@ VALIDATORS: dict[str, Callable[[tuple, dict], None]] = {
     "mask_gather": _v_mask_gather,
     "preference_loss": _v_preference_loss,
     "policy_loss": _v_policy_loss,
+    "token_scores": _v_token_scores,
     "balance_loss": _v_balance_loss,
     "qk_norm_rope": _v_qk_norm_rope,
 }

@@ -8,7 +8,7 @@ one and rows of *q* to length *scale*,
     ``S <- exp(g) S``, ``S <- S + k (beta (v - S^T k))^T``, ``o = S^T q``
 
 for every value head, ``H / Hk`` of which share a key head.  On sm_100 the kernels of
-``csrc/delta_rule.cu`` and ``csrc/delta_step.cu``; the same formulas in PyTorch serve CPU tensors.
+``csrc/delta_*.cu``; the same formulas in PyTorch serve CPU tensors.
 """
 
 from __future__ import annotations

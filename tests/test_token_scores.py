@@ -277,3 +277,30 @@ def test_alternatives_crowded_into_few_places(device):
         check(x[:, :4], labels[:, :4], top_k=32)
         got = ops.token_scores(x[:, 4:], labels[:, 4:], top_k=5)
         assert got.top_ids[0, 0].tolist() == [7, 0, 1, 2, 3] and got.entropy[0, 0] == 0
+
+
+def test_launch_checks_name_a_bad_label():
+    from dattri_llm_b200.ops import checks
+
+    labels = torch.tensor([[0, IGNORE, 9]])
+    checks.VALIDATORS["token_scores"]((torch.zeros(1, 3, 10), labels, 0, 1.0, IGNORE, None), {})
+    with pytest.raises(ValueError, match="token_scores"):
+        checks.VALIDATORS["token_scores"]((torch.zeros(1, 3, 9), labels, 0, 1.0, IGNORE, None), {})
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [148 * 32 - 4, 148 * 32])
+def test_middle_rows_by_warps_and_by_blocks(rows):
+    """Rows of 9,001 logits, few enough for a block to each and many enough for a warp."""
+    gen = torch.Generator().manual_seed(rows)
+    logits = (torch.randn(4, rows // 4, 9001, generator=gen) * 3).to(torch.bfloat16)
+    labels = torch.randint(0, 9001, (4, rows // 4), generator=gen)
+    got = ops.token_scores(logits.cuda(), labels.cuda(), top_k=7)
+    cut = (slice(None), slice(0, 40))
+    logs = torch.log_softmax(logits[cut].double(), -1)
+    want = logs.gather(2, labels[cut].unsqueeze(-1)).squeeze(-1)
+    assert ((got.logps[cut].cpu().double() - want).abs() <= TOL * (1 + want.abs())).all()
+    entropy = -(logs.exp() * logs).sum(-1)
+    assert ((got.entropy[cut].cpu().double() - entropy).abs() <= TOL * (1 + entropy)).all()
+    ids = torch.sort(logits[cut].double(), dim=-1, descending=True, stable=True).indices[..., :7]
+    assert torch.equal(got.top_ids[cut].cpu(), ids)
