@@ -383,7 +383,7 @@ template <typename T>
 void fwd_of(const ScoreArgs& a, cudaStream_t s) {
   // A warp to a row while it is short, or while there are rows for all warps: 2^28 bf16 logits in rows of 6,144 take 101 us with a
   // warp and 202 with 256 threads, in rows of 12,288 100 and 163, of 16,384 101 and 127 (with 20 alternatives 198 and 388, 188
-  // and 252, 212 and 191). Of few rows, each is a chain by itself, an eighth as long with 256 threads.
+  // and 252, 212 and 191); 4,736 rows of 12,288 34 and 44. Of few rows, each is a chain by itself, an eighth as long with 256 threads.
   const int n = a.rows.V / kVecOf<T>;
   if (n <= 768 || (n <= 1536 && (long long)a.rows.B * a.rows.T >= 148 * 32)) return fwd<T, 32>(a, s);
   fwd<T, 256>(a, s);

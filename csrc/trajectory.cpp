@@ -39,7 +39,7 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
   const bool bits8 = scales.has_value();
   const auto moment = bits8 ? torch::kFloat8_e4m3fn : torch::kFloat32;
   std::unordered_set<const void*> seen;
-  seen.reserve(2 * count);
+  seen.reserve(3 * count);
   std::vector<Tensor> held;  // gradients laid out like their parameters
   for (size_t i = 0; i < count; ++i) {
     const Tensor &p = params[i], &g = grads[i];
@@ -64,7 +64,8 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
                         "scales must be contiguous float32 (2, blocks of ", std::to_string(bw::kMomentBlock), " elements)");
     }
     if (p.numel() > 0)
-      TORCH_CHECK_VALUE(seen.insert(p.data_ptr()).second, "a parameter is given twice");
+      for (const Tensor* t : {&p, &exp_avgs[i], &exp_avg_sqs[i]})
+        TORCH_CHECK_VALUE(seen.insert(t->data_ptr()).second, "a parameter or a moment is given twice");
   }
   bw::AdamwTable<bw::kAdamwMany> table;
   table.s.beta1 = (float)beta1;

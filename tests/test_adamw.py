@@ -167,6 +167,8 @@ def test_refusals(device):
     ok = {"step": 1, "lr": 0.1}
     with pytest.raises(ValueError, match="twice"):
         ops.adamw_step([p, p], [g, g], [m, m.clone()], [v, v.clone()], **ok)
+    with pytest.raises(ValueError, match="twice"):
+        ops.adamw_step([p], [g], [m], [m], **ok)
     with pytest.raises(ValueError, match="needs a gradient"):
         ops.adamw_step([p], [], [m], [v], **ok)
     with pytest.raises(ValueError, match="shape"):

@@ -160,6 +160,14 @@ def test_fp16(shape):
     check(shape, torch.float16, "cuda")
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 70, 1, 5, 72, 64), (2, 66, 1, 6, 64, 128), (1, 130, 2, 7, 128, 64), (1, 70, 1, 8, 128, 128), (1, 65, 2, 10, 128, 200)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_many_value_heads_of_a_key_head(dtype, shape):
+    """Their rows of dq and dk are added up in clusters of 5 to 8, each of which owns a multiple of 16 rows."""
+    check(shape, dtype, "cuda")
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("layout", ["odd", "heads first"])
 def test_layouts(device, layout):
