@@ -42,6 +42,10 @@
 namespace bw {
 namespace {
 
+// Beside the workers and the warp that copies and multiplies, two warps compute the next chunk's factors. With 64 of the workers,
+// whose other warps then waited for them, a chunk took 1,700 of 10,200 cycles more.
+constexpr int kThreads = kWorkers + 32 + kChunk;
+
 // Of a chunk's tokens: what the products' columns are multiplied by.
 struct Factors {
   float grown_k[kChunk];  // exp(G) rk
@@ -98,7 +102,7 @@ struct StateMem {
                        kTiles = P + 2 * kTok;
 };
 
-enum StateBar { kGotKQ, kGotKQ2, kLoadedT, kLoadedP, kStateSet, kRhsSet, kWritesSet, kReadDone, kSolveDone, kStateDone, kOutDone, kFactorsSet, kStateBars };
+enum StateBar { kGotKQ, kGotKQ2, kLoadedT, kLoadedP, kHalfSet, kStateSet, kRhsSet, kWritesSet, kReadDone, kSolveDone, kStateDone, kOutDone, kFactorsSet, kStateBars };
 
 struct StateShared {
   uint64_t bar[kStateBars];
@@ -110,9 +114,9 @@ struct StateShared {
 // One slice of a head's state, chunk after chunk. Tensor memory: S^T (128 x DK), twice K S and Q S, then E and
 // after it P V', each in two halves.
 template <typename I, int DK, int DV>
-__global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd a) {
+__global__ void __launch_bounds__(kThreads, 1) state_kernel(const DeltaFwd a) {
   using Mem = StateMem<I, DK, DV>;
-  constexpr int P = kParts<I>, kSteps = DK / 16;
+  constexpr int P = kParts<I>;
   extern __shared__ __align__(1024) unsigned char mem[];
   StateShared& sh = *reinterpret_cast<StateShared*>(mem + Mem::kTiles);
   const DeltaDims& d = a.d;
@@ -123,7 +127,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
   const int tid = threadIdx.x, warp = tid >> 5;
   if (tid == 0) {
     for (int i = 0; i < kStateBars; ++i)
-      mbar_init(&sh.bar[i], i == kStateSet || i == kRhsSet || i == kWritesSet ? kWorkers : 1);
+      mbar_init(&sh.bar[i], i == kFactorsSet ? kChunk : i == kHalfSet || i == kStateSet || i == kRhsSet || i == kWritesSet ? kWorkers : 1);
     fence_barrier_init();
   }
   if (warp == kControl) tmem_alloc(&sh.tmem, 512);
@@ -171,10 +175,17 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
       int c = 0;
       for (; c < chunks; ++c) {
         const Operand KQ{base + Mem::KQ + (c & 1) * Mem::kStageKQ, Mem::kPanelKQ};
-        if (!wait(&sh.bar[kStateSet], c)) break;
         if (!wait(&sh.bar[c & 1 ? kGotKQ2 : kGotKQ], c >> 1)) break;
+        if constexpr (Mem::kPanels == 2) {  // the first half's products run while the second half is set
+          if (!wait(&sh.bar[kHalfSet], c)) break;
+          tc_fence_after();
+          multiply_parts<4, 128, false, false, 2, P>(tm + cK + (c & 1) * 128, S, Mem::kPlaneS, KQ, Mem::kPlaneKQ, false);
+        }
+        if (!wait(&sh.bar[kStateSet], c)) break;
         tc_fence_after();
-        multiply_parts<kSteps, 128, false, false, 2, P>(tm + cK + (c & 1) * 128, S, Mem::kPlaneS, KQ, Mem::kPlaneKQ, false);
+        constexpr int kLast = Mem::kPanels - 1;
+        multiply_parts<4, 128, false, false, 2, P>(tm + cK + (c & 1) * 128, Operand{S.addr + kLast * Mem::kPanelS, Mem::kPanelS}, Mem::kPlaneS,
+                                                   Operand{KQ.addr + kLast * Mem::kPanelKQ, Mem::kPanelKQ}, Mem::kPlaneKQ, kLast > 0);
         tc_commit(&sh.bar[kReadDone]);
         store_state(c);
         if (!wait(&sh.bar[kRhsSet], c)) break;
@@ -189,7 +200,6 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
         multiply_parts<4, DK, false, true, 2, P>(tm + cS, X, Mem::kPlaneX, KQ, Mem::kPlaneKQ, true);
         bulk_read_done();  // so is the state
         tc_commit(&sh.bar[kStateDone]);
-        mbar_arrive(&sh.bar[kFactorsSet]);
         if (!wait(&sh.bar[kLoadedP], c)) break;
         multiply_wide<4, 128, false, false, 2>(tm + cP, W, Mem::kPlaneX, At, false);
         tc_commit(&sh.bar[kOutDone]);
@@ -203,6 +213,14 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
         if (c + 1 < chunks) load_square(Mem::P, a.keep.attend, c + 1, &sh.bar[kLoadedP]);
       }
       bulk_done();
+    }
+  } else if (warp > kControl) {
+    const int i = tid - kWorkers - 32;
+    for (int c = 0; c + 1 < chunks; ++c) {
+      parts.read(a.keep, n0 + c + 1, m0 + c + 1, i);
+      if (!wait(&sh.bar[kStateSet], c)) break;  // all are done with the factors before this chunk's
+      parts.fill(sh.f[(c + 1) & 1], sh.grown_q[(c + 1) % 3], i);
+      mbar_arrive(&sh.bar[kFactorsSet]);
     }
   } else {
     const Seat seat;
@@ -248,13 +266,13 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
     for (int i = 0; i < 16; ++i) x[i] = ElemOf<I>::down(0.f);
     if (chunks > 0) take_values(0);
     for (int c = 0; c <= chunks; ++c) {
-      if (c > 0 && (!wait(&sh.bar[kStateDone], c - 1) || !wait(&sh.bar[kFactorsSet], c - 1))) break;
+      if (c > 0 && (!wait(&sh.bar[kStateDone], c - 1) || (c < chunks && !wait(&sh.bar[kFactorsSet], c - 1)))) break;
       tc_fence_after();
       const Factors& fac = sh.f[c & 1];
       const float left = c < chunks ? fac.left : 0.f;
 #pragma unroll
       for (int k = 0; k < kCols / 16; ++k) {
-        const int col = seat.part * kCols + k * 16;
+        const int col = k * 64 + seat.part * 16;
         float f[16];
         if (c > 0) {
           tmem_row(tm + seat.lanes + cS + col, f);
@@ -269,6 +287,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
             if (col + i < d.dk) a.last[(head * d.dk + col + i) * d.dv + v0 + seat.row] = f[i];
         }
         set_state(f, col, left);
+        if (k + 1 < kCols / 16) hand_over(&sh.bar[kHalfSet]);
       }
       tmem_st_wait();
       hand_over(&sh.bar[kStateSet]);
@@ -293,10 +312,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
         }
       }
       hand_over(&sh.bar[kRhsSet]);
-      if (c + 1 < chunks) {
-        take_values(c + 1);
-        if (tid < kChunk) parts.read(a.keep, n0 + c + 1, m0 + c + 1, tid);
-      }
+      if (c + 1 < chunks) take_values(c + 1);
       if (!wait(&sh.bar[kSolveDone], c)) break;
       tc_fence_after();
       tmem_sum(tm + seat.lanes + cE + tt, tm + seat.lanes + cE + 64 + tt, f);
@@ -313,7 +329,6 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) state_kernel(const DeltaFwd 
           put8(mem + Mem::X + at, mem + Mem::X + Mem::kPlaneX + at, y);
         }
       }
-      if (c + 1 < chunks && tid < kChunk) parts.fill(sh.f[(c + 1) & 1], sh.grown_q[(c + 1) % 3], tid);
       hand_over(&sh.bar[kWritesSet]);
     }
   }
@@ -336,7 +351,7 @@ struct DstateMem {
                        Q = K + kStages * kParts_ * kPlaneK, P = Q + kParts_ * kPlaneK, T = P + 2 * kTok, kTiles = T + 2 * kTok;
 };
 
-enum DstateBar { kGotK, kGotK2, kGotQ, kGotT, kDstateSet, kOutsSet, kGradSet, kReadsSet, kMixDone, kOutsDone, kBackDone, kDstateDone, kTilesFree, kPartsSet, kDstateBars };
+enum DstateBar { kGotK, kGotK2, kGotQ, kGotT, kHalfDset, kDstateSet, kOutsSet, kGradSet, kReadsSet, kMixDone, kOutsDone, kBackDone, kDstateDone, kTilesFree, kPartsSet, kDstateBars };
 
 struct DstateShared {
   uint64_t bar[kDstateBars];
@@ -348,9 +363,9 @@ struct DstateShared {
 // One slice of the gradient of a head's state, from the last chunk to the first. Tensor memory: dS^T (128 x DK), K dS',
 // P^T dO and dV in two halves each.
 template <typename I, int DK, int DV>
-__global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd a) {
+__global__ void __launch_bounds__(kThreads, 1) dstate_kernel(const DeltaBwd a) {
   using Mem = DstateMem<I, DK, DV>;
-  constexpr int P = kParts<I>, kSteps = DK / 16, kStages = Mem::kStages;
+  constexpr int P = kParts<I>, kStages = Mem::kStages;
   extern __shared__ __align__(1024) unsigned char mem[];
   DstateShared& sh = *reinterpret_cast<DstateShared*>(mem + Mem::kTiles);
   const DeltaDims& d = a.d;
@@ -361,7 +376,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
   const int tid = threadIdx.x, warp = tid >> 5;
   if (tid == 0) {
     for (int i = 0; i < kDstateBars; ++i)
-      mbar_init(&sh.bar[i], i == kDstateSet || i == kOutsSet || i == kGradSet || i == kReadsSet ? kWorkers : 1);
+      mbar_init(&sh.bar[i], i == kPartsSet ? kChunk : i == kHalfDset || i == kDstateSet || i == kOutsSet || i == kGradSet || i == kReadsSet ? kWorkers : 1);
     fence_barrier_init();
   }
   if (warp == kControl) tmem_alloc(&sh.tmem, 512);
@@ -400,10 +415,17 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
           O{base + Mem::O, Mem::kPlaneX}, Q{base + Mem::Q, kTok}, At{base + Mem::P, kTok}, T{base + Mem::T, kTok};
       for (int r = 0; r < chunks; ++r) {
         const Operand K{base + Mem::K + r % kStages * P * Mem::kPlaneK, kTok};
-        if (!wait(&sh.bar[kDstateSet], r)) break;
         if (!wait(&sh.bar[kStages == 2 && (r & 1) ? kGotK2 : kGotK], kStages == 2 ? r >> 1 : r)) break;
+        if constexpr (Mem::kPanels == 2) {
+          if (!wait(&sh.bar[kHalfDset], r)) break;
+          tc_fence_after();
+          multiply_parts<4, 64, false, false, 2, P>(tm + cK, S, Mem::kPlaneS, K, Mem::kPlaneK, false);
+        }
+        if (!wait(&sh.bar[kDstateSet], r)) break;
         tc_fence_after();
-        multiply_parts<kSteps, 64, false, false, 2, P>(tm + cK, S, Mem::kPlaneS, K, Mem::kPlaneK, false);
+        constexpr int kLast = Mem::kPanels - 1;
+        multiply_parts<4, 64, false, false, 2, P>(tm + cK, Operand{S.addr + kLast * Mem::kPanelS, Mem::kPanelS}, Mem::kPlaneS,
+                                                  Operand{K.addr + kLast * kTok, kTok}, Mem::kPlaneK, kLast > 0);
         if (!wait(&sh.bar[kOutsSet], r)) break;
         if (!wait(&sh.bar[kGotQ], r)) break;
         tc_fence_after();
@@ -428,7 +450,6 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
         multiply_parts<4, DK, false, true, 2, P>(tm + cS, X, Mem::kPlaneX, K, Mem::kPlaneK, true);
         bulk_read_done();  // dS' and dO are copied: their places may be written once this product is done
         tc_commit(&sh.bar[kDstateDone]);
-        mbar_arrive(&sh.bar[kPartsSet]);
         bulk_store(a.dreads + at_n * 2 * Mem::kPlaneX, mem + Mem::Y, 2 * Mem::kPlaneX);
         bulk_commit();
         bulk_read_done();
@@ -437,6 +458,14 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
         if (r + kStages < chunks) load_k(r + kStages);
       }
       bulk_done();
+    }
+  } else if (warp > kControl) {
+    const int i = tid - kWorkers - 32;
+    for (int r = 0; r + 1 < chunks; ++r) {
+      parts.read(a.keep, n0 + chunks - 2 - r, m0 + chunks - 2 - r, i);
+      if (!wait(&sh.bar[kDstateSet], r)) break;  // all are done with the factors before this chunk's
+      parts.fill(sh.f[(r + 1) & 1], sh.grown_q[(r + 1) & 1], i);
+      mbar_arrive(&sh.bar[kPartsSet]);
     }
   } else {
     const Seat seat;
@@ -455,13 +484,13 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
     if (chunks > 0) take_outs(chunks - 1);
     for (int r = 0; r <= chunks; ++r) {
       const int c = chunks - 1 - r;
-      if (r > 0 && (!wait(&sh.bar[kDstateDone], r - 1) || !wait(&sh.bar[kPartsSet], r - 1))) break;
+      if (r > 0 && (!wait(&sh.bar[kDstateDone], r - 1) || (c >= 0 && !wait(&sh.bar[kPartsSet], r - 1)))) break;
       tc_fence_after();
       const Factors& fac = sh.f[r & 1];
       const float left = c >= 0 ? fac.left : 0.f;
 #pragma unroll
       for (int k = 0; k < kCols / 16; ++k) {
-        const int col = seat.part * kCols + k * 16;
+        const int col = k * 64 + seat.part * 16;
         float f[16];
         if (r > 0) {
           tmem_row(tm + seat.lanes + cS + col, f);
@@ -492,6 +521,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
 #pragma unroll
         for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(f[i] * left);
         tmem_st_32x32b_x16(tm + seat.lanes + cS + col, u);
+        if (k + 1 < kCols / 16) hand_over(&sh.bar[kHalfDset]);
       }
       if (c < 0) break;
       tmem_st_wait();
@@ -512,10 +542,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
         }
       }
       hand_over(&sh.bar[kOutsSet]);
-      if (c > 0) {
-        take_outs(c - 1);
-        if (tid < kChunk) parts.read(a.keep, n0 + c - 1, m0 + c - 1, tid);
-      }
+      if (c > 0) take_outs(c - 1);
       if (!wait(&sh.bar[kMixDone], r)) break;
       tc_fence_after();
       float f[16], y16[16];
@@ -551,7 +578,6 @@ __global__ void __launch_bounds__(kWorkers + 32, 1) dstate_kernel(const DeltaBwd
           put8(mem + Mem::X + at, mem + Mem::X + Mem::kPlaneX + at, y);
         }
       }
-      if (c > 0 && tid < kChunk) parts.fill(sh.f[(r + 1) & 1], sh.grown_q[(r + 1) & 1], tid);
       hand_over(&sh.bar[kReadsSet]);
       const int t = c * kChunk + tt;
       if (in) put_column(dv + t * step, step, d.T - t, f);
@@ -570,7 +596,7 @@ void state(const DeltaFwd& a, cudaStream_t s) {
   constexpr int bytes = StateMem<I, DK, DV>::kTiles + (int)sizeof(StateShared);
   static_assert(bytes <= 227 * 1024, "shared memory");
   cudaFuncSetAttribute(state_kernel<I, DK, DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  state_kernel<I, DK, DV><<<(unsigned)(a.d.B * a.d.H * a.d.slices), kWorkers + 32, bytes, s>>>(a);
+  state_kernel<I, DK, DV><<<(unsigned)(a.d.B * a.d.H * a.d.slices), kThreads, bytes, s>>>(a);
 }
 
 template <typename I, int DK, int DV>
@@ -578,7 +604,7 @@ void dstate(const DeltaBwd& a, cudaStream_t s) {
   constexpr int bytes = DstateMem<I, DK, DV>::kTiles + (int)sizeof(DstateShared);
   static_assert(bytes <= 227 * 1024, "shared memory");
   cudaFuncSetAttribute(dstate_kernel<I, DK, DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  dstate_kernel<I, DK, DV><<<(unsigned)(a.d.B * a.d.H * a.d.slices), kWorkers + 32, bytes, s>>>(a);
+  dstate_kernel<I, DK, DV><<<(unsigned)(a.d.B * a.d.H * a.d.slices), kThreads, bytes, s>>>(a);
 }
 
 template <typename I>

@@ -60,6 +60,19 @@ def recurrence(x, first, scale=None):
     return torch.stack(outs, 1), state
 
 
+def gate_terms(x, out, g_out, dv):
+    """On the CPU the log-decay's gradient at a token is a sum over the rest of its chunk of what tokens give less what they
+    take (q . dq - v . dv), whose terms cancel: up to 64 of them with errors of random sign, 8 times one's. Those errors' size
+    for each gate's gradient."""
+    wide = {n: x[n].detach().double().cpu() for n in ("a", "a_log", "dt_bias", "v")}
+    each = (out * g_out.double().cpu()).sum(-1).abs() + (wide["v"] * dv).sum(-1).abs()
+    dt = wide["a"] + wide["dt_bias"]
+    da = 8 * each.square().mean((0, 1)).sqrt() * wide["a_log"].exp() * torch.sigmoid(dt).square().mean((0, 1)).sqrt()
+    n = each[..., 0].numel() ** 0.5
+    ratio = (torch.nn.functional.softplus(dt) / torch.sigmoid(dt)).square().mean((0, 1)).sqrt()
+    return {"a": da.detach(), "dt_bias": (da * n).detach(), "a_log": (da * n * ratio).detach()}
+
+
 def gate_sums(x, da):
     """The gradients of a_log and dt_bias are sums of all tokens' shares, of either sign, each with errors of its own size: what such
     a sum comes to where signs are random, whatever they happen to cancel to in one head."""
@@ -111,7 +124,7 @@ def check(shape, dtype, device, *, state=False, layout="sliced", g_state=False, 
     cpu = device == "cpu"
     close("out", out, want, dtype, terms * 2.0 ** (-18 if cpu else -9))
     close("state", last, want_last, torch.float32, terms * 2.0 ** (-18 if cpu else -12))
-    sums = gate_sums(x, grads["a"])
+    sums = gate_terms(x, want.detach(), g_out, grads["v"]) if cpu else gate_sums(x, grads["a"])
     for n, g in zip((*NAMES, "state"), got, strict=False):
         close("d" + n, g, grads[n], g.dtype, terms * 2.0 ** (-16 if cpu else -9), sums.get(n, 0.0))
 
@@ -161,7 +174,7 @@ def test_fp16(shape):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("shape", [(1, 70, 1, 5, 72, 64), (2, 66, 1, 6, 64, 128), (1, 130, 2, 7, 128, 64), (1, 70, 1, 8, 128, 128), (1, 65, 2, 10, 128, 200)])
+@pytest.mark.parametrize("shape", [(1, 70, 1, 5, 72, 64), (2, 66, 1, 6, 64, 128), (1, 130, 2, 14, 128, 64), (1, 70, 1, 8, 128, 128), (1, 65, 2, 10, 128, 200)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_many_value_heads_of_a_key_head(dtype, shape):
     """Their rows of dq and dk are added up in clusters of 5 to 8, each of which owns a multiple of 16 rows."""
