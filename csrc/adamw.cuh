@@ -40,7 +40,7 @@ struct AdamwTable {
 };
 
 // Elements of a CTA for a step of `total`: the more there are, the more a CTA takes before the next one has to find its tensor
-// and fill its pipeline again; a few CTAs for each SM at least. 137,000 weights take 2.8 us in chunks of 2048 and 7.5 in chunks
+// and fill its pipeline again; a few CTAs for each SM at least. 125,000 weights take 2.8 us in chunks of 2048 and 7.5 in chunks
 // of 32768.
 inline int adamw_chunk(int64_t total, bool bits8) {
   const int most = bits8 ? 32768 : 8192;

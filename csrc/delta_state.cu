@@ -34,8 +34,8 @@
 // multiplies; sixteen warps turn sums into halves.
 //
 // What bounds it: a chunk's chain of three products and three conversions, each waiting for the one before. 4 x 2048 tokens, 32
-// heads of 128 x 128, bf16 (128 CTAs, 32 chunks each): state 172 us, dstate 164 us, 5.3 us a chunk, while the bytes (0.85
-// GB each) would take 130 us. On instructions of single warps (state and outputs as kernels of their own):
+// heads of 128 x 128, bf16 (128 CTAs, 32 chunks each): state 152 us, dstate 165 us, 5 us a chunk, while the bytes (0.85
+// GB each) would take 130 us. The first half of a state's columns is multiplied while the second is turned into halves. On instructions of single warps (state and outputs as kernels of their own):
 // 354 + 195 us and 594 us. Eight converting warps instead of sixteen: a training pass 1085 us instead of 1000.
 #include "delta_tiles.cuh"
 
