@@ -45,7 +45,8 @@ def _mixer_forward(self, hidden_states: torch.Tensor, cache_params=None, attenti
     """The mixer's forward through :mod:`dattri_llm_b200.ops.delta`."""
     layer = cache_params.layers[self.layer_idx] if cache_params is not None else None
     started = layer is not None and layer.has_previous_state
-    if not _supported(self, hidden_states) or (started and hidden_states.shape[1] > 1):
+    tracked = torch.is_grad_enabled() and (hidden_states.requires_grad or any(p.requires_grad for p in self.parameters()))
+    if not _supported(self, hidden_states) or (started and (hidden_states.shape[1] > 1 or tracked)):  # the step has no gradient
         return type(self).forward(self, hidden_states, cache_params=cache_params, attention_mask=attention_mask, **kwargs)
     if attention_mask is not None and attention_mask.shape[0] > 1 and attention_mask.shape[1] > 1:
         hidden_states = (hidden_states * attention_mask[:, :, None]).to(hidden_states.dtype)  # padding writes nothing

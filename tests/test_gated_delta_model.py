@@ -89,6 +89,23 @@ def test_generation_goes_on_from_the_cached_state(device):
     assert (torch.cat(got, 1) - want).abs().max() <= tol * want.abs().max()
 
 
+def test_a_cached_token_does_not_lose_gradients_in_silence():
+    """The step in place has none: where they are wanted, the mixer runs its own forward, and a backward does what the
+    library's does (it raises: the cached state was updated in place)."""
+    logits = []
+    for fast in (False, True):
+        model = _model()
+        if fast:
+            accelerate_gated_delta(model, linears=False)
+        ids = _ids(2, 9)
+        with torch.no_grad():
+            cache = model(input_ids=ids[:, :8], use_cache=True).past_key_values
+        logits.append(model(input_ids=ids[:, 8:], past_key_values=cache, use_cache=True).logits)
+        with pytest.raises(RuntimeError, match="inplace"):
+            logits[-1].square().sum().backward()
+    torch.testing.assert_close(logits[1], logits[0], rtol=1e-4, atol=1e-4 * float(logits[0].detach().abs().max()))
+
+
 @pytest.mark.gpu
 def test_bf16_model_stays_near_the_library_model_in_fp32():
     theirs = _model("cuda")
