@@ -11,7 +11,7 @@
 //
 // What bounds it: one CTA of 208 KB of tiles to an SM, whose steps (tiles in, three products, the small matrices, three more, rows
 // out) wait for one another: 2,600 instructions a warp fill 39 % of the issue slots, memory runs at a quarter of its rate. 4 x
-// 2048 tokens, 16 key and 32 value heads of 128 x 128, bf16: 391 us (1734 on instructions of single warps); 1.05 GB to read
+// 2048 tokens, 16 key and 32 value heads of 128 x 128, bf16: 395 us (1734 on instructions of single warps); 1.05 GB to read
 // and write, 160 us. Clusters that stay and take chunk after chunk: 451 us, the last rows and the next tiles share their place.
 #include <cooperative_groups.h>
 

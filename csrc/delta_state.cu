@@ -30,13 +30,15 @@
 // state is 1e-6 to 6e-6 of its norm off.
 //
 // Layout: a CTA has up to 128 value elements of a head, one a lane of tensor memory, so that all of a token's factors are by columns
-// and the state's rows are the lanes: S^T, its reads by keys and queries, E and the outputs. The last warp's first lane copies and
-// multiplies; sixteen warps turn sums into halves.
+// and the state's rows are the lanes: S^T, its reads by keys and queries, E and the outputs. One warp's first lane copies and
+// multiplies, sixteen warps turn sums into halves, two compute the tokens' factors a chunk ahead.
 //
 // What bounds it: a chunk's chain of three products and three conversions, each waiting for the one before. 4 x 2048 tokens, 32
 // heads of 128 x 128, bf16 (128 CTAs, 32 chunks each): state 152 us, dstate 165 us, 5 us a chunk, while the bytes (0.85
-// GB each) would take 130 us. The first half of a state's columns is multiplied while the second is turned into halves. On instructions of single warps (state and outputs as kernels of their own):
-// 354 + 195 us and 594 us. Eight converting warps instead of sixteen: a training pass 1085 us instead of 1000.
+// GB each) would take 130 us. The first half of a state's columns is multiplied while the second is turned into halves. States are
+// copied out behind the products that read them: in front of them, 156 and 181 us, since both read shared memory. On
+// instructions of single warps (state and outputs as kernels of their own): 354 + 195 us and 594 us. Eight converting warps
+// instead of sixteen: a training pass 1085 us instead of 1000.
 #include "delta_tiles.cuh"
 
 namespace bw {

@@ -303,3 +303,23 @@ def test_gradients_whose_squares_overflow_move_nothing(device, bits):
     m, v, s = ops.adamw_state(p, bits)
     ops.adamw_step([p], [g], [m], [v], None if s is None else [s], step=1, lr=0.1, weight_decay=0.0)
     assert torch.equal(p, torch.ones_like(p))  # m / inf
+
+
+@pytest.mark.gpu
+def test_elements_that_32_bits_do_not_count():
+    """The last elements of a tensor of more than 2^31 move as they do by themselves (whole blocks before them)."""
+    n = 2**31 + 700
+    p, g = torch.zeros(n, dtype=torch.bfloat16, device="cuda"), torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    m, v, s = ops.adamw_state(p, 8)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    for x in (p, g):
+        x[2**31 - 256:] = torch.randn(956, generator=gen, device="cuda")
+    few = [x[2**31 - 256:].clone() for x in (p, g)]
+    fm, fv, fs = ops.adamw_state(few[0], 8)
+    for step in (1, 2):
+        ops.adamw_step([p], [g], [m], [v], [s], step=step, lr=0.1)
+        ops.adamw_step([few[0]], [few[1]], [fm], [fv], [fs], step=step, lr=0.1)
+    assert torch.equal(p[2**31 - 256:], few[0]) and not p[:2**31 - 256].any()
+    assert torch.equal(m[2**31 - 256:].view(torch.uint8), fm.view(torch.uint8))
+    assert torch.equal(v[2**31 - 256:].view(torch.uint8), fv.view(torch.uint8))
+    assert torch.equal(s[:, -fs.shape[1]:], fs)

@@ -389,3 +389,38 @@ def test_the_same_call_gives_the_same_bits_and_two_graphs_share_nothing():
     for z, grads in zip((x, y), late, strict=True):
         alone = torch.autograd.grad(ops.gated_delta_rule(*(z[n] for n in NAMES))[0], [z[n] for n in NAMES], g)
         assert all(torch.equal(a, b) for a, b in zip(alone, grads, strict=True))
+
+
+@pytest.mark.gpu
+def test_the_last_of_many_sequences_is_as_it_is_alone():
+    """Workspaces of more than 2^32 bytes (eight sequences of 8,192 tokens): every sequence's results are its own, to the bit."""
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    b, t, hk, h, d = 8, 8192, 8, 16, 128
+    rnd = functools.partial(torch.randn, generator=gen, device="cuda", dtype=torch.bfloat16)
+    x = [rnd(b, t, hk, d), rnd(b, t, hk, d), rnd(b, t, h, d), rnd(b, t, h), rnd(b, t, h)]
+    shared = [torch.zeros(h, device="cuda"), torch.full((h,), -3.0, device="cuda")]
+    g = rnd(b, t, h, d)
+    results = []
+    for cut in (slice(None), slice(b - 1, b)):
+        own = [y[cut].detach().requires_grad_(True) for y in x]
+        out, last = ops.gated_delta_rule(*own, *shared, output_final_state=True)
+        results.append([y[-1] for y in (out, last, *torch.autograd.grad(out, own, g[cut]))])
+    assert all(torch.isfinite(y).all() for y in results[1])
+    assert all(torch.equal(p, q) for p, q in zip(*results, strict=True))
+
+
+@pytest.mark.gpu
+def test_states_that_32_bits_do_not_count():
+    """2^31 elements of state and more: the last sequences step as they do by themselves."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    b, few, hk, h, d = 2**31 // (16 * 128 * 128) + 20, 20, 8, 16, 128  # few * h: enough for the blocks that stay
+    rnd = functools.partial(torch.randn, generator=gen, device="cuda")
+    x = [y.to(torch.bfloat16) for y in (rnd(b, 1, hk, d), rnd(b, 1, hk, d), rnd(b, 1, h, d), rnd(b, 1, h), rnd(b, 1, h))]
+    shared = [torch.zeros(h, device="cuda"), torch.full((h,), -3.0, device="cuda")]
+    state = torch.zeros(b, h, d, d, device="cuda")
+    state[-few:] = rnd(few, h, d, d)
+    own = state[-few:].clone()
+    with torch.no_grad():
+        out = ops.gated_delta_step(*x, *shared, state)
+        want = ops.gated_delta_step(*(y[-few:] for y in x), *shared, own)
+    assert torch.equal(out[-few:], want) and torch.equal(state[-few:], own)

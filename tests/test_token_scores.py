@@ -304,3 +304,18 @@ def test_middle_rows_by_warps_and_by_blocks(rows):
     assert ((got.entropy[cut].cpu().double() - entropy).abs() <= TOL * (1 + entropy)).all()
     ids = torch.sort(logits[cut].double(), dim=-1, descending=True, stable=True).indices[..., :7]
     assert torch.equal(got.top_ids[cut].cpu(), ids)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v", [1000, 20000])
+def test_rows_further_apart_than_32_bits_count(v):
+    """Two rows 2^31 elements apart: their scores and gradients are those of the rows side by side."""
+    far = torch.zeros(2**31 + v, dtype=torch.bfloat16, device="cuda").as_strided((1, 2, v), (0, 2**31, 1))
+    near, labels = make(1, 2, v, torch.bfloat16, "cuda")
+    far.copy_(near)
+    got = []
+    for x in (far, near):
+        x = x.detach().requires_grad_(True)
+        r = ops.token_scores(x, labels, top_k=3)
+        got.append((r.logps, r.entropy, r.top_logps, r.top_ids, torch.autograd.grad((r.logps.sum() + r.entropy.sum()), x)[0]))
+    assert all(torch.equal(a, b) for a, b in zip(*got, strict=True))
