@@ -123,7 +123,8 @@ __global__ void __launch_bounds__(kThreads) adamw32_kernel(const __grid_constant
 }
 
 // An e4m3 code's exponent and significand as the low exponent bits and the significand of an fp32 number are that number
-// times 2^-120, small codes included; 2^120 joins the scale. The codes of NaN never come: a NaN goes into the scale.
+// times 2^-120, small codes included. 2^120 is a product of its own, which is exact: with it in the scale, scales from 256 on would
+// be infinite. The codes of NaN never come: a NaN goes into the scale.
 constexpr float kF8Up = 1329227995784915872903807060280344576.f;  // 2^120
 
 // Code k of a word, with and without a sign.
@@ -241,8 +242,8 @@ __global__ void __launch_bounds__(kThreads, 4) adamw8_kernel(const __grid_consta
     fetch8<G>(b.g, g + from, wide, n);
     b.m = fetch_codes(m + from, wide, n);
     b.v = fetch_codes(v + from, wide, n);
-    b.sm = scale[block] * kF8Up;
-    b.sv = scale[blocks + block] * kF8Up;
+    b.sm = scale[block];
+    b.sv = scale[blocks + block];
   };
   long long block = first + (threadIdx.x >> 5);
   if (block >= end) return;
@@ -261,8 +262,10 @@ __global__ void __launch_bounds__(kThreads, 4) adamw8_kernel(const __grid_consta
 #pragma unroll
     for (int k = 0; k < kN; k += 2) {
       const float2 g2 = make_float2(gf[k], gf[k + 1]);
-      const float2 r = __fmul2_rn(make_float2(f8_up_plus(vw[k / 4], k % 4), f8_up_plus(vw[k / 4], k % 4 + 1)), two(now.sv));
-      const float2 old = __fmul2_rn(make_float2(f8_up(mw[k / 4], k % 4), f8_up(mw[k / 4], k % 4 + 1)), two(now.sm));
+      const float2 v_code = make_float2(f8_up_plus(vw[k / 4], k % 4), f8_up_plus(vw[k / 4], k % 4 + 1));
+      const float2 m_code = make_float2(f8_up(mw[k / 4], k % 4), f8_up(mw[k / 4], k % 4 + 1));
+      const float2 r = __fmul2_rn(__fmul2_rn(v_code, two(kF8Up)), two(now.sv));
+      const float2 old = __fmul2_rn(__fmul2_rn(m_code, two(kF8Up)), two(now.sm));
       const float2 m2 = sum_of(__fmul2_rn(two(a.s.beta1), old), __fmul2_rn(two(a.s.one_beta1), g2));
       const float2 v2 = sum_of(__fmul2_rn(two(a.s.beta2), __fmul2_rn(r, r)), __fmul2_rn(__fmul2_rn(two(a.s.one_beta2), g2), g2));
       const float2 root = roots_of(v2), den = __ffma2_rn(root, two(a.s.inv_root2), two(a.s.eps));

@@ -323,3 +323,56 @@ def test_elements_that_32_bits_do_not_count():
     assert torch.equal(m[2**31 - 256:].view(torch.uint8), fm.view(torch.uint8))
     assert torch.equal(v[2**31 - 256:].view(torch.uint8), fv.view(torch.uint8))
     assert torch.equal(s[:, -fs.shape[1]:], fs)
+
+
+def check_one_step(p, g, m, v, scales, step, *, lr, betas, eps):
+    """A step without weight decay against the formula in 64 bits on the moments that the state stood for before it.  Beside what
+    the module's tolerances count, a sum of products below fp32's normal range is rounded to steps of 2^-149, in four
+    roundings by 2^-148 together, half of it relative to the root."""
+    bits8 = scales is not None
+    old = p.double()
+    m0, v0 = (x.double() for x in ops.adamw_moments(m, v, scales))
+    g = g.double()
+    ops.adamw_step([p], [g.to(p.dtype)], [m], [v], [scales] if bits8 else None, step=step, lr=lr, betas=betas, eps=eps, weight_decay=0.0)
+    b1, b2 = betas
+    wm, wv = b1 * m0 + (1 - b1) * g, b2 * v0 + (1 - b2) * g * g
+    terms = b1 * m0.abs() + (1 - b1) * g.abs()
+    root_off = torch.where(wv > 0, (2.0 ** -149 / wv.clamp(min=1e-300)).clamp(max=1.0), 0.0)
+    by = lr / (1 - b1 ** step) / ((wv / (1 - b2 ** step)).sqrt() + eps)
+    by = torch.where(terms > 0, by, 0.0)
+    want = old - by * wm
+    half = torch.finfo(p.dtype).eps / 2
+    assert torch.isfinite(p).all()
+    assert ((p.double() - want).abs() <= half * want.abs() + (SLACK + 2 * root_off) * (old.abs() + by * terms)).all()
+    gm, gv = (x.double() for x in ops.adamw_moments(m, v, scales))
+    if not bits8:
+        assert ((gm - wm).abs() <= SLACK * terms + 2.0 ** -148).all()
+        assert ((gv - wv).abs() <= SLACK * wv + 2.0 ** -148).all()
+        return
+    n = p.numel()
+    roots = v.double() * scales[1].double().repeat_interleave(256)[:n]  # not through the reader, which squares them in 32 bits
+    for got, true, off, smallest in ((gm, wm, 0.0, 2.0 ** -10), (roots, wv.sqrt(), root_off, 2.0 ** -9)):
+        flat = torch.nn.functional.pad((true.abs() * (1 + off)).reshape(-1), (0, -n % 256)).view(-1, 256)
+        each = (flat.amax(1) / 448).repeat_interleave(256)[:n].view(p.shape)
+        spread = SLACK * terms if true is wm else 0.0
+        assert ((got - true).abs() <= (2.0 ** -4 + SLACK + off) * true.abs() + (smallest + SLACK) * each + spread).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_large_finite_moments_stay_numbers(device, bits, dtype):
+    """Gradients up to 1e17, whose moments' scales pass 256 from 1.2e6 on, in some elements of some blocks, over several steps: none of the
+    elements beside them is lost.  One tensor moves by whole vectors, one by single elements."""
+    gen = torch.Generator().manual_seed(5)
+    for offset in (0, 1):
+        n = 256 * 5 + 40
+        p = (torch.randn(n + offset, generator=gen)).to(device, dtype)[offset:]
+        m, v, s = ops.adamw_state(p, bits)
+        for step in range(1, 6):
+            g = torch.randn(n, generator=gen)
+            if step != 4:
+                for block, size in enumerate((1.0, 1.3e6, 2e6, 1e10, 1e15)):
+                    g[block * 256 + 7 * step] *= size
+                g[-3] = -1e17
+            check_one_step(p, g.to(device, dtype), m, v, s, step, lr=3e-3, betas=(0.9, 0.99), eps=1e-8)
