@@ -22,10 +22,11 @@ namespace {
 constexpr int kThreads = 256, kN = 8;  // elements of a thread's step
 constexpr float kF8Max = 448.f, kF8Tiny = 0.001953125f;
 
-// Square root and reciprocal to an ulp or two, in one instruction each where the compiler's correctly rounded ones take ten.
+// Square root and reciprocal to an ulp or two, in a few instructions where the compiler's correctly rounded ones take ten. The root
+// takes numbers below the normal range, squares of gradients under 1e-19; the reciprocal is of a root, 3e-23 at least, or of eps.
 __device__ __forceinline__ float root_of(float v) {
   float r;
-  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
 __device__ __forceinline__ float inverse_of(float v) {
@@ -158,14 +159,15 @@ __device__ __forceinline__ float2 two(float x) { return make_float2(x, x); }
 // Sums of products that are rounded first: no product joins the addition as a fused one.
 __device__ __forceinline__ float2 sum_of(float2 x, float2 y) { return make_float2(__fadd_rn(x.x, y.x), __fadd_rn(x.y, y.y)); }
 
-// Square roots of two values, to half an ulp or so: the estimate of the reciprocal root and a step of Newton's method on the
-// largest number at most; what an infinity has over that comes on top. 0 stays 0.
+// Square roots of two values, to half an ulp or so (an ulp or two below the normal range, where the rest is rounded to its steps):
+// the estimate of the reciprocal root and a step of Newton's method on the largest number at most; what an infinity has over
+// that comes on top. 0 stays 0.
 __device__ __forceinline__ float2 roots_of(float2 v) {
   float2 r, w;
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(w.x) : "f"(v.x), "f"(3.4028234663852886e38f));
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(w.y) : "f"(v.y), "f"(3.4028234663852886e38f));
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(fmaxf(w.x, 1.2e-38f)));
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(fmaxf(w.y, 1.2e-38f)));
+  asm("rsqrt.approx.f32 %0, %1;" : "=f"(r.x) : "f"(fmaxf(w.x, 1.4e-45f)));
+  asm("rsqrt.approx.f32 %0, %1;" : "=f"(r.y) : "f"(fmaxf(w.y, 1.4e-45f)));
   const float2 s = __fmul2_rn(w, r), over = __fadd2_rn(v, make_float2(-w.x, -w.y));
   const float2 rest = __ffma2_rn(make_float2(-s.x, -s.y), s, w);
   return __fadd2_rn(__ffma2_rn(rest, __fmul2_rn(r, two(0.5f)), s), over);

@@ -376,3 +376,17 @@ def test_large_finite_moments_stay_numbers(device, bits, dtype):
                     g[block * 256 + 7 * step] *= size
                 g[-3] = -1e17
             check_one_step(p, g.to(device, dtype), m, v, s, step, lr=3e-3, betas=(0.9, 0.99), eps=1e-8)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [8, 32])
+def test_roots_below_the_normal_range(device, bits):
+    """Gradients of 1e-21 to 1e-17 with eps = 0: their squares are subnormal numbers of fp32 (from 1e-44 on), their roots are not."""
+    gen = torch.Generator().manual_seed(6)
+    for offset in (0, 1):
+        n = 256 * 3 + 40
+        p = torch.randn(n + offset, generator=gen).to(device)[offset:]
+        m, v, s = ops.adamw_state(p, bits)
+        for step in range(1, 4):
+            g = 10.0 ** (-21 + 4 * torch.rand(n, generator=gen)) * (1 - 2 * (torch.rand(n, generator=gen) < 0.5).float())
+            check_one_step(p, g.to(device), m, v, s, step, lr=3e-3, betas=(0.9, 0.99), eps=0.0)
