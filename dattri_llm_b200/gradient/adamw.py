@@ -18,7 +18,8 @@ class AdamW(torch.optim.AdamW):
 
     Args:
         state_bits: 32 (fp32 moments, whatever the parameters' type) or 8 (e4m3 codes with a
-            scale for every 256 elements); also a setting of a parameter group.
+            scale for every 256 elements); also a setting of a parameter group.  It says how the
+            states of new parameters are held: loaded ones keep the form that they were saved in.
 
     The update counts are kept on the host: a step is not captured into a CUDA graph, which
     would repeat one count's bias correction.  Parameters sharded as DTensors (FSDP2) are not supported.
@@ -85,8 +86,13 @@ class AdamW(torch.optim.AdamW):
         return m if key == "exp_avg" else v
 
     def load_state_dict(self, state_dict: dict) -> None:
-        """As ``torch.optim``'s, without its cast of the states to the parameters' type."""
+        """As ``torch.optim``'s, without its cast of the states to the parameters' type.  A state of
+        ``torch.optim.AdamW`` is taken too; ``state_bits``, which it does not have, stay as they are."""
+        bits = [group["state_bits"] for group in self.param_groups]
         super().load_state_dict(state_dict)
+        for group, own in zip(self.param_groups, bits, strict=True):
+            group.setdefault("state_bits", own)
+            self._settle(group)
         saved = state_dict["state"]
         ids = (i for group in state_dict["param_groups"] for i in group["params"])
         params = (p for group in self.param_groups for p in group["params"])

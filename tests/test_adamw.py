@@ -390,3 +390,33 @@ def test_roots_below_the_normal_range(device, bits):
         for step in range(1, 4):
             g = 10.0 ** (-21 + 4 * torch.rand(n, generator=gen)) * (1 - 2 * (torch.rand(n, generator=gen) < 0.5).float())
             check_one_step(p, g.to(device), m, v, s, step, lr=3e-3, betas=(0.9, 0.99), eps=0.0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_state_of_torchs_own_adamw_goes_on(device, bits, dtype):
+    """Its moments are taken as they are, its groups' settings too; a parameter that it has no state of gets one of `bits`."""
+    torch.manual_seed(7)
+    kw = {"lr": 1e-2, "betas": (0.9, 0.95), "weight_decay": 0.2}
+    first, late = (torch.nn.Parameter(torch.randn(40, 9, device=device).to(dtype)) for _ in range(2))
+    theirs = torch.optim.AdamW([first, late], **kw)
+    _steps(theirs, first, [torch.randn_like(first) for _ in range(3)])
+    mine = bw.AdamW([first, late], lr=5.0, state_bits=bits)
+    mine.load_state_dict(copy.deepcopy(theirs.state_dict()))
+    group = mine.param_groups[0]
+    assert group["lr"] == kw["lr"] and group["state_bits"] == bits
+    m0, v0 = (theirs.state[first][key].double() for key in ("exp_avg", "exp_avg_sq"))
+    for key, was in (("exp_avg", m0), ("exp_avg_sq", v0)):
+        assert torch.equal(mine.moment(first, key).double(), was)
+    old, g = first.detach().double(), torch.randn_like(first)
+    first.grad, late.grad = g, g.clone()
+    mine.step()
+    (b1, b2), g = kw["betas"], g.double()
+    m, v = b1 * m0 + (1 - b1) * g, b2 * v0 + (1 - b2) * g * g
+    by = kw["lr"] / (1 - b1 ** 4) / ((v / (1 - b2 ** 4)).sqrt() + 1e-8)
+    want, terms = old * (1 - kw["lr"] * kw["weight_decay"]) - by * m, by * (b1 * m0.abs() + (1 - b1) * g.abs())
+    off = (first.double() - want).abs()
+    assert (off <= torch.finfo(dtype).eps / 2 * want.abs() + SLACK * (old.abs() + terms)).all()
+    assert int(mine.state[first]["step"]) == 4 and int(mine.state[late]["step"]) == 1
+    assert mine.state[late]["exp_avg"].dtype == (torch.float32 if bits == 32 else torch.float8_e4m3fn)
