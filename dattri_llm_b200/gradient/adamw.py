@@ -13,6 +13,13 @@ import torch
 from dattri_llm_b200.ops.optim import adamw_moments, adamw_state, adamw_step
 
 
+def _refuse(group: dict) -> None:
+    """Settings of ``torch.optim.AdamW``'s groups that would change the update and are not implemented here."""
+    for key in ("amsgrad", "differentiable"):
+        if group.get(key):
+            raise NotImplementedError(f"AdamW of this library does not implement {key}=True")
+
+
 class AdamW(torch.optim.AdamW):
     """``torch.optim.AdamW`` whose step is one launch for all tensors of a group and type.
 
@@ -22,7 +29,8 @@ class AdamW(torch.optim.AdamW):
             states of new parameters are held: loaded ones keep the form that they were saved in.
 
     The update counts are kept on the host: a step is not captured into a CUDA graph, which
-    would repeat one count's bias correction.  Parameters sharded as DTensors (FSDP2) are not supported.
+    would repeat one count's bias correction.  Parameters sharded as DTensors (FSDP2) are not
+    supported, nor are ``amsgrad`` and ``differentiable``, in a group or in a loaded state.
     """
 
     def __init__(self, params, lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
@@ -33,6 +41,7 @@ class AdamW(torch.optim.AdamW):
             self._settle(group)
 
     def _settle(self, group: dict) -> None:
+        _refuse(group)
         bits = group.setdefault("state_bits", self.defaults["state_bits"])
         if bits not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32, got {bits}")
@@ -41,6 +50,7 @@ class AdamW(torch.optim.AdamW):
                 raise NotImplementedError("AdamW of this library steps whole tensors, not DTensors")
 
     def add_param_group(self, param_group: dict) -> None:
+        _refuse(param_group)
         super().add_param_group(param_group)
         if "state_bits" in self.defaults:  # not while the base class is being made
             self._settle(self.param_groups[-1])
@@ -88,6 +98,8 @@ class AdamW(torch.optim.AdamW):
     def load_state_dict(self, state_dict: dict) -> None:
         """As ``torch.optim``'s, without its cast of the states to the parameters' type.  A state of
         ``torch.optim.AdamW`` is taken too; ``state_bits``, which it does not have, stay as they are."""
+        for group in state_dict["param_groups"]:
+            _refuse(group)
         bits = [group["state_bits"] for group in self.param_groups]
         super().load_state_dict(state_dict)
         for group, own in zip(self.param_groups, bits, strict=True):

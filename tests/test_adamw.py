@@ -420,3 +420,22 @@ def test_a_state_of_torchs_own_adamw_goes_on(device, bits, dtype):
     assert (off <= torch.finfo(dtype).eps / 2 * want.abs() + SLACK * (old.abs() + terms)).all()
     assert int(mine.state[first]["step"]) == 4 and int(mine.state[late]["step"]) == 1
     assert mine.state[late]["exp_avg"].dtype == (torch.float32 if bits == 32 else torch.float8_e4m3fn)
+
+
+@pytest.mark.parametrize("key", ["amsgrad", "differentiable"])
+def test_settings_that_would_be_dropped_are_refused(key):
+    p = torch.nn.Parameter(torch.randn(5))
+    theirs = torch.optim.AdamW([p], **{key: True})
+    if key == "amsgrad":  # a differentiable step needs weights that are no leaves
+        p.grad = torch.ones_like(p)
+        theirs.step()
+    p = torch.nn.Parameter(p.detach().clone())
+    mine = bw.AdamW([p])
+    with pytest.raises(NotImplementedError, match=key):
+        mine.load_state_dict(theirs.state_dict())
+    assert not mine.state and not mine.param_groups[0][key]  # it is as it was
+    with pytest.raises(NotImplementedError, match=key):
+        mine.add_param_group({"params": [torch.nn.Parameter(torch.ones(2))], key: True})
+    assert len(mine.param_groups) == 1
+    with pytest.raises(NotImplementedError, match=key):
+        bw.AdamW([{"params": [p], key: True}])
