@@ -110,7 +110,7 @@ class AdamW(torch.optim.AdamW):
         params = (p for group in self.param_groups for p in group["params"])
         for i, p in zip(ids, params, strict=True):
             for key, value in saved.get(i, {}).items():
-                if isinstance(value, torch.Tensor) and value.dim() > 0:
+                if isinstance(value, torch.Tensor) and key != "step":
                     moved = value.detach().to(p.device, copy=True)
                     if key != "scales" and moved.stride() != p.stride():  # codes and moments lie as the parameter does
                         moved = torch.empty_like(p, dtype=value.dtype, requires_grad=False).copy_(moved)

@@ -439,3 +439,20 @@ def test_settings_that_would_be_dropped_are_refused(key):
     assert len(mine.param_groups) == 1
     with pytest.raises(NotImplementedError, match=key):
         bw.AdamW([{"params": [p], key: True}])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_parameter_without_axes_goes_on_after_it_is_loaded(device, bits):
+    torch.manual_seed(8)
+    p = torch.nn.Parameter(torch.tensor(0.5, device=device, dtype=torch.bfloat16))
+    grads = [torch.randn((), device=device, dtype=torch.bfloat16) for _ in range(6)]
+    opt = bw.AdamW([p], state_bits=bits)
+    _steps(opt, p, grads[:3])
+    saved, q = copy.deepcopy(opt.state_dict()), torch.nn.Parameter(p.detach().clone())
+    other = bw.AdamW([q], state_bits=bits)
+    other.load_state_dict(saved)
+    assert torch.equal(other.moment(q, "exp_avg"), opt.moment(p, "exp_avg"))
+    _steps(opt, p, grads[3:])
+    _steps(other, q, grads[3:])
+    assert torch.equal(p, q) and torch.equal(other.moment(q, "exp_avg_sq"), opt.moment(p, "exp_avg_sq"))
