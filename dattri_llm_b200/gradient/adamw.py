@@ -109,6 +109,8 @@ class AdamW(torch.optim.AdamW):
         ids = (i for group in state_dict["param_groups"] for i in group["params"])
         params = (p for group in self.param_groups for p in group["params"])
         for i, p in zip(ids, params, strict=True):
+            if "step" in saved.get(i, {}):  # fused and capturable optimizers count on the GPU, where each step would wait for it
+                self.state[p]["step"] = torch.tensor(float(saved[i]["step"]))
             for key, value in saved.get(i, {}).items():
                 if isinstance(value, torch.Tensor) and key != "step":
                     moved = value.detach().to(p.device, copy=True)

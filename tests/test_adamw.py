@@ -456,3 +456,18 @@ def test_a_parameter_without_axes_goes_on_after_it_is_loaded(device, bits):
     _steps(opt, p, grads[3:])
     _steps(other, q, grads[3:])
     assert torch.equal(p, q) and torch.equal(other.moment(q, "exp_avg_sq"), opt.moment(p, "exp_avg_sq"))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_counts_of_a_fused_optimizer_are_kept_on_the_host(device):
+    p = torch.nn.Parameter(torch.randn(30, device=device))
+    theirs = torch.optim.AdamW([p], fused=True)
+    _steps(theirs, p, [torch.randn(30, device=device) for _ in range(2)])
+    saved = copy.deepcopy(theirs.state_dict())
+    for copied in (saved, {**saved, "state": {0: {**saved["state"][0], "step": 2}}}):  # a number, as old checkpoints have it
+        mine = bw.AdamW([p])
+        mine.load_state_dict(copied)
+        step = mine.state[p]["step"]
+        assert step.device.type == "cpu" and float(step) == 2.0
+        _steps(mine, p, [torch.randn(30, device=device)])
+        assert float(step) == 3.0 and float(theirs.state[p]["step"]) == 2.0
