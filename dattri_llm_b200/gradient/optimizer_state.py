@@ -73,7 +73,18 @@ def optimizer_from_state_dict(model: nn.Module, state_dict: dict, param_names: I
                               *, optimizer_cls: type = torch.optim.AdamW) -> torch.optim.Optimizer:
     """An *optimizer_cls* over *model* restored from a saved ``state_dict``; saved parameter
     indices are mapped to *model*'s parameters through *param_names* (default: the
-    Hugging Face Trainer order)."""
+    Hugging Face Trainer order).  Moments saved in 8 bits by
+    :class:`dattri_llm_b200.gradient.adamw.AdamW` are codes, which that class alone reads: it takes
+    the place of ``torch.optim.AdamW``, and another class is refused."""
+    if any(isinstance(saved, dict) and "scales" in saved and getattr(saved.get("exp_avg"), "dtype", None) == torch.float8_e4m3fn
+           for saved in state_dict["state"].values()):
+        from dattri_llm_b200.gradient.adamw import AdamW
+
+        if issubclass(AdamW, optimizer_cls):
+            optimizer_cls = AdamW
+        elif not issubclass(optimizer_cls, AdamW):
+            raise ValueError(f"the saved moments are 8-bit codes of {AdamW.__module__}.AdamW, which "
+                             f"{optimizer_cls.__name__} would read as numbers")
     by_name = dict(model.named_parameters())
     order = list(param_names) if param_names is not None else hf_trainer_param_names(model)
     groups = [{**{k: v for k, v in saved.items() if k != "params"},

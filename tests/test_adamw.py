@@ -471,3 +471,39 @@ def test_counts_of_a_fused_optimizer_are_kept_on_the_host(device):
         assert step.device.type == "cpu" and float(step) == 2.0
         _steps(mine, p, [torch.randn(30, device=device)])
         assert float(step) == 3.0 and float(theirs.state[p]["step"]) == 2.0
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_restored_without_a_class_coded_states_are_read_as_numbers(device):
+    from dattri_llm_b200.gradient.optimizer_state import OptimizerSnapshot, optimizer_from_state_dict
+
+    torch.manual_seed(9)
+    model = torch.nn.Sequential(torch.nn.Linear(9, 5)).to(device)
+    names = [n for n, _ in model.named_parameters()]
+    saved = {}
+    for bits in (8, 32):
+        opt = bw.AdamW(model.parameters(), state_bits=bits)
+        model(torch.randn(4, 9, device=device)).square().sum().backward()
+        opt.step()
+        saved[bits] = copy.deepcopy(opt.state_dict())
+        again = optimizer_from_state_dict(model, saved[bits], names)
+        assert isinstance(again, bw.AdamW) == (bits == 8)
+        for key in ("exp_avg", "exp_avg_sq"):
+            assert torch.equal(OptimizerSnapshot(model, again).state("0", key), OptimizerSnapshot(model, opt).state("0", key))
+    with pytest.raises(ValueError, match="8-bit codes"):
+        optimizer_from_state_dict(model, saved[8], names, optimizer_cls=torch.optim.NAdam)
+
+
+class _Mine(bw.AdamW):
+    pass
+
+
+def test_a_class_that_reads_codes_is_kept():
+    from dattri_llm_b200.gradient.optimizer_state import optimizer_from_state_dict
+
+    model = torch.nn.Linear(3, 2)
+    opt = bw.AdamW(model.parameters(), state_bits=8)
+    model(torch.ones(1, 3)).sum().backward()
+    opt.step()
+    again = optimizer_from_state_dict(model, opt.state_dict(), [n for n, _ in model.named_parameters()], optimizer_cls=_Mine)
+    assert type(again) is _Mine and again.state[model.weight]["exp_avg"].dtype == torch.float8_e4m3fn
