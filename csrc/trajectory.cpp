@@ -39,7 +39,7 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
   const bool bits8 = scales.has_value();
   const auto moment = bits8 ? torch::kFloat8_e4m3fn : torch::kFloat32;
   std::unordered_set<const void*> seen;
-  seen.reserve(3 * count);
+  seen.reserve(4 * count);
   std::vector<Tensor> held;  // gradients laid out like their parameters
   for (size_t i = 0; i < count; ++i) {
     const Tensor &p = params[i], &g = grads[i];
@@ -63,9 +63,11 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
                             s.size(0) == 2 && s.size(1) == (p.numel() + bw::kMomentBlock - 1) / bw::kMomentBlock,
                         "scales must be contiguous float32 (2, blocks of ", std::to_string(bw::kMomentBlock), " elements)");
     }
-    if (p.numel() > 0)
+    if (p.numel() > 0) {
       for (const Tensor* t : {&p, &exp_avgs[i], &exp_avg_sqs[i]})
         TORCH_CHECK_VALUE(seen.insert(t->data_ptr()).second, "a parameter or a moment is given twice");
+      TORCH_CHECK_VALUE(!bits8 || seen.insert((*scales)[i].data_ptr()).second, "scales are given twice");
+    }
   }
   bw::AdamwTable<bw::kAdamwMany> table;
   table.s.beta1 = (float)beta1;

@@ -113,7 +113,7 @@ def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor], exp_avgs: 
         step: the number of this update, from 1 on.  A captured graph repeats the update of the
             step that it was captured with.
 
-    A parameter or a moment given twice raises; so do sparse gradients.
+    A parameter, a moment or scales given twice raise; so do sparse gradients.
     """
     from dattri_llm_b200.ops import native, use_native
 
@@ -131,6 +131,9 @@ def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor], exp_avgs: 
     written = [x.data_ptr() for x in (*params, *exp_avgs, *exp_avg_sqs) if x.numel()]
     if len(set(written)) != len(written):
         raise ValueError("a parameter or a moment is given twice")
+    written += [s.data_ptr() for s in scales or () if s.numel()]
+    if len(set(written)) != len(written):
+        raise ValueError("scales are given twice")
     moment = torch.float32 if scales is None else torch.float8_e4m3fn
     for i, (p, g, m, v) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs, strict=True)):
         if g.layout != torch.strided:

@@ -507,3 +507,16 @@ def test_a_class_that_reads_codes_is_kept():
     opt.step()
     again = optimizer_from_state_dict(model, opt.state_dict(), [n for n, _ in model.named_parameters()], optimizer_cls=_Mine)
     assert type(again) is _Mine and again.state[model.weight]["exp_avg"].dtype == torch.float8_e4m3fn
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_scales_given_twice_are_refused(device):
+    params = [torch.ones(300, device=device) for _ in range(2)]
+    m, v, s = zip(*(ops.adamw_state(p, 8) for p in params), strict=True)
+    before = [x.clone() for x in (*params, *s)]
+    with pytest.raises(ValueError, match="twice"):
+        ops.adamw_step(params, [p.clone() for p in params], m, v, [s[0], s[0]], step=1, lr=0.1)
+    assert all(torch.equal(x, y) for x, y in zip((*params, *s), before, strict=True))
+    empty = [torch.ones(0, device=device) for _ in range(2)]  # nothing to write
+    m, v, s = zip(*(ops.adamw_state(p, 8) for p in empty), strict=True)
+    ops.adamw_step(empty, [p.clone() for p in empty], m, v, [s[0], s[0]], step=1, lr=0.1)
