@@ -436,6 +436,19 @@ std::pair<Tensor, OptTensor> gated_delta_rule(Tensor q, Tensor k, Tensor v, Tens
   return {out[0], want_last ? OptTensor(out[1]) : std::nullopt};
 }
 
+// Whether no two heads of a state, each dense in itself, share memory.
+bool heads_apart(const Tensor& state) {
+  const int64_t B = state.size(0), H = state.size(1), sb = state.stride(0), sh = state.stride(1), one = state.size(2) * state.size(3);
+  if (state.numel() == 0 || (B == 1 && H == 1)) return true;
+  if ((B > 1 && sb < one) || (H > 1 && sh < one)) return false;
+  if (B == 1 || H == 1 || sb >= (H - 1) * sh + one || sh >= (B - 1) * sb + one) return true;
+  for (int64_t h = 1; h < H; ++h) {  // the two sequences whose first head is nearest to head h of another one
+    const int64_t b = h * sh / sb, past = h * sh - b * sb;
+    if ((b < B && past < one) || (b + 1 < B && sb - past < one)) return false;
+  }
+  return true;
+}
+
 Tensor gated_delta_step(Tensor q, Tensor k, Tensor v, Tensor a, Tensor b, Tensor a_log, Tensor dt_bias, Tensor state,
                         std::optional<double> scale, Tensor err) {
   DeltaIn x{q, k, v, a, b, a_log, dt_bias};
@@ -448,8 +461,7 @@ Tensor gated_delta_step(Tensor q, Tensor k, Tensor v, Tensor a, Tensor b, Tensor
   TORCH_CHECK_VALUE((state.stride(3) == 1 && state.stride(2) == dv && state.stride(1) % 4 == 0 && state.stride(0) % 4 == 0 &&
                      at_multiple(state.data_ptr(), 16)) || state.numel() == 0,
                     "state must be contiguous along dk and dv, each head's on a 16-byte boundary");
-  TORCH_CHECK_VALUE(state.numel() == 0 || ((state.size(1) == 1 || state.stride(1) >= dk * dv) && (state.size(0) == 1 || state.stride(0) >= dk * dv)),
-                    "state: the heads must not overlap");
+  TORCH_CHECK_VALUE(heads_apart(state), "state: the heads must not overlap");
   const c10::cuda::CUDAGuard guard(x.q.device());
   bw::DeltaStep s;
   s.d = delta_dims(x, by);

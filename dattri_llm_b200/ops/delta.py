@@ -52,6 +52,21 @@ def _check_state(name: str, state, q, v) -> None:
         raise TypeError(f"{name} must be float32, got {state.dtype}")
 
 
+def _overlaps(state) -> bool:
+    """Whether elements of a state share memory."""
+    reach, nested = 0, True
+    for step, size in sorted(zip(state.stride(), state.shape, strict=True)):
+        if size > 1:  # each axis steps further than those of smaller steps reach together
+            nested = nested and step > reach
+            reach += (size - 1) * step
+    if nested or state.numel() == 0:
+        return False
+    place = torch.zeros((), dtype=torch.int64)
+    for step, size in zip(state.stride(), state.shape, strict=True):
+        place = place.unsqueeze(-1) + step * torch.arange(size)
+    return place.unique().numel() < state.numel()
+
+
 def _parts(q, k, v, a, b, a_log, dt_bias, scale):
     """Scaled rows of every value head, values, log-decays and write strengths, in 32 bits or more."""
     wide = torch.promote_types(q.dtype, torch.float32)
@@ -134,6 +149,8 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, a: torch
         return native().gated_delta_step(q, k, v, a, b, a_log, dt_bias, state, scale, error_word(q.device))
     scale = _check(q, k, v, a, b, a_log, dt_bias, scale)
     _check_state("state", state, q, v)
+    if _overlaps(state):
+        raise ValueError("state: the heads must not overlap")
     if torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, v, a, b, a_log, dt_bias, state)):
         raise RuntimeError("gated_delta_step has no gradient: call it under torch.no_grad(), or gated_delta_rule")
     q32, k32, v32, g, beta = _parts(q, k, v, a, b, a_log, dt_bias, scale)

@@ -424,3 +424,23 @@ def test_states_that_32_bits_do_not_count():
         out = ops.gated_delta_step(*x, *shared, state)
         want = ops.gated_delta_step(*(y[-few:] for y in x), *shared, own)
     assert torch.equal(out[-few:], want) and torch.equal(state[-few:], own)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_states_whose_heads_share_memory_are_refused(device):
+    """Strides that are large enough each by itself, but not together: head (0, 1) is head (1, 0)."""
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    x, first = make(3, 1, 1, 2, 16, 16, dtype, device, state=True)
+    args = [x[n] for n in NAMES]
+    one = 16 * 16
+    memory = torch.zeros(8 * one, device=device)
+    for outer in ((one, one), (one, 2 * one), (one, one + 16), (2 * one, 2 * one + 16), (0, one), (one, 0)):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.gated_delta_step(*args, memory.as_strided((3, 2, 16, 16), (*outer, 16, 1)))
+    assert not memory.any()
+    want = first.clone()
+    out = ops.gated_delta_step(*args, want)
+    for outer in ((2 * one, one), (one, 3 * one), (2 * one + 64, one + 16), (one + 16, 4 * one), (2 * one, 3 * one)):  # apart
+        state = memory.as_strided((3, 2, 16, 16), (*outer, 16, 1))
+        state.copy_(first)
+        assert torch.equal(ops.gated_delta_step(*args, state), out) and torch.equal(state, want)
