@@ -704,7 +704,7 @@ class GradientStreamer(GradientSource):
             fused = bool(params) and all(p.is_cuda and p.is_floating_point() for p in params)
             opt = torch.optim.AdamW(groups, lr=a.learning_rate, betas=(a.adam_beta1, a.adam_beta2),
                                     eps=a.adam_epsilon, fused=True if fused else None)
-        elif a.optim in ("adamw_8bit", "adamw_bnb_8bit"):
+        elif a.optim == "adamw_8bit":
             from dattri_llm_b200.gradient.adamw import AdamW
 
             opt = AdamW(groups, lr=a.learning_rate, betas=(a.adam_beta1, a.adam_beta2), eps=a.adam_epsilon, state_bits=8)

@@ -145,3 +145,11 @@ def test_sample_hashes_come_from_host_copies(monkeypatch):
     want = [hash_batch({"x": host["x"], "y": host["y"], "labels": host["y"]}, host["x"].shape[0])
             for host, _ in moved]
     assert got == want
+
+
+@pytest.mark.parametrize("optim", ["adamw_bnb_8bit", "adamw_torch_8bit"])
+def test_other_libraries_8_bit_optimizers_are_not_taken_for_this_ones(optim):
+    """They hold moments in other codes: a trajectory of theirs would be another one."""
+    args = bw.AttributionArguments(output_dir=tempfile.mkdtemp(), learning_rate=LR, optim=optim, lr_scheduler_type="constant", seed=SEED)
+    with pytest.raises(ValueError, match="not supported by the streamer"):
+        bw.GradientStreamer(tiny.make_model(seed=1), _dataset(), args, batch_size=BATCH, enable_update=True, loss_fn=tiny.sq_loss)
