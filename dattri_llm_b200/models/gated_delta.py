@@ -45,7 +45,8 @@ def _mixer_forward(self, hidden_states: torch.Tensor, cache_params=None, attenti
     """The mixer's forward through :mod:`dattri_llm_b200.ops.delta`."""
     layer = cache_params.layers[self.layer_idx] if cache_params is not None else None
     started = layer is not None and layer.has_previous_state
-    tracked = torch.is_grad_enabled() and (hidden_states.requires_grad or any(p.requires_grad for p in self.parameters()))
+    tracked = torch.is_grad_enabled() and (hidden_states.requires_grad or any(p.requires_grad for p in self.parameters())
+                                           or (started and layer.recurrent_states.requires_grad))
     if not _supported(self, hidden_states) or (started and (hidden_states.shape[1] > 1 or tracked)):  # the step has no gradient
         return type(self).forward(self, hidden_states, cache_params=cache_params, attention_mask=attention_mask, **kwargs)
     if attention_mask is not None and attention_mask.shape[0] > 1 and attention_mask.shape[1] > 1:
@@ -75,8 +76,7 @@ def _mixer_forward(self, hidden_states: torch.Tensor, cache_params=None, attenti
             cache_params.update_recurrent_state(held, self.layer_idx)
     else:
         out, last = gated_delta_rule(*heads, *gates, output_final_state=layer is not None)
-        if layer is not None:
-            last = last.detach()
+        if layer is not None:  # with its gradient: later tokens may send one back through it
             if layer.is_recurrent_states_initialized:
                 cache_params.update_recurrent_state(last, self.layer_idx)
             else:  # held in 32 bits: the cache itself would take the convolution's type

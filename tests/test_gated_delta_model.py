@@ -226,3 +226,37 @@ def test_moments_of_coded_states_are_recorded():
     records = [r["layers"]["model.layers.0.linear_attn.out_proj"] for r in callback.pre.values()]
     assert not records[0][0].any() and records[1][0].dtype == torch.float32
     assert records[1][0].numel() == weight.numel() and records[1][0].abs().max() > 0 and records[1][1].min() >= 0
+
+
+def _state_gradients(model, ids, loss):
+    """Gradients of a mixer's projection, the only one trained, from a prompt whose cache goes on."""
+    weight = model.requires_grad_(False).model.layers[0].linear_attn.in_proj_qkvz.weight.requires_grad_(True)
+    cache = model(input_ids=ids[:, :12], use_cache=True).past_key_values
+    loss(model, cache).backward()
+    return weight.grad
+
+
+def test_a_prompt_gets_the_gradients_of_cached_tokens():
+    """A loss on a cached token reaches the prompt's projections through the state too, as in the library's model."""
+    ids = _ids(2, 13)
+    grads = []
+    for fast in (False, True):
+        model = _model()
+        if fast:
+            accelerate_gated_delta(model, linears=False)
+        grads.append(_state_gradients(model, ids, lambda m, cache: m(input_ids=ids[:, 12:], past_key_values=cache,
+                                                                      use_cache=True).logits.square().sum()))
+    torch.testing.assert_close(grads[1], grads[0], rtol=1e-3, atol=1e-5 * float(grads[0].abs().max()))
+
+
+@pytest.mark.gpu
+def test_a_prompts_state_has_its_gradient_on_the_gpu():
+    def loss(_model, cache):
+        return cache.layers[0].recurrent_states.float().square().sum()
+
+    want = _state_gradients(_model("cuda"), _ids(2, 13, "cuda"), loss)  # fp32: the model itself
+    mine = _model("cuda", torch.bfloat16)
+    accelerate_gated_delta(mine)
+    got = _state_gradients(mine, _ids(2, 13, "cuda"), loss)
+    cos = torch.nn.functional.cosine_similarity(want.flatten().double(), got.flatten().double(), dim=0)
+    assert cos > 0.95  # gradients of bf16 activations: the direction is that of fp32
