@@ -35,7 +35,7 @@ def _supported(mixer: nn.Module, x: torch.Tensor) -> bool:
 def _convolved(mixer: nn.Module, mixed: torch.Tensor) -> torch.Tensor:
     """``silu(conv1d(mixed))`` over the tokens of ``(B, T, C)``."""
     conv = mixer.conv1d
-    watched = conv._forward_hooks or conv._forward_pre_hooks or conv._backward_hooks
+    watched = conv._forward_hooks or conv._forward_pre_hooks or conv._backward_hooks or conv._backward_pre_hooks
     if not watched and mixer.activation in ("silu", "swish") and fused.causal_conv_silu_enabled(mixed, conv):
         return fused.causal_conv_silu(mixed, conv.weight, conv.bias)
     return F.silu(conv(mixed.transpose(1, 2))[..., :mixed.shape[1]]).transpose(1, 2)

@@ -260,3 +260,19 @@ def test_a_prompts_state_has_its_gradient_on_the_gpu():
     got = _state_gradients(mine, _ids(2, 13, "cuda"), loss)
     cos = torch.nn.functional.cosine_similarity(want.flatten().double(), got.flatten().double(), dim=0)
     assert cos > 0.95  # gradients of bf16 activations: the direction is that of fp32
+
+
+@pytest.mark.parametrize("register", ["register_forward_hook", "register_forward_pre_hook", "register_full_backward_hook",
+                                      "register_full_backward_pre_hook"])
+def test_a_watched_convolution_is_called_as_a_module(register, monkeypatch):
+    """Whatever kind of hook it has, also where the fused kernel would take it."""
+    mixer = next(m for m in _model().modules() if gd.is_gated_delta_mixer(m))
+    monkeypatch.setattr(gd.fused, "causal_conv_silu_enabled", lambda x, conv: True)
+    monkeypatch.setattr(gd.fused, "causal_conv_silu", lambda x, weight, bias: x * 0)
+    seen = []
+    handle = getattr(mixer.conv1d, register)(lambda *a: seen.append(1))
+    x = torch.randn(2, 5, mixer.conv_dim, requires_grad=True)
+    gd._convolved(mixer, x).sum().backward()
+    assert seen
+    handle.remove()
+    assert not gd._convolved(mixer, x).any()
