@@ -69,7 +69,8 @@ def _mixer_forward(self, hidden_states: torch.Tensor, cache_params=None, attenti
     gates = (a, b, self.A_log, self.dt_bias)
     if started:
         state = layer.recurrent_states
-        held = state if state.dtype == torch.float32 and state.is_contiguous() else state.float().contiguous()
+        wide = torch.promote_types(query.dtype, torch.float32)
+        held = state if state.dtype == wide and state.is_contiguous() else state.to(wide).contiguous()
         with torch.no_grad():
             out = gated_delta_step(*heads, *gates, held)
         if held is not state:

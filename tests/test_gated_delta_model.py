@@ -276,3 +276,19 @@ def test_a_watched_convolution_is_called_as_a_module(register, monkeypatch):
     assert seen
     handle.remove()
     assert not gd._convolved(mixer, x).any()
+
+
+def test_cached_tokens_of_a_model_in_64_bits():
+    model = _model(dtype=torch.float64)
+    accelerate_gated_delta(model, linears=False)
+    ids = _ids(2, 12)
+    with torch.no_grad():
+        want = model(input_ids=ids).logits[:, 9:]
+        out = model(input_ids=ids[:, :9], use_cache=True)
+        got = []
+        for t in range(9, 12):
+            out = model(input_ids=ids[:, t:t + 1], past_key_values=out.past_key_values, use_cache=True)
+            got.append(out.logits)
+    assert out.past_key_values.layers[0].recurrent_states.dtype == torch.float64
+    # the mixer and its state stay in 64 bits; the model's own norms and angles round to 32, in another order of sums
+    assert (torch.cat(got, 1) - want).abs().max() <= 1e-5 * want.abs().max()
