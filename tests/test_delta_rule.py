@@ -444,3 +444,15 @@ def test_states_whose_heads_share_memory_are_refused(device):
         state = memory.as_strided((3, 2, 16, 16), (*outer, 16, 1))
         state.copy_(first)
         assert torch.equal(ops.gated_delta_step(*args, state), out) and torch.equal(state, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("shape", [(330, 1, 1, 1, 64, 64), (75, 2, 2, 4, 128, 96), (60, 3, 1, 5, 8, 104), (149, 2, 2, 2, 120, 120)])
+def test_many_heads_of_few_and_of_many_columns(dtype, shape):
+    """On either side of the width from which on CTAs stay."""
+    x, state = make(*shape, dtype, "cuda", state=True)
+    want, want_last = recurrence({n: y.double() for n, y in x.items()}, state.double())
+    out = ops.gated_delta_step(*(x[n] for n in NAMES), state)
+    close("out", out, want.cpu(), dtype, 2.0 ** -18)
+    close("state", state, want_last.cpu(), torch.float32, 2.0 ** -18)
