@@ -9,7 +9,12 @@
 // code at least, so that no weight is divided by eps alone because its neighbours' gradients are large. The step
 // itself uses the moments before they are rounded to codes.
 //
-// What bounds it: memory. A bf16 weight moves 22 bytes with moments in 32 bits and 10 with moments in 8.
+// Sums of squares are fp32: a gradient whose square passes its range (1e20 or so) leaves an infinite root. The codes of its block of
+// 256 then have an infinite scale, and the next step makes NaN of them, as an infinite gradient does at once.
+//
+// What bounds it: a bf16 weight moves 22 bytes with moments in 32 bits, at the rate of a copy: 486 M weights take 1,590 us. With
+// moments in 8 bits it moves 10, in 1,180 us: 60 instructions an element fill 70 % of the issue slots while memory runs at 60 % of a
+// copy's rate; 64 registers leave 32 warps to an SM, too few to fill either.
 #include "adamw.cuh"
 
 #include <cuda_fp8.h>

@@ -128,7 +128,8 @@ __global__ void __launch_bounds__(kThreads, 4) step_kernel(const DeltaStep s) {
 
 // Many sequences: CTAs that stay and take head after head, the states of the next ones on their way by bulk copies while one is
 // worked on in registers and another goes back. A thread takes four neighbouring columns of every 16th row; sums over rows go by
-// shuffles over four of them, then through shared memory. 2,048 heads of 128 x 128: 64 us, 4.2 TB/s.
+// shuffles over four of them, then through shared memory. 2,048 heads of 128 x 128: 62 us, 4.3 TB/s. What bounds it: one group of
+// threads takes a head's waits, its two sums and its way back one behind the other, 4.5 us a head; the bytes would take 41 us.
 constexpr int kStayThreads = 512, kStayRows = kMostKeyDim / 16, kBuffers = 3, kStayCols = 128,
               kStayFloats = kMostKeyDim * kStayCols;
 

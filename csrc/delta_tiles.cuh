@@ -203,7 +203,7 @@ struct Seat {
   }
 };
 
-// Threads of the sixteen warps that convert (eight leave half of the issue slots empty: a training pass took 1085 us with them);
+// Threads of the sixteen warps that convert (eight leave half of the issue slots empty: a training pass took 8 % longer with them);
 // another warp's first lane copies and multiplies.
 constexpr int kWorkers = 512, kControl = kWorkers / 32;
 

@@ -96,7 +96,11 @@ def is_gated_delta_mixer(module: nn.Module) -> bool:
 
 def accelerate_gated_delta(model: nn.Module, *, linears: bool = True) -> int:
     """Install the library's gated delta rule on every such mixer of *model* (and, with *linears*,
-    put its bias-free linears on the tcgen05 kernels).  Returns the number of mixers."""
+    put its bias-free linears on the tcgen05 kernels).  Returns the number of mixers.
+
+    On the GPU a mixer runs the rule where its hidden states are bf16 or fp16 and its heads are of sizes that
+    :func:`~dattri_llm_b200.ops.gated_delta_rule` takes; otherwise its own forward.  Weights in fp32 have hidden states in fp32, under
+    autocast too.  Mixers whose projections are cut otherwise than Qwen3-Next's are left alone and not counted."""
     mixers = [m for m in model.modules() if is_gated_delta_mixer(m)]
     for mixer in mixers:
         mixer.forward = types.MethodType(_mixer_forward, mixer)

@@ -120,7 +120,9 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, a: torch
 
     Returns:
         ``(out (B, T, H, dv), final state (B, H, dk, dv) fp32 or None)``.  Both backpropagate into
-        all inputs.  For the backward the forward keeps the state before every chunk.  A token
+        all inputs.  For the backward the forward keeps the state before every chunk and the chunks'
+        matrices: 2.3 KB a token and value head of 128 x 128 on the GPU, where two value heads share a
+        key head.  Operands of the products carry 16 bits there: a final state is 1e-6 to 6e-6 of its norm off.  A token
         with ``b = -inf`` writes nothing; one with ``a = +inf`` forgets everything before it.
     """
     if use_native(q):

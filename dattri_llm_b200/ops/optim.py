@@ -108,7 +108,8 @@ def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor], exp_avgs: 
         grads: of the parameters' types, or fp32.
         exp_avgs, exp_avg_sqs: the moments, laid out like the parameters: fp32, or with *scales*
             e4m3 codes, 256 elements to a scale (see :func:`adamw_state`).  What stands for ``v``
-            is its root; a root that is not zero keeps a code that is not zero.
+            is its root; a root that is not zero keeps a code that is not zero.  A gradient whose square
+            is infinite in fp32 makes NaN of its block's moments, as an infinite one does.
         scales: ``None``, or for each parameter fp32 ``(2, blocks)``.
         step: the number of this update, from 1 on.  A captured graph repeats the update of the
             step that it was captured with.
