@@ -76,20 +76,20 @@ def optimizer_from_state_dict(model: nn.Module, state_dict: dict, param_names: I
     Hugging Face Trainer order).  Moments saved in 8 bits by
     :class:`dattri_llm_b200.gradient.adamw.AdamW` are codes, which that class alone reads: it takes
     the place of ``torch.optim.AdamW``, and another class is refused."""
-    if any(isinstance(saved, dict) and "scales" in saved and getattr(saved.get("exp_avg"), "dtype", None) == torch.float8_e4m3fn
-           for saved in state_dict["state"].values()):
-        from dattri_llm_b200.gradient.adamw import AdamW
+    from dattri_llm_b200.gradient.adamw import AdamW
 
-        if issubclass(AdamW, optimizer_cls):
-            optimizer_cls = AdamW
-        elif not issubclass(optimizer_cls, AdamW):
-            raise ValueError(f"the saved moments are 8-bit codes of {AdamW.__module__}.AdamW, which "
-                             f"{optimizer_cls.__name__} would read as numbers")
+    coded = any(isinstance(saved, dict) and "scales" in saved and getattr(saved.get("exp_avg"), "dtype", None) == torch.float8_e4m3fn
+                for saved in state_dict["state"].values())
+    if coded and isinstance(optimizer_cls, type) and issubclass(AdamW, optimizer_cls):
+        optimizer_cls = AdamW
     by_name = dict(model.named_parameters())
     order = list(param_names) if param_names is not None else hf_trainer_param_names(model)
     groups = [{**{k: v for k, v in saved.items() if k != "params"},
                "params": [by_name[order[i]] for i in saved["params"]]} for saved in state_dict["param_groups"]]
     restored = optimizer_cls(groups)
+    if coded and not isinstance(restored, AdamW):
+        raise ValueError(f"the saved moments are 8-bit codes of {AdamW.__module__}.AdamW, which {type(restored).__name__} would "
+                         "read as numbers")
     restored.load_state_dict(state_dict)
     return restored
 

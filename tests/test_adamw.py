@@ -520,3 +520,19 @@ def test_scales_given_twice_are_refused(device):
     empty = [torch.ones(0, device=device) for _ in range(2)]  # nothing to write
     m, v, s = zip(*(ops.adamw_state(p, 8) for p in empty), strict=True)
     ops.adamw_step(empty, [p.clone() for p in empty], m, v, [s[0], s[0]], step=1, lr=0.1)
+
+
+def test_coded_states_are_restored_by_a_function_that_makes_the_class():
+    import functools
+
+    from dattri_llm_b200.gradient.optimizer_state import optimizer_from_state_dict
+
+    model = torch.nn.Linear(3, 2)
+    names = [n for n, _ in model.named_parameters()]
+    opt = bw.AdamW(model.parameters(), state_bits=8)
+    model(torch.ones(1, 3)).sum().backward()
+    opt.step()
+    again = optimizer_from_state_dict(model, opt.state_dict(), names, optimizer_cls=functools.partial(bw.AdamW, state_bits=8))
+    assert torch.equal(again.moment(model.weight, "exp_avg"), opt.moment(model.weight, "exp_avg"))
+    with pytest.raises(ValueError, match="8-bit codes"):
+        optimizer_from_state_dict(model, opt.state_dict(), names, optimizer_cls=functools.partial(torch.optim.AdamW))
