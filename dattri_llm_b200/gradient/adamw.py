@@ -98,13 +98,30 @@ class AdamW(torch.optim.AdamW):
     def load_state_dict(self, state_dict: dict) -> None:
         """As ``torch.optim``'s, without its cast of the states to the parameters' type.  A state of
         ``torch.optim.AdamW`` is taken too; ``state_bits``, which it does not have, stay as they are."""
-        for group in state_dict["param_groups"]:
-            _refuse(group)
         bits = [group["state_bits"] for group in self.param_groups]
-        super().load_state_dict(state_dict)
-        for group, own in zip(self.param_groups, bits, strict=True):
-            group.setdefault("state_bits", own)
-            self._settle(group)
+        final: dict = {}  # what the user's hooks make of the dictionary
+
+        def look(_optimizer, given: dict) -> None:
+            for group in given["param_groups"]:
+                _refuse(group)
+            final.update(given)
+
+        def keep(_optimizer) -> None:
+            for group, own in zip(self.param_groups, bits, strict=True):
+                group.setdefault("state_bits", own)
+                self._settle(group)
+            self._keep_types(final)
+
+        # Behind the other hooks on the dictionary, before those on the loaded optimizer.
+        hooks = [self.register_load_state_dict_pre_hook(look), self.register_load_state_dict_post_hook(keep, prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    def _keep_types(self, state_dict: dict) -> None:
+        """The states as they were saved, which ``torch.optim`` has cast to the parameters' types."""
         saved = state_dict["state"]
         ids = (i for group in state_dict["param_groups"] for i in group["params"])
         params = (p for group in self.param_groups for p in group["params"])

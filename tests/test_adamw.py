@@ -536,3 +536,27 @@ def test_coded_states_are_restored_by_a_function_that_makes_the_class():
     assert torch.equal(again.moment(model.weight, "exp_avg"), opt.moment(model.weight, "exp_avg"))
     with pytest.raises(ValueError, match="8-bit codes"):
         optimizer_from_state_dict(model, opt.state_dict(), names, optimizer_cls=functools.partial(torch.optim.AdamW))
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_hooks_on_loading_are_followed(bits):
+    """A hook's dictionary is the one that is loaded, and hooks on the loaded optimizer see its states' own types."""
+    torch.manual_seed(10)
+    first, second = (torch.nn.Parameter(torch.randn(20).to(torch.bfloat16)) for _ in range(2))
+    opt = bw.AdamW([first, second], state_bits=bits)
+    first.grad, second.grad = torch.randn_like(first), torch.randn_like(second)
+    opt.step()
+    other = bw.AdamW([first, second], state_bits=bits)
+
+    def swap(_optimizer, given):
+        return {**given, "state": {0: given["state"][1], 1: given["state"][0]}}
+
+    seen = []
+    other.register_load_state_dict_pre_hook(swap)
+    other.register_load_state_dict_post_hook(lambda o: seen.append(o.state[first]["exp_avg"].dtype))
+    other.load_state_dict(opt.state_dict())
+    assert torch.equal(other.moment(first, "exp_avg"), opt.moment(second, "exp_avg"))
+    assert torch.equal(other.moment(second, "exp_avg_sq"), opt.moment(first, "exp_avg_sq"))
+    assert seen == [torch.float32 if bits == 32 else torch.float8_e4m3fn]
+    other.load_state_dict(opt.state_dict())
+    assert len(seen) == 2
