@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import torch
 
-from dattri_llm_b200.ops.optim import adamw_moments, adamw_state, adamw_step
+from dattri_llm_b200.ops.optim import adamw_moments, adamw_state, adamw_state_like, adamw_step
 
 
 def _refuse(group: dict) -> None:
@@ -130,9 +130,11 @@ class AdamW(torch.optim.AdamW):
                 self.state[p]["step"] = torch.tensor(float(saved[i]["step"]))
             for key, value in saved.get(i, {}).items():
                 if isinstance(value, torch.Tensor) and key != "step":
-                    moved = value.detach().to(p.device, copy=True)
-                    if key != "scales" and moved.stride() != p.stride():  # codes and moments lie as the parameter does
-                        moved = torch.empty_like(p, dtype=value.dtype, requires_grad=False).copy_(moved)
-                    if key in ("exp_avg", "exp_avg_sq") and moved.dtype != torch.float8_e4m3fn:
-                        moved = moved.float()  # moments that another AdamW kept in the parameters' type
-                    self.state[p][key] = moved
+                    self.state[p][key] = value.detach().to(p.device, copy=True)
+            state = self.state.get(p, {})
+            if "scales" in state:
+                keys = ("exp_avg", "exp_avg_sq", "scales")
+                state.update(zip(keys, adamw_state_like(p, *(state[key] for key in keys)), strict=True))
+                continue
+            for key in {"exp_avg", "exp_avg_sq"} & state.keys():  # another AdamW may keep them in the parameters' type
+                state[key] = torch.empty_like(p, dtype=torch.float32, requires_grad=False).copy_(state[key])

@@ -74,6 +74,20 @@ def adamw_moments(exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor,
     return _spread(exp_avg, scales[0]), _spread(exp_avg_sq, scales[1]).square()
 
 
+def adamw_state_like(param: torch.Tensor, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor,
+                     scales: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """A state of 8-bit moments in the layout of *param*.  Blocks go by the order of memory: where that differs, the
+    moments are written as codes once more."""
+    if [t for n, t in zip(param.shape, exp_avg.stride(), strict=True) if n > 1] == [
+            t for n, t in zip(param.shape, param.stride(), strict=True) if n > 1]:
+        return *(torch.empty_like(param, dtype=x.dtype, requires_grad=False).copy_(x) for x in (exp_avg, exp_avg_sq)), scales
+    m, v, s = adamw_state(param, 8)
+    for codes, to, row in ((exp_avg, m, 0), (exp_avg_sq, v, 1)):
+        wide = torch.empty_like(param, dtype=torch.float32, requires_grad=False).copy_(_spread(codes, scales[row]))
+        _encode(wide, to, s[row], bool(row))
+    return m, v, s
+
+
 def _adamw_torch(p, g, exp_avg, exp_avg_sq, scales, step, lr, betas, eps, weight_decay, maximize) -> None:
     wide = torch.promote_types(p.dtype, torch.float32)
     m, v = (x.to(wide) for x in adamw_moments(exp_avg, exp_avg_sq, scales))

@@ -405,7 +405,7 @@ def test_a_state_of_torchs_own_adamw_goes_on(device, bits, dtype):
     mine = bw.AdamW([first, late], lr=5.0, state_bits=bits)
     mine.load_state_dict(copy.deepcopy(theirs.state_dict()))
     group = mine.param_groups[0]
-    assert group["lr"] == kw["lr"] and group["state_bits"] == bits
+    assert group["lr"] == kw["lr"] and group["state_bits"] == bits and late not in mine.state
     m0, v0 = (theirs.state[first][key].double() for key in ("exp_avg", "exp_avg_sq"))
     for key, was in (("exp_avg", m0), ("exp_avg_sq", v0)):
         assert torch.equal(mine.moment(first, key).double(), was)
@@ -560,3 +560,52 @@ def test_hooks_on_loading_are_followed(bits):
     assert seen == [torch.float32 if bits == 32 else torch.float8_e4m3fn]
     other.load_state_dict(opt.state_dict())
     assert len(seen) == 2
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_state_is_loaded_into_a_parameter_that_lies_otherwise(device, bits):
+    """Blocks of 256 elements go by the order of memory, which the loaded parameter need not share.  A moment that is written as
+    a code for a second time is off by another 2^-4 of itself or half a step of the smallest codes."""
+    torch.manual_seed(11)
+    w = torch.randn(40, 33, device=device)
+    w[:, 5] *= 100  # blocks of one order and of the other have other scales
+    g = w * torch.rand(40, 33, device=device)
+    p = torch.nn.Parameter(w.t().contiguous().t())
+    opt = bw.AdamW([p], state_bits=bits)
+    _steps(opt, p, [g, 2 * g])
+    q = torch.nn.Parameter(w.clone())
+    other = bw.AdamW([q], state_bits=bits)
+    other.load_state_dict(copy.deepcopy(opt.state_dict()))
+    assert q.stride() != p.stride() and other.state[q]["exp_avg"].stride() == q.stride()
+    for key in ("exp_avg", "exp_avg_sq"):
+        want, got = opt.moment(p, key).double(), other.moment(q, key).double()
+        if bits == 32:
+            assert torch.equal(got, want)
+            continue
+        if key == "exp_avg_sq":
+            want, got = want.sqrt(), got.sqrt()
+        each = (want.abs().reshape(-1)[:1280].view(5, 256).amax(1) / 448).repeat_interleave(256)
+        off, size = (x.reshape(-1)[:1280] for x in ((got - want).abs(), want.abs()))
+        assert (off <= (2.0 ** -4 + SLACK) * size + (2.0 ** -9 + SLACK) * each).all()
+    _steps(other, q, [g])
+    assert torch.isfinite(q).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_axes_of_one_element_do_not_change_the_order(device):
+    """Their steps say nothing of where an element lies: codes are loaded as they are."""
+    torch.manual_seed(12)
+    p = torch.nn.Parameter(torch.randn(1, 300, device=device))
+    opt = bw.AdamW([p], state_bits=8)
+    _steps(opt, p, [torch.randn(1, 300, device=device) for _ in range(3)])
+    q = torch.nn.Parameter(torch.empty_strided((1, 300), (7, 1), device=device).copy_(p.detach()))
+    other = bw.AdamW([q], state_bits=8)
+    other.load_state_dict(copy.deepcopy(opt.state_dict()))
+    for key in ("exp_avg", "exp_avg_sq"):
+        assert torch.equal(other.state[q][key].view(torch.uint8), opt.state[p][key].view(torch.uint8))
+    assert torch.equal(other.state[q]["scales"], opt.state[p]["scales"])
+    g = torch.randn(1, 300, device=device)
+    _steps(opt, p, [g])
+    _steps(other, q, [g])
+    assert torch.equal(p, q)
