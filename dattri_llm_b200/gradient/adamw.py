@@ -132,6 +132,8 @@ class AdamW(torch.optim.AdamW):
                 if isinstance(value, torch.Tensor) and key != "step":
                     self.state[p][key] = value.detach().to(p.device, copy=True)
             state = self.state.get(p, {})
+            if any(state[key].shape != p.shape for key in {"exp_avg", "exp_avg_sq"} & state.keys()):
+                continue  # of another parameter: the step refuses it
             if "scales" in state:
                 keys = ("exp_avg", "exp_avg_sq", "scales")
                 state.update(zip(keys, adamw_state_like(p, *(state[key] for key in keys)), strict=True))

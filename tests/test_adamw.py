@@ -609,3 +609,13 @@ def test_axes_of_one_element_do_not_change_the_order(device):
     _steps(opt, p, [g])
     _steps(other, q, [g])
     assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_state_of_another_shape_is_not_spread_over_a_parameter(bits):
+    p, q = torch.nn.Parameter(torch.randn(1, 300)), torch.nn.Parameter(torch.randn(3, 300))
+    opt, other = bw.AdamW([p], state_bits=bits), bw.AdamW([q], state_bits=bits)
+    _steps(opt, p, [torch.randn(1, 300)])
+    other.load_state_dict(copy.deepcopy(opt.state_dict()))  # as torch.optim loads it
+    with pytest.raises(ValueError):
+        _steps(other, q, [torch.randn(3, 300)])
