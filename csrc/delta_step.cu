@@ -316,8 +316,9 @@ __global__ void __launch_bounds__(kStayThreads, 1) step_stay_kernel(const DeltaS
 template <typename I>
 void launch(const DeltaStep& s, cudaStream_t stream) {
   const long long heads = (long long)s.d.B * s.d.H;
-  // The pipeline pays for wide heads from some three of them for each SM on; below, more and smaller CTAs do, and so they do for heads
-  // of 96 columns or fewer, which leave a quarter of the staying threads or more without a column. bf16, us with staying CTAs
+  // The pipeline pays for wide heads from some three of them for each SM on, and is taken from two on, where it costs 8 % at most: calls
+  // of few and of many more heads then give the same bits. Below, more and smaller CTAs pay, and so they do for heads of 96
+  // columns or fewer, which leave a quarter of the staying threads or more without a column. bf16, us with staying CTAs
   // and with a CTA to each 32 columns: heads of 128 x 128, 32 of them 5.5 and 4.0, 160 10.8 and 9.3, 320 15.0 and 13.9, 512 19.6
   // and 20.5, 1,024 33 and 39, 2,048 62 and 81; of 32 x 128, 512 14.0 and 14.9, 2,048 43 and 53; of 128 x 112, 320 14.8 and 14.3,
   // 2,048 61 and 78; of 96 x 96, 320 13.2 and 10.6, 2,048 53 and 51; of 64 x 64, 320 11.0 and 7.7, 2,048 43 and 30.
