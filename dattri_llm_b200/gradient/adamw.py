@@ -77,14 +77,16 @@ class AdamW(torch.optim.AdamW):
                     state["exp_avg"], state["exp_avg_sq"], scales = adamw_state(p, bits)
                     if scales is not None:
                         state["scales"] = scales
-                state["step"] += 1
-                lists = batches.setdefault((p.device, int(state["step"]), "scales" in state), [[], [], [], [], []])
-                for to, x in zip(lists, (p, p.grad, state["exp_avg"], state["exp_avg_sq"], state.get("scales")), strict=True):
+                lists = batches.setdefault((p.device, int(state["step"]) + 1, "scales" in state), [[], [], [], [], [], []])
+                for to, x in zip(lists, (p, p.grad, state["exp_avg"], state["exp_avg_sq"], state.get("scales"), state["step"]),
+                                 strict=True):
                     to.append(x)
-            for (_device, step, coded), (params, grads, m, v, scales) in batches.items():
+            for (_device, step, coded), (params, grads, m, v, scales, counts) in batches.items():
                 adamw_step(params, grads, m, v, scales if coded else None, step=step, lr=float(group["lr"]),
                            betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
                            maximize=group["maximize"])
+                for count in counts:  # a refused step is not counted
+                    count += 1
         return loss
 
     def moment(self, param: torch.Tensor, key: str) -> torch.Tensor | None:

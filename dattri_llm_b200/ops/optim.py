@@ -159,4 +159,5 @@ def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor], exp_avgs: 
             raise TypeError(f"moments must be {moment}, got {m.dtype} and {v.dtype}")
         if scales is not None and scales[i].shape != (2, -(-p.numel() // MOMENT_BLOCK)):
             raise ValueError(f"scales must be (2, blocks of {MOMENT_BLOCK} elements), got {tuple(scales[i].shape)}")
+    for i, (p, g, m, v) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs, strict=True)):
         _adamw_torch(p, g, m, v, None if scales is None else scales[i], step, lr, betas, eps, weight_decay, maximize)

@@ -619,3 +619,19 @@ def test_a_state_of_another_shape_is_not_spread_over_a_parameter(bits):
     other.load_state_dict(copy.deepcopy(opt.state_dict()))  # as torch.optim loads it
     with pytest.raises(ValueError):
         _steps(other, q, [torch.randn(3, 300)])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_refused_step_changes_nothing(device):
+    torch.manual_seed(13)
+    p, q = torch.nn.Parameter(torch.randn(4, 3, device=device)), torch.nn.Parameter(torch.randn(4, 3, device=device))
+    opt, start = bw.AdamW([p, q]), p.detach().clone()
+    p.grad, q.grad = torch.ones_like(p), torch.ones_like(q).to_sparse()
+    with pytest.raises(NotImplementedError):
+        opt.step()
+    assert all(float(opt.state[x]["step"]) == 0 for x in (p, q)) and torch.equal(p, start)
+    old, q.grad = q.detach().clone(), torch.ones_like(q)
+    opt.step()
+    assert all(float(opt.state[x]["step"]) == 1 for x in (p, q))
+    # the first step: by lr whatever the gradient's size, and the weight's decay
+    assert ((old * (1 - 1e-5) - 1e-3 - q).abs() <= 4 * torch.finfo(torch.float32).eps * (1 + old.abs())).all()
